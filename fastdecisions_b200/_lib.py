@@ -52,6 +52,20 @@ SIGNATURES = {
     "fdk_slot_readout": (i32, [vp, i32, vp, i64, vp, vp, i64, vp, i32, vp, i64, f32, f32, vp, vp, vp]),
 }
 
+SIGNATURES.update({
+    "fdk_paged_kv_write": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp,
+                                 vp, i64, i64, i64, i64, vp]),
+    "fdk_paged_kv_read": (i32, [vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64, i64, i64,
+                                i64, vp, vp, vp]),
+    "fdk_paged_gqa_workspace_size": (sz, [i64, i64, i64, i64, i64, i64, i64]),
+    "fdk_paged_gqa_fwd": (i32, [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64,
+                                i64, i64, i64, i64, i64, i64, f32, vp, i64, i32, vp, vp, sz, vp]),
+    "fdk_recurrent_gated_delta_rule_fwd": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64,
+                                                 f32, i32, vp, vp, i64, vp, vp, i64, vp, vp]),
+    "fdk_packed_conv_state": (i32, [vp, i64, vp, vp, i64, i64, i64, i32, i64, i64, vp, vp, i64, vp, vp, i64, vp, vp,
+                                    vp, vp]),
+})
+
 _lib = None
 
 

@@ -753,6 +753,12 @@ extern "C" int fdk_poll_device_error(int* code) {
   const int gm = fdk::gemm_take_device_error();
   if (gm < 0) return set_error(FDK_ERR_DEVICE, "poll_device_error: cannot read the device error word");
   if (gm) h |= 16;  // a GEMM wait ran out
+  const int kv = fdk::paged_kv_take_device_error(), pa = fdk::paged_attn_take_device_error();
+  const int sp = fdk::state_take_device_error();
+  if (kv < 0 || pa < 0 || sp < 0)
+    return set_error(FDK_ERR_DEVICE, "poll_device_error: cannot read the device error word");
+  if (kv || (pa & 1)) h |= 32;  // a paged-cache call found an invalid segment range, length or page id
+  if (sp) h |= 64;              // a state-pool call found an invalid segment range or slot
   if (code) *code = h;
   return FDK_OK;
 }

@@ -26,6 +26,10 @@ int ensure_smem_attr(const void* func, int bytes, const char* what);
 int delta_take_device_error();
 // Reads and clears the GEMM kernel's device error word.
 int gemm_take_device_error();
+// Read and clear the error words of the paged-cache and state-pool kernels (invalid device metadata).
+int paged_kv_take_device_error();
+int paged_attn_take_device_error();
+int state_take_device_error();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,696 @@
+// Causal GQA attention of the newest tokens of packed sequences over a paged KV cache.
+//
+// Segment s's n = cu[s+1] - cu[s] tokens are the last of its kv_lens[s] cached positions (their own keys
+// are already written): token i attends to positions 0 .. kv_lens[s] - n + i.  A token whose mask leaves
+// nothing gets zeros.  The query heads of a KV head are packed with the tokens into rows (row = token *
+// group + head), so every cached row brought into shared memory feeds them all.
+//
+// This file: the few-row kernel (mma.sync tiles of 16 rows, split over the keys) and the join of splits.
+// Its work is bound by reading the cache: at one token a sequence each cached byte is used by `group`
+// rows only, far below the tensor cores' rate, so the 16-row warp-level MMA -- which needs no padding to
+// 128 rows and keeps S and P in registers -- loses nothing to the memory time it hides behind.
+//
+//   CTA: BM = 16 WM rows of one (segment, KV head), keys [k0, k1) in tiles of 64; 4 warps = WM row
+//   groups x WK = 4 / WM key groups.  Tiles stream through a ring of cp.async stages.  Each warp keeps
+//   its own running maximum, sum and O (fp32) over its keys; key groups are joined through shared memory
+//   at the end, splits through a float32 workspace by the second kernel.
+//   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S's column, V's
+//   multiplies P's column before its rounding to fp16, relative to the largest V scale so far (O is
+//   rescaled when that grows, as for the maximum).  q is brought to fp16 with a power of two a row.
+#include <math.h>
+
+#include "paged.cuh"
+#include "sm100.cuh"
+
+namespace fdk {
+namespace pattn {
+using paged::scale_value;
+using sm100::ex2;
+
+__device__ int g_error = 0;
+
+struct Params {
+  const bf16* q;
+  int64_t ld_q;
+  const uint8_t* k_cache;  // bytes
+  const uint8_t* v_cache;
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  int64_t kpage, vpage;  // bytes between pages
+  int64_t kscale_page, vscale_page;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* cu;
+  const int32_t* kv_lens;
+  int64_t tokens, num_pages;
+  int nseg, max_pages, page_shift, hq, hkv, group, nsplit, row_blocks;
+  float sl2;  // softmax scale * log2(e)
+  const bf16* gate;
+  int64_t ld_gate;
+  int gate_hstride;
+  bf16* out;
+  float* part_o;   // [nsplit][tokens * hq][D], unnormalised
+  float2* part_ml; // [nsplit][tokens * hq]: (running max in the exp2 domain, sum)
+};
+
+// One segment's metadata, checked.  n: new tokens, past: cached positions before them (may be negative:
+// then the first -past tokens see nothing).  Invalid metadata reads as "no keys" and is reported.
+struct Seg {
+  int begin, n;
+  int64_t past;
+};
+__device__ __forceinline__ Seg segment(const Params& p, int s, bool report) {
+  Seg r;
+  int end;
+  if (!paged::segment_range(p.cu, s, p.tokens, r.begin, end)) {
+    if (report) atomicOr(&g_error, 1);
+    r.begin = end = 0;
+  }
+  r.n = end - r.begin;
+  int64_t len = p.kv_lens[s];
+  if (len < 0 || len > ((int64_t)p.max_pages << p.page_shift)) {
+    if (report) atomicOr(&g_error, 1);
+    len = 0;
+  }
+  r.past = len - r.n;
+  return r;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int BN = 64;        // keys a tile
+constexpr int THREADS = 128;
+
+template <int D, bool QUANT>
+struct Geo {
+  static constexpr int ROW = QUANT ? D : 2 * D;   // bytes of a cached row
+  static constexpr int CH = ROW / 16;             // 16-byte chunks of it
+  static constexpr int TILE = BN * ROW;
+  static constexpr int STAGE = 2 * TILE + (QUANT ? 2 * BN : 0);
+  // stages in flight and CTAs an SM: about 100 KB of loads in flight an SM in every form
+  static constexpr int STAGES = QUANT ? (D == 128 ? 4 : 3) : 3;
+  static constexpr int RING = STAGES * STAGE;
+};
+
+// 16-byte chunk c of row r of a tile: the chunk index is XORed with the row so that the eight rows of an
+// 8x8 matrix fall into different banks
+template <int CH>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) { return (uint32_t)((r * CH + (c ^ (r & 7))) * 16); }
+
+template <int D, bool QUANT, int WM>
+__global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
+  using G = Geo<D, QUANT>;
+  constexpr int WK = 4 / WM;        // key groups
+  constexpr int KPW = BN / WK;      // keys a warp and tile
+  constexpr int NT = KPW / 8;       // 8-key column tiles of S
+  constexpr int BM = 16 * WM;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wm = warp % WM, wk = warp / WM;
+  const int g = lane >> 2, t4 = lane & 3;
+
+  // grid: x = (segment, kv head, row block) with the kv head fastest, y = split
+  const int hk = (int)(blockIdx.x % (unsigned)p.hkv);
+  const int srb = (int)(blockIdx.x / (unsigned)p.hkv);
+  const int s = srb / p.row_blocks, rb = srb % p.row_blocks;
+  const int split = blockIdx.y;
+  const Seg seg = segment(p, s, tid == 0 && hk == 0 && rb == 0 && split == 0);
+  const int rows = seg.n * p.group;
+  const int row0 = rb * BM;
+  if (tid == 0 && hk == 0 && rb == 0 && split == 0 && rows > p.row_blocks * BM) atomicOr(&g_error, 1);
+  if (row0 >= rows) return;
+  const int last_tok = (min(row0 + BM, rows) - 1) / p.group;
+  const int64_t kend64 = seg.past + last_tok + 1;
+  const int kend = kend64 > 0 ? (int)kend64 : 0;       // keys the row block can see
+  const int per = ((kend + p.nsplit * BN - 1) / (p.nsplit * BN)) * BN;
+  const int kb = min(kend, split * per), ke = min(kend, kb + per);
+  const int ntiles = (ke - kb + BN - 1) / BN;
+
+  // this lane's two rows (g and g + 8 of the warp's 16)
+  int rr[2], lim[2];
+  int64_t qrow[2];
+  bool live[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    rr[i] = row0 + wm * 16 + g + 8 * i;
+    live[i] = rr[i] < rows;
+    const int tok = live[i] ? rr[i] / p.group : 0;
+    const int head = hk * p.group + (live[i] ? rr[i] % p.group : 0);
+    lim[i] = live[i] ? (int)(seg.past + tok) : -1;   // last visible key
+    qrow[i] = (int64_t)(seg.begin + tok) * p.hq + head;
+  }
+
+  // Q fragments.  bf16: columns 2t, 2t+1 (+8) of each 16; 8-bit cache: columns 4t .. 4t+3 of each 16, in
+  // the order the byte-wise K fragments come in, as fp16 scaled by a power of two a row.
+  uint32_t qf[D / 16][4];
+  float qs[2] = {p.sl2, p.sl2};
+  if (!QUANT) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bf16* src = p.q + (qrow[i] / p.hq) * p.ld_q + (qrow[i] % p.hq) * D;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][i] = live[i] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 2 * t4) : 0u;
+        qf[kk][2 + i] = live[i] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + 2 * t4) : 0u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bf16* src = p.q + (qrow[i] / p.hq) * p.ld_q + (qrow[i] % p.hq) * D;
+      uint2 raw[D / 16];
+      float a = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        raw[kk] = live[i] ? *reinterpret_cast<const uint2*>(src + kk * 16 + 4 * t4) : make_uint2(0u, 0u);
+        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].x));
+        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].y));
+        a = fmaxf(fmaxf(a, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+      // the row's largest magnitude goes to [1, 2): fp16 keeps bf16's 8 bits down to 2^-14 of it
+      const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+      const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+      qs[i] = p.sl2 * __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].x));
+        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].y));
+        qf[kk][i] = pack_f16x2(x.x * inv, x.y * inv);
+        qf[kk][2 + i] = pack_f16x2(y.x * inv, y.y * inv);
+      }
+    }
+  }
+
+  // tile loads: chunk tid % CH of rows tid / CH + j * (128 / CH)
+  constexpr int RPP = THREADS / G::CH;   // rows a pass
+  constexpr int PASSES = BN / RPP;
+  const int lc = tid % G::CH, lr = tid / G::CH;
+  const int32_t* table = p.table + (int64_t)s * p.ld_table;
+  const int page_mask = (1 << p.page_shift) - 1;
+  auto page_of = [&](int key) -> int64_t {  // -1: the key is past the range or its page id is invalid
+    if (key >= ke) return -1;
+    const int64_t id = __ldg(table + (key >> p.page_shift));
+    if (id < 0 || id >= p.num_pages) {
+      atomicOr(&g_error, 1);
+      return -1;
+    }
+    return id;
+  };
+  auto load_tile = [&](int j) {
+    const int key0 = kb + j * BN;
+    const uint32_t dst = sbase + (uint32_t)(j % G::STAGES) * G::STAGE;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = lr + i * RPP;
+      const int64_t id = page_of(key0 + r);
+      const int64_t at = ((int64_t)(hk << p.page_shift) + ((key0 + r) & page_mask)) * G::ROW + lc * 16;
+      const uint32_t bytes = id >= 0 ? 16u : 0u;   // rows past the range are zero-filled
+      const int64_t pg = id >= 0 ? id : 0;
+      const uint32_t to = dst + tile_at<G::CH>(r, lc);
+      cp_async16(to, p.k_cache + pg * p.kpage + (id >= 0 ? at : 0), bytes);
+      cp_async16(to + G::TILE, p.v_cache + pg * p.vpage + (id >= 0 ? at : 0), bytes);
+    }
+    if (QUANT && tid < 8) {  // scale bytes: 16 keys at a time (page sizes are multiples of 16)
+      const int r = (tid & 3) * 16;
+      const int64_t id = page_of(key0 + r);
+      const int64_t at = (int64_t)(hk << p.page_shift) + ((key0 + r) & page_mask);
+      const uint8_t* src = tid < 4 ? p.k_scale : p.v_scale;
+      const int64_t ld = tid < 4 ? p.kscale_page : p.vscale_page;
+      cp_async16(dst + 2 * G::TILE + (tid < 4 ? 0 : BN) + r, src + (id >= 0 ? id * ld + at : 0), id >= 0 ? 16u : 0u);
+    }
+  };
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  int ev = 0;  // O is in units of 2^(ev - 127) (8-bit cache)
+
+#pragma unroll
+  for (int j = 0; j < G::STAGES - 1; ++j) {
+    if (j < ntiles) load_tile(j);
+    cp_commit();
+  }
+  for (int j = 0; j < ntiles; ++j) {
+    cp_wait<G::STAGES - 2>();
+    __syncthreads();  // tile j is in, and every warp is done with the stage that tile j + STAGES - 1 takes
+    if (j + G::STAGES - 1 < ntiles) load_tile(j + G::STAGES - 1);
+    cp_commit();
+    const uint32_t kt = sbase + (uint32_t)(j % G::STAGES) * G::STAGE, vt = kt + G::TILE;
+    const int krow = wk * KPW;  // first key of this warp in the tile
+    const int key0 = kb + j * BN + krow;
+
+    // S = Q K^T
+    float sc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sc[i][c] = 0.f;
+    if (!QUANT) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {  // 16 keys x 16 columns a load
+          uint32_t b[4];
+          ldsm4(b, kt + tile_at<G::CH>(krow + i * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+          mma<false>(sc[i], qf[kk], b[0], b[1]);
+          mma<false>(sc[i + 1], qf[kk], b[2], b[3]);
+        }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk += 2)
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {  // 16 keys x 32 columns a load
+          uint32_t b[4];
+          ldsm4(b, kt + tile_at<G::CH>(krow + i * 8 + (lane & 7) + ((lane >> 4) << 3), kk + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            mma<true>(sc[i + (u >> 1)], qf[kk + (u & 1)], paged::e4m3x2_to_f16x2((uint16_t)b[u]),
+                      paged::e4m3x2_to_f16x2((uint16_t)(b[u] >> 16)));
+        }
+    }
+    // scale, mask, row maximum.  Element (i, c): row c / 2, key 8 i + 2 t4 + (c & 1).
+    float vs[NT][2];
+    int etile = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (QUANT) {
+        const uint16_t kb2 = *reinterpret_cast<const uint16_t*>(smem + (kt - sbase) + 2 * G::TILE + krow + i * 8 + 2 * t4);
+        const uint16_t vb2 = *reinterpret_cast<const uint16_t*>(smem + (kt - sbase) + 2 * G::TILE + BN + krow + i * 8 + 2 * t4);
+        const float k0 = scale_value(kb2 & 255), k1 = scale_value(kb2 >> 8);
+        sc[i][0] *= k0 * qs[0];
+        sc[i][1] *= k1 * qs[0];
+        sc[i][2] *= k0 * qs[1];
+        sc[i][3] *= k1 * qs[1];
+        const int key = key0 + i * 8 + 2 * t4;
+        const int v0 = key < ke ? vb2 & 255 : 0, v1 = key + 1 < ke ? vb2 >> 8 : 0;
+        etile = max(etile, max(v0, v1));
+        vs[i][0] = __int_as_float(v0);
+        vs[i][1] = __int_as_float(v1);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[i][c] *= p.sl2;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (key0 + i * 8 + 2 * t4 + (c & 1) > min(lim[c >> 1], ke - 1)) sc[i][c] = -INFINITY;
+    }
+    float corr[2], mu[2];
+    bool grow = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mx = fmaxf(mx, fmaxf(sc[i][2 * r], sc[i][2 * r + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx);
+      mu[r] = mn == -INFINITY ? 0.f : mn;      // a row without keys so far: exp2(-inf - 0) = 0
+      corr[r] = mn > m[r] ? ex2(m[r] - mu[r]) : 1.f;
+      grow |= mn > m[r];
+      m[r] = mn;
+      l[r] *= corr[r];
+    }
+    float fv = 1.f;
+    if (QUANT) {
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) etile = max(etile, __shfl_xor_sync(0xffffffffu, etile, off));
+      if (etile > ev) {  // a larger V scale: O moves to its units
+        fv = ev == 0 ? 0.f : scale_value(max(ev - etile + 127, 0));
+        ev = etile;
+        grow = true;
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= corr[0] * fv;
+        o[i][1] *= corr[0] * fv;
+        o[i][2] *= corr[1] * fv;
+        o[i][3] *= corr[1] * fv;
+      }
+    }
+    // P, the row sums (of the unrounded p), and O += P V
+#pragma unroll
+    for (int i = 0; i < NT; i += 2) {
+      uint32_t a[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float p0 = ex2(sc[i + u][0] - mu[0]), p1 = ex2(sc[i + u][1] - mu[0]);
+        const float p2 = ex2(sc[i + u][2] - mu[1]), p3 = ex2(sc[i + u][3] - mu[1]);
+        l[0] += p0 + p1;
+        l[1] += p2 + p3;
+        if (QUANT) {
+          // times 2^(scale - ev + 12): p * scale <= 2^12 keeps fp16's 11 bits for weights down to 2^-26
+          const float w0 = scale_value(max(__float_as_int(vs[i + u][0]) - ev + 139, 0));
+          const float w1 = scale_value(max(__float_as_int(vs[i + u][1]) - ev + 139, 0));
+          a[2 * u] = pack_f16x2(p0 * w0, p1 * w1);
+          a[2 * u + 1] = pack_f16x2(p2 * w0, p3 * w1);
+        } else {
+          a[2 * u] = pack_bf16x2(p0, p1);
+          a[2 * u + 1] = pack_bf16x2(p2, p3);
+        }
+      }
+      const int vrow = krow + i * 8 + (lane & 15);
+      if (!QUANT) {
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd) {  // 16 keys x 16 columns a load
+          uint32_t b[4];
+          ldsm4t(b, vt + tile_at<G::CH>(vrow, dd * 2 + (lane >> 4)));
+          mma<false>(o[2 * dd], a, b[0], b[1]);
+          mma<false>(o[2 * dd + 1], a, b[2], b[3]);
+        }
+      } else {
+        // b16 pairs are two neighbouring columns of a key: after the transpose each register holds keys
+        // (2t, 2t+1) x columns (2n, 2n+1); reordered bytes give the even columns' and the odd columns'
+        // fragments, so o[2 dd] holds columns 0, 2, .. and o[2 dd + 1] columns 1, 3, .. of 16
+#pragma unroll
+        for (int dd = 0; dd < D / 16; dd += 2) {  // 16 keys x 32 columns a load
+          uint32_t b[4];
+          ldsm4t(b, vt + tile_at<G::CH>(vrow, dd + (lane >> 4)));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t x = __byte_perm(b[2 * u], 0, 0x3120), y = __byte_perm(b[2 * u + 1], 0, 0x3120);
+            mma<true>(o[2 * (dd + u)], a, paged::e4m3x2_to_f16x2((uint16_t)x), paged::e4m3x2_to_f16x2((uint16_t)y));
+            mma<true>(o[2 * (dd + u) + 1], a, paged::e4m3x2_to_f16x2((uint16_t)(x >> 16)),
+                      paged::e4m3x2_to_f16x2((uint16_t)(y >> 16)));
+          }
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();  // the ring is free: it holds the join now
+
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  // join of the key groups: [wk][row][D] floats (columns in their own order) and [wk][row] (m, l)
+  float* so = reinterpret_cast<float*>(smem);
+  float2* sml = reinterpret_cast<float2*>(smem + WK * BM * D * 4);
+  const int lrow = wm * 16 + g;
+  if (t4 == 0) {
+    sml[wk * BM + lrow] = make_float2(m[0], l[0]);
+    sml[wk * BM + lrow + 8] = make_float2(m[1], l[1]);
+  }
+  __syncthreads();
+  float mj[2], f[2];
+  const float unit = QUANT ? scale_value(ev) * (1.f / 4096.f) : 1.f;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    mj[r] = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) mj[r] = fmaxf(mj[r], sml[w * BM + lrow + 8 * r].x);
+    f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mj[r]);
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float* dst = so + (wk * BM + lrow + 8 * r) * D + i * 16;
+      const float a0 = o[2 * i][2 * r] * f[r] * unit, a1 = o[2 * i][2 * r + 1] * f[r] * unit;
+      const float b0 = o[2 * i + 1][2 * r] * f[r] * unit, b1 = o[2 * i + 1][2 * r + 1] * f[r] * unit;
+      if (QUANT) {
+        *reinterpret_cast<float4*>(dst + 4 * t4) = make_float4(a0, b0, a1, b1);
+      } else {
+        *reinterpret_cast<float2*>(dst + 2 * t4) = make_float2(a0, a1);
+        *reinterpret_cast<float2*>(dst + 8 + 2 * t4) = make_float2(b0, b1);
+      }
+    }
+  __syncthreads();
+  // 8 columns a thread: sum of the key groups, then the result or this split's part
+  for (int e = tid; e < BM * (D / 8); e += THREADS) {
+    const int row = e / (D / 8), c = (e % (D / 8)) * 8;
+    const int gr = row0 + row;
+    if (gr >= rows) continue;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) mm = fmaxf(mm, sml[w * BM + row].x);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float2 x = sml[w * BM + row];
+      if (x.x != -INFINITY) ll += x.y * ex2(x.x - mm);
+    }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float4 a = *reinterpret_cast<const float4*>(so + (w * BM + row) * D + c);
+      const float4 b = *reinterpret_cast<const float4*>(so + (w * BM + row) * D + c + 4);
+      y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
+      y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
+    }
+    const int64_t tok = seg.begin + gr / p.group;
+    const int head = hk * p.group + gr % p.group;
+    const int64_t idx = tok * p.hq + head;
+    if (p.nsplit > 1) {
+      float* dst = p.part_o + ((int64_t)split * p.tokens * p.hq + idx) * D + c;
+      *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
+      if (c == 0) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(mm, ll);
+    } else {
+      const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= inv;
+      if (p.gate) {
+        float gv[8];
+        unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
+      }
+      *reinterpret_cast<uint4*>(p.out + idx * D + c) = pack8(y);
+    }
+  }
+}
+
+// Join of the splits: one warp a (token, head) row, 8 columns a lane (two rows a warp at D = 128).
+template <int D>
+__global__ void __launch_bounds__(128) join_kernel(const Params p) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int64_t per_tok = (p.hq + RPW - 1) / RPW;   // warps a token
+  const int64_t tok = w / per_tok;
+  if (tok >= p.tokens) return;
+  const int s = paged::find_segment_warp(p.cu, p.nseg, (int)tok, lane);
+  if (s < 0 || s >= p.nseg) return;                 // behind the last segment
+  const int end = p.cu[s + 1];
+  if (end <= tok || end > p.tokens || p.cu[s] < 0) return;
+  const int head = (int)(w % per_tok) * RPW + lane / LPR, c = (lane % LPR) * 8;
+  if (head >= p.hq) return;
+  const int64_t idx = tok * p.hq + head, plane = p.tokens * p.hq;
+  float mm = -INFINITY;
+  for (int i = 0; i < p.nsplit; ++i) mm = fmaxf(mm, p.part_ml[i * plane + idx].x);
+  float ll = 0.f, y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = 0.f;
+  if (mm != -INFINITY)
+    for (int i = 0; i < p.nsplit; ++i) {
+      const float2 ml = p.part_ml[i * plane + idx];
+      if (ml.x == -INFINITY) continue;
+      const float f = ex2(ml.x - mm);
+      const float* src = p.part_o + (i * plane + idx) * D + c;
+      const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+      ll = fmaf(f, ml.y, ll);
+      y[0] = fmaf(f, a.x, y[0]); y[1] = fmaf(f, a.y, y[1]); y[2] = fmaf(f, a.z, y[2]); y[3] = fmaf(f, a.w, y[3]);
+      y[4] = fmaf(f, b.x, y[4]); y[5] = fmaf(f, b.y, y[5]); y[6] = fmaf(f, b.z, y[6]); y[7] = fmaf(f, b.w, y[7]);
+    }
+  const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= inv;
+  if (p.gate) {
+    float gv[8];
+    unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
+  }
+  *reinterpret_cast<uint4*>(p.out + idx * D + c) = pack8(y);
+}
+
+template <int D, bool QUANT, int WM>
+static int launch_few(const Params& p, cudaStream_t s) {
+  using G = Geo<D, QUANT>;
+  constexpr int BM = 16 * WM, WK = 4 / WM;
+  constexpr int join = WK * BM * D * 4 + WK * BM * 8;
+  constexpr int bytes = G::RING > join ? G::RING : join;
+  const void* fn = (const void*)few_rows_kernel<D, QUANT, WM>;
+  if (int st = ensure_smem_attr(fn, bytes, "paged_gqa")) return st;
+  const dim3 grid((unsigned)((int64_t)p.nseg * p.row_blocks * p.hkv), (unsigned)p.nsplit);
+  few_rows_kernel<D, QUANT, WM><<<grid, THREADS, bytes, s>>>(p);
+  return check_launch("paged_gqa");
+}
+
+template <int D, bool QUANT>
+static int launch_rows(const Params& p, int wm, cudaStream_t s) {
+  return wm == 1 ? launch_few<D, QUANT, 1>(p, s) : wm == 2 ? launch_few<D, QUANT, 2>(p, s) : launch_few<D, QUANT, 4>(p, s);
+}
+
+// Tiling of a call: 16-row groups a CTA and the split of the keys.  Both follow from host-side sizes
+// only, so a captured call replays with any lengths.
+struct Plan {
+  int wm, row_blocks, nsplit;
+};
+constexpr int MAX_SPLIT = 64;
+constexpr int MIN_KEYS_A_SPLIT = 128;
+static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t hkv, int64_t group) {
+  Plan r;
+  const int64_t rows = max_seqlen * group;
+  r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  r.row_blocks = (int)((rows + 16 * r.wm - 1) / (16 * r.wm));
+  const int64_t ctas = num_segments * hkv * r.row_blocks;
+  int64_t split = (2 * sm_count() + ctas - 1) / (ctas > 0 ? ctas : 1);
+  const int64_t most = (max_kv + MIN_KEYS_A_SPLIT - 1) / MIN_KEYS_A_SPLIT;
+  if (split > most) split = most;
+  if (split > MAX_SPLIT) split = MAX_SPLIT;
+  r.nsplit = split < 1 ? 1 : (int)split;
+  return r;
+}
+
+}  // namespace pattn
+
+int paged_attn_take_device_error() {
+  int h = 0;
+  if (cudaMemcpyFromSymbol(&h, pattn::g_error, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (h) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(pattn::g_error, &zero, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace fdk
+
+using namespace fdk;
+
+static bool sizes_ok(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len, int64_t tokens, int64_t hq,
+                     int64_t hkv, int64_t head_dim) {
+  return num_segments >= 1 && num_segments <= 0x7ffffffe && max_seqlen >= 0 && max_seqlen <= 0x7fffffff &&
+         max_kv_len >= 0 && tokens >= 0 && tokens <= 0x7fffffff && hkv >= 1 && hq >= 1 && hq <= 4096 &&
+         hq % hkv == 0 && (head_dim == 128 || head_dim == 256);
+}
+
+extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
+                                               int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim) {
+  if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
+  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv);
+  return pl.nsplit > 1 ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
+}
+
+extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,
+                                 const void* v_cache, int64_t ld_vpage, int cache_is_e4m3, const void* k_scale,
+                                 int64_t ld_kscale_page, const void* v_scale, int64_t ld_vscale_page,
+                                 int64_t num_pages, int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                                 int64_t max_pages, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                 int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len, int64_t tokens,
+                                 int64_t hq, int64_t hkv, int64_t head_dim, float scale, const void* gate,
+                                 int64_t ld_gate, int gate_interleaved, void* out, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  using namespace fdk::pattn;
+  if (int st = check_device()) return st;
+  const char* what = "paged_gqa";
+  if (head_dim != 128 && head_dim != 256)
+    return set_error(FDK_ERR_UNSUPPORTED, "%s: head_dim=%lld (128 and 256 supported)", what, (long long)head_dim);
+  if (hkv < 1 || hq < 1 || hq % hkv) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: hq must be a multiple of hkv", what);
+  if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad segment count or sizes", what);
+  int shift = 0;
+  for (int i = 4; i <= 8; ++i)
+    if (page_size == (int64_t)1 << i) shift = i;
+  if (!shift) return set_error(FDK_ERR_UNSUPPORTED, "%s: page_size=%lld (16, 32, 64, 128 or 256)", what, (long long)page_size);
+  if (tokens == 0 || max_seqlen == 0) return FDK_OK;
+  if (!q || !k_cache || !v_cache || !page_table || !cu_seqlens || !kv_lens || !out)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const bool quant = cache_is_e4m3 != 0;
+  if (quant && (!k_scale || !v_scale))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: an e4m3 cache needs k_scale and v_scale", what);
+  if (num_pages < 1 || num_pages > 0x7fffffff || max_pages < 1 || ld_table < max_pages ||
+      max_pages * page_size > 0x7fffff00)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad page counts (at most 2^31 positions a sequence)", what);
+  const int64_t page_elems = page_size * hkv * head_dim;
+  if (ld_kpage < page_elems || ld_vpage < page_elems ||
+      (quant && (ld_kscale_page < page_size * hkv || ld_vscale_page < page_size * hkv)))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: page stride too small", what);
+  if (ld_q < hq * head_dim || (gate && ld_gate < hq * head_dim))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: row stride too small", what);
+  const int esz = quant ? 1 : 2;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || ld_q % 8 ||
+      ld_kpage * esz % 16 || ld_vpage * esz % 16 || (gate && (!aligned16(gate) || ld_gate % 8)) ||
+      (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
+    return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
+  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv);
+  if (max_seqlen * (hq / hkv) > 0x7fffffff || num_segments * hkv * pl.row_blocks > 0x7fffffff)
+    return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
+  Params p = {};
+  p.q = static_cast<const bf16*>(q); p.ld_q = ld_q;
+  p.k_cache = static_cast<const uint8_t*>(k_cache); p.v_cache = static_cast<const uint8_t*>(v_cache);
+  p.k_scale = static_cast<const uint8_t*>(k_scale); p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.kpage = ld_kpage * esz; p.vpage = ld_vpage * esz;
+  p.kscale_page = ld_kscale_page; p.vscale_page = ld_vscale_page;
+  p.table = page_table; p.ld_table = ld_table; p.cu = cu_seqlens; p.kv_lens = kv_lens;
+  p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
+  p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
+  p.nsplit = pl.nsplit; p.row_blocks = pl.row_blocks;
+  p.sl2 = scale * 1.4426950408889634f;
+  p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
+  p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);
+  p.out = static_cast<bf16*>(out);
+  if (pl.nsplit > 1) {
+    const size_t need = fdk_paged_gqa_workspace_size(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim);
+    if (!workspace || workspace_bytes < need)
+      return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes needed", what, need);
+    if (!aligned16(workspace)) return set_error(FDK_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", what);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)pl.nsplit * tokens * hq * head_dim);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int st;
+  if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.wm, s) : launch_rows<128, false>(p, pl.wm, s);
+  else st = quant ? launch_rows<256, true>(p, pl.wm, s) : launch_rows<256, false>(p, pl.wm, s);
+  if (st || pl.nsplit == 1) return st;
+  const int64_t rpw = head_dim == 128 ? 2 : 1;
+  const int64_t warps = tokens * ((hq + rpw - 1) / rpw);
+  const unsigned grid = (unsigned)((warps + 3) / 4);
+  if (head_dim == 128) join_kernel<128><<<grid, 128, 0, s>>>(p);
+  else join_kernel<256><<<grid, 128, 0, s>>>(p);
+  return check_launch("paged_gqa (join of splits)");
+}

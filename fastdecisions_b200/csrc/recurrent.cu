@@ -1,0 +1,430 @@
+// The Gated-DeltaNet mixer continued from cached state, for few tokens a sequence: the recurrent gated
+// delta rule over a pool of states, and the packed causal conv + SiLU over a pool of input histories.
+//
+// Pools: segment s starts from slot state_indices[s] (negative: from zero) and leaves its new state in
+// slot final_indices[s] (negative: nowhere).  The two may be the same slot (a sequence that advances) or
+// differ (a fork: many segments may start from one slot).  A slot that one segment writes must not be
+// read or written by another segment of the same call.
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace fdk {
+namespace recur {
+
+__device__ int g_state_error = 0;
+
+__device__ __forceinline__ void flag_error() { atomicOr(&g_state_error, 1); }
+
+// A segment's slot in a pool of `slots`: -1 for none; an id outside the pool is treated as none and
+// reported.
+__device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t slots, bool report) {
+  const int64_t i = idx ? idx[s] : s;
+  if (i >= slots) {
+    if (report) flag_error();
+    return -1;
+  }
+  return i < 0 ? -1 : i;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Recurrent gated delta rule.  Per token, with the state S [dk][dv] (float32) of one head:
+//     S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
+// Columns of S evolve on their own, so a warp owns 16 of the 128 columns and never talks to another:
+// lane (r, c) = (lane / 4, lane % 4) holds rows 16 r .. 16 r + 15 of columns 4 c .. 4 c + 3 in 64
+// registers.  S^T k and S^T q of the old state are reduced together (one pass over the registers, one
+// round of shuffles), as o = scale (e^g S^T q + (k . q) u).
+constexpr int DK = 128, DV = 128, CPW = 16;   // columns a warp
+constexpr int WARPS = 4;
+
+struct DeltaParams {
+  const bf16* q;
+  const bf16* k;
+  const bf16* v;
+  const float* g;
+  const bf16* beta;
+  int64_t ld_q, ld_k, ld_v;
+  const int32_t* cu;
+  int64_t period;       // tokens a segment when cu is null
+  int64_t tokens;
+  int nseg, heads, group;  // group: value heads a key head
+  float scale;
+  int l2norm;
+  const float* state_in;
+  const int32_t* in_idx;
+  int64_t in_slots;
+  float* state_out;
+  const int32_t* out_idx;
+  int64_t out_slots;
+  bf16* out;
+};
+
+__device__ __forceinline__ void load16(const bf16* p, float (&f)[16]) {
+  float a[8], b[8];
+  unpack8(__ldg(reinterpret_cast<const uint4*>(p)), a);
+  unpack8(__ldg(reinterpret_cast<const uint4*>(p) + 1), b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f[i] = a[i];
+    f[8 + i] = b[i];
+  }
+}
+
+__global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const DeltaParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int slice = (int)(w & (DV / CPW - 1));
+  const int64_t sh = w / (DV / CPW);
+  const int s = (int)(sh / p.heads), h = (int)(sh - (int64_t)s * p.heads);
+  if (s >= p.nseg) return;
+  int64_t t0, t1;
+  if (p.cu) {
+    int b, e;
+    if (!paged::segment_range(p.cu, s, p.tokens, b, e)) {
+      if (lane == 0) flag_error();
+      b = e = 0;
+    }
+    t0 = b;
+    t1 = e;
+  } else {
+    t0 = s * p.period;
+    t1 = t0 + p.period;
+  }
+  const int r = lane >> 2, c = lane & 3;
+  const int col = slice * CPW + c * 4;
+  const int hk = h / p.group;
+  const int64_t from = p.state_in ? slot_of(p.in_idx, s, p.in_slots, lane == 0) : -1;
+  const int64_t to = p.state_out ? slot_of(p.out_idx, s, p.out_slots, lane == 0) : -1;
+  const int64_t in_slot = (int64_t)r * 16 * DV + col;
+  float4 S[16];
+  if (from >= 0) {
+    const float* src = p.state_in + (from * p.heads + h) * (DK * DV) + in_slot;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) S[i] = *reinterpret_cast<const float4*>(src + i * DV);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    float k[16], q[16];
+    load16(p.k + t * p.ld_k + hk * DK + r * 16, k);
+    load16(p.q + t * p.ld_q + hk * DK + r * 16, q);
+    const uint2 vr = __ldg(reinterpret_cast<const uint2*>(p.v + t * p.ld_v + h * DV + col));
+    const float eg = expf(p.g[t * p.heads + h]);
+    const float beta = __bfloat162float(p.beta[t * p.heads + h]);
+    float red[11];
+#pragma unroll
+    for (int i = 0; i < 11; ++i) red[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      red[0] = fmaf(S[i].x, k[i], red[0]);
+      red[1] = fmaf(S[i].y, k[i], red[1]);
+      red[2] = fmaf(S[i].z, k[i], red[2]);
+      red[3] = fmaf(S[i].w, k[i], red[3]);
+      red[4] = fmaf(S[i].x, q[i], red[4]);
+      red[5] = fmaf(S[i].y, q[i], red[5]);
+      red[6] = fmaf(S[i].z, q[i], red[6]);
+      red[7] = fmaf(S[i].w, q[i], red[7]);
+      red[8] = fmaf(k[i], q[i], red[8]);
+      red[9] = fmaf(k[i], k[i], red[9]);
+      red[10] = fmaf(q[i], q[i], red[10]);
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 11; ++i) red[i] += __shfl_xor_sync(0xffffffffu, red[i], o);
+    const float rk = p.l2norm ? rsqrtf(red[9] + 1e-6f) : 1.f;
+    const float rq = (p.l2norm ? rsqrtf(red[10] + 1e-6f) : 1.f) * p.scale;
+    const float2 v01 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&vr.x));
+    const float2 v23 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&vr.y));
+    const float er = eg * rk;
+    float4 u;  // rk * beta * (v - S^T k)
+    u.x = rk * beta * (v01.x - er * red[0]);
+    u.y = rk * beta * (v01.y - er * red[1]);
+    u.z = rk * beta * (v23.x - er * red[2]);
+    u.w = rk * beta * (v23.y - er * red[3]);
+    if (r == 0) {
+      uint2 o;
+      o.x = pack_bf16x2(rq * fmaf(red[8], u.x, eg * red[4]), rq * fmaf(red[8], u.y, eg * red[5]));
+      o.y = pack_bf16x2(rq * fmaf(red[8], u.z, eg * red[6]), rq * fmaf(red[8], u.w, eg * red[7]));
+      *reinterpret_cast<uint2*>(p.out + (t * p.heads + h) * DV + col) = o;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      S[i].x = fmaf(k[i], u.x, eg * S[i].x);
+      S[i].y = fmaf(k[i], u.y, eg * S[i].y);
+      S[i].z = fmaf(k[i], u.z, eg * S[i].z);
+      S[i].w = fmaf(k[i], u.w, eg * S[i].w);
+    }
+  }
+  if (to >= 0) {
+    float* dst = p.state_out + (to * p.heads + h) * (DK * DV) + in_slot;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(dst + i * DV) = S[i];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Packed causal conv (width KW <= 4) + SiLU with history.  The rows before a segment are its slot's
+// KW - 1 cached input rows; its last KW - 1 rows (of history and input together) are the new ones.
+// Two kinds of work in one grid: jobs below nseg are a segment's head -- its first KW - 1 outputs, the
+// only ones that read the history, and the new history, so an in-place update cannot race -- and the
+// rest take eight consecutive tokens each and compute those at least KW - 1 tokens into their segment.
+constexpr int RPT = 8;
+
+struct ConvParams {
+  const bf16* x;
+  int64_t ld_x;
+  const bf16* w;
+  const int32_t* cu;
+  int64_t period, tokens;
+  int nseg, channels, key_dim, cblocks;
+  const bf16* hist_in;
+  const int32_t* in_idx;
+  int64_t in_slots;
+  bf16* hist_out;
+  const int32_t* out_idx;
+  int64_t out_slots;
+  bf16* q;
+  bf16* k;
+  bf16* v;
+};
+
+template <int KW>
+__device__ __forceinline__ void conv_row(const uint4 (&rows)[KW], const float (&w)[KW][8], bf16* dst) {
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < KW; ++j) {
+    float f[8];
+    unpack8(rows[j], f);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[c] = j == 0 ? w[0][c] * f[c] : fmaf(w[j][c], f[c], acc[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < 8; ++c) acc[c] = silu_tanh(acc[c]);
+  *reinterpret_cast<uint4*>(dst) = pack8(acc);
+}
+
+template <int KW>
+__global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
+  constexpr int HR = KW - 1;  // history rows
+  const int lane = threadIdx.x & 31;
+  const int cblk = (int)(blockIdx.x % (unsigned)p.cblocks);
+  const int c0 = (cblk * 32 + lane) * 8;
+  const bool active = c0 < p.channels;
+  const int64_t job = (int64_t)(blockIdx.x / (unsigned)p.cblocks) * 4 + (threadIdx.x >> 5);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  bf16* dst;
+  int64_t ldd;
+  if (c0 < p.key_dim) { dst = p.q + c0; ldd = p.key_dim; }
+  else if (c0 < 2 * p.key_dim) { dst = p.k + (c0 - p.key_dim); ldd = p.key_dim; }
+  else { dst = p.v + (c0 - 2 * p.key_dim); ldd = p.channels - 2 * p.key_dim; }
+  auto load_w = [&](float (&w)[KW][8]) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+      for (int j = 0; j < KW; ++j) w[j][c] = __bfloat162float(p.w[(int64_t)(c0 + c) * KW + j]);
+  };
+  if (job < p.nseg) {
+    const int s = (int)job;
+    int64_t t0, t1;
+    if (p.cu) {
+      int b, e;
+      if (!paged::segment_range(p.cu, s, p.tokens, b, e)) {
+        if (lane == 0 && cblk == 0) flag_error();
+        b = e = 0;
+      }
+      t0 = b;
+      t1 = e;
+    } else {
+      t0 = s * p.period;
+      t1 = t0 + p.period;
+    }
+    if (!active) return;
+    const bool report = lane == 0 && cblk == 0;
+    const int64_t from = p.hist_in ? slot_of(p.in_idx, s, p.in_slots, report) : -1;
+    const int64_t to = p.hist_out ? slot_of(p.out_idx, s, p.out_slots, report) : -1;
+    const int64_t n = t1 - t0;
+    // rows: history, then the first HR inputs
+    uint4 rows[2 * HR];
+#pragma unroll
+    for (int j = 0; j < HR; ++j) {
+      rows[j] = from >= 0 ? *reinterpret_cast<const uint4*>(p.hist_in + (from * HR + j) * p.channels + c0) : zero;
+      rows[HR + j] = j < n ? ldg_stream(p.x + (t0 + j) * p.ld_x + c0) : zero;
+    }
+    uint4 last[HR] = {};  // the new history: rows n .. n + HR - 1 of (history, inputs)
+#pragma unroll
+    for (int j = 0; j < HR; ++j) {
+      const int64_t i = n + j;
+      if (i >= 2 * HR) {
+        last[j] = ldg_stream(p.x + (t0 + i - HR) * p.ld_x + c0);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2 * HR; ++m)
+          if (m == i) last[j] = rows[m];
+      }
+    }
+    if (to >= 0) {
+#pragma unroll
+      for (int j = 0; j < HR; ++j)
+        *reinterpret_cast<uint4*>(p.hist_out + (to * HR + j) * p.channels + c0) = last[j];
+    }
+    if (n == 0) return;
+    float w[KW][8];
+    load_w(w);
+#pragma unroll
+    for (int j = 0; j < HR; ++j) {
+      if (j >= n) break;
+      uint4 win[KW];
+#pragma unroll
+      for (int m = 0; m < KW; ++m) win[m] = rows[j + m];
+      conv_row<KW>(win, w, dst + (t0 + j) * ldd);
+    }
+    return;
+  }
+  const int64_t r0 = (job - p.nseg) * RPT;
+  if (r0 >= p.tokens) return;
+  const int64_t r1 = r0 + RPT < p.tokens ? r0 + RPT : p.tokens;
+  int s;
+  if (p.cu) {
+    s = paged::find_segment_warp(p.cu, p.nseg, (int)r0, lane);
+    if (s < 0) s = 0;
+  } else {
+    s = (int)(r0 / p.period);
+  }
+  if (!active) return;
+  uint4 raw[RPT + HR];
+#pragma unroll
+  for (int j = 0; j < RPT + HR; ++j) {
+    const int64_t t = r0 - HR + j;
+    raw[j] = t >= 0 && t < r1 ? ldg_stream(p.x + t * p.ld_x + c0) : zero;
+  }
+  float w[KW][8];
+  load_w(w);
+  int64_t begin = -1, end = -1;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int64_t t = r0 + i;
+    if (t >= r1) break;
+    while (t >= end && s < p.nseg) {  // the segment that holds t (none: behind the last one)
+      begin = p.cu ? p.cu[s] : s * p.period;
+      end = p.cu ? p.cu[s + 1] : begin + p.period;
+      ++s;
+    }
+    if (t >= end || begin < 0 || end > p.tokens || t < begin + HR) continue;
+    uint4 win[KW];
+#pragma unroll
+    for (int m = 0; m < KW; ++m) win[m] = raw[i + m];
+    conv_row<KW>(win, w, dst + t * ldd);
+  }
+}
+
+}  // namespace recur
+
+int state_take_device_error() {
+  int h = 0;
+  if (cudaMemcpyFromSymbol(&h, recur::g_state_error, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (h) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(recur::g_state_error, &zero, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace fdk
+
+using namespace fdk;
+
+extern "C" int fdk_recurrent_gated_delta_rule_fwd(
+    const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v, const float* g,
+    const void* beta, const int32_t* cu_seqlens, int64_t num_segments, int64_t tokens, int64_t key_heads,
+    int64_t heads, int64_t dk, int64_t dv, float scale, int use_qk_l2norm, const float* initial_state,
+    const int32_t* state_indices, int64_t initial_slots, float* final_state, const int32_t* final_indices,
+    int64_t final_slots, void* out, void* stream) {
+  using namespace fdk::recur;
+  if (int st = check_device()) return st;
+  const char* what = "recurrent_gated_delta_rule";
+  if (dk != DK || dv != DV) return set_error(FDK_ERR_UNSUPPORTED, "%s: head dims must be 128", what);
+  if (heads < 1 || key_heads < 1 || heads % key_heads || heads > 65535)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: heads must be a multiple of the key heads", what);
+  if (num_segments < 1 || num_segments > 0x7ffffffe || tokens < 0 || tokens > 0x7fffffff)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad segment count or tokens", what);
+  if (!cu_seqlens && tokens % num_segments)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: without cu_seqlens every segment has tokens / num_segments tokens", what);
+  if (tokens && (!q || !k || !v || !g || !beta || !out)) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if ((initial_state && initial_slots < 1) || (final_state && final_slots < 1) ||
+      (initial_state && !state_indices && initial_slots < num_segments) ||
+      (final_state && !final_indices && final_slots < num_segments))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: fewer state slots than segments", what);
+  if (ld_q < key_heads * DK || ld_k < key_heads * DK || ld_v < heads * DV)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: row stride too small", what);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(initial_state) ||
+      !aligned16(final_state) || ld_q % 8 || ld_k % 8 || ld_v % 8)
+    return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
+  DeltaParams p = {};
+  p.q = static_cast<const bf16*>(q); p.k = static_cast<const bf16*>(k); p.v = static_cast<const bf16*>(v);
+  p.g = g; p.beta = static_cast<const bf16*>(beta);
+  p.ld_q = ld_q; p.ld_k = ld_k; p.ld_v = ld_v;
+  p.cu = cu_seqlens; p.period = tokens / num_segments; p.tokens = tokens;
+  p.nseg = (int)num_segments; p.heads = (int)heads; p.group = (int)(heads / key_heads);
+  p.scale = scale; p.l2norm = use_qk_l2norm;
+  p.state_in = initial_state; p.in_idx = state_indices; p.in_slots = initial_slots;
+  p.state_out = final_state; p.out_idx = final_indices; p.out_slots = final_slots;
+  p.out = static_cast<bf16*>(out);
+  const int64_t warps = num_segments * heads * (DV / CPW);
+  const int64_t blocks = (warps + WARPS - 1) / WARPS;
+  if (blocks > 0x7fffffff) return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments", what);
+  recurrent_delta_kernel<<<(unsigned)blocks, 32 * WARPS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return check_launch(what);
+}
+
+extern "C" int fdk_packed_conv_state(const void* x, int64_t ld_x, const void* weight, const int32_t* cu_seqlens,
+                                     int64_t num_segments, int64_t tokens, int64_t channels, int kernel_width,
+                                     int64_t key_dim, int64_t value_dim, const void* history,
+                                     const int32_t* state_indices, int64_t history_slots, void* new_history,
+                                     const int32_t* final_indices, int64_t new_history_slots, void* q, void* k,
+                                     void* v, void* stream) {
+  using namespace fdk::recur;
+  if (int st = check_device()) return st;
+  const char* what = "packed_conv_state";
+  if (channels <= 0 || key_dim <= 0 || value_dim <= 0 || channels != 2 * key_dim + value_dim || channels > 0x7fffff00)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: channels=%lld must equal 2*key_dim + value_dim", what, (long long)channels);
+  if (kernel_width < 2 || kernel_width > 4)
+    return set_error(FDK_ERR_UNSUPPORTED, "%s: kernel_width=%d (2..4 supported)", what, kernel_width);
+  if (key_dim % 8 || value_dim % 8) return set_error(FDK_ERR_UNSUPPORTED, "%s: key/value dims must be multiples of 8", what);
+  if (num_segments < 1 || num_segments > 0x7ffffffe || tokens < 0 || tokens > 0x7fffffff)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad segment count or tokens", what);
+  if (!cu_seqlens && tokens % num_segments)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: without cu_seqlens every segment has tokens / num_segments tokens", what);
+  if (!weight || (tokens && (!x || !q || !k || !v))) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if ((history && history_slots < 1) || (new_history && new_history_slots < 1) ||
+      (history && !state_indices && history_slots < num_segments) ||
+      (new_history && !final_indices && new_history_slots < num_segments))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: fewer history slots than segments", what);
+  if (ld_x < channels) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: ld_x < channels", what);
+  if (!aligned16(x) || ld_x % 8 || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(history) ||
+      !aligned16(new_history))
+    return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and row stride must be 16-byte aligned", what);
+  ConvParams p = {};
+  p.x = static_cast<const bf16*>(x); p.ld_x = ld_x; p.w = static_cast<const bf16*>(weight);
+  p.cu = cu_seqlens; p.period = tokens / num_segments; p.tokens = tokens;
+  p.nseg = (int)num_segments; p.channels = (int)channels; p.key_dim = (int)key_dim;
+  p.hist_in = static_cast<const bf16*>(history); p.in_idx = state_indices; p.in_slots = history_slots;
+  p.hist_out = static_cast<bf16*>(new_history); p.out_idx = final_indices; p.out_slots = new_history_slots;
+  p.q = static_cast<bf16*>(q); p.k = static_cast<bf16*>(k); p.v = static_cast<bf16*>(v);
+  const int64_t jobs = num_segments + (tokens + RPT - 1) / RPT;
+  const int64_t rows = (jobs + 3) / 4;
+  p.cblocks = (int)((channels / 8 + 31) / 32);
+  if (rows * p.cblocks > 0x7fffffff) return set_error(FDK_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  const unsigned grid = (unsigned)(rows * p.cblocks);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (kernel_width) {
+    case 4: conv_state_kernel<4><<<grid, 128, 0, s>>>(p); break;
+    case 3: conv_state_kernel<3><<<grid, 128, 0, s>>>(p); break;
+    default: conv_state_kernel<2><<<grid, 128, 0, s>>>(p); break;
+  }
+  return check_launch(what);
+}

@@ -222,12 +222,133 @@ int fdk_gqa_fwd(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const 
                 void* stream);
 
 /*
+ * ---- Continuing sequences from cached state ---------------------------------------------------
+ * A paged KV cache for the attention layers and pools of states for the Gated-DeltaNet layers, so
+ * a common prefix is computed once and any number of continuations run behind it (the reference
+ * forks transformers' dense caches instead, src/decider/shared_prefix.py:42-200).
+ *
+ * Paged cache, shared by the three fdk_paged_* entry points:
+ *     k_cache, v_cache: [num_pages][hkv][page_size][head_dim], page strides ld_kpage / ld_vpage
+ *         (elements, >= hkv * page_size * head_dim); bf16, or e4m3 when cache_is_e4m3 != 0;
+ *     k_scale, v_scale (e4m3 only): uint8 [num_pages][hkv][page_size], page strides ld_*scale_page:
+ *         byte b makes the row stand for e4m3 value * 2^(b - 127) (exact in bf16);
+ *     page_table: int32 [num_segments][>= max_pages], row stride ld_table: segment s's position p is
+ *         row p % page_size of page page_table[s][p / page_size]; entries past kv_lens[s] are not
+ *         read; several segments may share pages;
+ *     cu_seqlens: int32 [num_segments + 1] as elsewhere; kv_lens: int32 [num_segments], positions of
+ *         segment s INCLUDING its tokens of this call: its tokens cu[s] .. cu[s + 1] - 1 are its last
+ *         ones, token t at position kv_lens[s] - (cu[s + 1] - t).
+ * page_size 16, 32, 64, 128 or 256; head_dim 128 or 256.  All of these live on the device and are
+ * checked there, never read out of range: an invalid segment range counts as empty, an invalid length
+ * (negative, or more than max_pages * page_size) as no cached rows, an invalid page id as rows of
+ * zeros (a write skips it); each sets bit 32 of the device error word.  Rows behind the last segment
+ * are left as they were.  A page that one segment writes must not be written by another of the call.
+ */
+
+/*
+ * Writes the rows k, v [tokens][hkv][head_dim] (bf16, token strides ld_k, ld_v, head stride
+ * head_dim) into the cache.  e4m3: per row, scale 2^e with the smallest e in [-127, 127] such that
+ * the row's largest magnitude is <= 448 * 2^e, then round to nearest even (NaN stays NaN).  Tokens
+ * at negative positions (kv_lens[s] less than the segment's tokens) are not written.
+ */
+int fdk_paged_kv_write(const void* k, int64_t ld_k, const void* v, int64_t ld_v, void* k_cache,
+                       int64_t ld_kpage, void* v_cache, int64_t ld_vpage, int cache_is_e4m3,
+                       void* k_scale, int64_t ld_kscale_page, void* v_scale,
+                       int64_t ld_vscale_page, int64_t num_pages, int64_t page_size,
+                       const int32_t* page_table, int64_t ld_table, int64_t max_pages,
+                       const int32_t* cu_seqlens, const int32_t* kv_lens, int64_t num_segments,
+                       int64_t tokens, int64_t hkv, int64_t head_dim, void* stream);
+
+/*
+ * The other way round: rows k_out, v_out [tokens][hkv][head_dim] (bf16, contiguous) from the cache
+ * (cu_seqlens = running sums of kv_lens reads whole contexts).  Tokens without a cached row read as
+ * zeros.
+ */
+int fdk_paged_kv_read(const void* k_cache, int64_t ld_kpage, const void* v_cache, int64_t ld_vpage,
+                      int cache_is_e4m3, const void* k_scale, int64_t ld_kscale_page,
+                      const void* v_scale, int64_t ld_vscale_page, int64_t num_pages,
+                      int64_t page_size, const int32_t* page_table, int64_t ld_table,
+                      int64_t max_pages, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                      int64_t num_segments, int64_t tokens, int64_t hkv, int64_t head_dim,
+                      void* k_out, void* v_out, void* stream);
+
+/* Scratch bytes fdk_paged_gqa_fwd needs (0 when the call does not split the keys). */
+size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
+                                    int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim);
+
+/*
+ * Causal GQA attention of the newest tokens over the paged cache: token i of segment s's n attends
+ * to positions 0 .. kv_lens[s] - n + i (its own keys are in the cache already); a token that sees
+ * nothing gets zeros.  q, gate, out, scale and the head mapping as fdk_gqa_fwd (any hq / hkv).
+ * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows past the bound are
+ * not computed).  max_kv_len is a hint for how far the keys are split: any lengths up to
+ * max_pages * page_size are right with any hint.  Softmax statistics and accumulation are float32; P
+ * is rounded to bf16 (bf16 cache) or fp16 (e4m3 cache) before P.V.  A non-finite V row may reach every
+ * row of its call that shares a tile with it, masked ones included; K rows and rows past kv_lens[s]
+ * never do.  The caller's workspace holds float32 partial results; calls that overlap on the GPU
+ * need separate ones.
+ */
+int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,
+                      const void* v_cache, int64_t ld_vpage, int cache_is_e4m3,
+                      const void* k_scale, int64_t ld_kscale_page, const void* v_scale,
+                      int64_t ld_vscale_page, int64_t num_pages, int64_t page_size,
+                      const int32_t* page_table, int64_t ld_table, int64_t max_pages,
+                      const int32_t* cu_seqlens, const int32_t* kv_lens, int64_t num_segments,
+                      int64_t max_seqlen, int64_t max_kv_len, int64_t tokens, int64_t hq,
+                      int64_t hkv, int64_t head_dim, float scale, const void* gate,
+                      int64_t ld_gate, int gate_interleaved, void* out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Recurrent gated delta rule ([tf]:314-353): the token-by-token form of
+ * fdk_chunk_gated_delta_rule_fwd for few tokens a segment, over a pool of states.
+ *     q, k [tokens][key_heads][dk], v [tokens][heads][dv] bf16 (token strides ld_q, ld_k, ld_v),
+ *     value head h reads key head h / (heads / key_heads); g float32, beta bf16 [tokens][heads];
+ *     cu_seqlens NULL: num_segments segments of tokens / num_segments tokens each;
+ *     initial_state float32 [initial_slots][heads][dk][dv] (NULL: all from zero): segment s starts
+ *         from slot state_indices[s] (NULL: slot s; a negative index: from zero);
+ *     final_state float32 [final_slots][heads][dk][dv] (NULL: not kept): segment s leaves its state in
+ *         slot final_indices[s] (NULL: slot s; negative: nowhere).  An empty segment's state is its
+ *         initial one;
+ *     out [tokens][heads][dv] bf16 contiguous.
+ * The pools may be the same array and a segment's two slots the same slot; a slot that one segment
+ * writes must not be read or written by another segment of the call.  Indices past the pool count as
+ * negative and set bit 64 of the device error word, as an invalid segment range does (it counts as
+ * empty).  dk == dv == 128; float32 states and arithmetic.
+ */
+int fdk_recurrent_gated_delta_rule_fwd(
+    const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
+    const float* g, const void* beta, const int32_t* cu_seqlens, int64_t num_segments,
+    int64_t tokens, int64_t key_heads, int64_t heads, int64_t dk, int64_t dv, float scale,
+    int use_qk_l2norm, const float* initial_state, const int32_t* state_indices,
+    int64_t initial_slots, float* final_state, const int32_t* final_indices, int64_t final_slots,
+    void* out, void* stream);
+
+/*
+ * fdk_packed_conv_silu continued from cached inputs ([tf]:451-464, the conv state of a decoding
+ * step, for any number of tokens): x [tokens][channels] (row stride ld_x); the kernel_width - 1 rows
+ * before segment s are history [history_slots][kernel_width - 1][channels] (bf16, oldest first)
+ * at slot state_indices[s], and its last kernel_width - 1 rows -- of history and inputs together --
+ * go to new_history's slot final_indices[s].  Pools, indices, cu_seqlens and errors as
+ * fdk_recurrent_gated_delta_rule_fwd; q, k, v and the dims as fdk_packed_conv_silu, kernel_width
+ * 2 to 4.  Updating a slot in place is safe.
+ */
+int fdk_packed_conv_state(const void* x, int64_t ld_x, const void* weight,
+                          const int32_t* cu_seqlens, int64_t num_segments, int64_t tokens,
+                          int64_t channels, int kernel_width, int64_t key_dim, int64_t value_dim,
+                          const void* history, const int32_t* state_indices,
+                          int64_t history_slots, void* new_history, const int32_t* final_indices,
+                          int64_t new_history_slots, void* q, void* k, void* v, void* stream);
+
+/*
  * Reads and clears the device-side error word of the current device.  Kernels that wait on
  * mbarriers (fdk_gqa_fwd, the delta rule) bound every wait; a wait that runs out sets a bit of
  * this word, frees its resources and returns without finishing its tile.  Bits: 1 an attention
  * wait ran out, 2 a delta-rule wait ran out, 4 the bounded-wait self-test, 8 the delta rule found
  * cu_seqlens invalid on the device (cu[0] != 0, decreasing, or cu[num_segments] != tokens) and
- * treated every segment as empty, 16 a GEMM wait ran out.  Synchronises with the device.
+ * treated every segment as empty, 16 a GEMM wait ran out, 32 a paged-cache call found an invalid
+ * segment range, length or page id, 64 a state-pool call found an invalid segment range or slot.
+ * Synchronises with the device.
  * No reference counterpart (the reference's Triton kernels have no device waits).
  */
 int fdk_poll_device_error(int* code);
