@@ -757,6 +757,7 @@ extern "C" int fdk_poll_device_error(int* code) {
   const int sp = fdk::state_take_device_error();
   if (kv < 0 || pa < 0 || sp < 0)
     return set_error(FDK_ERR_DEVICE, "poll_device_error: cannot read the device error word");
+  if (pa & 2) h |= 1;            // a wait of the paged attention ran out
   if (kv || (pa & 1)) h |= 32;  // a paged-cache call found an invalid segment range, length or page id
   if (sp) h |= 64;              // a state-pool call found an invalid segment range or slot
   if (code) *code = h;

@@ -5,8 +5,9 @@
 // nothing gets zeros.  The query heads of a KV head are packed with the tokens into rows (row = token *
 // group + head), so every cached row brought into shared memory feeds them all.
 //
-// This file: the few-row kernel (mma.sync tiles of 16 rows, split over the keys) and the join of splits.
-// Its work is bound by reading the cache: at one token a sequence each cached byte is used by `group`
+// Calls with more than 64 rows a KV head run the tcgen05 kernel of paged_attention_chunk.cuh.  This file:
+// the few-row kernel (mma.sync tiles of 16 rows, split over the keys) and the join of splits.  Its work
+// is bound by reading the cache: at one token a sequence each cached byte is used by `group`
 // rows only, far below the tensor cores' rate, so the 16-row warp-level MMA -- which needs no padding to
 // 128 rows and keeps S and P in registers -- loses nothing to the memory time it hides behind.
 //
@@ -562,21 +563,36 @@ static int launch_rows(const Params& p, int wm, cudaStream_t s) {
   return wm == 1 ? launch_few<D, QUANT, 1>(p, s) : wm == 2 ? launch_few<D, QUANT, 2>(p, s) : launch_few<D, QUANT, 4>(p, s);
 }
 
-// Tiling of a call: 16-row groups a CTA and the split of the keys.  Both follow from host-side sizes
-// only, so a captured call replays with any lengths.
+// Tiling of a call: the kernel, its rows a CTA and the split of the keys.  All follow from host-side
+// sizes only, so a captured call replays with any lengths.
 struct Plan {
-  int wm, row_blocks, nsplit;
+  bool many;           // the tcgen05 kernel
+  int wm;              // few-row kernel: 16-row groups a CTA
+  int64_t row_blocks;  // row blocks (tiles) of a segment and KV head
+  int nsplit;
 };
+constexpr int SMS = 148;
 constexpr int MAX_SPLIT = 64;
-constexpr int MIN_KEYS_A_SPLIT = 128;
-static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t hkv, int64_t group) {
-  Plan r;
+constexpr int FEW_ROWS = 64;
+constexpr int MIN_KEYS_A_SPLIT = 128;       // few rows: two tiles
+constexpr int MIN_KEYS_A_SPLIT_MANY = 512;  // many rows: four or eight blocks
+static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t hkv, int64_t group, int64_t d) {
+  Plan r = {};
   const int64_t rows = max_seqlen * group;
-  r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  r.row_blocks = (int)((rows + 16 * r.wm - 1) / (16 * r.wm));
-  const int64_t ctas = num_segments * hkv * r.row_blocks;
-  int64_t split = (2 * sm_count() + ctas - 1) / (ctas > 0 ? ctas : 1);
-  const int64_t most = (max_kv + MIN_KEYS_A_SPLIT - 1) / MIN_KEYS_A_SPLIT;
+  int64_t split, most;
+  r.many = rows > FEW_ROWS && group <= 128;
+  if (r.many) {
+    const int64_t tokens = (d == 128 ? 2 : 1) * (128 / group);  // of a CTA
+    r.row_blocks = (max_seqlen + tokens - 1) / tokens;
+    split = SMS / (num_segments * hkv * r.row_blocks);
+    most = max_kv / MIN_KEYS_A_SPLIT_MANY;
+  } else {
+    r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    r.row_blocks = (rows + 16 * r.wm - 1) / (16 * r.wm);
+    const int64_t ctas = num_segments * hkv * (r.row_blocks > 0 ? r.row_blocks : 1);
+    split = (2 * SMS + ctas - 1) / ctas;
+    most = (max_kv + MIN_KEYS_A_SPLIT - 1) / MIN_KEYS_A_SPLIT;
+  }
   if (split > most) split = most;
   if (split > MAX_SPLIT) split = MAX_SPLIT;
   r.nsplit = split < 1 ? 1 : (int)split;
@@ -584,6 +600,11 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
 }
 
 }  // namespace pattn
+}  // namespace fdk
+
+#include "paged_attention_chunk.cuh"
+
+namespace fdk {
 
 int paged_attn_take_device_error() {
   int h = 0;
@@ -612,7 +633,7 @@ static bool sizes_ok(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_le
 extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
                                                int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
-  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv);
+  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv, head_dim);
   return pl.nsplit > 1 ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
 }
 
@@ -633,6 +654,8 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   if (hkv < 1 || hq < 1 || hq % hkv) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: hq must be a multiple of hkv", what);
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim))
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad segment count or sizes", what);
+  if (!(scale > 0.f) || !(scale < 1e30f))
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", what);
   int shift = 0;
   for (int i = 4; i <= 8; ++i)
     if (page_size == (int64_t)1 << i) shift = i;
@@ -650,15 +673,16 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   if (ld_kpage < page_elems || ld_vpage < page_elems ||
       (quant && (ld_kscale_page < page_size * hkv || ld_vscale_page < page_size * hkv)))
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: page stride too small", what);
-  if (ld_q < hq * head_dim || (gate && ld_gate < hq * head_dim))
+  if (ld_q < hq * head_dim || (gate && ld_gate < (gate_interleaved ? 2 * hq - 1 : hq) * head_dim))
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: row stride too small", what);
   const int esz = quant ? 1 : 2;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || ld_q % 8 ||
       ld_kpage * esz % 16 || ld_vpage * esz % 16 || (gate && (!aligned16(gate) || ld_gate % 8)) ||
       (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
-  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv);
-  if (max_seqlen * (hq / hkv) > 0x7fffffff || num_segments * hkv * pl.row_blocks > 0x7fffffff)
+  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv, head_dim);
+  if (max_seqlen * (hq / hkv) > 0x7fffffff || num_segments * hkv * (pl.many ? 1 : pl.row_blocks) > 0x7fffffff ||
+      (pl.many && pl.row_blocks > 65535))
     return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
   Params p = {};
   p.q = static_cast<const bf16*>(q); p.ld_q = ld_q;
@@ -669,7 +693,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.table = page_table; p.ld_table = ld_table; p.cu = cu_seqlens; p.kv_lens = kv_lens;
   p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
-  p.nsplit = pl.nsplit; p.row_blocks = pl.row_blocks;
+  p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks;
   p.sl2 = scale * 1.4426950408889634f;
   p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
   p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);
@@ -684,7 +708,12 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st;
-  if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.wm, s) : launch_rows<128, false>(p, pl.wm, s);
+  if (pl.many) {
+    if (head_dim == 128)
+      st = quant ? chunk::launch<128, true>(p, pl.row_blocks, s) : chunk::launch<128, false>(p, pl.row_blocks, s);
+    else
+      st = quant ? chunk::launch<256, true>(p, pl.row_blocks, s) : chunk::launch<256, false>(p, pl.row_blocks, s);
+  } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.wm, s) : launch_rows<128, false>(p, pl.wm, s);
   else st = quant ? launch_rows<256, true>(p, pl.wm, s) : launch_rows<256, false>(p, pl.wm, s);
   if (st || pl.nsplit == 1) return st;
   const int64_t rpw = head_dim == 128 ? 2 : 1;

@@ -696,50 +696,83 @@ E4M3 = torch.float8_e4m3fn
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
+def _device_of(*ts) -> int:
+    """Index of the one CUDA device of all given tensors (``_need_cuda`` for calls of a few microseconds)."""
+    dev = None
+    for t in ts:
+        if t is not None:
+            d = t.get_device()
+            if d != dev:
+                if d < 0:
+                    raise ValueError("fastdecisions_b200 ops run on CUDA tensors only (no CPU fallback)")
+                if dev is not None:
+                    raise ValueError("all tensors must share one CUDA device")
+                dev = d
+    return dev
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(dev: int, name: str, *args):
+    """``_lib.call_block`` on ``dev`` and its current stream."""
+    if torch.cuda.current_device() == dev:
+        _lib.call_block(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call_block(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
 def _int32_vector(name: str, what: str, t: torch.Tensor, n: int):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         raise ValueError(f"{name}: {what} must be a contiguous int32 vector of {n} elements")
 
 
 def _paged_args(name: str, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale):
-    """Checks the cache and its metadata; the argument list of the C entry points from the cache on."""
-    quant = k_cache.dtype == E4M3
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or not (
-            quant or k_cache.dtype == BF16):
+    """Checks the cache and its metadata; the arguments of the C entry points from the cache on, and the
+    cache's shape."""
+    dtype, shape = k_cache.dtype, k_cache.shape
+    quant = dtype == E4M3
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dtype or not (quant or dtype == BF16):
         raise ValueError(f"{name}: caches must be [pages, kv heads, page size, head_dim], both bf16 or both e4m3")
-    pages, hkv, page_size, D = k_cache.shape
+    pages, hkv, page_size, D = shape
     if page_size not in PAGE_SIZES or D not in (128, 256):
         raise ValueError(f"{name}: page sizes {PAGE_SIZES} and head_dim 128 or 256 supported")
-    for t in (k_cache, v_cache):
-        if t.stride()[1:] != (page_size * D, D, 1):
-            raise ValueError(f"{name}: a cache page must be contiguous (only the page stride is free)")
+    kst, vst = k_cache.stride(), v_cache.stride()
+    want = (page_size * D, D, 1)
+    if kst[1:] != want or vst[1:] != want:
+        raise ValueError(f"{name}: a cache page must be contiguous (only the page stride is free)")
     if quant:
-        for t in (k_scale, v_scale):
-            if t is None or t.dtype != torch.uint8 or t.shape != (pages, hkv, page_size) or t.stride()[1:] != (
-                    page_size, 1):
-                raise ValueError(f"{name}: an e4m3 cache needs uint8 k_scale and v_scale [pages, kv heads, page size]")
-        scales = (k_scale.data_ptr(), k_scale.stride(0), v_scale.data_ptr(), v_scale.stride(0))
+        if k_scale is None or v_scale is None or k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8 or (
+                k_scale.shape != (pages, hkv, page_size) or v_scale.shape != (pages, hkv, page_size)):
+            raise ValueError(f"{name}: an e4m3 cache needs uint8 k_scale and v_scale [pages, kv heads, page size]")
+        kss, vss = k_scale.stride(), v_scale.stride()
+        if kss[1:] != (page_size, 1) or vss[1:] != (page_size, 1):
+            raise ValueError(f"{name}: the scales of a page must be contiguous (only the page stride is free)")
+        scales = (k_scale.data_ptr(), kss[0], v_scale.data_ptr(), vss[0])
     elif k_scale is not None or v_scale is not None:
         raise ValueError(f"{name}: a bf16 cache has no scales")
     else:
-        scales = (None, 0, None, 0)
+        scales = (0, 0, 0, 0)
     S = kv_lens.numel()
     _int32_vector(name, "kv_lens", kv_lens, S)
     _int32_vector(name, "cu_seqlens", cu_seqlens, S + 1)
-    if S < 1 or page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != S or (
-            page_table.shape[1] < 1 or page_table.stride(1) != 1):
+    tshape, tst = page_table.shape, page_table.stride()
+    if S < 1 or page_table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != S or tshape[1] < 1 or (
+            tshape[1] > 1 and tst[1] != 1):
         raise ValueError(f"{name}: page_table must be int32 [segments, pages] with unit column stride")
-    max_pages = page_table.shape[1]
-    cache = (k_cache.data_ptr(), k_cache.stride(0), v_cache.data_ptr(), v_cache.stride(0), int(quant), *scales)
-    return cache, (pages, page_size, page_table.data_ptr(), page_table.stride(0) if S > 1 else max_pages, max_pages,
-                   cu_seqlens.data_ptr(), kv_lens.data_ptr(), S)
+    return ((k_cache.data_ptr(), kst[0], v_cache.data_ptr(), vst[0], int(quant)) + scales +
+            (pages, page_size, page_table.data_ptr(), tst[0] if S > 1 else tshape[1], tshape[1],
+             cu_seqlens.data_ptr(), kv_lens.data_ptr(), S)), shape
 
 
-def _token_rows(name: str, what: str, t: torch.Tensor, heads: int, D: int):
-    if t.dim() != 3 or t.shape[1:] != (heads, D) or t.dtype != BF16 or t.stride(2) != 1 or (
-            heads > 1 and t.stride(1) != D):
+def _token_rows(name: str, what: str, t: torch.Tensor, heads: int, D: int) -> int:
+    """Token stride of bf16 rows ``[tokens, heads, D]``."""
+    st = t.stride()
+    if t.shape[1:] != (heads, D) or t.dtype != BF16 or st[2] != 1 or (heads > 1 and st[1] != D):
         raise ValueError(f"{name}: {what} must be bf16 [tokens, {heads}, {D}] with head stride {D}")
-    return t.stride(0) if t.shape[0] > 1 else heads * D
+    return st[0] if t.shape[0] > 1 else heads * D
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -751,16 +784,15 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     cu_seqlens[s + 1] - 1`` are the last of its ``kv_lens[s]`` positions; position p is row ``p % page
     size`` of page ``page_table[s, p // page size]``.  Invalid device metadata is skipped and reported
     by the device error word."""
-    _need_cuda(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale)
-    cache, meta = _paged_args("paged_kv_write", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale)
-    _, hkv, _, D = k_cache.shape
+    dev = _device_of(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale)
+    args, (_, hkv, _, D) = _paged_args("paged_kv_write", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
+                                       v_scale)
     ldk = _token_rows("paged_kv_write", "k", k, hkv, D)
     ldv = _token_rows("paged_kv_write", "v", v, hkv, D)
-    if k.shape[0] != v.shape[0]:
+    T = k.shape[0]
+    if v.shape[0] != T:
         raise ValueError("paged_kv_write: k and v must have the same tokens")
-    with torch.cuda.device(k.device):
-        _lib.call("fdk_paged_kv_write", k.data_ptr(), ldk, v.data_ptr(), ldv, *cache, *meta, k.shape[0], hkv, D,
-                  _stream(k))
+    _launch(dev, "fdk_paged_kv_write", k.data_ptr(), ldk, v.data_ptr(), ldv, *args, T, hkv, D)
 
 
 def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -770,22 +802,20 @@ def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
     """The last ``cu_seqlens[s + 1] - cu_seqlens[s]`` cached rows of every segment as packed bf16 ``(k, v)
     [tokens, Hkv, D]`` (the inverse of ``paged_kv_write``; ``cu_seqlens`` = running sums of ``kv_lens``
     reads whole contexts).  Rows behind the last segment are left as they were."""
-    _need_cuda(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, k_out, v_out)
-    cache, meta = _paged_args("paged_kv_read", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale)
-    _, hkv, _, D = k_cache.shape
+    dev = _device_of(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, k_out, v_out)
+    args, (_, hkv, _, D) = _paged_args("paged_kv_read", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
+                                       v_scale)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError("paged_kv_read: tokens must not be negative")
+    for t in (k_out, v_out):
+        if t is not None and (t.shape != (tokens, hkv, D) or t.dtype != BF16 or not t.is_contiguous()):
+            raise ValueError("paged_kv_read: outputs must be contiguous bf16 [tokens, kv heads, head_dim]")
     if k_out is None:
         k_out = torch.empty((tokens, hkv, D), device=k_cache.device, dtype=BF16)
     if v_out is None:
         v_out = torch.empty((tokens, hkv, D), device=k_cache.device, dtype=BF16)
-    for t in (k_out, v_out):
-        if t.shape != (tokens, hkv, D) or t.dtype != BF16 or not t.is_contiguous():
-            raise ValueError("paged_kv_read: outputs must be contiguous bf16 [tokens, kv heads, head_dim]")
-    with torch.cuda.device(k_cache.device):
-        _lib.call("fdk_paged_kv_read", *cache, *meta, tokens, hkv, D, k_out.data_ptr(), v_out.data_ptr(),
-                  _stream(k_cache))
+    _launch(dev, "fdk_paged_kv_read", *args, tokens, hkv, D, k_out.data_ptr(), v_out.data_ptr())
     return k_out, v_out
 
 
@@ -805,39 +835,42 @@ def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     n attends to positions ``0 .. kv_lens[s] - n + i``; one that sees nothing gets zeros.  ``max_seqlen``
     bounds the tokens of a segment; ``max_kv_len`` (default: the page table's reach) only guides how the
     keys are split.  ``gate`` / ``gate_interleaved`` / ``scale`` as ``gqa_attention_varlen_``."""
-    _need_cuda(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, gate, out, workspace)
-    cache, meta = _paged_args("paged_gqa_attention", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
-                              v_scale)
-    _, hkv, page_size, D = k_cache.shape
-    if q.dim() != 3 or q.shape[1] % hkv:
+    dev = _device_of(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, gate, out, workspace)
+    args, (_, hkv, page_size, D) = _paged_args("paged_gqa_attention", k_cache, v_cache, page_table, cu_seqlens, kv_lens,
+                                               k_scale, v_scale)
+    qshape = q.shape
+    if len(qshape) != 3 or qshape[1] < 1 or qshape[1] % hkv:
         raise ValueError("paged_gqa_attention: q must be [tokens, query heads, head_dim], whole groups of query heads")
-    T, hq, _ = q.shape
+    T, hq, _ = qshape
     ldq = _token_rows("paged_gqa_attention", "q", q, hq, D)
     ldg = 0
     if gate is not None:
-        span = hq * D * (2 if gate_interleaved else 1) - (D if gate_interleaved else 0)
-        if gate.dim() != 2 or gate.dtype != BF16 or gate.shape[0] != T or gate.shape[1] < span or gate.stride(1) != 1:
+        span = (2 * hq - 1) * D if gate_interleaved else hq * D
+        gshape, gst = gate.shape, gate.stride()
+        if len(gshape) != 2 or gate.dtype != BF16 or gshape[0] != T or gshape[1] < span or gst[1] != 1:
             raise ValueError(f"paged_gqa_attention: gate must be bf16 [tokens, >= {span}] with unit column stride")
-        ldg = gate.stride(0) if T > 1 else gate.shape[1]
+        ldg = gst[0] if T > 1 else (gshape[1] + 7) // 8 * 8
     if out is None:
-        out = torch.empty((T, hq, D), device=q.device, dtype=BF16)
-    elif out.shape != (T, hq, D) or out.dtype != BF16 or not out.is_contiguous():
+        out = torch.empty(qshape, device=q.device, dtype=BF16)
+    elif out.shape != qshape or out.dtype != BF16 or not out.is_contiguous():
         raise ValueError("paged_gqa_attention: out must be contiguous bf16 shaped like q")
     max_seqlen = min(int(max_seqlen), T)
     if max_seqlen < 0:
         raise ValueError("paged_gqa_attention: max_seqlen must not be negative")
-    if max_kv_len is None:
-        max_kv_len = page_table.shape[1] * page_size
-    max_kv_len = int(max_kv_len)
-    S = kv_lens.numel()
-    with torch.cuda.device(q.device):
-        need = paged_gqa_workspace_bytes(S, max_seqlen, max_kv_len, T, hq, hkv, D)
-        if need and workspace is None:
-            workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
-        _lib.call("fdk_paged_gqa_fwd", q.data_ptr(), ldq, *cache, *meta, max_seqlen, max_kv_len, T, hq, hkv, D,
-                  float(D ** -0.5 if scale is None else scale), _ptr(gate), ldg, int(gate_interleaved),
-                  out.data_ptr(), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-                  _stream(q))
+    max_kv_len = page_table.shape[1] * page_size if max_kv_len is None else int(max_kv_len)
+    if max_kv_len < 0:
+        raise ValueError("paged_gqa_attention: max_kv_len must not be negative")
+    if workspace is None:
+        have = paged_gqa_workspace_bytes(kv_lens.numel(), max_seqlen, max_kv_len, T, hq, hkv, D)
+        if have:
+            workspace = torch.empty(have, device=q.device, dtype=torch.uint8)
+    else:
+        if not workspace.is_contiguous():
+            raise ValueError("paged_gqa_attention: workspace must be contiguous")
+        have = workspace.numel() * workspace.element_size()
+    _launch(dev, "fdk_paged_gqa_fwd", q.data_ptr(), ldq, *args, max_seqlen, max_kv_len, T, hq, hkv, D,
+            float(D ** -0.5 if scale is None else scale), _addr(gate), ldg, int(gate_interleaved), out.data_ptr(),
+            _addr(workspace), have)
     return out
 
 
@@ -846,22 +879,25 @@ def _segments_of(name: str, B: int, T: int, cu_seqlens: Optional[torch.Tensor]) 
         return B
     if B != 1:
         raise ValueError(f"{name}: cu_seqlens needs batch size 1")
-    _int32_vector(name, "cu_seqlens", cu_seqlens, cu_seqlens.numel())
-    if cu_seqlens.numel() < 2:
+    n = cu_seqlens.numel()
+    _int32_vector(name, "cu_seqlens", cu_seqlens, n)
+    if n < 2:
         raise ValueError(f"{name}: cu_seqlens must have at least two elements")
-    return cu_seqlens.numel() - 1
+    return n - 1
 
 
 def _heads_stride(name: str, what: str, t: torch.Tensor, B: int, T: int, H: int, D: int):
     """``[B, T, H, D]`` as rows of one token stride (a copy when the layout has none)."""
     if t.dtype != BF16:
         raise ValueError(f"{name}: {what} must be bf16")
-    if not (t.stride(3) == 1 and (H == 1 or t.stride(2) == D) and (B == 1 or t.stride(0) == T * t.stride(1))):
+    st = t.stride()
+    if not (st[3] == 1 and (H == 1 or st[2] == D) and (B == 1 or T == 1 or st[0] == T * st[1])):
         t = t.contiguous()
-    return t, (t.stride(1) if T > 1 else t.stride(0) if B > 1 else H * D)
+        st = t.stride()
+    return t, (st[1] if T > 1 else st[0] if B > 1 else H * D)
 
 
-def _recurrent(name, query, key, value, g, beta, l2norm, cu_seqlens, initial, initial_idx, final, final_idx, out):
+def _recurrent(name, dev, query, key, value, g, beta, l2norm, cu_seqlens, initial, initial_idx, final, final_idx, out):
     if query.dim() != 4 or key.shape != query.shape or value.dim() != 4:
         raise ValueError(f"{name}: expected [B, T, H, D] query/key/value")
     B, T, Hk, Dk = key.shape
@@ -891,12 +927,14 @@ def _recurrent(name, query, key, value, g, beta, l2norm, cu_seqlens, initial, in
     q, ldq = _heads_stride(name, "query", query, B, T, Hk, Dk)
     k, ldk = _heads_stride(name, "key", key, B, T, Hk, Dk)
     v, ldv = _heads_stride(name, "value", value, B, T, H, Dv)
-    gg, bb = g.float().contiguous(), beta.to(BF16).contiguous()
-    with torch.cuda.device(v.device):
-        _lib.call("fdk_recurrent_gated_delta_rule_fwd", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
-                  gg.data_ptr(), bb.data_ptr(), _ptr(cu_seqlens), S, B * T, Hk, H, Dk, Dv, float(Dk ** -0.5),
-                  int(l2norm), _ptr(initial), _ptr(initial_idx), 0 if initial is None else initial.shape[0],
-                  _ptr(final), _ptr(final_idx), 0 if final is None else final.shape[0], out.data_ptr(), _stream(v))
+    if g.dtype != torch.float32 or not g.is_contiguous():
+        g = g.float().contiguous()
+    if beta.dtype != BF16 or not beta.is_contiguous():
+        beta = beta.to(BF16).contiguous()
+    _launch(dev, "fdk_recurrent_gated_delta_rule_fwd", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+            g.data_ptr(), beta.data_ptr(), _addr(cu_seqlens), S, B * T, Hk, H, Dk, Dv, Dk ** -0.5, int(l2norm),
+            _addr(initial), _addr(initial_idx), 0 if initial is None else initial.shape[0], _addr(final),
+            _addr(final_idx), 0 if final is None else final.shape[0], out.data_ptr())
     return out
 
 
@@ -911,10 +949,10 @@ def recurrent_gated_delta_rule_(query: torch.Tensor, key: torch.Tensor, value: t
     negative: nowhere), so a slot can be advanced or forked.  A slot written by one segment must not be
     read or written by another of the call.  ``query, key [B, T, Hk, 128]``, ``value [B, T, H, 128]`` bf16
     (H a multiple of Hk), ``g`` (log decay) and ``beta [B, T, H]``; returns ``o [B, T, H, 128]`` bf16."""
-    _need_cuda(query, key, value, g, beta, state, state_indices, final_indices, cu_seqlens, out)
+    dev = _device_of(query, key, value, g, beta, state, state_indices, final_indices, cu_seqlens, out)
     if final_indices is None:
         final_indices = state_indices
-    return _recurrent("recurrent_gated_delta_rule_", query, key, value, g, beta, use_qk_l2norm_in_kernel, cu_seqlens,
+    return _recurrent("recurrent_gated_delta_rule_", dev, query, key, value, g, beta, use_qk_l2norm_in_kernel, cu_seqlens,
                       state, state_indices, state, final_indices, out)
 
 
@@ -924,7 +962,7 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
     ``chunk_gated_delta_rule``): returns ``(o [B, T, H, Dv] bf16, final_state [N, H, Dk, Dv] float32 or
     None)``.  For few tokens a sequence (decoding, short continuations); the chunked form is faster for
     long ones."""
-    _need_cuda(query, key, value, g, beta, initial_state, cu_seqlens)
+    dev = _device_of(query, key, value, g, beta, initial_state, cu_seqlens)
     if query.dim() != 4 or value.dim() != 4:
         raise ValueError("recurrent_gated_delta_rule: expected [B, T, H, D] query/key/value")
     cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
@@ -937,7 +975,7 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
         init = initial_state.float().contiguous()
     final = torch.empty(shape, device=value.device, dtype=torch.float32) if output_final_state else None
     q, k, v = (t if t.dtype == BF16 else t.to(BF16) for t in (query, key, value))
-    o = _recurrent("recurrent_gated_delta_rule", q, k, v, g, beta, use_qk_l2norm_in_kernel, cu, init, None, final,
+    o = _recurrent("recurrent_gated_delta_rule", dev, q, k, v, g, beta, use_qk_l2norm_in_kernel, cu, init, None, final,
                    None, None)
     return o, final
 
@@ -950,23 +988,24 @@ def packed_conv_state_(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     ``K - 1`` input rows of each sequence (oldest first) and is updated in place; ``state_indices`` /
     ``final_indices`` as ``recurrent_gated_delta_rule_`` (a negative index: zeros before the segment).
     ``x [B, T, C]`` (unit column stride, any row stride) -> ``q, k, v [B, T, heads, head_dim]``."""
-    _need_cuda(x, weight, state, state_indices, final_indices, cu_seqlens)
+    dev = _device_of(x, weight, state, state_indices, final_indices, cu_seqlens)
     name = "packed_conv_state_"
     if x.dim() != 3 or x.dtype != BF16 or weight.dtype != BF16:
         raise ValueError(f"{name}: expected bf16 x [B, T, C] and weight")
     B, T, C = x.shape
-    if weight.dim() == 3 and weight.shape[1] == 1:
-        weight = weight.reshape(weight.shape[0], weight.shape[2])
-    if weight.dim() != 2 or weight.shape[0] != C or not weight.is_contiguous() or not 2 <= weight.shape[1] <= 4:
+    wshape = weight.shape
+    if (len(wshape) != 2 and (len(wshape) != 3 or wshape[1] != 1)) or wshape[0] != C or not 2 <= wshape[-1] <= 4 or (
+            not weight.is_contiguous()):
         raise ValueError(f"{name}: weight must be a contiguous [C, K] or [C, 1, K] tensor with K from 2 to 4")
-    K = weight.shape[1]
+    K = wshape[-1]
     if key_dim is None:
         key_dim = C // 3
     if value_dim is None:
         value_dim = C - 2 * key_dim
     if 2 * key_dim + value_dim != C or key_dim % head_dim or value_dim % head_dim or min(key_dim, value_dim) < 1:
         raise ValueError(f"{name}: C must equal 2*key_dim + value_dim with whole heads")
-    if state.dim() != 3 or state.shape[1:] != (K - 1, C) or state.dtype != BF16 or not state.is_contiguous():
+    slots = state.shape[0]
+    if state.shape != (slots, K - 1, C) or state.dtype != BF16 or not state.is_contiguous():
         raise ValueError(f"{name}: state must be contiguous bf16 [slots, {K - 1}, {C}]")
     S = _segments_of(name, B, T, cu_seqlens)
     if final_indices is None:
@@ -974,19 +1013,19 @@ def packed_conv_state_(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     for idx in (state_indices, final_indices):
         if idx is not None:
             _int32_vector(name, "slot indices", idx, S)
-        elif state.shape[0] < S:
+        elif slots < S:
             raise ValueError(f"{name}: {S} segments need at least as many state slots")
-    if x.stride(2) != 1 or (B > 1 and x.stride(0) != T * x.stride(1)):
+    st = x.stride()
+    if st[2] != 1 or (B > 1 and T > 1 and st[0] != T * st[1]):
         x = x.contiguous()
-    ldx = x.stride(1) if T > 1 else x.stride(0) if B > 1 else C
-    _aligned(x, state)
-    q = torch.empty((B, T, key_dim // head_dim, head_dim), device=x.device, dtype=BF16)
-    k = torch.empty_like(q)
-    v = torch.empty((B, T, value_dim // head_dim, head_dim), device=x.device, dtype=BF16)
-    if S == 0:
-        return q, k, v
-    with torch.cuda.device(x.device):
-        _lib.call("fdk_packed_conv_state", x.data_ptr(), ldx, weight.data_ptr(), _ptr(cu_seqlens), S, B * T, C, K,
-                  key_dim, value_dim, state.data_ptr(), _ptr(state_indices), state.shape[0], state.data_ptr(),
-                  _ptr(final_indices), state.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), _stream(x))
+        st = x.stride()
+    ldx = st[1] if T > 1 else st[0] if B > 1 else C
+    hk, hv = key_dim // head_dim, value_dim // head_dim
+    q = torch.empty((B, T, hk, head_dim), device=x.device, dtype=BF16)
+    k = torch.empty((B, T, hk, head_dim), device=x.device, dtype=BF16)
+    v = torch.empty((B, T, hv, head_dim), device=x.device, dtype=BF16)
+    if S:
+        _launch(dev, "fdk_packed_conv_state", x.data_ptr(), ldx, weight.data_ptr(), _addr(cu_seqlens), S, B * T, C, K,
+                key_dim, value_dim, state.data_ptr(), _addr(state_indices), slots, state.data_ptr(),
+                _addr(final_indices), slots, q.data_ptr(), k.data_ptr(), v.data_ptr())
     return q, k, v

@@ -153,6 +153,32 @@ def test_attention_chunks(hq, hkv, D, quant):
 
 
 @pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("most", [4, 8, 16])
+def test_attention_few_tokens(hq, hkv, D, quant, most):
+    # 16, 32 and 64 rows a CTA at four heads a group
+    q = [1, most, 2, most - 1, 3]
+    run_attn(q, [1, most, 200, 90, 1000], hq, hkv, D, 16, quant, seed=most, gate=True)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS + [(12, 1, 128), (7, 1, 256)])
+def test_attention_many_tokens(hq, hkv, D, quant):
+    # full and ragged row tiles, a second tile without rows, blocks that end inside a page or at kv_lens
+    q = [64, 65, 33, 128, 1, 257, 0]
+    run_attn(q, [64, 321, 33, 1000, 700, 260, 9], hq, hkv, D, 16, quant, seed=hq)
+    run_attn([200], [201], hq, hkv, D, 128, quant, seed=hq + 1, interleaved=True, strided=True, gate=True)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
+def test_attention_many_tokens_split_keys(hq, hkv, D, quant):
+    # few row tiles behind a long history: keys split over CTAs, some parts without a visible key
+    run_attn([100], [6000], hq, hkv, D, 64, quant, seed=40, gate=True)
+    run_attn([70, 30], [4500, 60], hq, hkv, D, 32, quant, seed=41)
+
+
+@pytest.mark.parametrize("quant", [False, True])
 def test_attention_empty_rows_and_segments(quant):
     # no tokens; no keys; more tokens than positions (the first ones see nothing and give zeros)
     run_attn([0, 4, 0, 6, 1, 2], [10, 0, 0, 3, 0, 2], 16, 4, 128, 16, quant, seed=3)
