@@ -77,6 +77,26 @@ __device__ __forceinline__ Seg segment(const Params& p, int s, bool report) {
   return r;
 }
 
+// Page ids of the 16-key groups from `key0` on (page sizes are multiples of 16).  The index is clamped to
+// the range's last key, so the loads need no branch and are all in flight at once; they are issued a
+// tile ahead of their use.  An id outside the cache gives -1 (rows of zeros) and is reported.
+template <int N>
+__device__ __forceinline__ void load_page_ids(const Params& p, const int32_t* table, int key0, int last, int (&id)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) id[i] = __ldg(table + (min(key0 + 16 * i, last) >> p.page_shift));
+}
+template <int N>
+__device__ __forceinline__ void check_page_ids(const Params& p, int (&id)[N]) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if ((uint32_t)id[i] >= (uint32_t)p.num_pages) {
+      id[i] = -1;
+      bad = true;
+    }
+  if (bad) atomicOr(&g_error, 1);
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -220,37 +240,34 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int lc = tid % G::CH, lr = tid / G::CH;
   const int32_t* table = p.table + (int64_t)s * p.ld_table;
   const int page_mask = (1 << p.page_shift) - 1;
-  auto page_of = [&](int key) -> int64_t {  // -1: the key is past the range or its page id is invalid
-    if (key >= ke) return -1;
-    const int64_t id = __ldg(table + (key >> p.page_shift));
-    if (id < 0 || id >= p.num_pages) {
-      atomicOr(&g_error, 1);
-      return -1;
-    }
-    return id;
-  };
+  int ids[BN / 16];  // of the next tile to load
+  if (ntiles > 0) load_page_ids(p, table, kb, ke - 1, ids);
   auto load_tile = [&](int j) {
     const int key0 = kb + j * BN;
     const uint32_t dst = sbase + (uint32_t)(j % G::STAGES) * G::STAGE;
+    check_page_ids(p, ids);
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int r = lr + i * RPP;
-      const int64_t id = page_of(key0 + r);
-      const int64_t at = ((int64_t)(hk << p.page_shift) + ((key0 + r) & page_mask)) * G::ROW + lc * 16;
-      const uint32_t bytes = id >= 0 ? 16u : 0u;   // rows past the range are zero-filled
-      const int64_t pg = id >= 0 ? id : 0;
+      const int id = ids[i * RPP / 16];
+      const bool ok = id >= 0 && key0 + r < ke;
+      const int64_t pg = ok ? id : 0;
+      const int at = ((hk << p.page_shift) + ((key0 + r) & page_mask)) * G::ROW + lc * 16;
+      const uint32_t bytes = ok ? 16u : 0u;   // rows past the range are zero-filled
       const uint32_t to = dst + tile_at<G::CH>(r, lc);
-      cp_async16(to, p.k_cache + pg * p.kpage + (id >= 0 ? at : 0), bytes);
-      cp_async16(to + G::TILE, p.v_cache + pg * p.vpage + (id >= 0 ? at : 0), bytes);
+      cp_async16(to, p.k_cache + (pg * p.kpage + at), bytes);
+      cp_async16(to + G::TILE, p.v_cache + (pg * p.vpage + at), bytes);
     }
-    if (QUANT && tid < 8) {  // scale bytes: 16 keys at a time (page sizes are multiples of 16)
-      const int r = (tid & 3) * 16;
-      const int64_t id = page_of(key0 + r);
-      const int64_t at = (int64_t)(hk << p.page_shift) + ((key0 + r) & page_mask);
-      const uint8_t* src = tid < 4 ? p.k_scale : p.v_scale;
-      const int64_t ld = tid < 4 ? p.kscale_page : p.vscale_page;
-      cp_async16(dst + 2 * G::TILE + (tid < 4 ? 0 : BN) + r, src + (id >= 0 ? id * ld + at : 0), id >= 0 ? 16u : 0u);
+    if (QUANT && tid < 8) {  // scale bytes: 16 keys at a time
+      const int u = tid & 3, r = u * 16;
+      const int id = u == 0 ? ids[0] : u == 1 ? ids[1] : u == 2 ? ids[2] : ids[3];
+      const bool ok = id >= 0 && key0 + r < ke;
+      const int64_t pg = ok ? id : 0;
+      const int at = (hk << p.page_shift) + ((key0 + r) & page_mask);
+      cp_async16(dst + 2 * G::TILE + (tid < 4 ? 0 : BN) + r,
+                 tid < 4 ? p.k_scale + (pg * p.kscale_page + at) : p.v_scale + (pg * p.vscale_page + at), ok ? 16u : 0u);
     }
+    load_page_ids(p, table, key0 + BN, ke - 1, ids);
   };
 
   float o[D / 8][4];

@@ -16,11 +16,15 @@
 //   outside the cache is an out-of-range coordinate, which TMA fills with zeros.  V rows at or behind
 //   kv_lens[s] may hold anything (0 * NaN would reach the sums): the block that has them is zeroed there
 //   after its load and before the MMA warp sees it.
-//   8-bit cache: four warps load rows with ordinary 16-byte loads, convert e4m3 -> fp16 (exact), multiply by
-//   the row's scale relative to the largest one of the CTA's key range (exact for scales within 2^15 of
-//   it; smaller ones lose bits below 2^-33 of the range's largest element) and store them in the
-//   operand layout.  The largest K scale then folds into the softmax scale, V's into the final
-//   normalisation, so the softmax costs what it does for bf16.  q goes to fp16 with a power of two a row.
+//   8-bit cache: TMA brings the raw e4m3 rows; four converter warps turn them into fp16 operands (e4m3 ->
+//   fp16 is exact) multiplied by the row's scale relative to the largest one of the CTA's key range
+//   (exact for scales within 2^15 of it; smaller ones lose bits below 2^-33 of the range's largest
+//   element).  The largest K scale then folds into the softmax scale, V's into the final normalisation,
+//   so the softmax costs what it does for bf16.  q goes to fp16 with a power of two a row.
+//
+//   K and V blocks share one ring of operand slots, in the order K_0 V_0 K_1 V_1 ..: four slots for bf16,
+//   three for the 8-bit cache (PV of block j and S of block j + 1 hold two, the converters fill the
+//   third), which leaves room for a ring of four raw tiles.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -37,23 +41,34 @@ struct Geo {
   static constexpr int NBX = D / 64;                   // 64-column (128-byte) boxes of a row
   static constexpr uint32_t QBOX = 128 * 128, KBOX = (uint32_t)BN * 128;
   static constexpr uint32_t QT = NBX * QBOX, KT = NBX * KBOX;
-  static constexpr uint32_t OFF_Q = 0, OFF_K = NT * QT, OFF_V = OFF_K + 2 * KT, OFF_BAR = OFF_V + 2 * KT;
   static constexpr uint32_t TM_S(int i) { return (uint32_t)(BN * i); }         // tile i, or ping-pong buffer i
   static constexpr uint32_t TM_O(int i) { return 256u + 128u * (uint32_t)i; }  // tile i
 };
-// barriers: two of each KF KE VF VE S P; VT: V of the block that ends past kv_lens, before its tail is zeroed
-enum { B_Q = 0, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_VT = B_P + 2,
+// Shared memory: Q tiles, operand ring, raw ring (8-bit cache), barriers and small state.
+// barriers: F / E operand slot full / empty, RF / RE raw slot full / empty, S and P per tile or buffer;
+// VT: V of the block that ends past kv_lens, before its tail is zeroed
+enum { B_Q = 0, B_F, B_E = B_F + 4, B_RF = B_E + 4, B_RE = B_RF + 4, B_S = B_RE + 4, B_P = B_S + 2, B_VT = B_P + 2,
        B_PV, B_O, NBAR };
-constexpr uint32_t OFF_MISC = 8 * NBAR;                // abort flag, TMEM address, scale maxima, row scales of q
-constexpr uint32_t MISC_BYTES = 32 + 2 * 128 * 4 + 64;
-template <int D>
-constexpr uint32_t smem_bytes() { return Geo<D>::OFF_BAR + OFF_MISC + MISC_BYTES + 1024; }
+constexpr int RAW_SLOTS = 4;
+template <int D, bool QUANT>
+struct Smem {
+  using G = Geo<D>;
+  static constexpr int SLOTS = QUANT ? 3 : 4;
+  static constexpr uint32_t RAWT = QUANT ? (uint32_t)(G::BN * D) : 0;  // bytes of a raw tile
+  static constexpr uint32_t OFF_Q = 0, OFF_KV = G::NT * G::QT, OFF_RAW = OFF_KV + SLOTS * G::KT,
+                            OFF_BAR = OFF_RAW + RAW_SLOTS * RAWT, OFF_MISC = OFF_BAR + 8 * NBAR,
+                            OFF_QS = OFF_MISC + 64,                       // row scale exponents of q: 256 bytes
+                            OFF_FT = OFF_QS + (QUANT ? 256 : 0),          // row factors of two tiles: half2
+                            BYTES = OFF_FT + (QUANT ? 1024 : 0) + 1024;   // + slack for 1024-byte alignment
+  static_assert(OFF_MISC % 16 == 0, "alignment of the small state");
+  static_assert(BYTES <= 232448, "shared memory of a CTA");
+};
 constexpr uint32_t TM_COLS = 512;
 constexpr float P_SHIFT = 6.f;  // fp16 P is scaled by 2^6: weights down to 2^-30 of the row's largest stay
 constexpr long long DRAIN_BUDGET = 2000000000LL;
 
-// warps: NT * 4 softmax, then one producer (bf16 cache), one MMA issuer and TMEM allocator; with the 8-bit
-// cache four converter warps on a warpgroup boundary
+// warps: NT * 4 softmax, one producer, one MMA issuer and TMEM allocator; with the 8-bit cache four
+// converter warps on a warpgroup boundary
 template <int D, bool QUANT>
 struct Roles {
   static constexpr int PRODUCER = Geo<D>::NT * 4, MMA = PRODUCER + 1, CONV = PRODUCER + 4;
@@ -75,6 +90,14 @@ __device__ __forceinline__ bool drain(uint32_t bar, uint32_t parity) {
 __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_mn_major, bool f16) {
   return idesc_bf16(M, N, false, b_mn_major) & (f16 ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
+__device__ __forceinline__ uint32_t half2_bits(float x) {
+  const __half2 h = __float2half2_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N>
@@ -91,19 +114,21 @@ __global__ void __launch_bounds__(Roles<D, QUANT>::THREADS, 1)
 many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const Params p) {
   using G = Geo<D>;
+  using M = Smem<D, QUANT>;
   using R = Roles<D, QUANT>;
   constexpr int NT = G::NT, BN = G::BN, NBX = G::NBX;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const uint32_t bar0 = base + G::OFF_BAR;
+  const uint32_t bar0 = base + M::OFF_BAR;
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + G::OFF_BAR + OFF_MISC);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + G::OFF_BAR + OFF_MISC + 4);
-  volatile int* scale_max = reinterpret_cast<volatile int*>(gbase + G::OFF_BAR + OFF_MISC + 8);  // K, V bytes
-  float* q_scale = reinterpret_cast<float*>(gbase + G::OFF_BAR + OFF_MISC + 32);                 // [NT * 128]
-  int* warp_max = reinterpret_cast<int*>(q_scale + 256);                                         // [4][2]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + M::OFF_MISC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + M::OFF_MISC + 4);
+  volatile int* scale_max = reinterpret_cast<volatile int*>(gbase + M::OFF_MISC + 8);  // largest K, V scale byte
+  int* warp_max = reinterpret_cast<int*>(gbase + M::OFF_MISC + 16);                    // [4][2]
+  uint8_t* q_exp = gbase + M::OFF_QS;
+  uint32_t* factor = reinterpret_cast<uint32_t*>(gbase + M::OFF_FT);                   // [2][BN] half2
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // grid: x = (segment, KV head) with the head fastest, y = row tile from the last one down (the longest
@@ -146,7 +171,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;
       if (i == B_P || i == B_P + 1) count = 128;
-      if (QUANT && (i == B_Q || i == B_KF || i == B_KF + 1 || i == B_VF || i == B_VF + 1)) count = 128;
+      if (QUANT && (i == B_Q || (i >= B_F && i < B_F + 4) || (i >= B_RE && i < B_RE + 4))) count = 128;
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -163,14 +188,44 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   const int32_t* table = p.table + (int64_t)s * p.ld_table;
   const int page_mask = (1 << p.page_shift) - 1;
 
-  if (!QUANT && warp == R::PRODUCER) {
-    // ------------------------------------------------------------------ TMA producer (whole warp)
+  // ------------------------------------------------------------------ TMA producer (one whole warp)
+  // items 2 j and 2 j + 1 are K and V of block j; ring of operand slots (bf16) or raw slots (8-bit cache)
+  auto producer = [&]() {
+    constexpr int RING = QUANT ? RAW_SLOTS : M::SLOTS;
+    constexpr int FULL = QUANT ? B_RF : B_F, EMPTY = QUANT ? B_RE : B_E;
+    constexpr uint32_t BYTES = QUANT ? M::RAWT : G::KT;
     // a block's boxes: keys in pages of 2^page_shift, at most BN a box; lane i issues box i, i + 32, ..
     const int box_keys = min(BN, 1 << p.page_shift);
-    const int boxes = (BN / box_keys) * NBX;
-    auto load_block = [&](const CUtensorMap* map, uint32_t dst, uint32_t fb, int key0) {
+    constexpr int COLS = QUANT ? 1 : NBX;  // boxes across a row: the raw row, or 64 bf16 columns each
+    const int boxes = (BN / box_keys) * COLS;
+    if (lane == 0) {
+      prefetch_tmap(&tk);
+      prefetch_tmap(&tv);
+      if (!QUANT) {
+        const int tiles = two ? 2 : 1;
+        mbar_expect_tx(bar(B_Q), (uint32_t)(tiles * NBX) * 128u * (uint32_t)rpt);
+        for (int i = 0; i < tiles; ++i)
+          for (int b = 0; b < NBX; ++b)
+            tma_load_3d(base + M::OFF_Q + i * G::QT + b * G::QBOX, &tq, bar(B_Q), b * 64, hk * p.group,
+                        seg.begin + tok0 + i * tpt);
+      }
+    }
+    int issued = 0;
+    for (int i = 0; i < 2 * n_kv; ++i) {
+      const int slot = i % RING;
+      if (i >= RING &&
+          !__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + slot), (uint32_t)(i / RING - 1) & 1u, abort_flag) ? 1 : 0))
+        break;
+      const bool is_v = i & 1;
+      const int key0 = kb + (i >> 1) * BN;
+      const int live = kv_len - key0;                      // rows of the block that are cached positions
+      const bool tail = !QUANT && is_v && live < BN;       // at most the last block
+      const uint32_t fb = bar(tail ? B_VT : FULL + slot);
+      const uint32_t dst = base + (QUANT ? M::OFF_RAW + slot * M::RAWT : M::OFF_KV + slot * G::KT);
+      if (lane == 0) mbar_expect_tx(fb, BYTES);
+      __syncwarp();
       for (int b = lane; b < boxes; b += 32) {
-        const int sub = b / NBX, col = b % NBX;
+        const int sub = b / COLS, col = b % COLS;
         const int key = key0 + sub * box_keys;
         int page = (int)p.num_pages;  // out of range: zeros
         if (key < ke) {
@@ -178,70 +233,46 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           if (id >= 0 && id < p.num_pages) page = id;
           else atomicOr(&g_error, 1);
         }
-        tma_load_4d(dst + (uint32_t)col * G::KBOX + (uint32_t)(sub * box_keys) * 128u, map, fb, col * 64,
-                    key & page_mask, hk, page);
+        const uint32_t at = QUANT ? (uint32_t)(sub * box_keys * D) : (uint32_t)col * G::KBOX + (uint32_t)(sub * box_keys) * 128u;
+        tma_load_4d(dst + at, is_v ? &tv : &tk, fb, col * 64, key & page_mask, hk, page);
       }
-    };
-    if (lane == 0) {
-      prefetch_tmap(&tq);
-      prefetch_tmap(&tk);
-      prefetch_tmap(&tv);
-      const int tiles = two ? 2 : 1;
-      mbar_expect_tx(bar(B_Q), (uint32_t)(tiles * NBX) * 128u * (uint32_t)rpt);
-      for (int i = 0; i < tiles; ++i)
-        for (int b = 0; b < NBX; ++b)
-          tma_load_3d(base + G::OFF_Q + i * G::QT + b * G::QBOX, &tq, bar(B_Q), b * 64, hk * p.group,
-                      seg.begin + tok0 + i * tpt);
-    }
-    int issued_k = 0, issued_v = 0;
-    bool ok = true;
-    for (int j = 0; ok && j < n_kv; ++j) {
-      const int st = j & 1;
-      ok = __all_sync(0xffffffffu, (j < 2 || mbar_wait(bar(B_KE + st), ((j >> 1) - 1) & 1, abort_flag)) ? 1 : 0);
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(bar(B_KF + st), G::KT);
-      __syncwarp();
-      load_block(&tk, base + G::OFF_K + st * G::KT, bar(B_KF + st), kb + j * BN);
-      issued_k = j + 1;
-      ok = __all_sync(0xffffffffu, (j < 2 || mbar_wait(bar(B_VE + st), ((j >> 1) - 1) & 1, abort_flag)) ? 1 : 0);
-      if (!ok) break;
-      const int live = kv_len - (kb + j * BN);  // rows of the block that are cached positions
-      const bool tail = live < BN;              // at most the last block
-      const uint32_t vdst = base + G::OFF_V + st * G::KT;
-      if (lane == 0) mbar_expect_tx(bar(tail ? B_VT : B_VF + st), G::KT);
-      __syncwarp();
-      load_block(&tv, vdst, bar(tail ? B_VT : B_VF + st), kb + j * BN);
-      issued_v = j + 1;
+      issued = i + 1;
       if (tail) {
         drain(bar(B_VT), 0);
         __syncwarp();
-        uint8_t* v = gbase + G::OFF_V + st * G::KT;
+        uint8_t* v = gbase + M::OFF_KV + slot * G::KT;
         for (int e = lane; e < (BN - live) * NBX * 8; e += 32) {
           const int r = live + e / (NBX * 8), c = e % (NBX * 8);
           *reinterpret_cast<uint4*>(v + chunk_at<G::KBOX>(r, c)) = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_VF + st));
+        if (lane == 0) mbar_arrive(bar(FULL + slot));
       }
     }
     // drain: every issued load must have landed before shared memory is released
     if (lane == 0) {
-      drain(bar(B_Q), 0);
-      for (int j = (issued_k > 2 ? issued_k - 2 : 0); j < issued_k; ++j) drain(bar(B_KF + (j & 1)), (j >> 1) & 1);
-      for (int j = (issued_v > 2 ? issued_v - 2 : 0); j < issued_v; ++j) drain(bar(B_VF + (j & 1)), (j >> 1) & 1);
+      if (!QUANT) drain(bar(B_Q), 0);
+      for (int i = (issued > RING ? issued - RING : 0); i < issued; ++i) drain(bar(FULL + i % RING), (uint32_t)(i / RING) & 1u);
     }
+  };
+
+  if (warp == R::PRODUCER && !R::SPLIT_REGS) {
+    producer();
   } else if (QUANT ? warp >= R::PRODUCER && warp < R::CONV : warp == R::MMA) {
     // With the 8-bit cache at head_dim 128, 512 threads are launched with 128 registers each; the softmax
-    // needs more (a row of S and of P), the other warpgroups less: 256 * 176 + 128 * (40 + 120) = 65536.
-    if constexpr (R::SPLIT_REGS) reg_dec<40>();
+    // needs more (a row of S and of P), the other warpgroups less: 256 * 192 + 128 * (40 + 88) = 65536.
+    if constexpr (R::SPLIT_REGS) {
+      reg_dec<40>();
+      if (warp == R::PRODUCER) producer();
+    }
     // ------------------------------------------------------------------ MMA issuer
     if (warp == R::MMA && lane == 0) {
       constexpr uint32_t ID_QK = idesc(128, BN, false, QUANT);
       constexpr uint32_t ID_PV = idesc(128, D, true, QUANT);  // V is MN-major (columns contiguous)
       auto issue_s = [&](int j, int tile, uint32_t tm) {
-        const uint64_t dq = sdesc_sw128(base + G::OFF_Q + tile * G::QT, 16, 1024);
-        const uint64_t dk = sdesc_sw128(base + G::OFF_K + (j & 1) * G::KT, 16, 1024);
+        const uint64_t dq = sdesc_sw128(base + M::OFF_Q + tile * G::QT, 16, 1024);
+        const uint64_t dk = sdesc_sw128(base + M::OFF_KV + (2 * j % M::SLOTS) * G::KT, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t qo = ((kk >> 2) * G::QBOX + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * G::KBOX + (kk & 3) * 32) >> 4;
@@ -249,13 +280,15 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         }
       };
       auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o) {
-        const uint64_t dv = sdesc_sw128(base + G::OFF_V + (j & 1) * G::KT, G::KBOX, 1024);
+        const uint64_t dv = sdesc_sw128(base + M::OFF_KV + ((2 * j + 1) % M::SLOTS) * G::KT, G::KBOX, 1024);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
           umma_ts(tmem + tm_o, tmem + tm_p + 8 * kk, dv + (uint32_t)(kk * 2048 >> 4), ID_PV, (j > 0 || kk > 0) ? 1u : 0u);
       };
       auto wait = [&](int i, int parity) { return mbar_wait(bar(i), (uint32_t)parity & 1u, abort_flag); };
-      bool ok = wait(B_Q, 0) && wait(B_KF, 0);
+      auto full = [&](int item) { return wait(B_F + item % M::SLOTS, item / M::SLOTS); };
+      auto release = [&](int item) { umma_commit(bar(B_E + item % M::SLOTS)); };
+      bool ok = wait(B_Q, 0) && full(0);
       if (NT == 2) {
         if (ok) {
           tc_fence_after();
@@ -265,15 +298,15 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
             issue_s(0, 1, G::TM_S(1));
             umma_commit(bar(B_S + 1));
           }
-          umma_commit(bar(B_KE));
+          release(0);
         }
         for (int j = 0; ok && j < n_kv; ++j) {
           const bool more = j + 1 < n_kv;
-          if (!wait(B_VF + (j & 1), j >> 1) || !wait(B_P, j)) break;
+          if (!full(2 * j + 1) || !wait(B_P, j)) break;
           tc_fence_after();
           issue_pv(j, G::TM_S(0), G::TM_O(0));
           if (more) {
-            if (!wait(B_KF + ((j + 1) & 1), (j + 1) >> 1)) break;
+            if (!full(2 * j + 2)) break;
             tc_fence_after();
             issue_s(j + 1, 0, G::TM_S(0));
             umma_commit(bar(B_S));
@@ -283,37 +316,37 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
             tc_fence_after();
             issue_pv(j, G::TM_S(1), G::TM_O(1));
           }
-          umma_commit(bar(B_VE + (j & 1)));
+          release(2 * j + 1);
           if (more) {
             if (two) {
               issue_s(j + 1, 1, G::TM_S(1));
               umma_commit(bar(B_S + 1));
             }
-            umma_commit(bar(B_KE + ((j + 1) & 1)));
+            release(2 * j + 2);
           }
         }
       } else {
         auto s_block = [&](int j) {
           issue_s(j, 0, G::TM_S(j & 1));
           umma_commit(bar(B_S + (j & 1)));
-          umma_commit(bar(B_KE + (j & 1)));
+          release(2 * j);
         };
         if (ok) {
           tc_fence_after();
           s_block(0);
-          if (n_kv > 1 && (ok = wait(B_KF + 1, 0))) {
+          if (n_kv > 1 && (ok = full(2))) {
             tc_fence_after();
             s_block(1);
           }
         }
         for (int j = 0; ok && j < n_kv; ++j) {
-          if (!wait(B_VF + (j & 1), j >> 1) || !wait(B_P + (j & 1), j >> 1)) break;
+          if (!full(2 * j + 1) || !wait(B_P + (j & 1), j >> 1)) break;
           tc_fence_after();
           issue_pv(j, G::TM_S(j & 1), G::TM_O(0));
           umma_commit(bar(B_PV));
-          umma_commit(bar(B_VE + (j & 1)));
+          release(2 * j + 1);
           if (j + 2 < n_kv) {
-            if (!wait(B_KF + (j & 1), (j + 2) >> 1)) break;
+            if (!full(2 * j + 4)) break;
             tc_fence_after();
             s_block(j + 2);
           }
@@ -324,23 +357,14 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     }
   } else if (QUANT && warp >= R::CONV) {
     // ------------------------------------------------------------------ converters (128 threads)
-    if constexpr (R::SPLIT_REGS) reg_dec<120>();
+    if constexpr (R::SPLIT_REGS) reg_dec<88>();
     const int ct = tid - R::CONV * 32, cw = ct >> 5;
-    auto page_of = [&](int key) -> int64_t {  // -1: behind the range, or an invalid id
-      if (key >= ke) return -1;
-      const int64_t id = __ldg(table + (key >> p.page_shift));
-      if (id < 0 || id >= p.num_pages) {
-        atomicOr(&g_error, 1);
-        return -1;
-      }
-      return id;
-    };
-    auto slot_of = [&](int key) { return (int64_t)(hk << p.page_shift) + (key & page_mask); };
+    auto slot_of = [&](int key) { return (hk << p.page_shift) + (key & page_mask); };
     // largest scale bytes of the range, 16 keys a load
     uint32_t mk = 0, mv = 0;
     for (int key = kb + ct * 16; key < ke; key += 128 * 16) {
-      const int64_t id = page_of(key);
-      if (id < 0) continue;
+      const int64_t id = __ldg(table + (key >> p.page_shift));
+      if (id < 0 || id >= p.num_pages) continue;  // reported by the loads below
       const uint4 a = __ldg(reinterpret_cast<const uint4*>(p.k_scale + id * p.kscale_page + slot_of(key)));
       const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.v_scale + id * p.vscale_page + slot_of(key)));
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
@@ -384,76 +408,77 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       }
       const int e = a == 0.f ? 127 : min(max((int)(__float_as_uint(a) >> 23), 1), 253);
       const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-      q_scale[i * 128 + ct] = __uint_as_float((uint32_t)e << 23);
+      q_exp[i * 128 + ct] = (uint8_t)e;  // q's row is fp16 * 2^(e - 127)
       for (int c = 0; c < D / 8; ++c) {
         float f[8];
         unpack8(live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u), f);
         const uint4 h = make_uint4(pack_f16x2(f[0] * inv, f[1] * inv), pack_f16x2(f[2] * inv, f[3] * inv),
                                    pack_f16x2(f[4] * inv, f[5] * inv), pack_f16x2(f[6] * inv, f[7] * inv));
-        *reinterpret_cast<uint4*>(gbase + G::OFF_Q + i * G::QT + chunk_at<G::QBOX>(ct, c)) = h;
+        *reinterpret_cast<uint4*>(gbase + M::OFF_Q + i * G::QT + chunk_at<G::QBOX>(ct, c)) = h;
       }
     }
     fence_proxy_async_smem();
     mbar_arrive(bar(B_Q));
-    // K and V blocks: D / 16 threads a row of 16-byte pieces
-    constexpr int TPR = D / 16, RPP = 128 / TPR, PASSES = BN / RPP;
+    // Items: thread ct is row ct's keeper (its scale byte, loaded a block ahead) and, for the conversion,
+    // piece lc (8 columns) of rows lr, lr + RPP, ..: 8 raw bytes become one 16-byte operand chunk.  Eight
+    // neighbouring threads read 64 consecutive bytes and store all eight chunk positions: no conflicts.
+    constexpr int TPR = D / 8, RPP = 128 / TPR, PASSES = BN / RPP;
     const int lc = ct % TPR, lr = ct / TPR;
-    uint4 kraw[PASSES], vraw[PASSES];
-    int kexp[PASSES], vexp[PASSES];
-    auto load_rows = [&](int key0, const uint8_t* cache, int64_t page_bytes, const uint8_t* scales, int64_t scale_page,
-                         uint4 (&w)[PASSES], int (&e)[PASSES]) {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int key = key0 + lr + i * RPP;
-        const int64_t id = page_of(key);
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        e[i] = 0;
-        if (id >= 0) {
-          w[i] = ldg_stream(cache + id * page_bytes + slot_of(key) * D + lc * 16);
-          e[i] = __ldg(scales + id * scale_page + slot_of(key));
-        }
-      }
+    const int my = ct < BN ? ct : 0;
+    auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
+    auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
+      const bool live = (uint32_t)id < (uint32_t)p.num_pages && key < ke;  // a bad id is reported by the producer
+      const int b = __ldg(scales + ((live ? id : 0) * page_ld + slot_of(key)));
+      return live ? b : 0;
     };
-    auto store_rows = [&](uint32_t off, const uint4 (&w)[PASSES], const int (&e)[PASSES], int emax) {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int r = lr + i * RPP;
-        const __half2 f = __float2half2_rn(scale_value(max(e[i] - emax + 127, 0)));
-        const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t lo = paged::e4m3x2_to_f16x2((uint16_t)ww[u]), hi = paged::e4m3x2_to_f16x2((uint16_t)(ww[u] >> 16));
-          const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&lo), f);
-          const __half2 b = __hmul2(*reinterpret_cast<const __half2*>(&hi), f);
-          h[2 * u] = *reinterpret_cast<const uint32_t*>(&a);
-          h[2 * u + 1] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        // two 16-byte chunks; the upper half of a row's threads stores its odd one first, so that the eight
-        // threads of a store phase hit all eight chunk positions
-        uint8_t* dst = gbase + off;
-        const int flip = (lc >> 2) & 1;
-        const uint4 c0 = make_uint4(h[0], h[1], h[2], h[3]), c1 = make_uint4(h[4], h[5], h[6], h[7]);
-        *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(r, 2 * lc + flip)) = flip ? c1 : c0;
-        *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(r, 2 * lc + 1 - flip)) = flip ? c0 : c1;
-      }
-      fence_proxy_async_smem();
-    };
-    load_rows(kb, p.k_cache, p.kpage, p.k_scale, p.kscale_page, kraw, kexp);
+    int id = page_at(kb + my);
+    int kbyte = scale_at(p.k_scale, p.kscale_page, kb + my, id), vbyte = scale_at(p.v_scale, p.vscale_page, kb + my, id);
+    id = page_at(kb + BN + my);
+    // once a wait has run out, a thread only keeps step at the named barrier (the others may be behind it)
+    bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
-      const int st = j & 1;
-      load_rows(kb + j * BN, p.v_cache, p.vpage, p.v_scale, p.vscale_page, vraw, vexp);
-      if (j >= 2 && !mbar_wait(bar(B_KE + st), ((j >> 1) - 1) & 1, abort_flag)) break;
-      store_rows(G::OFF_K + st * G::KT, kraw, kexp, ek);
-      mbar_arrive(bar(B_KF + st));
-      if (j + 1 < n_kv) load_rows(kb + (j + 1) * BN, p.k_cache, p.kpage, p.k_scale, p.kscale_page, kraw, kexp);
-      if (j >= 2 && !mbar_wait(bar(B_VE + st), ((j >> 1) - 1) & 1, abort_flag)) break;
-      store_rows(G::OFF_V + st * G::KT, vraw, vexp, ev);
-      mbar_arrive(bar(B_VF + st));
+      const int key0 = kb + j * BN;
+      const uint32_t fk = half2_bits(scale_value(max(kbyte - ek + 127, 0))), fv = half2_bits(scale_value(max(vbyte - ev + 127, 0)));
+      // rows behind the range may hold anything, NaN included: their operands are zeros, not 0 * NaN
+      const int live = ke - key0;
+      kbyte = scale_at(p.k_scale, p.kscale_page, key0 + BN + my, id);
+      vbyte = scale_at(p.v_scale, p.vscale_page, key0 + BN + my, id);
+      id = page_at(key0 + 2 * BN + my);
+#pragma unroll 1
+      for (int which = 0; which < 2; ++which) {
+        const int item = 2 * j + which, raw_slot = item % RAW_SLOTS, slot = item % M::SLOTS;
+        if (ct < BN) factor[which * BN + ct] = which ? fv : fk;
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");  // factors written; also: nobody still reads the other table
+        ok = ok && mbar_wait(bar(B_RF + raw_slot), (uint32_t)(item / RAW_SLOTS) & 1u, abort_flag) &&
+             (item < M::SLOTS || mbar_wait(bar(B_E + slot), (uint32_t)(item / M::SLOTS - 1) & 1u, abort_flag));
+        if (!ok) continue;
+        const uint8_t* src = gbase + M::OFF_RAW + raw_slot * M::RAWT + lr * D + lc * 8;
+        uint8_t* dst = gbase + M::OFF_KV + slot * G::KT;
+        const uint32_t* fac = factor + which * BN + lr;
+        auto convert = [&](bool partial) {
+#pragma unroll
+          for (int i = 0; i < PASSES; ++i) {
+            uint2 w = *reinterpret_cast<const uint2*>(src + i * RPP * D);
+            if (partial && lr + i * RPP >= live) w = make_uint2(0u, 0u);
+            const uint32_t f = fac[i * RPP];
+            uint4 h;
+            h.x = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w.x), f);
+            h.y = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w.x >> 16)), f);
+            h.z = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w.y), f);
+            h.w = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w.y >> 16)), f);
+            *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(lr + i * RPP, lc)) = h;
+          }
+        };
+        if (live >= BN) convert(false);
+        else convert(true);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(B_F + slot));
+        mbar_arrive(bar(B_RE + raw_slot));
+      }
     }
   } else {
     // ------------------------------------------------------------------ softmax
-    if constexpr (R::SPLIT_REGS) reg_inc<176>();
+    if constexpr (R::SPLIT_REGS) reg_inc<192>();
     const int tile = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -468,7 +493,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     if (QUANT && ok) {
       ok = __all_sync(0xffffffffu, mbar_wait(bar(B_Q), 0, abort_flag) ? 1 : 0);
       // never 0: a masked score is -inf * sl2
-      if (ok) sl2 = fmaxf(sl2 * q_scale[tile * 128 + row] * scale_value(scale_max[0]), 1e-37f);
+      if (ok) sl2 = fmaxf(sl2 * scale_value(q_exp[tile * 128 + row]) * scale_value(scale_max[0]), 1e-37f);
     }
     const int n_blocks = ok ? n_kv : 0;
     for (int j = 0; j < n_blocks; ++j) {
@@ -625,13 +650,15 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-static int encode(CUtensorMap* m, const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+// bf16 with the 128-byte swizzle, or plain bytes
+static int encode(CUtensorMap* m, const void* ptr, bool bytes, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                   const cuuint32_t* box) {
   EncodeFn enc = encode_fn();
   if (!enc) return set_error(FDK_ERR_DEVICE, "paged_gqa: cuTensorMapEncodeTiled unavailable");
   const cuuint32_t one[4] = {1, 1, 1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box,
-                         one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = enc(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+                         const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(FDK_ERR_INVALID_ARGUMENT, "paged_gqa: tensor map encode failed (%d)", (int)r);
   return FDK_OK;
@@ -641,20 +668,20 @@ template <int D, bool QUANT>
 static int launch(const Params& p, int64_t row_tiles, cudaStream_t s) {
   using G = Geo<D>;
   CUtensorMap mq = {}, mk = {}, mv = {};
+  const cuuint64_t esz = QUANT ? 1 : 2, ps = (cuuint64_t)1 << p.page_shift;
+  const cuuint64_t kd[4] = {(cuuint64_t)D, ps, (cuuint64_t)p.hkv, (cuuint64_t)p.num_pages};
+  const cuuint32_t kb[4] = {QUANT ? (cuuint32_t)D : 64u, (cuuint32_t)(ps < (cuuint64_t)G::BN ? ps : (cuuint64_t)G::BN), 1, 1};
+  const cuuint64_t ks[3] = {(cuuint64_t)D * esz, ps * D * esz, (cuuint64_t)p.kpage};
+  const cuuint64_t vs[3] = {(cuuint64_t)D * esz, ps * D * esz, (cuuint64_t)p.vpage};
+  if (int st = encode(&mk, p.k_cache, QUANT, 4, kd, ks, kb)) return st;
+  if (int st = encode(&mv, p.v_cache, QUANT, 4, kd, vs, kb)) return st;
   if (!QUANT) {
     const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)p.hq, (cuuint64_t)p.tokens};
     const cuuint64_t qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)p.ld_q * 2};
     const cuuint32_t qb[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(128 / p.group)};
-    if (int st = encode(&mq, p.q, 3, qd, qs, qb)) return st;
-    const cuuint64_t ps = (cuuint64_t)1 << p.page_shift;
-    const cuuint64_t kd[4] = {(cuuint64_t)D, ps, (cuuint64_t)p.hkv, (cuuint64_t)p.num_pages};
-    const cuuint32_t kb[4] = {64, (cuuint32_t)(ps < G::BN ? ps : G::BN), 1, 1};
-    const cuuint64_t ks[3] = {(cuuint64_t)D * 2, ps * D * 2, (cuuint64_t)p.kpage};
-    const cuuint64_t vs[3] = {(cuuint64_t)D * 2, ps * D * 2, (cuuint64_t)p.vpage};
-    if (int st = encode(&mk, p.k_cache, 4, kd, ks, kb)) return st;
-    if (int st = encode(&mv, p.v_cache, 4, kd, vs, kb)) return st;
+    if (int st = encode(&mq, p.q, false, 3, qd, qs, qb)) return st;
   }
-  constexpr uint32_t bytes = smem_bytes<D>();
+  constexpr uint32_t bytes = Smem<D, QUANT>::BYTES;
   const void* fn = (const void*)many_rows_kernel<D, QUANT>;
   if (int st = ensure_smem_attr(fn, (int)bytes, "paged_gqa")) return st;
   const dim3 grid((unsigned)((int64_t)p.nseg * p.hkv), (unsigned)row_tiles, (unsigned)p.nsplit);
