@@ -45,6 +45,8 @@ struct Params {
   const int32_t* kv_lens;
   int64_t tokens, num_pages;
   int nseg, max_pages, page_shift, hq, hkv, group, nsplit, row_blocks;
+  int split_keys;  // keys a split (a multiple of every tile's), the last one takes what is left
+  int picked;      // many rows: x counts the call's row tiles, longest first
   float sl2;  // softmax scale * log2(e)
   const bf16* gate;
   int64_t ld_gate;
@@ -75,6 +77,17 @@ __device__ __forceinline__ Seg segment(const Params& p, int s, bool report) {
   }
   r.past = len - r.n;
   return r;
+}
+
+// Keys [kb, ke) of a split of a row block that sees keys [0, kend).  The split size is fixed, so short
+// sequences use few of the grid's splits.
+__device__ __forceinline__ void split_range(const Params& p, int split, int kend, int& kb, int& ke) {
+  kb = (int)min((int64_t)kend, (int64_t)split * p.split_keys);
+  ke = split == p.nsplit - 1 ? kend : (int)min((int64_t)kend, (int64_t)kb + p.split_keys);
+}
+// Parts of a row that sees `visible` keys: the splits that hold one of them (at least one is written).
+__device__ __forceinline__ int parts_of(const Params& p, int64_t visible) {
+  return visible <= p.split_keys ? 1 : (int)min((int64_t)p.nsplit, (visible + p.split_keys - 1) / p.split_keys);
 }
 
 // Page ids of the 16-key groups from `key0` on (page sizes are multiples of 16).  The index is clamped to
@@ -173,8 +186,9 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int last_tok = (min(row0 + BM, rows) - 1) / p.group;
   const int64_t kend64 = seg.past + last_tok + 1;
   const int kend = kend64 > 0 ? (int)kend64 : 0;       // keys the row block can see
-  const int per = ((kend + p.nsplit * BN - 1) / (p.nsplit * BN)) * BN;
-  const int kb = min(kend, split * per), ke = min(kend, kb + per);
+  int kb, ke;
+  split_range(p, split, kend, kb, ke);
+  if (kb >= ke && split > 0) return;  // the join does not read this part
   const int ntiles = (ke - kb + BN - 1) / BN;
 
   // this lane's two rows (g and g + 8 of the warp's 16)
@@ -534,13 +548,16 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int head = (int)(w % per_tok) * RPW + lane / LPR, c = (lane % LPR) * 8;
   if (head >= p.hq) return;
   const int64_t idx = tok * p.hq + head, plane = p.tokens * p.hq;
+  int64_t len = p.kv_lens[s];
+  if (len < 0 || len > ((int64_t)p.max_pages << p.page_shift)) len = 0;
+  const int parts = parts_of(p, len - (end - tok) + 1);
   float mm = -INFINITY;
-  for (int i = 0; i < p.nsplit; ++i) mm = fmaxf(mm, p.part_ml[i * plane + idx].x);
+  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, p.part_ml[i * plane + idx].x);
   float ll = 0.f, y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = 0.f;
   if (mm != -INFINITY)
-    for (int i = 0; i < p.nsplit; ++i) {
+    for (int i = 0; i < parts; ++i) {
       const float2 ml = p.part_ml[i * plane + idx];
       if (ml.x == -INFINITY) continue;
       const float f = ex2(ml.x - mm);
@@ -585,34 +602,57 @@ static int launch_rows(const Params& p, int wm, cudaStream_t s) {
 struct Plan {
   bool many;           // the tcgen05 kernel
   int wm;              // few-row kernel: 16-row groups a CTA
-  int64_t row_blocks;  // row blocks (tiles) of a segment and KV head
-  int nsplit;
+  int64_t row_blocks;  // row blocks (tiles) of the longest segment, a KV head
+  int64_t tiles;       // many rows: row tiles in the grid, a KV head
+  bool picked;
+  int nsplit, split_keys;
 };
 constexpr int SMS = 148;
 constexpr int MAX_SPLIT = 64;
 constexpr int FEW_ROWS = 64;
-constexpr int MIN_KEYS_A_SPLIT = 128;       // few rows: two tiles
-constexpr int MIN_KEYS_A_SPLIT_MANY = 512;  // many rows: four or eight blocks
-static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t hkv, int64_t group, int64_t d) {
+// Few rows: a part costs little (16 to 64 rows of float32) and ragged contexts need many to spread over the
+// SMs.  Measured, 64 one-token segments of 500 to 8192 positions, e4m3: 98 us with 2 CTAs an SM, 80 with 4,
+// 75 with 8, 73 with 16; parts below 256 keys gain nothing more.
+constexpr int FEW_CTAS_AN_SM = 16;
+constexpr int MIN_SPLIT_KEYS_FEW = 256;
+// Many rows: a part costs its rows in float32 twice, about as much as 250 keys of work, and a CTA's start
+// about 10 us.  Measured, eight segments of 100 to 700 tokens behind 600 to 6902 positions, e4m3: 164 us
+// unsplit, 140 aiming at two CTAs an SM, 155 at three; 48 segments of 9 to 70 tokens behind 1490, bf16:
+// 59 us unsplit, 66 in two parts of 896 keys.
+constexpr int MIN_SPLIT_KEYS_MANY = 2048;
+static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
+                      int64_t group, int64_t d) {
   Plan r = {};
   const int64_t rows = max_seqlen * group;
-  int64_t split, most;
+  int64_t split, least;
   r.many = rows > FEW_ROWS && group <= 128;
   if (r.many) {
-    const int64_t tokens = (d == 128 ? 2 : 1) * (128 / group);  // of a CTA
-    r.row_blocks = (max_seqlen + tokens - 1) / tokens;
-    split = SMS / (num_segments * hkv * r.row_blocks);
-    most = max_kv / MIN_KEYS_A_SPLIT_MANY;
+    const int64_t per = (d == 128 ? 2 : 1) * (128 / group);  // tokens a CTA
+    r.row_blocks = (max_seqlen + per - 1) / per;
+    // CTAs that have work: from the tokens, half a tile more a segment, not from the longest segment
+    int64_t ctas = hkv * (tokens / per + (num_segments + 1) / 2);
+    if (ctas > num_segments * hkv * r.row_blocks) ctas = num_segments * hkv * r.row_blocks;
+    // row tiles that can exist; few segments are sorted on the device (see pick_tile)
+    r.picked = num_segments <= 64 && tokens < 1 << 24;
+    r.tiles = num_segments * r.row_blocks;
+    if (r.picked && tokens / per + num_segments < r.tiles) r.tiles = tokens / per + num_segments;
+    split = (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1);
+    least = MIN_SPLIT_KEYS_MANY;
   } else {
     r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     r.row_blocks = (rows + 16 * r.wm - 1) / (16 * r.wm);
     const int64_t ctas = num_segments * hkv * (r.row_blocks > 0 ? r.row_blocks : 1);
-    split = (2 * SMS + ctas - 1) / ctas;
-    most = (max_kv + MIN_KEYS_A_SPLIT - 1) / MIN_KEYS_A_SPLIT;
+    split = (FEW_CTAS_AN_SM * SMS + ctas - 1) / ctas;
+    least = MIN_SPLIT_KEYS_FEW;
   }
-  if (split > most) split = most;
   if (split > MAX_SPLIT) split = MAX_SPLIT;
-  r.nsplit = split < 1 ? 1 : (int)split;
+  if (split < 1) split = 1;
+  int64_t keys = (max_kv + split - 1) / split;
+  if (keys < least) keys = least;
+  keys = (keys + 127) / 128 * 128;
+  r.split_keys = (int)keys;
+  r.nsplit = (int)((max_kv + keys - 1) / keys);
+  if (r.nsplit < 1) r.nsplit = 1;
   return r;
 }
 
@@ -643,14 +683,14 @@ using namespace fdk;
 static bool sizes_ok(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len, int64_t tokens, int64_t hq,
                      int64_t hkv, int64_t head_dim) {
   return num_segments >= 1 && num_segments <= 0x7ffffffe && max_seqlen >= 0 && max_seqlen <= 0x7fffffff &&
-         max_kv_len >= 0 && tokens >= 0 && tokens <= 0x7fffffff && hkv >= 1 && hq >= 1 && hq <= 4096 &&
+         max_kv_len >= 0 && max_kv_len <= 0x7fffff00 && tokens >= 0 && tokens <= 0x7fffffff && hkv >= 1 && hq >= 1 && hq <= 4096 &&
          hq % hkv == 0 && (head_dim == 128 || head_dim == 256);
 }
 
 extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
                                                int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
-  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv, head_dim);
+  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim);
   return pl.nsplit > 1 ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
 }
 
@@ -697,9 +737,8 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       ld_kpage * esz % 16 || ld_vpage * esz % 16 || (gate && (!aligned16(gate) || ld_gate % 8)) ||
       (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
-  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, hkv, hq / hkv, head_dim);
-  if (max_seqlen * (hq / hkv) > 0x7fffffff || num_segments * hkv * (pl.many ? 1 : pl.row_blocks) > 0x7fffffff ||
-      (pl.many && pl.row_blocks > 65535))
+  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim);
+  if (max_seqlen * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.tiles : num_segments * pl.row_blocks) > 0x7fffffff)
     return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
   Params p = {};
   p.q = static_cast<const bf16*>(q); p.ld_q = ld_q;
@@ -710,7 +749,8 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.table = page_table; p.ld_table = ld_table; p.cu = cu_seqlens; p.kv_lens = kv_lens;
   p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
-  p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks;
+  p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks; p.split_keys = pl.split_keys;
+  p.picked = pl.picked;
   p.sl2 = scale * 1.4426950408889634f;
   p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
   p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);
@@ -727,9 +767,9 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   int st;
   if (pl.many) {
     if (head_dim == 128)
-      st = quant ? chunk::launch<128, true>(p, pl.row_blocks, s) : chunk::launch<128, false>(p, pl.row_blocks, s);
+      st = quant ? chunk::launch<128, true>(p, pl.tiles, s) : chunk::launch<128, false>(p, pl.tiles, s);
     else
-      st = quant ? chunk::launch<256, true>(p, pl.row_blocks, s) : chunk::launch<256, false>(p, pl.row_blocks, s);
+      st = quant ? chunk::launch<256, true>(p, pl.tiles, s) : chunk::launch<256, false>(p, pl.tiles, s);
   } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.wm, s) : launch_rows<128, false>(p, pl.wm, s);
   else st = quant ? launch_rows<256, true>(p, pl.wm, s) : launch_rows<256, false>(p, pl.wm, s);
   if (st || pl.nsplit == 1) return st;

@@ -98,6 +98,11 @@ __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N>
@@ -107,6 +112,78 @@ __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.al
 template <uint32_t BOX>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)(c >> 3) * BOX + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) * 16);
+}
+
+// The `rank`-th longest row tile of the call (a warp's work): tiles of all segments in descending order of
+// the keys they see, so that the grid starts with the longest and the launched tiles are the ones that
+// exist.  Tile rb of a segment sees kend(rb) = past + min((rb + 1) tokens, n) keys; the number of tiles with
+// at least L keys has a closed form a segment, so L is found by bisection with the segments spread over
+// the lanes.  False when there are no more than `rank` tiles.  At most 32 * PICK segments.
+constexpr int PICK = 2;
+struct Unit {
+  int s, rb;
+};
+__device__ __forceinline__ bool pick_tile(const Params& p, int tokens, int rank, int lane, Unit& u) {
+  int past[PICK], n[PICK], tiles[PICK], most = 0;
+  // x / tokens as a multiplication, exact for x < 2^32 / tokens: here x < 2^24 (the host's rule)
+  const uint32_t inv = 0xffffffffu / (uint32_t)tokens + 1u;
+  auto div_up = [&](int x) { return (int)__umulhi((uint32_t)(x + tokens - 1), inv); };
+#pragma unroll
+  for (int i = 0; i < PICK; ++i) {
+    const int s = lane * PICK + i;
+    n[i] = past[i] = tiles[i] = 0;
+    if (s < p.nseg) {
+      const Seg g = segment(p, s, false);
+      n[i] = g.n;
+      past[i] = (int)g.past;
+      tiles[i] = div_up(g.n);
+      most = max(most, past[i] + n[i]);
+    }
+  }
+  auto count1 = [&](int i, int L) {  // tiles of the lane's segment i that see at least L keys
+    if (L <= 0) return tiles[i];
+    if (tiles[i] == 0 || past[i] + n[i] < L) return 0;
+    const int need = max(min(L - past[i], n[i]), 1);  // the first tile with (rb + 1) tokens >= need
+    return tiles[i] - div_up(need) + 1;
+  };
+  auto count = [&](int L) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < PICK; ++i) c += count1(i, L);
+    return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+  };
+  if (count(0) <= rank) return false;
+  int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1;  // count(lo) > rank >= count(hi)
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (count(mid) > rank) lo = mid;
+    else hi = mid;
+  }
+  // of the tiles with exactly lo keys, in segment order
+  int skip = rank - count(lo + 1), mine = 0, eq[PICK];
+#pragma unroll
+  for (int i = 0; i < PICK; ++i) mine += eq[i] = count1(i, lo) - count1(i, lo + 1);
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  skip -= before - mine;
+  int found = -1, rb = 0;
+#pragma unroll
+  for (int i = 0; i < PICK; ++i) {
+    if (found < 0 && skip >= 0 && skip < eq[i]) {
+      found = lane * PICK + i;
+      rb = tiles[i] - count1(i, lo) + skip;
+    }
+    skip -= eq[i];
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, found >= 0);
+  const int src = __ffs(who) - 1;
+  u.s = __shfl_sync(0xffffffffu, found, src);
+  u.rb = __shfl_sync(0xffffffffu, rb, src);
+  return true;
 }
 
 template <int D, bool QUANT>
@@ -131,27 +208,51 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   uint32_t* factor = reinterpret_cast<uint32_t*>(gbase + M::OFF_FT);                   // [2][BN] half2
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // grid: x = (segment, KV head) with the head fastest, y = row tile from the last one down (the longest
-  // key ranges first), z = split of the keys
-  const int s = (int)(blockIdx.x / (unsigned)p.hkv), hk = (int)(blockIdx.x % (unsigned)p.hkv);
-  const int rb = (int)gridDim.y - 1 - (int)blockIdx.y;
-  const int split = (int)blockIdx.z;
-  const bool first = hk == 0 && rb == 0 && split == 0;
-  const Seg seg = segment(p, s, tid == 0 && first);
   const int tpt = 128 / p.group;                 // tokens a tile
   const int rpt = tpt * p.group;                 // rows of it in use
+  // grid: x = (row tiles of all segments, KV head) with the head fastest, y = split of the keys from the
+  // last one (only long ranges have it: short tiles come at the end).  With few
+  // segments the tiles are taken longest first (short calls end on their longest CTA, and only the device
+  // knows the lengths); with many, x counts each segment's tiles up to the longest one's number, from
+  // the last tile down.
+  const int hk = (int)(blockIdx.x % (unsigned)p.hkv), item = (int)(blockIdx.x / (unsigned)p.hkv);
+  const int split = p.nsplit - 1 - (int)blockIdx.y;
+  int s, rb;
+  if (p.picked) {
+    int* pick = reinterpret_cast<int*>(gbase + M::OFF_MISC + 48);
+    if (warp == 0) {
+      Unit u = {-1, 0};
+      const bool some = pick_tile(p, NT * tpt, item, lane, u);
+      if (lane == 0) {
+        pick[0] = some ? u.s : -1;
+        pick[1] = u.rb;
+      }
+    }
+    __syncthreads();
+    s = pick[0];
+    rb = pick[1];
+  } else {
+    s = item % p.nseg;
+    rb = p.row_blocks - 1 - item / p.nseg;
+  }
+  if (item == 0 && hk == 0 && split == 0) {  // one CTA reports what is wrong with the segments
+    for (int i = tid; i < p.nseg; i += R::THREADS)
+      if (segment(p, i, true).n > p.row_blocks * NT * tpt) atomicOr(&g_error, 1);
+  }
+  if (s < 0) return;
+  const Seg seg = segment(p, s, false);
   const int rows = seg.n * p.group;
   const int tok0 = rb * NT * tpt;                // first token of the CTA
-  if (tid == 0 && first && seg.n > (int)gridDim.y * NT * tpt) atomicOr(&g_error, 1);
   if (tok0 >= seg.n) return;
   const int last_tok = min(tok0 + NT * tpt, seg.n) - 1;
   const int64_t kend64 = seg.past + last_tok + 1;
   const int kend = kend64 > 0 ? (int)kend64 : 0;
   const int kv_len = (int)(seg.past + seg.n);
-  const int per = ((kend + p.nsplit * BN - 1) / (p.nsplit * BN)) * BN;
-  const int kb = min(kend, split * per), ke = min(kend, kb + per);
+  int kb, ke;
+  split_range(p, split, kend, kb, ke);
+  if (kb >= ke && split > 0) return;  // the join does not read this part
   const int n_kv = (ke - kb + BN - 1) / BN;
-  if (n_kv == 0) {  // nothing to see: zeros, or an empty part
+  if (n_kv == 0) {  // no keys at all: zeros, or an empty part
     for (int e = tid; e < NT * rpt; e += R::THREADS) {
       const int64_t gr = (int64_t)tok0 * p.group + e;
       if (gr >= rows) break;
@@ -171,7 +272,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;
       if (i == B_P || i == B_P + 1) count = 128;
-      if (QUANT && (i == B_Q || (i >= B_F && i < B_F + 4) || (i >= B_RE && i < B_RE + 4))) count = 128;
+      if (QUANT && i == B_Q) count = two ? 256 : 128;
+      if (QUANT && ((i >= B_F && i < B_F + 4) || (i >= B_RE && i < B_RE + 4))) count = 128;
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -194,7 +296,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     constexpr int RING = QUANT ? RAW_SLOTS : M::SLOTS;
     constexpr int FULL = QUANT ? B_RF : B_F, EMPTY = QUANT ? B_RE : B_E;
     constexpr uint32_t BYTES = QUANT ? M::RAWT : G::KT;
-    // a block's boxes: keys in pages of 2^page_shift, at most BN a box; lane i issues box i, i + 32, ..
+    // a block's boxes: keys in pages of 2^page_shift, at most BN a box
     const int box_keys = min(BN, 1 << p.page_shift);
     constexpr int COLS = QUANT ? 1 : NBX;  // boxes across a row: the raw row, or 64 bf16 columns each
     const int boxes = (BN / box_keys) * COLS;
@@ -210,8 +312,16 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
                         seg.begin + tok0 + i * tpt);
       }
     }
+    // at most 16 boxes: lane b issues box b.  Its page id is loaded a block ahead.
+    const int sub = lane / COLS, col = lane % COLS;
+    auto page_of = [&](int j) { return __ldg(table + (min(kb + j * BN + sub * box_keys, ke - 1) >> p.page_shift)); };
+    int id = 0, id_next = page_of(0);
     int issued = 0;
     for (int i = 0; i < 2 * n_kv; ++i) {
+      if ((i & 1) == 0) {
+        id = id_next;
+        id_next = page_of((i >> 1) + 1);
+      }
       const int slot = i % RING;
       if (i >= RING &&
           !__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + slot), (uint32_t)(i / RING - 1) & 1u, abort_flag) ? 1 : 0))
@@ -224,12 +334,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       const uint32_t dst = base + (QUANT ? M::OFF_RAW + slot * M::RAWT : M::OFF_KV + slot * G::KT);
       if (lane == 0) mbar_expect_tx(fb, BYTES);
       __syncwarp();
-      for (int b = lane; b < boxes; b += 32) {
-        const int sub = b / COLS, col = b % COLS;
+      if (lane < boxes) {
         const int key = key0 + sub * box_keys;
         int page = (int)p.num_pages;  // out of range: zeros
         if (key < ke) {
-          const int id = __ldg(table + (key >> p.page_shift));
           if (id >= 0 && id < p.num_pages) page = id;
           else atomicOr(&g_error, 1);
         }
@@ -390,40 +498,16 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       ek = max(ek, warp_max[2 * i]);
       ev = max(ev, warp_max[2 * i + 1]);
     }
-    if (ct == 0) {
+    if (ct == 0) {  // the softmax reads them behind the first S, the epilogue later still
       scale_max[0] = ek;
       scale_max[1] = ev;
     }
-    // q: a row a thread, fp16 with its largest magnitude in [1, 2)
-    for (int i = 0; i < (two ? 2 : 1); ++i) {
-      const int tok = tok0 + i * tpt + ct / p.group;
-      const bool live = ct < rpt && tok < seg.n;
-      const bf16* src = p.q + (int64_t)(seg.begin + (live ? tok : 0)) * p.ld_q + (int64_t)(hk * p.group + (live ? ct % p.group : 0)) * D;
-      float a = 0.f;
-      for (int c = 0; c < D / 8; ++c) {
-        float f[8];
-        unpack8(live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u), f);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) a = fmaxf(a, fabsf(f[u]));
-      }
-      const int e = a == 0.f ? 127 : min(max((int)(__float_as_uint(a) >> 23), 1), 253);
-      const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-      q_exp[i * 128 + ct] = (uint8_t)e;  // q's row is fp16 * 2^(e - 127)
-      for (int c = 0; c < D / 8; ++c) {
-        float f[8];
-        unpack8(live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u), f);
-        const uint4 h = make_uint4(pack_f16x2(f[0] * inv, f[1] * inv), pack_f16x2(f[2] * inv, f[3] * inv),
-                                   pack_f16x2(f[4] * inv, f[5] * inv), pack_f16x2(f[6] * inv, f[7] * inv));
-        *reinterpret_cast<uint4*>(gbase + M::OFF_Q + i * G::QT + chunk_at<G::QBOX>(ct, c)) = h;
-      }
-    }
-    fence_proxy_async_smem();
-    mbar_arrive(bar(B_Q));
+    constexpr int TPR = D / 8, RPP = 128 / TPR;  // threads a row, rows a pass (of 128 threads)
+    const int lc = ct % TPR, lr = ct / TPR;
     // Items: thread ct is row ct's keeper (its scale byte, loaded a block ahead) and, for the conversion,
     // piece lc (8 columns) of rows lr, lr + RPP, ..: 8 raw bytes become one 16-byte operand chunk.  Eight
     // neighbouring threads read 64 consecutive bytes and store all eight chunk positions: no conflicts.
-    constexpr int TPR = D / 8, RPP = 128 / TPR, PASSES = BN / RPP;
-    const int lc = ct % TPR, lr = ct / TPR;
+    constexpr int PASSES = BN / RPP;
     const int my = ct < BN ? ct : 0;
     auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
     auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
@@ -491,7 +575,41 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     bool ok = tile == 0 || two;
     float sl2 = p.sl2;
     if (QUANT && ok) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_Q), 0, abort_flag) ? 1 : 0);
+      // this tile's q: D / 8 threads a row, fp16 with the row's largest magnitude in [1, 2)
+      constexpr int TPR = D / 8, RPP = 128 / TPR;
+      const int ct = tid & 127, lc = ct % TPR, lr = ct / TPR;
+      const int inv_group = 65536 / p.group + 1;  // x / group == x * inv_group >> 16 for x < 128
+#pragma unroll 1
+      for (int r0 = lr; r0 < 128; r0 += 8 * RPP) {
+        uint4 w[8];  // eight rows' loads in flight, from a valid row where there is none
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int r = r0 + u * RPP, dt = r * inv_group >> 16, t = tok0 + tile * tpt + dt;
+          const bool live = r < rpt && t < seg.n;
+          w[u] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)(seg.begin + (live ? t : 0)) * p.ld_q +
+                                                      (int64_t)(hk * p.group + (live ? r - dt * p.group : 0)) * D + lc * 8));
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int r = r0 + u * RPP;
+          float f[8], a = 0.f;
+          unpack8(w[u], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
+#pragma unroll
+          for (int o = TPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+          const int e = a == 0.f ? 127 : min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+          const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+          if (lc == 0) q_exp[tile * 128 + r] = (uint8_t)e;  // q's row is fp16 * 2^(e - 127)
+          *reinterpret_cast<uint4*>(gbase + M::OFF_Q + tile * G::QT + chunk_at<G::QBOX>(r, lc)) =
+              make_uint4(pack_f16x2(f[0] * inv, f[1] * inv), pack_f16x2(f[2] * inv, f[3] * inv),
+                         pack_f16x2(f[4] * inv, f[5] * inv), pack_f16x2(f[6] * inv, f[7] * inv));
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bar(B_Q));
+      // S of the first block follows every thread's q and the scale maxima
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_S + (NT == 2 ? tile : 0)), 0, abort_flag) ? 1 : 0);
       // never 0: a masked score is -inf * sl2
       if (ok) sl2 = fmaxf(sl2 * scale_value(q_exp[tile * 128 + row]) * scale_value(scale_max[0]), 1e-37f);
     }
@@ -519,13 +637,11 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       }
       float mx8[8];
 #pragma unroll
-      for (int a = 0; a < 8; ++a) mx8[a] = -INFINITY;
+      for (int a = 0; a < 8; ++a) mx8[a] = __uint_as_float(sr[0][a]);
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) mx8[i & 7] = fmaxf(mx8[i & 7], __uint_as_float(sr[c][i]));
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+      for (int i = 8; i < BN; i += 2)  // three-operand maximum, eight chains
+        mx8[(i >> 1) & 7] = max3(mx8[(i >> 1) & 7], __uint_as_float(sr[i >> 5][i & 31]), __uint_as_float(sr[(i + 1) >> 5][(i + 1) & 31]));
+      const float mx = fmaxf(max3(mx8[0], mx8[1], mx8[2]), max3(max3(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
       float alpha = 1.f;
       bool rescale = false;
       if (j == 0) {
@@ -538,29 +654,34 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       // a row that has seen nothing yet: every exponent below is -inf
       const float r0 = r_run == -INFINITY ? 0.f : r_run;
       const float shift = r0 * sl2 - (QUANT ? P_SHIFT : 0.f);
-      float sum8[8];
+      float2 sum4[4];  // packed float32: two columns an operation
 #pragma unroll
-      for (int a = 0; a < 8; ++a) sum8[a] = 0.f;
+      for (int a = 0; a < 4; ++a) sum4[a] = make_float2(0.f, 0.f);
       uint32_t pk[BN / 64][32];
       auto weights = [&](auto expo) {
 #pragma unroll
         for (int c = 0; c < BN / 2; ++c) {
-          const float e0 = ex2(expo(__uint_as_float(sr[(2 * c) >> 5][(2 * c) & 31])));
-          const float e1 = ex2(expo(__uint_as_float(sr[(2 * c + 1) >> 5][(2 * c + 1) & 31])));
-          sum8[(2 * c) & 7] += e0;
-          sum8[(2 * c + 1) & 7] += e1;
-          pk[c >> 5][c & 31] = QUANT ? pack_f16x2(e0, e1) : pack_bf16x2(e0, e1);
+          const float2 x = expo(make_float2(__uint_as_float(sr[(2 * c) >> 5][(2 * c) & 31]),
+                                            __uint_as_float(sr[(2 * c + 1) >> 5][(2 * c + 1) & 31])));
+          const float2 e = make_float2(ex2(x.x), ex2(x.y));
+          sum4[c & 3] = __fadd2_rn(sum4[c & 3], e);
+          pk[c >> 5][c & 31] = QUANT ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
         }
       };
+      const float2 sl2v = make_float2(sl2, sl2);
       // s * sl2 - shift in one operation, unless scores are so large that shift's own rounding (float32
       // spacing 0.25 and more) would show in the exponent
       if (!__any_sync(0xffffffffu, fabsf(shift) > 2097152.f))
-        weights([&](float x) { return fmaf(x, sl2, -shift); });
+        weights([&](float2 x) { return __ffma2_rn(x, sl2v, make_float2(-shift, -shift)); });
       else
-        weights([&](float x) { return fmaf(x - r0, sl2, QUANT ? P_SHIFT : 0.f); });
+        weights([&](float2 x) {
+          const float up = QUANT ? P_SHIFT : 0.f;
+          return __ffma2_rn(make_float2(x.x - r0, x.y - r0), sl2v, make_float2(up, up));
+        });
 #pragma unroll
       for (int c = 0; c < BN / 64; ++c) tmem_st32(tS + c * 32, pk[c]);
-      const float sum = ((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7]));
+      const float2 sum2 = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
+      const float sum = sum2.x + sum2.y;
       l_run = l_run * alpha + sum;
       if (__any_sync(0xffffffffu, rescale)) {  // O row *= alpha
         // NT == 2: S_j's commit covers PV(j-1) of this tile; NT == 1: it covers PV(j-2), so wait for PV(j-1)
@@ -597,8 +718,21 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       if (part && valid) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(r_run * sl2, l_run);
       bf16* orow = p.out + idx * D;
       const bf16* grow = p.gate ? p.gate + tk_ * p.ld_gate + (int64_t)head * p.gate_hstride : nullptr;
+      uint4 gate_next[4];  // the gate's next 32 columns, loaded a step ahead
+      const bool gated = grow != nullptr && valid && !part;
+      if (gated) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gate_next[i] = ldg_stream(grow + i * 8);
+      }
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
+        uint4 gate_now[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gate_now[i] = gate_next[i];
+        if (gated && c + 1 < D / 32) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) gate_next[i] = ldg_stream(grow + (c + 1) * 32 + i * 8);
+        }
         uint32_t o[32];
         tmem_ld32(tO + c * 32, o);
         tmem_ld_wait();
@@ -614,9 +748,9 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(o[v8 * 8 + i]) * inv;
-            if (grow) {
+            if (gated) {
               float gv[8];
-              unpack8(*reinterpret_cast<const uint4*>(grow + c * 32 + v8 * 8), gv);
+              unpack8(gate_now[v8], gv);
 #pragma unroll
               for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
             }
@@ -684,7 +818,7 @@ static int launch(const Params& p, int64_t row_tiles, cudaStream_t s) {
   constexpr uint32_t bytes = Smem<D, QUANT>::BYTES;
   const void* fn = (const void*)many_rows_kernel<D, QUANT>;
   if (int st = ensure_smem_attr(fn, (int)bytes, "paged_gqa")) return st;
-  const dim3 grid((unsigned)((int64_t)p.nseg * p.hkv), (unsigned)row_tiles, (unsigned)p.nsplit);
+  const dim3 grid((unsigned)(row_tiles * p.hkv), (unsigned)p.nsplit);
   many_rows_kernel<D, QUANT><<<grid, Roles<D, QUANT>::THREADS, bytes, s>>>(mq, mk, mv, p);
   return check_launch("paged_gqa (many rows)");
 }

@@ -857,7 +857,8 @@ def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     max_seqlen = min(int(max_seqlen), T)
     if max_seqlen < 0:
         raise ValueError("paged_gqa_attention: max_seqlen must not be negative")
-    max_kv_len = page_table.shape[1] * page_size if max_kv_len is None else int(max_kv_len)
+    reach = page_table.shape[1] * page_size
+    max_kv_len = reach if max_kv_len is None else min(int(max_kv_len), reach)
     if max_kv_len < 0:
         raise ValueError("paged_gqa_attention: max_kv_len must not be negative")
     if workspace is None:
