@@ -6,18 +6,22 @@
 // group + head), so every cached row brought into shared memory feeds them all.
 //
 // Calls with more than 64 rows a KV head run the tcgen05 kernel of paged_attention_chunk.cuh.  This file:
-// the few-row kernel (mma.sync tiles of 16 rows, split over the keys) and the join of splits.  Its work
-// is bound by reading the cache: at one token a sequence each cached byte is used by `group`
-// rows only, far below the tensor cores' rate, so the 16-row warp-level MMA -- which needs no padding to
-// 128 rows and keeps S and P in registers -- loses nothing to the memory time it hides behind.
+// the few-row kernel (mma.sync, split over the keys) and the join of splits.  Its work is bound by
+// reading the cache: at one token a sequence each cached byte is used by `group` rows only, far below the
+// tensor cores' rate, so warp-level MMAs -- which need no padding to 128 rows and keep S and P in
+// registers -- lose nothing to the memory time they hide behind.  What competes with the loads is
+// instruction issue, so the products are transposed: S^T = K Q^T and O^T = V^T P^T put 16 keys (columns
+// of V) on the MMA's 16-row side and the query rows on its 8-column side.  Four rows then waste half an
+// MMA instead of three quarters, and each K / V fragment is converted from e4m3 once for all rows.
 //
-//   CTA: BM = 16 WM rows of one (segment, KV head), keys [k0, k1) in tiles of 64; 4 warps = WM row
+//   CTA: BM = 8 NR WM rows of one (segment, KV head), keys [kb, ke) in tiles of 64; 4 warps = WM row
 //   groups x WK = 4 / WM key groups.  Tiles stream through a ring of cp.async stages.  Each warp keeps
-//   its own running maximum, sum and O (fp32) over its keys; key groups are joined through shared memory
-//   at the end, splits through a float32 workspace by the second kernel.
-//   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S's column, V's
-//   multiplies P's column before its rounding to fp16, relative to the largest V scale so far (O is
-//   rescaled when that grows, as for the maximum).  q is brought to fp16 with a power of two a row.
+//   its own running maximum (raised only when a score exceeds it by more than 2^8, so most tiles
+//   need no reduction across lanes), sum and O (fp32) over its keys; key groups are joined through
+//   shared memory at the end, splits through a float32 workspace by the second kernel.
+//   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S, V's multiplies
+//   P before its rounding to fp16, relative to the largest V scale so far (O is rescaled when that grows,
+//   as for the maximum).  q is brought to fp16 with a power of two a row.
 #include <math.h>
 
 #include "paged.cuh"
@@ -113,6 +117,9 @@ __device__ __forceinline__ void check_page_ids(const Params& p, int (&id)[N]) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
@@ -150,8 +157,7 @@ struct Geo {
   static constexpr int CH = ROW / 16;             // 16-byte chunks of it
   static constexpr int TILE = BN * ROW;
   static constexpr int STAGE = 2 * TILE + (QUANT ? 2 * BN : 0);
-  // stages in flight and CTAs an SM: about 100 KB of loads in flight an SM in every form
-  static constexpr int STAGES = QUANT ? (D == 128 ? 4 : 3) : 3;
+  static constexpr int STAGES = 3;                // 50 KB (e4m3, head_dim 128) to 192 KB (bf16, 256) a CTA
   static constexpr int RING = STAGES * STAGE;
 };
 
@@ -160,13 +166,26 @@ struct Geo {
 template <int CH>
 __device__ __forceinline__ uint32_t tile_at(int r, int c) { return (uint32_t)((r * CH + (c ^ (r & 7))) * 16); }
 
-template <int D, bool QUANT, int WM>
+// 2^(b - 127), with 0 for b <= 0
+__device__ __forceinline__ float pow2_byte(int b) { return __int_as_float(max(b, 0) << 23); }
+
+// transpose of an 8x8 matrix of 16-bit elements held two a lane
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
+  return r;
+}
+
+constexpr float GROW = 8.f;     // the running maximum lags by at most 2^GROW
+constexpr int V_SHIFT = 6;      // fp16 P: times 2^V_SHIFT; at most 2^(GROW + V_SHIFT), weights down to 2^-30 stay
+
+template <int D, bool QUANT, int WM, int NR>
 __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   using G = Geo<D, QUANT>;
   constexpr int WK = 4 / WM;        // key groups
   constexpr int KPW = BN / WK;      // keys a warp and tile
-  constexpr int NT = KPW / 8;       // 8-key column tiles of S
-  constexpr int BM = 16 * WM;
+  constexpr int BM = 8 * NR * WM;
+  constexpr int KK = D / 16;        // 16-column steps of D
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -178,10 +197,11 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int srb = (int)(blockIdx.x / (unsigned)p.hkv);
   const int s = srb / p.row_blocks, rb = srb % p.row_blocks;
   const int split = blockIdx.y;
-  const Seg seg = segment(p, s, tid == 0 && hk == 0 && rb == 0 && split == 0);
+  const bool first = tid == 0 && hk == 0 && rb == 0 && split == 0;
+  const Seg seg = segment(p, s, first);
   const int rows = seg.n * p.group;
   const int row0 = rb * BM;
-  if (tid == 0 && hk == 0 && rb == 0 && split == 0 && rows > p.row_blocks * BM) atomicOr(&g_error, 1);
+  if (first && rows > p.row_blocks * BM) atomicOr(&g_error, 1);
   if (row0 >= rows) return;
   const int last_tok = (min(row0 + BM, rows) - 1) / p.group;
   const int64_t kend64 = seg.past + last_tok + 1;
@@ -191,86 +211,40 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   if (kb >= ke && split > 0) return;  // the join does not read this part
   const int ntiles = (ke - kb + BN - 1) / BN;
 
-  // this lane's two rows (g and g + 8 of the warp's 16)
-  int rr[2], lim[2];
-  int64_t qrow[2];
-  bool live[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    rr[i] = row0 + wm * 16 + g + 8 * i;
-    live[i] = rr[i] < rows;
-    const int tok = live[i] ? rr[i] / p.group : 0;
-    const int head = hk * p.group + (live[i] ? rr[i] % p.group : 0);
-    lim[i] = live[i] ? (int)(seg.past + tok) : -1;   // last visible key
-    qrow[i] = (int64_t)(seg.begin + tok) * p.hq + head;
-  }
-
-  // Q fragments.  bf16: columns 2t, 2t+1 (+8) of each 16; 8-bit cache: columns 4t .. 4t+3 of each 16, in
-  // the order the byte-wise K fragments come in, as fp16 scaled by a power of two a row.
-  uint32_t qf[D / 16][4];
-  float qs[2] = {p.sl2, p.sl2};
-  if (!QUANT) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bf16* src = p.q + (qrow[i] / p.hq) * p.ld_q + (qrow[i] % p.hq) * D;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        qf[kk][i] = live[i] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 2 * t4) : 0u;
-        qf[kk][2 + i] = live[i] ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + 2 * t4) : 0u;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bf16* src = p.q + (qrow[i] / p.hq) * p.ld_q + (qrow[i] % p.hq) * D;
-      uint2 raw[D / 16];
-      float a = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        raw[kk] = live[i] ? *reinterpret_cast<const uint2*>(src + kk * 16 + 4 * t4) : make_uint2(0u, 0u);
-        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].x));
-        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].y));
-        a = fmaxf(fmaxf(a, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
-      }
-      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-      // the row's largest magnitude goes to [1, 2): fp16 keeps bf16's 8 bits down to 2^-14 of it
-      const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
-      const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-      qs[i] = p.sl2 * __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].x));
-        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[kk].y));
-        qf[kk][i] = pack_f16x2(x.x * inv, x.y * inv);
-        qf[kk][2 + i] = pack_f16x2(y.x * inv, y.y * inv);
-      }
-    }
-  }
-
-  // tile loads: chunk tid % CH of rows tid / CH + j * (128 / CH)
-  constexpr int RPP = THREADS / G::CH;   // rows a pass
-  constexpr int PASSES = BN / RPP;
+  // tile loads: chunk lc of rows lr + i * RPP; the rows of a pass lie in one group of 16 keys
+  constexpr int RPP = THREADS / G::CH, PASSES = BN / RPP, GROUPS = BN / 16;
   const int lc = tid % G::CH, lr = tid / G::CH;
   const int32_t* table = p.table + (int64_t)s * p.ld_table;
   const int page_mask = (1 << p.page_shift) - 1;
-  int ids[BN / 16];  // of the next tile to load
+  const int64_t head_at = (int64_t)(hk << p.page_shift) * G::ROW + lr * G::ROW + lc * 16;
+  int ids[GROUPS];  // of the next tile to load
   if (ntiles > 0) load_page_ids(p, table, kb, ke - 1, ids);
   auto load_tile = [&](int j) {
     const int key0 = kb + j * BN;
     const uint32_t dst = sbase + (uint32_t)(j % G::STAGES) * G::STAGE;
     check_page_ids(p, ids);
+    bool whole = key0 + BN <= ke;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = lr + i * RPP;
-      const int id = ids[i * RPP / 16];
-      const bool ok = id >= 0 && key0 + r < ke;
-      const int64_t pg = ok ? id : 0;
-      const int at = ((hk << p.page_shift) + ((key0 + r) & page_mask)) * G::ROW + lc * 16;
-      const uint32_t bytes = ok ? 16u : 0u;   // rows past the range are zero-filled
-      const uint32_t to = dst + tile_at<G::CH>(r, lc);
-      cp_async16(to, p.k_cache + (pg * p.kpage + at), bytes);
-      cp_async16(to + G::TILE, p.v_cache + (pg * p.vpage + at), bytes);
+    for (int u = 0; u < GROUPS; ++u) whole = whole && ids[u] >= 0;
+#pragma unroll
+    for (int u = 0; u < GROUPS; ++u) {
+      const int64_t pg = ids[u] >= 0 ? ids[u] : 0;
+      const int64_t at = head_at + ((key0 + 16 * u) & page_mask) * G::ROW;
+      const uint8_t* ks = p.k_cache + (pg * p.kpage + at);
+      const uint8_t* vs = p.v_cache + (pg * p.vpage + at);
+#pragma unroll
+      for (int i = 0; i < 16 / RPP; ++i) {
+        const int r = 16 * u + i * RPP;
+        const uint32_t to = dst + tile_at<G::CH>(lr + r, lc);
+        if (whole) {
+          cp_async16(to, ks + i * RPP * G::ROW);
+          cp_async16(to + G::TILE, vs + i * RPP * G::ROW);
+        } else {  // rows past the range or on a bad page are zero-filled
+          const uint32_t bytes = ids[u] >= 0 && key0 + lr + r < ke ? 16u : 0u;
+          cp_async16(to, ks + i * RPP * G::ROW, bytes);
+          cp_async16(to + G::TILE, vs + i * RPP * G::ROW, bytes);
+        }
+      }
     }
     if (QUANT && tid < 8) {  // scale bytes: 16 keys at a time
       const int u = tid & 3, r = u * 16;
@@ -283,163 +257,221 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     }
     load_page_ids(p, table, key0 + BN, ke - 1, ids);
   };
-
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  int ev = 0;  // O is in units of 2^(ev - 127) (8-bit cache)
-
 #pragma unroll
   for (int j = 0; j < G::STAGES - 1; ++j) {
     if (j < ntiles) load_tile(j);
     cp_commit();
   }
+
+  // B fragments of q: row 8 nr + g of this warp's rows.  bf16: columns 2t, 2t+1 (+8) of each 16; 8-bit
+  // cache: columns 4t .. 4t+3, in the order the byte-wise K fragments come in, as fp16 times a power of
+  // two a row.
+  uint32_t qf[NR][KK][2];
+  float qs[NR][2];   // of this lane's columns of S^T: rows 2t, 2t+1
+  int lim[NR][2];    // their last visible key
+  int wlim = 0x7fffffff;  // the smallest of the warp's live rows
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) {
+    const int base_row = row0 + (wm * NR + nr) * 8;
+    const int r = base_row + g;
+    const bool live = r < rows;
+    const int tok = live ? r / p.group : 0;
+    const bf16* src = p.q + (int64_t)(seg.begin + tok) * p.ld_q + (int64_t)(hk * p.group + (live ? r - tok * p.group : 0)) * D;
+    float unit = 1.f;
+    if (!QUANT) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        qf[nr][kk][0] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 2 * t4) : 0u;
+        qf[nr][kk][1] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + 2 * t4) : 0u;
+      }
+    } else {
+      float a = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const uint2 raw = live ? *reinterpret_cast<const uint2*>(src + kk * 16 + 4 * t4) : make_uint2(0u, 0u);
+        qf[nr][kk][0] = raw.x;
+        qf[nr][kk][1] = raw.y;
+        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+        a = fmaxf(fmaxf(a, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+      // the row's largest magnitude goes to [1, 2): fp16 keeps bf16's 8 bits down to 2^-14 of it
+      const int e = min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+      const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+      unit = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[nr][kk][u]));
+          qf[nr][kk][u] = pack_f16x2(x.x * inv, x.y * inv);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      qs[nr][u] = p.sl2 * (QUANT ? __shfl_sync(0xffffffffu, unit, (2 * t4 + u) * 4) : 1.f);
+      const int rr = base_row + 2 * t4 + u;
+      lim[nr][u] = rr < rows ? (int)(seg.past + rr / p.group) : -1;
+      wlim = min(wlim, rr < rows ? lim[nr][u] : 0x7fffffff);
+    }
+  }
+  wlim = min(__reduce_min_sync(0xffffffffu, wlim), ke - 1);  // every key up to here needs no mask
+
+  float o[KK][NR][4];  // O^T: columns (of D) down, rows across
+#pragma unroll
+  for (int i = 0; i < KK; ++i)
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[i][nr][c] = 0.f;
+  float m[NR][2], l[NR][2];
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[nr][u] = -INFINITY;
+      l[nr][u] = 0.f;
+    }
+  int ev = 0;  // O is in units of 2^(ev - 127) (8-bit cache)
+
   for (int j = 0; j < ntiles; ++j) {
     cp_wait<G::STAGES - 2>();
     __syncthreads();  // tile j is in, and every warp is done with the stage that tile j + STAGES - 1 takes
     if (j + G::STAGES - 1 < ntiles) load_tile(j + G::STAGES - 1);
     cp_commit();
     const uint32_t kt = sbase + (uint32_t)(j % G::STAGES) * G::STAGE, vt = kt + G::TILE;
-    const int krow = wk * KPW;  // first key of this warp in the tile
-    const int key0 = kb + j * BN + krow;
-
-    // S = Q K^T
-    float sc[NT][4];
+    const uint8_t* scales = smem + (kt - sbase) + 2 * G::TILE;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int kg = 0; kg < KPW / 16; ++kg) {
+      const int krow = wk * KPW + kg * 16;  // first of 16 keys in the tile
+      const int key0 = kb + j * BN + krow;
+      // S^T = K Q^T: element c of row tile nr is key g + 8 (c / 2), row 2 t + (c & 1)
+      float sc[NR][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sc[i][c] = 0.f;
-    if (!QUANT) {
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-        for (int i = 0; i < NT; i += 2) {  // 16 keys x 16 columns a load
-          uint32_t b[4];
-          ldsm4(b, kt + tile_at<G::CH>(krow + i * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
-          mma<false>(sc[i], qf[kk], b[0], b[1]);
-          mma<false>(sc[i + 1], qf[kk], b[2], b[3]);
-        }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < D / 16; kk += 2)
-#pragma unroll
-        for (int i = 0; i < NT; i += 2) {  // 16 keys x 32 columns a load
-          uint32_t b[4];
-          ldsm4(b, kt + tile_at<G::CH>(krow + i * 8 + (lane & 7) + ((lane >> 4) << 3), kk + ((lane >> 3) & 1)));
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            mma<true>(sc[i + (u >> 1)], qf[kk + (u & 1)], paged::e4m3x2_to_f16x2((uint16_t)b[u]),
-                      paged::e4m3x2_to_f16x2((uint16_t)(b[u] >> 16)));
-        }
-    }
-    // scale, mask, row maximum.  Element (i, c): row c / 2, key 8 i + 2 t4 + (c & 1).
-    float vs[NT][2];
-    int etile = 0;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      if (QUANT) {
-        const uint16_t kb2 = *reinterpret_cast<const uint16_t*>(smem + (kt - sbase) + 2 * G::TILE + krow + i * 8 + 2 * t4);
-        const uint16_t vb2 = *reinterpret_cast<const uint16_t*>(smem + (kt - sbase) + 2 * G::TILE + BN + krow + i * 8 + 2 * t4);
-        const float k0 = scale_value(kb2 & 255), k1 = scale_value(kb2 >> 8);
-        sc[i][0] *= k0 * qs[0];
-        sc[i][1] *= k1 * qs[0];
-        sc[i][2] *= k0 * qs[1];
-        sc[i][3] *= k1 * qs[1];
-        const int key = key0 + i * 8 + 2 * t4;
-        const int v0 = key < ke ? vb2 & 255 : 0, v1 = key + 1 < ke ? vb2 >> 8 : 0;
-        etile = max(etile, max(v0, v1));
-        vs[i][0] = __int_as_float(v0);
-        vs[i][1] = __int_as_float(v1);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sc[i][c] *= p.sl2;
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (key0 + i * 8 + 2 * t4 + (c & 1) > min(lim[c >> 1], ke - 1)) sc[i][c] = -INFINITY;
-    }
-    float corr[2], mu[2];
-    bool grow = false;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) mx = fmaxf(mx, fmaxf(sc[i][2 * r], sc[i][2 * r + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[r], mx);
-      mu[r] = mn == -INFINITY ? 0.f : mn;      // a row without keys so far: exp2(-inf - 0) = 0
-      corr[r] = mn > m[r] ? ex2(m[r] - mu[r]) : 1.f;
-      grow |= mn > m[r];
-      m[r] = mn;
-      l[r] *= corr[r];
-    }
-    float fv = 1.f;
-    if (QUANT) {
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) etile = max(etile, __shfl_xor_sync(0xffffffffu, etile, off));
-      if (etile > ev) {  // a larger V scale: O moves to its units
-        fv = ev == 0 ? 0.f : scale_value(max(ev - etile + 127, 0));
-        ev = etile;
-        grow = true;
-      }
-    }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= corr[0] * fv;
-        o[i][1] *= corr[0] * fv;
-        o[i][2] *= corr[1] * fv;
-        o[i][3] *= corr[1] * fv;
-      }
-    }
-    // P, the row sums (of the unrounded p), and O += P V
-#pragma unroll
-    for (int i = 0; i < NT; i += 2) {
-      uint32_t a[4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float p0 = ex2(sc[i + u][0] - mu[0]), p1 = ex2(sc[i + u][1] - mu[0]);
-        const float p2 = ex2(sc[i + u][2] - mu[1]), p3 = ex2(sc[i + u][3] - mu[1]);
-        l[0] += p0 + p1;
-        l[1] += p2 + p3;
-        if (QUANT) {
-          // times 2^(scale - ev + 12): p * scale <= 2^12 keeps fp16's 11 bits for weights down to 2^-26
-          const float w0 = scale_value(max(__float_as_int(vs[i + u][0]) - ev + 139, 0));
-          const float w1 = scale_value(max(__float_as_int(vs[i + u][1]) - ev + 139, 0));
-          a[2 * u] = pack_f16x2(p0 * w0, p1 * w1);
-          a[2 * u + 1] = pack_f16x2(p2 * w0, p3 * w1);
-        } else {
-          a[2 * u] = pack_bf16x2(p0, p1);
-          a[2 * u + 1] = pack_bf16x2(p2, p3);
-        }
-      }
-      const int vrow = krow + i * 8 + (lane & 15);
+        for (int c = 0; c < 4; ++c) sc[nr][c] = 0.f;
+      const int kr = krow + (lane & 15), vr = krow + (lane & 7) + ((lane >> 4) << 3);
       if (!QUANT) {
 #pragma unroll
-        for (int dd = 0; dd < D / 16; ++dd) {  // 16 keys x 16 columns a load
-          uint32_t b[4];
-          ldsm4t(b, vt + tile_at<G::CH>(vrow, dd * 2 + (lane >> 4)));
-          mma<false>(o[2 * dd], a, b[0], b[1]);
-          mma<false>(o[2 * dd + 1], a, b[2], b[3]);
+        for (int kk = 0; kk < KK; ++kk) {
+          uint32_t a[4];
+          ldsm4(a, kt + tile_at<G::CH>(kr, 2 * kk + (lane >> 4)));
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) mma<false>(sc[nr], a, qf[nr][kk][0], qf[nr][kk][1]);
         }
       } else {
-        // b16 pairs are two neighbouring columns of a key: after the transpose each register holds keys
-        // (2t, 2t+1) x columns (2n, 2n+1); reordered bytes give the even columns' and the odd columns'
-        // fragments, so o[2 dd] holds columns 0, 2, .. and o[2 dd + 1] columns 1, 3, .. of 16
 #pragma unroll
-        for (int dd = 0; dd < D / 16; dd += 2) {  // 16 keys x 32 columns a load
+        for (int kk = 0; kk < KK; kk += 2) {
           uint32_t b[4];
-          ldsm4t(b, vt + tile_at<G::CH>(vrow, dd + (lane >> 4)));
+          ldsm4(b, kt + tile_at<G::CH>(kr, kk + (lane >> 4)));
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t x = __byte_perm(b[2 * u], 0, 0x3120), y = __byte_perm(b[2 * u + 1], 0, 0x3120);
-            mma<true>(o[2 * (dd + u)], a, paged::e4m3x2_to_f16x2((uint16_t)x), paged::e4m3x2_to_f16x2((uint16_t)y));
-            mma<true>(o[2 * (dd + u) + 1], a, paged::e4m3x2_to_f16x2((uint16_t)(x >> 16)),
-                      paged::e4m3x2_to_f16x2((uint16_t)(y >> 16)));
+            const uint32_t a[4] = {paged::e4m3x2_to_f16x2((uint16_t)b[2 * u]), paged::e4m3x2_to_f16x2((uint16_t)b[2 * u + 1]),
+                                   paged::e4m3x2_to_f16x2((uint16_t)(b[2 * u] >> 16)),
+                                   paged::e4m3x2_to_f16x2((uint16_t)(b[2 * u + 1] >> 16))};
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma<true>(sc[nr], a, qf[nr][kk + u][0], qf[nr][kk + u][1]);
+          }
+        }
+      }
+      int vb[2] = {0, 0};
+      if (QUANT) {
+        const float k0 = pow2_byte(scales[krow + g]), k1 = pow2_byte(scales[krow + g + 8]);
+        vb[0] = key0 + g < ke ? scales[BN + krow + g] : 0;
+        vb[1] = key0 + g + 8 < ke ? scales[BN + krow + g + 8] : 0;
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+          sc[nr][0] *= k0 * qs[nr][0];
+          sc[nr][1] *= k0 * qs[nr][1];
+          sc[nr][2] *= k1 * qs[nr][0];
+          sc[nr][3] *= k1 * qs[nr][1];
+        }
+      } else {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[nr][c] *= p.sl2;
+      }
+      if (key0 + 15 > wlim) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key0 + g + 8 * (c >> 1) > min(lim[nr][c & 1], ke - 1)) sc[nr][c] = -INFINITY;
+      }
+      // raise the maxima (and the unit of O) only where needed
+      bool up = QUANT && max(vb[0], vb[1]) > ev;
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) up |= fmaxf(sc[nr][u], sc[nr][2 + u]) > m[nr][u] + GROW;
+      if (__any_sync(0xffffffffu, up)) {
+        float fv = 1.f;
+        if (QUANT) {
+          const int e = __reduce_max_sync(0xffffffffu, max(vb[0], vb[1]));
+          if (e > ev) {
+            fv = ev == 0 ? 0.f : pow2_byte(ev - e + 127);
+            ev = e;
+          }
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float mx = fmaxf(sc[nr][u], sc[nr][2 + u]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            float corr = 1.f;
+            if (mx > m[nr][u]) {
+              corr = ex2(m[nr][u] - mx);  // 0 when nothing was visible before
+              m[nr][u] = mx;
+            }
+            l[nr][u] *= corr;
+            corr *= fv;
+#pragma unroll
+            for (int i = 0; i < KK; ++i) {
+              o[i][nr][u] *= corr;
+              o[i][nr][2 + u] *= corr;
+            }
+          }
+      }
+      // P^T, this lane's part of the row sums (of the unrounded weights), and O^T += V^T P^T
+      const float w0 = QUANT ? pow2_byte(vb[0] - ev + 127 + V_SHIFT) : 1.f, w1 = QUANT ? pow2_byte(vb[1] - ev + 127 + V_SHIFT) : 1.f;
+      uint32_t pb[NR][2];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        const float m0 = m[nr][0] == -INFINITY ? 0.f : m[nr][0], m1 = m[nr][1] == -INFINITY ? 0.f : m[nr][1];
+        const float p0 = ex2(sc[nr][0] - m0), p1 = ex2(sc[nr][1] - m1), p2 = ex2(sc[nr][2] - m0), p3 = ex2(sc[nr][3] - m1);
+        l[nr][0] += p0 + p2;
+        l[nr][1] += p1 + p3;
+        pb[nr][0] = transpose8(QUANT ? pack_f16x2(p0 * w0, p1 * w0) : pack_bf16x2(p0, p1));
+        pb[nr][1] = transpose8(QUANT ? pack_f16x2(p2 * w1, p3 * w1) : pack_bf16x2(p2, p3));
+      }
+      if (!QUANT) {
+#pragma unroll
+        for (int i = 0; i < KK; ++i) {
+          uint32_t a[4];
+          ldsm4t(a, vt + tile_at<G::CH>(vr, 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) mma<false>(o[i][nr], a, pb[nr][0], pb[nr][1]);
+        }
+      } else {
+        // b16 pairs are two neighbouring columns of a key: after the transpose a register holds columns
+        // (2g, 2g+1) x keys (2t, 2t+1); its bytes reordered give rows g (even columns) and g + 8 (odd)
+#pragma unroll
+        for (int i = 0; i < KK; i += 2) {
+          uint32_t b[4];
+          ldsm4t(b, vt + tile_at<G::CH>(vr, i + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t x = __byte_perm(b[u], 0, 0x3120), y = __byte_perm(b[2 + u], 0, 0x3120);
+            const uint32_t a[4] = {paged::e4m3x2_to_f16x2((uint16_t)x), paged::e4m3x2_to_f16x2((uint16_t)(x >> 16)),
+                                   paged::e4m3x2_to_f16x2((uint16_t)y), paged::e4m3x2_to_f16x2((uint16_t)(y >> 16))};
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma<true>(o[i + u][nr], a, pb[nr][0], pb[nr][1]);
           }
         }
       }
@@ -448,41 +480,35 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   cp_wait<0>();
   __syncthreads();  // the ring is free: it holds the join now
 
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-  }
-  // join of the key groups: [wk][row][D] floats (columns in their own order) and [wk][row] (m, l)
+  // join of the key groups: [wk][row][D + 4] floats (the padding spreads the four row pairs of a store
+  // over the banks) and [wk][row] (m, l)
+  constexpr int LDO = D + 4;
   float* so = reinterpret_cast<float*>(smem);
-  float2* sml = reinterpret_cast<float2*>(smem + WK * BM * D * 4);
-  const int lrow = wm * 16 + g;
-  if (t4 == 0) {
-    sml[wk * BM + lrow] = make_float2(m[0], l[0]);
-    sml[wk * BM + lrow + 8] = make_float2(m[1], l[1]);
-  }
+  float2* sml = reinterpret_cast<float2*>(smem + WK * BM * LDO * 4);
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[nr][u] += __shfl_xor_sync(0xffffffffu, l[nr][u], off);
+      if (g == 0) sml[wk * BM + (wm * NR + nr) * 8 + 2 * t4 + u] = make_float2(m[nr][u], l[nr][u]);
+    }
   __syncthreads();
-  float mj[2], f[2];
-  const float unit = QUANT ? scale_value(ev) * (1.f / 4096.f) : 1.f;
+  const float unit = QUANT ? scale_value(ev) * (1.f / (1 << V_SHIFT)) : 1.f;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    mj[r] = -INFINITY;
+  for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-    for (int w = 0; w < WK; ++w) mj[r] = fmaxf(mj[r], sml[w * BM + lrow + 8 * r].x);
-    f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mj[r]);
-  }
+    for (int u = 0; u < 2; ++u) {
+      const int row = (wm * NR + nr) * 8 + 2 * t4 + u;
+      float mj = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
+      for (int w = 0; w < WK; ++w) mj = fmaxf(mj, sml[w * BM + row].x);
+      const float f = m[nr][u] == -INFINITY ? 0.f : ex2(m[nr][u] - mj) * unit;
+      float* dst = so + (wk * BM + row) * LDO;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float* dst = so + (wk * BM + lrow + 8 * r) * D + i * 16;
-      const float a0 = o[2 * i][2 * r] * f[r] * unit, a1 = o[2 * i][2 * r + 1] * f[r] * unit;
-      const float b0 = o[2 * i + 1][2 * r] * f[r] * unit, b1 = o[2 * i + 1][2 * r + 1] * f[r] * unit;
-      if (QUANT) {
-        *reinterpret_cast<float4*>(dst + 4 * t4) = make_float4(a0, b0, a1, b1);
-      } else {
-        *reinterpret_cast<float2*>(dst + 2 * t4) = make_float2(a0, a1);
-        *reinterpret_cast<float2*>(dst + 8 + 2 * t4) = make_float2(b0, b1);
+      for (int i = 0; i < KK; ++i) {
+        dst[i * 16 + (QUANT ? 2 * g : g)] = o[i][nr][u] * f;
+        dst[i * 16 + (QUANT ? 2 * g + 1 : g + 8)] = o[i][nr][2 + u] * f;
       }
     }
   __syncthreads();
@@ -490,7 +516,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   for (int e = tid; e < BM * (D / 8); e += THREADS) {
     const int row = e / (D / 8), c = (e % (D / 8)) * 8;
     const int gr = row0 + row;
-    if (gr >= rows) continue;
+    if (gr >= rows) break;
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < WK; ++w) mm = fmaxf(mm, sml[w * BM + row].x);
@@ -504,8 +530,8 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     for (int i = 0; i < 8; ++i) y[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
-      const float4 a = *reinterpret_cast<const float4*>(so + (w * BM + row) * D + c);
-      const float4 b = *reinterpret_cast<const float4*>(so + (w * BM + row) * D + c + 4);
+      const float4 a = *reinterpret_cast<const float4*>(so + (w * BM + row) * LDO + c);
+      const float4 b = *reinterpret_cast<const float4*>(so + (w * BM + row) * LDO + c + 4);
       y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
       y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
     }
@@ -579,29 +605,37 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   *reinterpret_cast<uint4*>(p.out + idx * D + c) = pack8(y);
 }
 
-template <int D, bool QUANT, int WM>
+template <int D, bool QUANT, int WM, int NR>
 static int launch_few(const Params& p, cudaStream_t s) {
   using G = Geo<D, QUANT>;
-  constexpr int BM = 16 * WM, WK = 4 / WM;
-  constexpr int join = WK * BM * D * 4 + WK * BM * 8;
+  constexpr int BM = 8 * NR * WM, WK = 4 / WM;
+  constexpr int join = WK * BM * (D + 4) * 4 + WK * BM * 8;
   constexpr int bytes = G::RING > join ? G::RING : join;
-  const void* fn = (const void*)few_rows_kernel<D, QUANT, WM>;
+  const void* fn = (const void*)few_rows_kernel<D, QUANT, WM, NR>;
   if (int st = ensure_smem_attr(fn, bytes, "paged_gqa")) return st;
   const dim3 grid((unsigned)((int64_t)p.nseg * p.row_blocks * p.hkv), (unsigned)p.nsplit);
-  few_rows_kernel<D, QUANT, WM><<<grid, THREADS, bytes, s>>>(p);
+  few_rows_kernel<D, QUANT, WM, NR><<<grid, THREADS, bytes, s>>>(p);
   return check_launch("paged_gqa");
 }
 
+// `rows` (8, 16, 32 or 64) a CTA.  O of 32 rows at head_dim 128, 16 at 256, takes 128 registers a lane;
+// more rows go to more warps.
 template <int D, bool QUANT>
-static int launch_rows(const Params& p, int wm, cudaStream_t s) {
-  return wm == 1 ? launch_few<D, QUANT, 1>(p, s) : wm == 2 ? launch_few<D, QUANT, 2>(p, s) : launch_few<D, QUANT, 4>(p, s);
+static int launch_rows(const Params& p, int rows, cudaStream_t s) {
+  constexpr int most = D == 128 ? 4 : 2;
+  switch (rows) {
+    case 8: return launch_few<D, QUANT, 1, 1>(p, s);
+    case 16: return launch_few<D, QUANT, 1, 2>(p, s);
+    case 32: return launch_few<D, QUANT, 4 / most, most>(p, s);
+    default: return launch_few<D, QUANT, 8 / most, most>(p, s);
+  }
 }
 
 // Tiling of a call: the kernel, its rows a CTA and the split of the keys.  All follow from host-side
 // sizes only, so a captured call replays with any lengths.
 struct Plan {
   bool many;           // the tcgen05 kernel
-  int wm;              // few-row kernel: 16-row groups a CTA
+  int rows;            // few-row kernel: rows a CTA
   int64_t row_blocks;  // row blocks (tiles) of the longest segment, a KV head
   int64_t tiles;       // many rows: row tiles in the grid, a KV head
   bool picked;
@@ -639,8 +673,8 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
     split = (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1);
     least = MIN_SPLIT_KEYS_MANY;
   } else {
-    r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    r.row_blocks = (rows + 16 * r.wm - 1) / (16 * r.wm);
+    r.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    r.row_blocks = (rows + r.rows - 1) / r.rows;
     const int64_t ctas = num_segments * hkv * (r.row_blocks > 0 ? r.row_blocks : 1);
     split = (FEW_CTAS_AN_SM * SMS + ctas - 1) / ctas;
     least = MIN_SPLIT_KEYS_FEW;
@@ -770,8 +804,8 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       st = quant ? chunk::launch<128, true>(p, pl.tiles, s) : chunk::launch<128, false>(p, pl.tiles, s);
     else
       st = quant ? chunk::launch<256, true>(p, pl.tiles, s) : chunk::launch<256, false>(p, pl.tiles, s);
-  } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.wm, s) : launch_rows<128, false>(p, pl.wm, s);
-  else st = quant ? launch_rows<256, true>(p, pl.wm, s) : launch_rows<256, false>(p, pl.wm, s);
+  } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.rows, s) : launch_rows<128, false>(p, pl.rows, s);
+  else st = quant ? launch_rows<256, true>(p, pl.rows, s) : launch_rows<256, false>(p, pl.rows, s);
   if (st || pl.nsplit == 1) return st;
   const int64_t rpw = head_dim == 128 ? 2 : 1;
   const int64_t warps = tokens * ((hq + rpw - 1) / rpw);
