@@ -58,7 +58,7 @@ SIGNATURES.update({
                                  vp, i64, i64, i64, i64, vp]),
     "fdk_paged_kv_read": (i32, [vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64, i64, i64,
                                 i64, vp, vp, vp]),
-    "fdk_paged_gqa_workspace_size": (sz, [i64, i64, i64, i64, i64, i64, i64]),
+    "fdk_paged_gqa_workspace_size": (sz, [i64, i64, i64, i64, i64, i64, i64, i32]),
     "fdk_paged_gqa_fwd": (i32, [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64,
                                 i64, i64, i64, i64, i64, i64, f32, vp, i64, i32, vp, vp, sz, vp]),
     "fdk_recurrent_gated_delta_rule_fwd": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64,

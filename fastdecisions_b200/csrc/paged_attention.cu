@@ -5,7 +5,7 @@
 // nothing gets zeros.  The query heads of a KV head are packed with the tokens into rows (row = token *
 // group + head), so every cached row brought into shared memory feeds them all.
 //
-// Calls with more than 64 rows a KV head run the tcgen05 kernel of paged_attention_chunk.cuh.  This file:
+// Calls with more than 16 to 32 rows a KV head run the tcgen05 kernel of paged_attention_chunk.cuh.  This file:
 // the few-row kernel (mma.sync, split over the keys) and the join of splits.  Its work is bound by
 // reading the cache: at one token a sequence each cached byte is used by `group` rows only, far below the
 // tensor cores' rate, so warp-level MMAs -- which need no padding to 128 rows and keep S and P in
@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     }
   }
   cp_wait<0>();
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   __syncthreads();  // the ring is free: it holds the join now
 
   // join of the key groups: [wk][row][D + 4] floats (the padding spreads the four row pairs of a store
@@ -559,8 +560,10 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
 }
 
 // Join of the splits: one warp a (token, head) row, 8 columns a lane (two rows a warp at D = 128).
+// It is launched while the kernel before it drains and waits here for its parts.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const Params p) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int LPR = D / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -618,16 +621,15 @@ static int launch_few(const Params& p, cudaStream_t s) {
   return check_launch("paged_gqa");
 }
 
-// `rows` (8, 16, 32 or 64) a CTA.  O of 32 rows at head_dim 128, 16 at 256, takes 128 registers a lane;
-// more rows go to more warps.
+// `rows` (8, 16 or 32) a CTA.  O of 32 rows at head_dim 128, 16 at 256, takes 128 registers a lane; the
+// other 16 go to other warps.
 template <int D, bool QUANT>
 static int launch_rows(const Params& p, int rows, cudaStream_t s) {
   constexpr int most = D == 128 ? 4 : 2;
   switch (rows) {
     case 8: return launch_few<D, QUANT, 1, 1>(p, s);
     case 16: return launch_few<D, QUANT, 1, 2>(p, s);
-    case 32: return launch_few<D, QUANT, 4 / most, most>(p, s);
-    default: return launch_few<D, QUANT, 8 / most, most>(p, s);
+    default: return launch_few<D, QUANT, 4 / most, most>(p, s);
   }
 }
 
@@ -643,23 +645,28 @@ struct Plan {
 };
 constexpr int SMS = 148;
 constexpr int MAX_SPLIT = 64;
-constexpr int FEW_ROWS = 64;
-// Few rows: a part costs little (16 to 64 rows of float32) and ragged contexts need many to spread over the
-// SMs.  Measured, 64 one-token segments of 500 to 8192 positions, e4m3: 98 us with 2 CTAs an SM, 80 with 4,
-// 75 with 8, 73 with 16; parts below 256 keys gain nothing more.
-constexpr int FEW_CTAS_AN_SM = 16;
+// The few-row kernel's time grows with the rows, the tcgen05 kernel's does not below a tile.  Measured, 64
+// segments x 8192 positions, 16 / 4 heads of 128 and 8 / 2 of 256, few against many rows in us, bf16: 16
+// rows 173 / 302 and 204 / 214, 32 rows 253 / 296 and 284 / 209, 64 rows 365 / 299 and 520 / 208; e4m3:
+// 32 rows 229 / 363 and 202 / 279, 64 rows 364 / 363 and 323 / 286.
+constexpr int few_rows_most(int64_t d, bool quant) { return d == 256 && !quant ? 16 : 32; }
+// Few rows, CTAs an SM to aim at.  A part costs its rows in float32 and a CTA's start, so equal contexts want
+// few (8 segments x 8192 positions, bf16: 31 us with 2 CTAs an SM, 35 with 4, 46 with 8); ragged ones want
+// many once every SM has one (64 segments of 500 to 8192, e4m3: 98, 80 and 75 us), the more rows the
+// fewer.  Parts below 256 keys gain nothing.
+constexpr int few_ctas(int64_t ctas, int rows) { return ctas < SMS ? 2 : rows <= 16 ? 8 : 4; }
 constexpr int MIN_SPLIT_KEYS_FEW = 256;
 // Many rows: a part costs its rows in float32 twice, about as much as 250 keys of work, and a CTA's start
 // about 10 us.  Measured, eight segments of 100 to 700 tokens behind 600 to 6902 positions, e4m3: 164 us
 // unsplit, 140 aiming at two CTAs an SM, 155 at three; 48 segments of 9 to 70 tokens behind 1490, bf16:
-// 59 us unsplit, 66 in two parts of 896 keys.
-constexpr int MIN_SPLIT_KEYS_MANY = 2048;
+// 59 us unsplit, 66 in two parts of 896 keys.  While half of the SMs have no CTA, parts may be short.
+constexpr int MIN_SPLIT_KEYS_MANY = 2048, MIN_SPLIT_KEYS_IDLE = 512;
 static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
-                      int64_t group, int64_t d) {
+                      int64_t group, int64_t d, bool quant) {
   Plan r = {};
   const int64_t rows = max_seqlen * group;
   int64_t split, least;
-  r.many = rows > FEW_ROWS && group <= 128;
+  r.many = rows > few_rows_most(d, quant) && group <= 128;
   if (r.many) {
     const int64_t per = (d == 128 ? 2 : 1) * (128 / group);  // tokens a CTA
     r.row_blocks = (max_seqlen + per - 1) / per;
@@ -671,12 +678,12 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
     r.tiles = num_segments * r.row_blocks;
     if (r.picked && tokens / per + num_segments < r.tiles) r.tiles = tokens / per + num_segments;
     split = (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1);
-    least = MIN_SPLIT_KEYS_MANY;
+    least = 2 * ctas <= SMS ? MIN_SPLIT_KEYS_IDLE : MIN_SPLIT_KEYS_MANY;
   } else {
-    r.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    r.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     r.row_blocks = (rows + r.rows - 1) / r.rows;
     const int64_t ctas = num_segments * hkv * (r.row_blocks > 0 ? r.row_blocks : 1);
-    split = (FEW_CTAS_AN_SM * SMS + ctas - 1) / ctas;
+    split = (few_ctas(ctas, r.rows) * SMS + ctas - 1) / ctas;
     least = MIN_SPLIT_KEYS_FEW;
   }
   if (split > MAX_SPLIT) split = MAX_SPLIT;
@@ -722,9 +729,10 @@ static bool sizes_ok(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_le
 }
 
 extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
-                                               int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim) {
+                                               int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
+                                               int cache_is_e4m3) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
-  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim);
+  const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, cache_is_e4m3 != 0);
   return pl.nsplit > 1 ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
 }
 
@@ -771,7 +779,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       ld_kpage * esz % 16 || ld_vpage * esz % 16 || (gate && (!aligned16(gate) || ld_gate % 8)) ||
       (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
-  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim);
+  Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, quant);
   if (max_seqlen * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.tiles : num_segments * pl.row_blocks) > 0x7fffffff)
     return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
   Params p = {};
@@ -790,7 +798,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);
   p.out = static_cast<bf16*>(out);
   if (pl.nsplit > 1) {
-    const size_t need = fdk_paged_gqa_workspace_size(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim);
+    const size_t need = fdk_paged_gqa_workspace_size(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim, quant);
     if (!workspace || workspace_bytes < need)
       return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes needed", what, need);
     if (!aligned16(workspace)) return set_error(FDK_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", what);
@@ -809,8 +817,16 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   if (st || pl.nsplit == 1) return st;
   const int64_t rpw = head_dim == 128 ? 2 : 1;
   const int64_t warps = tokens * ((hq + rpw - 1) / rpw);
-  const unsigned grid = (unsigned)((warps + 3) / 4);
-  if (head_dim == 128) join_kernel<128><<<grid, 128, 0, s>>>(p);
-  else join_kernel<256><<<grid, 128, 0, s>>>(p);
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((warps + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (head_dim == 128) cudaLaunchKernelEx(&cfg, join_kernel<128>, p);
+  else cudaLaunchKernelEx(&cfg, join_kernel<256>, p);
   return check_launch("paged_gqa (join of splits)");
 }

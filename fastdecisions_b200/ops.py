@@ -820,8 +820,9 @@ def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
 
 
 def paged_gqa_workspace_bytes(segments: int, max_seqlen: int, max_kv_len: int, tokens: int, hq: int, hkv: int,
-                              head_dim: int) -> int:
-    return int(_lib.load().fdk_paged_gqa_workspace_size(segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim))
+                              head_dim: int, e4m3: bool = False) -> int:
+    """Scratch bytes of ``paged_gqa_attention`` for these sizes (0 when the keys are not split)."""
+    return _lib.load().fdk_paged_gqa_workspace_size(segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim, e4m3)
 
 
 def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -862,7 +863,7 @@ def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if max_kv_len < 0:
         raise ValueError("paged_gqa_attention: max_kv_len must not be negative")
     if workspace is None:
-        have = paged_gqa_workspace_bytes(kv_lens.numel(), max_seqlen, max_kv_len, T, hq, hkv, D)
+        have = paged_gqa_workspace_bytes(kv_lens.numel(), max_seqlen, max_kv_len, T, hq, hkv, D, k_scale is not None)
         if have:
             workspace = torch.empty(have, device=q.device, dtype=torch.uint8)
     else:

@@ -274,7 +274,8 @@ int fdk_paged_kv_read(const void* k_cache, int64_t ld_kpage, const void* v_cache
 
 /* Scratch bytes fdk_paged_gqa_fwd needs (0 when the call does not split the keys). */
 size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, int64_t max_kv_len,
-                                    int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim);
+                                    int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
+                                    int cache_is_e4m3);
 
 /*
  * Causal GQA attention of the newest tokens over the paged cache: token i of segment s's n attends
