@@ -6,9 +6,9 @@ There is no fallback: if the shared library is missing every op raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import re
-import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libfdk.so")
@@ -65,16 +65,10 @@ SIGNATURES.update({
                                                  f32, i32, vp, vp, i64, vp, vp, i64, vp, vp]),
     "fdk_packed_conv_state": (i32, [vp, i64, vp, vp, i64, i64, i64, i32, i64, i64, vp, vp, i64, vp, vp, i64, vp, vp,
                                     vp, vp]),
-    "fdk_invoke": (i32, [i32, C.c_char_p, i64]),
 })
 
-# entry points called through fdk_invoke: (FDK_OP_* number, packer of their arguments)
-_BLOCKS = {name: (op, struct.Struct("".join("d" if a is f32 else "q" for a in SIGNATURES[name][1])),
-                  len(SIGNATURES[name][1]))
-           for op, name in enumerate(("fdk_paged_kv_write", "fdk_paged_kv_read", "fdk_paged_gqa_fwd",
-                                      "fdk_recurrent_gated_delta_rule_fwd", "fdk_packed_conv_state"), start=1)}
-
 _lib = None
+_binding = None
 
 
 class FdkError(RuntimeError):
@@ -102,6 +96,22 @@ def load(path: str = LIB_PATH):
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def binding():
+    """The native binding of the cached-state operators (``csrc/binding.cpp``), loaded on first use."""
+    global _binding
+    if _binding is None:
+        path = os.path.join(_PKG, "_fdk_torch.so")
+        if not os.path.exists(path):
+            raise FdkError(f"{path} is missing: build it with `python -m fastdecisions_b200.build`")
+        load()
+        spec = importlib.util.spec_from_file_location("_fdk_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.set_error_class(FdkError)
+        _binding = module
+    return _binding
 
 
 def poll_device_error() -> int:
@@ -134,16 +144,6 @@ def call(name: str, *args):
     if st != FDK_OK:
         _raise(name, st)
     return st
-
-
-def call_block(name: str, *args):
-    """``call`` for the entry points of ``fdk_invoke``: arguments packed into one block (0 for a null
-    pointer), a fifth of ``call``'s host time."""
-    op, packer, n = _BLOCKS[name]
-    call_counts[name] = call_counts.get(name, 0) + 1
-    st = (_lib or load()).fdk_invoke(op, packer.pack(*args), n)
-    if st != FDK_OK:
-        _raise(name, st)
 
 
 def _raise(name: str, st: int):

@@ -2,7 +2,8 @@
 
 ``python -m fastdecisions_b200.build`` compiles every ``csrc/*.cu`` to an object file under
 ``fastdecisions_b200/_build/`` (in parallel, skipped when up to date) and links
-``fastdecisions_b200/libfdk.so``.  No GPU is needed: nvcc cross-compiles for sm_100a.
+``fastdecisions_b200/libfdk.so``, and the Python binding of the cached-state operators,
+``_fdk_torch.so``, with g++.  No GPU is needed: nvcc cross-compiles for sm_100a.
 """
 from __future__ import annotations
 
@@ -62,7 +63,40 @@ def build(verbose_ptxas: bool = False, jobs: int | None = None) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    build_binding()
     return LIB
+
+
+BINDING = os.path.join(PKG, "_fdk_torch.so")
+
+
+def build_binding() -> str:
+    """The Python binding of the cached-state operators, _fdk_torch.so: csrc/binding.cpp against the installed
+    torch and libfdk.so (found beside it at run time).  Host code only."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    src = os.path.join(CSRC, "binding.cpp")
+    deps = [src, os.path.join(ROOT, "include", "fdk.h"), torch.__file__]
+    if os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps):
+        return BINDING
+    tmp = BINDING + ".tmp"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", sysconfig.get_paths()["include"], "-I", cuda]
+    for p in include_paths():
+        cmd += ["-isystem", p]
+    cmd += [src, "-o", tmp]
+    for p in library_paths():
+        cmd += ["-L", p, f"-Wl,-rpath,{p}"]
+    cmd += ["-L", PKG, "-l:libfdk.so", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+            "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for binding.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 PHASES_LIB = os.path.join(PKG, "libfdk_phases.so")

@@ -2,10 +2,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
-#include <cstring>
 #include <mutex>
-#include <type_traits>
-#include <utility>
 
 #include "common.cuh"
 
@@ -101,47 +98,3 @@ int sm_count() {
 extern "C" const char* fdk_version(void) { return "fastdecisions-b200 0.1.0 sm_100a"; }
 
 extern "C" const char* fdk_get_last_error_string(void) { return fdk::g_last_error; }
-
-namespace fdk {
-
-// One 64-bit slot as an argument of type T.
-template <typename T>
-static T slot_as(const char* args, size_t i) {
-  int64_t raw;
-  memcpy(&raw, args + 8 * i, 8);  // the block has no alignment of its own
-  if constexpr (std::is_floating_point_v<T>) {
-    double d;
-    memcpy(&d, &raw, 8);
-    return static_cast<T>(d);
-  } else if constexpr (std::is_pointer_v<T>) {
-    return reinterpret_cast<T>(static_cast<uintptr_t>(raw));
-  } else {
-    return static_cast<T>(raw);
-  }
-}
-
-template <typename... A, size_t... I>
-static int invoke(int (*fn)(A...), const char* args, std::index_sequence<I...>) {
-  return fn(slot_as<A>(args, I)...);
-}
-
-template <typename... A>
-static int invoke(int (*fn)(A...), const void* args, int64_t nargs) {
-  if (!args || nargs != (int64_t)sizeof...(A))
-    return set_error(FDK_ERR_INVALID_ARGUMENT, "invoke: %d arguments expected, %lld given", (int)sizeof...(A),
-                     (long long)nargs);
-  return invoke(fn, static_cast<const char*>(args), std::index_sequence_for<A...>{});
-}
-
-}  // namespace fdk
-
-extern "C" int fdk_invoke(int op, const void* args, int64_t nargs) {
-  switch (op) {
-    case FDK_OP_PAGED_KV_WRITE: return fdk::invoke(fdk_paged_kv_write, args, nargs);
-    case FDK_OP_PAGED_KV_READ: return fdk::invoke(fdk_paged_kv_read, args, nargs);
-    case FDK_OP_PAGED_GQA_FWD: return fdk::invoke(fdk_paged_gqa_fwd, args, nargs);
-    case FDK_OP_RECURRENT_GATED_DELTA_RULE_FWD: return fdk::invoke(fdk_recurrent_gated_delta_rule_fwd, args, nargs);
-    case FDK_OP_PACKED_CONV_STATE: return fdk::invoke(fdk_packed_conv_state, args, nargs);
-    default: return fdk::set_error(FDK_ERR_INVALID_ARGUMENT, "invoke: unknown entry point %d", op);
-  }
-}

@@ -692,87 +692,10 @@ def rmsnorm_add_partials(partials: torch.Tensor, slices: int, h: torch.Tensor, w
 # Continuing sequences from cached state: paged KV cache, recurrent delta rule, conv history
 # (what src/decider/shared_prefix.py:42-200 does with transformers' dense caches)
 # ------------------------------------------------------------------------------------------------
-E4M3 = torch.float8_e4m3fn
-PAGE_SIZES = (16, 32, 64, 128, 256)
-
-
-def _device_of(*ts) -> int:
-    """Index of the one CUDA device of all given tensors (``_need_cuda`` for calls of a few microseconds)."""
-    dev = None
-    for t in ts:
-        if t is not None:
-            d = t.get_device()
-            if d != dev:
-                if d < 0:
-                    raise ValueError("fastdecisions_b200 ops run on CUDA tensors only (no CPU fallback)")
-                if dev is not None:
-                    raise ValueError("all tensors must share one CUDA device")
-                dev = d
-    return dev
-
-
-def _addr(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _launch(dev: int, name: str, *args):
-    """``_lib.call_block`` on ``dev`` and its current stream."""
-    if torch.cuda.current_device() == dev:
-        _lib.call_block(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _lib.call_block(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-
-
-def _int32_vector(name: str, what: str, t: torch.Tensor, n: int):
-    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
-        raise ValueError(f"{name}: {what} must be a contiguous int32 vector of {n} elements")
-
-
-def _paged_args(name: str, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale):
-    """Checks the cache and its metadata; the arguments of the C entry points from the cache on, and the
-    cache's shape."""
-    dtype, shape = k_cache.dtype, k_cache.shape
-    quant = dtype == E4M3
-    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dtype or not (quant or dtype == BF16):
-        raise ValueError(f"{name}: caches must be [pages, kv heads, page size, head_dim], both bf16 or both e4m3")
-    pages, hkv, page_size, D = shape
-    if page_size not in PAGE_SIZES or D not in (128, 256):
-        raise ValueError(f"{name}: page sizes {PAGE_SIZES} and head_dim 128 or 256 supported")
-    kst, vst = k_cache.stride(), v_cache.stride()
-    want = (page_size * D, D, 1)
-    if kst[1:] != want or vst[1:] != want:
-        raise ValueError(f"{name}: a cache page must be contiguous (only the page stride is free)")
-    if quant:
-        if k_scale is None or v_scale is None or k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8 or (
-                k_scale.shape != (pages, hkv, page_size) or v_scale.shape != (pages, hkv, page_size)):
-            raise ValueError(f"{name}: an e4m3 cache needs uint8 k_scale and v_scale [pages, kv heads, page size]")
-        kss, vss = k_scale.stride(), v_scale.stride()
-        if kss[1:] != (page_size, 1) or vss[1:] != (page_size, 1):
-            raise ValueError(f"{name}: the scales of a page must be contiguous (only the page stride is free)")
-        scales = (k_scale.data_ptr(), kss[0], v_scale.data_ptr(), vss[0])
-    elif k_scale is not None or v_scale is not None:
-        raise ValueError(f"{name}: a bf16 cache has no scales")
-    else:
-        scales = (0, 0, 0, 0)
-    S = kv_lens.numel()
-    _int32_vector(name, "kv_lens", kv_lens, S)
-    _int32_vector(name, "cu_seqlens", cu_seqlens, S + 1)
-    tshape, tst = page_table.shape, page_table.stride()
-    if S < 1 or page_table.dtype != torch.int32 or len(tshape) != 2 or tshape[0] != S or tshape[1] < 1 or (
-            tshape[1] > 1 and tst[1] != 1):
-        raise ValueError(f"{name}: page_table must be int32 [segments, pages] with unit column stride")
-    return ((k_cache.data_ptr(), kst[0], v_cache.data_ptr(), vst[0], int(quant)) + scales +
-            (pages, page_size, page_table.data_ptr(), tst[0] if S > 1 else tshape[1], tshape[1],
-             cu_seqlens.data_ptr(), kv_lens.data_ptr(), S)), shape
-
-
-def _token_rows(name: str, what: str, t: torch.Tensor, heads: int, D: int) -> int:
-    """Token stride of bf16 rows ``[tokens, heads, D]``."""
-    st = t.stride()
-    if t.shape[1:] != (heads, D) or t.dtype != BF16 or st[2] != 1 or (heads > 1 and st[1] != D):
-        raise ValueError(f"{name}: {what} must be bf16 [tokens, {heads}, {D}] with head stride {D}")
-    return st[0] if t.shape[0] > 1 else heads * D
+def _counted(name: str):
+    """The native binding, counting one call of C entry point ``name``."""
+    _lib.call_counts[name] = _lib.call_counts.get(name, 0) + 1
+    return _lib._binding or _lib.binding()
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -784,15 +707,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     cu_seqlens[s + 1] - 1`` are the last of its ``kv_lens[s]`` positions; position p is row ``p % page
     size`` of page ``page_table[s, p // page size]``.  Invalid device metadata is skipped and reported
     by the device error word."""
-    dev = _device_of(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale)
-    args, (_, hkv, _, D) = _paged_args("paged_kv_write", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
-                                       v_scale)
-    ldk = _token_rows("paged_kv_write", "k", k, hkv, D)
-    ldv = _token_rows("paged_kv_write", "v", v, hkv, D)
-    T = k.shape[0]
-    if v.shape[0] != T:
-        raise ValueError("paged_kv_write: k and v must have the same tokens")
-    _launch(dev, "fdk_paged_kv_write", k.data_ptr(), ldk, v.data_ptr(), ldv, *args, T, hkv, D)
+    _counted("fdk_paged_kv_write").paged_kv_write(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
+                                                  v_scale)
 
 
 def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -802,21 +718,8 @@ def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
     """The last ``cu_seqlens[s + 1] - cu_seqlens[s]`` cached rows of every segment as packed bf16 ``(k, v)
     [tokens, Hkv, D]`` (the inverse of ``paged_kv_write``; ``cu_seqlens`` = running sums of ``kv_lens``
     reads whole contexts).  Rows behind the last segment are left as they were."""
-    dev = _device_of(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, k_out, v_out)
-    args, (_, hkv, _, D) = _paged_args("paged_kv_read", k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale,
-                                       v_scale)
-    tokens = int(tokens)
-    if tokens < 0:
-        raise ValueError("paged_kv_read: tokens must not be negative")
-    for t in (k_out, v_out):
-        if t is not None and (t.shape != (tokens, hkv, D) or t.dtype != BF16 or not t.is_contiguous()):
-            raise ValueError("paged_kv_read: outputs must be contiguous bf16 [tokens, kv heads, head_dim]")
-    if k_out is None:
-        k_out = torch.empty((tokens, hkv, D), device=k_cache.device, dtype=BF16)
-    if v_out is None:
-        v_out = torch.empty((tokens, hkv, D), device=k_cache.device, dtype=BF16)
-    _launch(dev, "fdk_paged_kv_read", *args, tokens, hkv, D, k_out.data_ptr(), v_out.data_ptr())
-    return k_out, v_out
+    return _counted("fdk_paged_kv_read").paged_kv_read(k_cache, v_cache, page_table, cu_seqlens, kv_lens, tokens,
+                                                       k_scale, v_scale, k_out, v_out)
 
 
 def paged_gqa_workspace_bytes(segments: int, max_seqlen: int, max_kv_len: int, tokens: int, hq: int, hkv: int,
@@ -835,109 +738,12 @@ def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     the paged cache (see ``paged_kv_write``, which has written their own keys): token i of a segment's
     n attends to positions ``0 .. kv_lens[s] - n + i``; one that sees nothing gets zeros.  ``max_seqlen``
     bounds the tokens of a segment; ``max_kv_len`` (default: the page table's reach) only guides how the
-    keys are split.  ``gate`` / ``gate_interleaved`` / ``scale`` as ``gqa_attention_varlen_``."""
-    dev = _device_of(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, gate, out, workspace)
-    args, (_, hkv, page_size, D) = _paged_args("paged_gqa_attention", k_cache, v_cache, page_table, cu_seqlens, kv_lens,
-                                               k_scale, v_scale)
-    qshape = q.shape
-    if len(qshape) != 3 or qshape[1] < 1 or qshape[1] % hkv:
-        raise ValueError("paged_gqa_attention: q must be [tokens, query heads, head_dim], whole groups of query heads")
-    T, hq, _ = qshape
-    ldq = _token_rows("paged_gqa_attention", "q", q, hq, D)
-    ldg = 0
-    if gate is not None:
-        span = (2 * hq - 1) * D if gate_interleaved else hq * D
-        gshape, gst = gate.shape, gate.stride()
-        if len(gshape) != 2 or gate.dtype != BF16 or gshape[0] != T or gshape[1] < span or gst[1] != 1:
-            raise ValueError(f"paged_gqa_attention: gate must be bf16 [tokens, >= {span}] with unit column stride")
-        ldg = gst[0] if T > 1 else (gshape[1] + 7) // 8 * 8
-    if out is None:
-        out = torch.empty(qshape, device=q.device, dtype=BF16)
-    elif out.shape != qshape or out.dtype != BF16 or not out.is_contiguous():
-        raise ValueError("paged_gqa_attention: out must be contiguous bf16 shaped like q")
-    max_seqlen = min(int(max_seqlen), T)
-    if max_seqlen < 0:
-        raise ValueError("paged_gqa_attention: max_seqlen must not be negative")
-    reach = page_table.shape[1] * page_size
-    max_kv_len = reach if max_kv_len is None else min(int(max_kv_len), reach)
-    if max_kv_len < 0:
-        raise ValueError("paged_gqa_attention: max_kv_len must not be negative")
-    if workspace is None:
-        have = paged_gqa_workspace_bytes(kv_lens.numel(), max_seqlen, max_kv_len, T, hq, hkv, D, k_scale is not None)
-        if have:
-            workspace = torch.empty(have, device=q.device, dtype=torch.uint8)
-    else:
-        if not workspace.is_contiguous():
-            raise ValueError("paged_gqa_attention: workspace must be contiguous")
-        have = workspace.numel() * workspace.element_size()
-    _launch(dev, "fdk_paged_gqa_fwd", q.data_ptr(), ldq, *args, max_seqlen, max_kv_len, T, hq, hkv, D,
-            float(D ** -0.5 if scale is None else scale), _addr(gate), ldg, int(gate_interleaved), out.data_ptr(),
-            _addr(workspace), have)
-    return out
-
-
-def _segments_of(name: str, B: int, T: int, cu_seqlens: Optional[torch.Tensor]) -> int:
-    if cu_seqlens is None:
-        return B
-    if B != 1:
-        raise ValueError(f"{name}: cu_seqlens needs batch size 1")
-    n = cu_seqlens.numel()
-    _int32_vector(name, "cu_seqlens", cu_seqlens, n)
-    if n < 2:
-        raise ValueError(f"{name}: cu_seqlens must have at least two elements")
-    return n - 1
-
-
-def _heads_stride(name: str, what: str, t: torch.Tensor, B: int, T: int, H: int, D: int):
-    """``[B, T, H, D]`` as rows of one token stride (a copy when the layout has none)."""
-    if t.dtype != BF16:
-        raise ValueError(f"{name}: {what} must be bf16")
-    st = t.stride()
-    if not (st[3] == 1 and (H == 1 or st[2] == D) and (B == 1 or T == 1 or st[0] == T * st[1])):
-        t = t.contiguous()
-        st = t.stride()
-    return t, (st[1] if T > 1 else st[0] if B > 1 else H * D)
-
-
-def _recurrent(name, dev, query, key, value, g, beta, l2norm, cu_seqlens, initial, initial_idx, final, final_idx, out):
-    if query.dim() != 4 or key.shape != query.shape or value.dim() != 4:
-        raise ValueError(f"{name}: expected [B, T, H, D] query/key/value")
-    B, T, Hk, Dk = key.shape
-    H, Dv = value.shape[2:]
-    if value.shape[:2] != (B, T) or g.shape != (B, T, H) or beta.shape != (B, T, H):
-        raise ValueError(f"{name}: shape mismatch between q/k/v/g/beta")
-    if Dk != 128 or Dv != 128:
-        raise ValueError(f"{name}: head dims must be 128")
-    if Hk < 1 or H % Hk:
-        raise ValueError(f"{name}: value heads must be a multiple of the key heads")
-    S = _segments_of(name, B, T, cu_seqlens)
-    for pool in (initial, final):
-        if pool is not None and (pool.dim() != 4 or pool.shape[1:] != (H, Dk, Dv) or pool.dtype != torch.float32
-                                 or not pool.is_contiguous()):
-            raise ValueError(f"{name}: states must be contiguous float32 [slots, {H}, {Dk}, {Dv}]")
-    for idx, pool in ((initial_idx, initial), (final_idx, final)):
-        if idx is not None:
-            _int32_vector(name, "slot indices", idx, S)
-        elif pool is not None and pool.shape[0] < S:
-            raise ValueError(f"{name}: {S} segments need at least as many state slots")
-    if out is None:
-        out = torch.empty((B, T, H, Dv), device=value.device, dtype=BF16)
-    elif out.shape != (B, T, H, Dv) or out.dtype != BF16 or not out.is_contiguous():
-        raise ValueError(f"{name}: out must be contiguous bf16 [B, T, H, Dv]")
-    if S == 0:
-        return out
-    q, ldq = _heads_stride(name, "query", query, B, T, Hk, Dk)
-    k, ldk = _heads_stride(name, "key", key, B, T, Hk, Dk)
-    v, ldv = _heads_stride(name, "value", value, B, T, H, Dv)
-    if g.dtype != torch.float32 or not g.is_contiguous():
-        g = g.float().contiguous()
-    if beta.dtype != BF16 or not beta.is_contiguous():
-        beta = beta.to(BF16).contiguous()
-    _launch(dev, "fdk_recurrent_gated_delta_rule_fwd", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
-            g.data_ptr(), beta.data_ptr(), _addr(cu_seqlens), S, B * T, Hk, H, Dk, Dv, Dk ** -0.5, int(l2norm),
-            _addr(initial), _addr(initial_idx), 0 if initial is None else initial.shape[0], _addr(final),
-            _addr(final_idx), 0 if final is None else final.shape[0], out.data_ptr())
-    return out
+    keys are split.  ``gate`` / ``gate_interleaved`` / ``scale`` as ``gqa_attention_varlen_``.  A
+    ``workspace`` (``paged_gqa_workspace_bytes``) may serve calls that do not overlap on the GPU; without
+    one it is allocated."""
+    return _counted("fdk_paged_gqa_fwd").paged_gqa_attention(
+        q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, max_seqlen, max_kv_len, k_scale, v_scale, scale, gate,
+        gate_interleaved, out, workspace)
 
 
 def recurrent_gated_delta_rule_(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: torch.Tensor,
@@ -951,11 +757,9 @@ def recurrent_gated_delta_rule_(query: torch.Tensor, key: torch.Tensor, value: t
     negative: nowhere), so a slot can be advanced or forked.  A slot written by one segment must not be
     read or written by another of the call.  ``query, key [B, T, Hk, 128]``, ``value [B, T, H, 128]`` bf16
     (H a multiple of Hk), ``g`` (log decay) and ``beta [B, T, H]``; returns ``o [B, T, H, 128]`` bf16."""
-    dev = _device_of(query, key, value, g, beta, state, state_indices, final_indices, cu_seqlens, out)
-    if final_indices is None:
-        final_indices = state_indices
-    return _recurrent("recurrent_gated_delta_rule_", dev, query, key, value, g, beta, use_qk_l2norm_in_kernel, cu_seqlens,
-                      state, state_indices, state, final_indices, out)
+    return _counted("fdk_recurrent_gated_delta_rule_fwd").recurrent_gated_delta_rule(
+        "recurrent_gated_delta_rule_", query, key, value, g, beta, state, state_indices, state,
+        state_indices if final_indices is None else final_indices, cu_seqlens, use_qk_l2norm_in_kernel, out)
 
 
 def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, output_final_state=False,
@@ -964,7 +768,7 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
     ``chunk_gated_delta_rule``): returns ``(o [B, T, H, Dv] bf16, final_state [N, H, Dk, Dv] float32 or
     None)``.  For few tokens a sequence (decoding, short continuations); the chunked form is faster for
     long ones."""
-    dev = _device_of(query, key, value, g, beta, initial_state, cu_seqlens)
+    _need_cuda(query, key, value, g, beta, initial_state, cu_seqlens)
     if query.dim() != 4 or value.dim() != 4:
         raise ValueError("recurrent_gated_delta_rule: expected [B, T, H, D] query/key/value")
     cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
@@ -977,8 +781,8 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state=None, o
         init = initial_state.float().contiguous()
     final = torch.empty(shape, device=value.device, dtype=torch.float32) if output_final_state else None
     q, k, v = (t if t.dtype == BF16 else t.to(BF16) for t in (query, key, value))
-    o = _recurrent("recurrent_gated_delta_rule", dev, q, k, v, g, beta, use_qk_l2norm_in_kernel, cu, init, None, final,
-                   None, None)
+    o = _counted("fdk_recurrent_gated_delta_rule_fwd").recurrent_gated_delta_rule(
+        "recurrent_gated_delta_rule", q, k, v, g, beta, init, None, final, None, cu, use_qk_l2norm_in_kernel, None)
     return o, final
 
 
@@ -990,44 +794,5 @@ def packed_conv_state_(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     ``K - 1`` input rows of each sequence (oldest first) and is updated in place; ``state_indices`` /
     ``final_indices`` as ``recurrent_gated_delta_rule_`` (a negative index: zeros before the segment).
     ``x [B, T, C]`` (unit column stride, any row stride) -> ``q, k, v [B, T, heads, head_dim]``."""
-    dev = _device_of(x, weight, state, state_indices, final_indices, cu_seqlens)
-    name = "packed_conv_state_"
-    if x.dim() != 3 or x.dtype != BF16 or weight.dtype != BF16:
-        raise ValueError(f"{name}: expected bf16 x [B, T, C] and weight")
-    B, T, C = x.shape
-    wshape = weight.shape
-    if (len(wshape) != 2 and (len(wshape) != 3 or wshape[1] != 1)) or wshape[0] != C or not 2 <= wshape[-1] <= 4 or (
-            not weight.is_contiguous()):
-        raise ValueError(f"{name}: weight must be a contiguous [C, K] or [C, 1, K] tensor with K from 2 to 4")
-    K = wshape[-1]
-    if key_dim is None:
-        key_dim = C // 3
-    if value_dim is None:
-        value_dim = C - 2 * key_dim
-    if 2 * key_dim + value_dim != C or key_dim % head_dim or value_dim % head_dim or min(key_dim, value_dim) < 1:
-        raise ValueError(f"{name}: C must equal 2*key_dim + value_dim with whole heads")
-    slots = state.shape[0]
-    if state.shape != (slots, K - 1, C) or state.dtype != BF16 or not state.is_contiguous():
-        raise ValueError(f"{name}: state must be contiguous bf16 [slots, {K - 1}, {C}]")
-    S = _segments_of(name, B, T, cu_seqlens)
-    if final_indices is None:
-        final_indices = state_indices
-    for idx in (state_indices, final_indices):
-        if idx is not None:
-            _int32_vector(name, "slot indices", idx, S)
-        elif slots < S:
-            raise ValueError(f"{name}: {S} segments need at least as many state slots")
-    st = x.stride()
-    if st[2] != 1 or (B > 1 and T > 1 and st[0] != T * st[1]):
-        x = x.contiguous()
-        st = x.stride()
-    ldx = st[1] if T > 1 else st[0] if B > 1 else C
-    hk, hv = key_dim // head_dim, value_dim // head_dim
-    q = torch.empty((B, T, hk, head_dim), device=x.device, dtype=BF16)
-    k = torch.empty((B, T, hk, head_dim), device=x.device, dtype=BF16)
-    v = torch.empty((B, T, hv, head_dim), device=x.device, dtype=BF16)
-    if S:
-        _launch(dev, "fdk_packed_conv_state", x.data_ptr(), ldx, weight.data_ptr(), _addr(cu_seqlens), S, B * T, C, K,
-                key_dim, value_dim, state.data_ptr(), _addr(state_indices), slots, state.data_ptr(),
-                _addr(final_indices), slots, q.data_ptr(), k.data_ptr(), v.data_ptr())
-    return q, k, v
+    return _counted("fdk_packed_conv_state").packed_conv_state(x, weight, state, state_indices, final_indices, key_dim,
+                                                               value_dim, head_dim, cu_seqlens)

@@ -342,20 +342,6 @@ int fdk_packed_conv_state(const void* x, int64_t ld_x, const void* weight,
                           int64_t new_history_slots, void* q, void* k, void* v, void* stream);
 
 /*
- * The entry points above from one block of arguments, for hosts whose foreign-function interface
- * pays per argument (Python's ctypes: about 0.2 us each, 33 arguments for the attention):
- * args[i] is the i-th argument of entry point `op` in a 64-bit slot -- integers and pointers as they
- * are, floats as the bits of a double -- and nargs must be its argument count.  Same checks, same
- * results, same status.
- */
-#define FDK_OP_PAGED_KV_WRITE 1
-#define FDK_OP_PAGED_KV_READ 2
-#define FDK_OP_PAGED_GQA_FWD 3
-#define FDK_OP_RECURRENT_GATED_DELTA_RULE_FWD 4
-#define FDK_OP_PACKED_CONV_STATE 5
-int fdk_invoke(int op, const void* args, int64_t nargs);
-
-/*
  * Reads and clears the device-side error word of the current device.  Kernels that wait on
  * mbarriers (fdk_gqa_fwd, the delta rule) bound every wait; a wait that runs out sets a bit of
  * this word, frees its resources and returns without finishing its tile.  Bits: 1 an attention
