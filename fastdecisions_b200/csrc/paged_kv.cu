@@ -63,70 +63,97 @@ __device__ __forceinline__ Where locate(const KvParams& p, int64_t t, int lane, 
 }
 
 // One warp a token: D / 8 lanes a row, so two rows (D = 128) or one (D = 256) at a time over the
-// 2 * hkv rows (k then v).  READ = false: rows into the cache; READ = true: cached rows out.
+// 2 * hkv rows (k then v), up to four of those in flight.  READ = false: rows into the cache (loaded
+// before the token's place is looked up); READ = true: cached rows out.
 template <int D, bool QUANT, bool READ>
 __global__ void __launch_bounds__(128) kv_rows_kernel(const KvParams p) {
   constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows an iteration
+  constexpr int BATCH = 4;
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (t >= p.tokens) return;
+  const int sub = lane / LPR, c = (lane % LPR) * 8;
+  const int rows = 2 * p.hkv;
+  uint4 raw[BATCH];
+  auto load_new = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int r = min(r0 + i * RPI + sub, rows - 1);
+      const bf16* src = r >= p.hkv ? p.v + t * p.ld_v + (r - p.hkv) * D : p.k + t * p.ld_k + r * D;
+      raw[i] = ldg_stream(src + c);
+    }
+  };
+  if (!READ) load_new(0);
   int64_t page = 0;
   int off = 0;
   const Where where = locate(p, t, lane, page, off);
   if (where == OUTSIDE || (!READ && where == NONE)) return;
-  const int sub = lane / LPR, c = (lane % LPR) * 8;
-  const int rows = 2 * p.hkv;
-  for (int r0 = 0; r0 < rows; r0 += RPI) {
-    const int r = r0 + sub;
-    const bool live = r < rows;
-    const bool is_v = r >= p.hkv;
-    const int h = is_v ? r - p.hkv : r;
-    const int64_t slot = ((int64_t)h << p.page_shift) + off;
-    const int64_t row_at = page * (is_v ? p.ld_vpage : p.ld_kpage) + slot * D + c;
-    const int64_t scale_at = page * (is_v ? p.ld_vscale_page : p.ld_kscale_page) + slot;
-    if (!READ) {
-      const bf16* src = (is_v ? p.v + t * p.ld_v : p.k + t * p.ld_k) + h * D + c;
-      const uint4 raw = live ? ldg_stream(src) : make_uint4(0u, 0u, 0u, 0u);
-      if (!QUANT) {
-        if (live) *reinterpret_cast<uint4*>(static_cast<bf16*>(is_v ? p.v_cache : p.k_cache) + row_at) = raw;
-      } else {
-        float f[8];
-        unpack8(raw, f);
-        float a = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += BATCH * RPI) {
+    if (READ) {
+      int bytes[BATCH];
+      uint2 q8[BATCH];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const int b = scale_byte(a);
-        const float inv = scale_inverse(b);
-        uint16_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = f32x2_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
-        if (live) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + row_at) =
-              make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
-          if (c == 0) (is_v ? p.v_scale : p.k_scale)[scale_at] = (uint8_t)b;
+      for (int i = 0; i < BATCH; ++i) {  // `page` and `off` are 0 where there is no row: a valid place
+        const int r = min(r0 + i * RPI + sub, rows - 1);
+        const bool is_v = r >= p.hkv;
+        const int64_t slot = ((int64_t)(is_v ? r - p.hkv : r) << p.page_shift) + off;
+        const int64_t at = page * (is_v ? p.ld_vpage : p.ld_kpage) + slot * D + c;
+        if (QUANT) {
+          q8[i] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + at));
+          bytes[i] = __ldg((is_v ? p.v_scale : p.k_scale) + page * (is_v ? p.ld_vscale_page : p.ld_kscale_page) + slot);
+        } else {
+          raw[i] = ldg_stream(static_cast<const bf16*>(is_v ? p.v_cache : p.k_cache) + at);
         }
       }
-    } else if (live) {
-      bf16* dst = (is_v ? p.v_out : p.k_out) + (t * p.hkv + h) * D + c;
-      if (where == NONE) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
-      } else if (!QUANT) {
-        *reinterpret_cast<uint4*>(dst) = ldg_stream(static_cast<const bf16*>(is_v ? p.v_cache : p.k_cache) + row_at);
-      } else {
-        const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + row_at);
-        const float s = scale_value((is_v ? p.v_scale : p.k_scale)[scale_at]);
-        const uint16_t q[4] = {(uint16_t)raw.x, (uint16_t)(raw.x >> 16), (uint16_t)raw.y, (uint16_t)(raw.y >> 16)};
-        float f[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t h2 = e4m3x2_to_f16x2(q[i]);
-          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-          f[2 * i] = w.x * s;
-          f[2 * i + 1] = w.y * s;
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = r0 + i * RPI + sub;
+        if (QUANT) {
+          const float s = scale_value(bytes[i]);
+          const uint16_t q[4] = {(uint16_t)q8[i].x, (uint16_t)(q8[i].x >> 16), (uint16_t)q8[i].y, (uint16_t)(q8[i].y >> 16)};
+          float f[8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t h2 = e4m3x2_to_f16x2(q[u]);
+            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+            f[2 * u] = w.x * s;
+            f[2 * u + 1] = w.y * s;
+          }
+          raw[i] = pack8(f);
         }
-        *reinterpret_cast<uint4*>(dst) = pack8(f);
+        if (where == NONE) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows)
+          *reinterpret_cast<uint4*>((r >= p.hkv ? p.v_out + (t * p.hkv + r - p.hkv) * D : p.k_out + (t * p.hkv + r) * D) + c) = raw[i];
+      }
+    } else {
+      if (r0 > 0) load_new(r0);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = r0 + i * RPI + sub;
+        const bool is_v = r >= p.hkv;
+        const int64_t slot = ((int64_t)(is_v ? r - p.hkv : r) << p.page_shift) + off;
+        const int64_t at = page * (is_v ? p.ld_vpage : p.ld_kpage) + slot * D + c;
+        if (!QUANT) {
+          if (r < rows) *reinterpret_cast<uint4*>(static_cast<bf16*>(is_v ? p.v_cache : p.k_cache) + at) = raw[i];
+        } else {
+          float f[8];
+          unpack8(raw[i], f);
+          float a = 0.f;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) a = fmaxf(a, fabsf(f[u]));
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+          const int b = scale_byte(a);
+          const float inv = scale_inverse(b);
+          uint16_t q[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) q[u] = f32x2_to_e4m3x2(f[2 * u] * inv, f[2 * u + 1] * inv);
+          if (r < rows) {
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + at) =
+                make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
+            if (c == 0) (is_v ? p.v_scale : p.k_scale)[page * (is_v ? p.ld_vscale_page : p.ld_kscale_page) + slot] = (uint8_t)b;
+          }
+        }
       }
     }
   }

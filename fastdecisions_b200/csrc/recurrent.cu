@@ -32,8 +32,14 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t sl
 //     S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
 // Columns of S evolve on their own, so a warp owns 16 of the 128 columns and never talks to another:
 // lane (r, c) = (lane / 4, lane % 4) holds rows 16 r .. 16 r + 15 of columns 4 c .. 4 c + 3 in 64
-// registers.  S^T k and S^T q of the old state are reduced together (one pass over the registers, one
-// round of shuffles), as o = scale (e^g S^T q + (k . q) u).
+// registers, as pairs of rows (one packed operation works on two).  S^T k and S^T q of the old state are
+// reduced together, as o = scale (e^g S^T q + (k . q) u); the reduction over r leaves one of the eight
+// sums in each lane (7 shuffles instead of 24).
+// The decay is not applied to the registers: they hold S / G with G the product of the decays so far, and
+// the update adds k (u / G), one operation an element instead of two.  When G leaves [1e-18, 1e18] it is
+// multiplied in and starts over at 1.
+// Bound by HBM where states dominate (64 KiB in, 64 KiB out a head and segment), by the float32 pipe at
+// several tokens a segment: about 240 operations a lane and token.
 constexpr int DK = 128, DV = 128, CPW = 16;   // columns a warp
 constexpr int WARPS = 4;
 
@@ -59,16 +65,11 @@ struct DeltaParams {
   bf16* out;
 };
 
-__device__ __forceinline__ void load16(const bf16* p, float (&f)[16]) {
-  float a[8], b[8];
-  unpack8(__ldg(reinterpret_cast<const uint4*>(p)), a);
-  unpack8(__ldg(reinterpret_cast<const uint4*>(p) + 1), b);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = a[i];
-    f[8 + i] = b[i];
-  }
-}
+// One token's inputs of a lane, loaded a token ahead.
+struct TokenIn {
+  uint4 k[2], q[2];
+  float v, g, beta;
+};
 
 __global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const DeltaParams p) {
   const int lane = threadIdx.x & 31;
@@ -96,71 +97,120 @@ __global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const Delta
   const int64_t from = p.state_in ? slot_of(p.in_idx, s, p.in_slots, lane == 0) : -1;
   const int64_t to = p.state_out ? slot_of(p.out_idx, s, p.out_slots, lane == 0) : -1;
   const int64_t in_slot = (int64_t)r * 16 * DV + col;
-  float4 S[16];
+  auto load = [&](int64_t t) {
+    TokenIn x;
+    const uint4* kp = reinterpret_cast<const uint4*>(p.k + t * p.ld_k + hk * DK + r * 16);
+    const uint4* qp = reinterpret_cast<const uint4*>(p.q + t * p.ld_q + hk * DK + r * 16);
+    x.k[0] = __ldg(kp);
+    x.k[1] = __ldg(kp + 1);
+    x.q[0] = __ldg(qp);
+    x.q[1] = __ldg(qp + 1);
+    x.v = __bfloat162float(p.v[t * p.ld_v + h * DV + col + (r & 3)]);
+    x.g = p.g[t * p.heads + h];
+    x.beta = __bfloat162float(p.beta[t * p.heads + h]);
+    return x;
+  };
+  TokenIn next = {};
+  if (t0 < t1) next = load(t0);
+  float2 S[4][8];  // [column][pair of rows]
   if (from >= 0) {
     const float* src = p.state_in + (from * p.heads + h) * (DK * DV) + in_slot;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) S[i] = *reinterpret_cast<const float4*>(src + i * DV);
+    for (int i = 0; i < 8; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(src + (2 * i) * DV);
+      const float4 b = *reinterpret_cast<const float4*>(src + (2 * i + 1) * DV);
+      S[0][i] = make_float2(a.x, b.x);
+      S[1][i] = make_float2(a.y, b.y);
+      S[2][i] = make_float2(a.z, b.z);
+      S[3][i] = make_float2(a.w, b.w);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[j][i] = make_float2(0.f, 0.f);
   }
+  float G = 1.f;
+  auto scale_state = [&](float f) {
+    const float2 f2 = make_float2(f, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) S[j][i] = __fmul2_rn(S[j][i], f2);
+  };
   for (int64_t t = t0; t < t1; ++t) {
-    float k[16], q[16];
-    load16(p.k + t * p.ld_k + hk * DK + r * 16, k);
-    load16(p.q + t * p.ld_q + hk * DK + r * 16, q);
-    const uint2 vr = __ldg(reinterpret_cast<const uint2*>(p.v + t * p.ld_v + h * DV + col));
-    const float eg = expf(p.g[t * p.heads + h]);
-    const float beta = __bfloat162float(p.beta[t * p.heads + h]);
-    float red[11];
+    const TokenIn x = next;
+    if (t + 1 < t1) next = load(t + 1);
+    float2 k[8], q[8];
+    const uint32_t kw[8] = {x.k[0].x, x.k[0].y, x.k[0].z, x.k[0].w, x.k[1].x, x.k[1].y, x.k[1].z, x.k[1].w};
+    const uint32_t qw[8] = {x.q[0].x, x.q[0].y, x.q[0].z, x.q[0].w, x.q[1].x, x.q[1].y, x.q[1].z, x.q[1].w};
 #pragma unroll
-    for (int i = 0; i < 11; ++i) red[i] = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      k[i] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&kw[i]));
+      q[i] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qw[i]));
+    }
+    G *= expf(x.g);
+    if (!(G >= 1e-18f && G <= 1e18f)) {  // warp-uniform
+      scale_state(G);
+      G = 1.f;
+    }
+    float2 dot[8], kq = make_float2(0.f, 0.f), kk = kq, qq = kq;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      red[0] = fmaf(S[i].x, k[i], red[0]);
-      red[1] = fmaf(S[i].y, k[i], red[1]);
-      red[2] = fmaf(S[i].z, k[i], red[2]);
-      red[3] = fmaf(S[i].w, k[i], red[3]);
-      red[4] = fmaf(S[i].x, q[i], red[4]);
-      red[5] = fmaf(S[i].y, q[i], red[5]);
-      red[6] = fmaf(S[i].z, q[i], red[6]);
-      red[7] = fmaf(S[i].w, q[i], red[7]);
-      red[8] = fmaf(k[i], q[i], red[8]);
-      red[9] = fmaf(k[i], k[i], red[9]);
-      red[10] = fmaf(q[i], q[i], red[10]);
+    for (int j = 0; j < 8; ++j) dot[j] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dot[j] = __ffma2_rn(S[j][i], k[i], dot[j]);
+        dot[4 + j] = __ffma2_rn(S[j][i], q[i], dot[4 + j]);
+      }
+      kq = __ffma2_rn(k[i], q[i], kq);
+      kk = __ffma2_rn(k[i], k[i], kk);
+      qq = __ffma2_rn(q[i], q[i], qq);
+    }
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = dot[j].x + dot[j].y;
+    float skq = kq.x + kq.y, skk = kk.x + kk.y, sqq = qq.x + qq.y;
+    // sum over r: lane r ends with sum r of S^T k (columns 0 .. 3), S^T q (columns 0 .. 3)
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1) {
+      const bool upper = (r & n) != 0;
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        const float mine = upper ? d[n + j] : d[j], other = upper ? d[j] : d[n + j];
+        d[j] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
+      }
     }
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1)
-#pragma unroll
-      for (int i = 0; i < 11; ++i) red[i] += __shfl_xor_sync(0xffffffffu, red[i], o);
-    const float rk = p.l2norm ? rsqrtf(red[9] + 1e-6f) : 1.f;
-    const float rq = (p.l2norm ? rsqrtf(red[10] + 1e-6f) : 1.f) * p.scale;
-    const float2 v01 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&vr.x));
-    const float2 v23 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&vr.y));
-    const float er = eg * rk;
-    float4 u;  // rk * beta * (v - S^T k)
-    u.x = rk * beta * (v01.x - er * red[0]);
-    u.y = rk * beta * (v01.y - er * red[1]);
-    u.z = rk * beta * (v23.x - er * red[2]);
-    u.w = rk * beta * (v23.y - er * red[3]);
-    if (r == 0) {
-      uint2 o;
-      o.x = pack_bf16x2(rq * fmaf(red[8], u.x, eg * red[4]), rq * fmaf(red[8], u.y, eg * red[5]));
-      o.y = pack_bf16x2(rq * fmaf(red[8], u.z, eg * red[6]), rq * fmaf(red[8], u.w, eg * red[7]));
-      *reinterpret_cast<uint2*>(p.out + (t * p.heads + h) * DV + col) = o;
+    for (int off = 4; off < 32; off <<= 1) {
+      skq += __shfl_xor_sync(0xffffffffu, skq, off);
+      skk += __shfl_xor_sync(0xffffffffu, skk, off);
+      sqq += __shfl_xor_sync(0xffffffffu, sqq, off);
     }
+    const float rk = p.l2norm ? rsqrtf(skk + 1e-6f) : 1.f;
+    const float rq = (p.l2norm ? rsqrtf(sqq + 1e-6f) : 1.f) * p.scale;
+    // lanes r < 4: u of column r times k's norm factor; lanes r >= 4 pick it up for their output
+    const float u = rk * x.beta * (x.v - G * rk * d[0]);
+    const float uo = __shfl_xor_sync(0xffffffffu, u, 16);
+    if (r >= 4) p.out[(t * p.heads + h) * DV + col + (r & 3)] = __float2bfloat16_rn(rq * fmaf(skq, uo, G * d[0]));
+    const float ug = u / G;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      S[i].x = fmaf(k[i], u.x, eg * S[i].x);
-      S[i].y = fmaf(k[i], u.y, eg * S[i].y);
-      S[i].z = fmaf(k[i], u.z, eg * S[i].z);
-      S[i].w = fmaf(k[i], u.w, eg * S[i].w);
+    for (int j = 0; j < 4; ++j) {
+      const float uj = __shfl_sync(0xffffffffu, ug, 4 * j + c);
+      const float2 uu = make_float2(uj, uj);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) S[j][i] = __ffma2_rn(k[i], uu, S[j][i]);
     }
   }
   if (to >= 0) {
+    if (t0 < t1) scale_state(G);
     float* dst = p.state_out + (to * p.heads + h) * (DK * DV) + in_slot;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) *reinterpret_cast<float4*>(dst + i * DV) = S[i];
+    for (int i = 0; i < 8; ++i) {
+      *reinterpret_cast<float4*>(dst + (2 * i) * DV) = make_float4(S[0][i].x, S[1][i].x, S[2][i].x, S[3][i].x);
+      *reinterpret_cast<float4*>(dst + (2 * i + 1) * DV) = make_float4(S[0][i].y, S[1][i].y, S[2][i].y, S[3][i].y);
+    }
   }
 }
 
@@ -190,19 +240,26 @@ struct ConvParams {
   bf16* v;
 };
 
+// One output row of 8 channels from its KW input rows, two channels an operation.
 template <int KW>
-__device__ __forceinline__ void conv_row(const uint4 (&rows)[KW], const float (&w)[KW][8], bf16* dst) {
-  float acc[8];
+__device__ __forceinline__ void conv_row(const uint4 (&rows)[KW], const float2 (&w)[KW][4], bf16* dst) {
+  uint4 out;
+  uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+  const float2 half2_ = make_float2(0.5f, 0.5f);
 #pragma unroll
-  for (int j = 0; j < KW; ++j) {
-    float f[8];
-    unpack8(rows[j], f);
+  for (int c = 0; c < 4; ++c) {
+    float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) acc[c] = j == 0 ? w[0][c] * f[c] : fmaf(w[j][c], f[c], acc[c]);
+    for (int j = 0; j < KW; ++j) {
+      const uint32_t b = c == 0 ? rows[j].x : c == 1 ? rows[j].y : c == 2 ? rows[j].z : rows[j].w;
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b));
+      acc = j == 0 ? __fmul2_rn(w[0][c], x) : __ffma2_rn(w[j][c], x, acc);
+    }
+    const float2 h = __fmul2_rn(half2_, acc);  // silu(x) = h + h tanh(h), h = x / 2
+    const float2 y = __ffma2_rn(h, make_float2(tanh_approx(h.x), tanh_approx(h.y)), h);
+    o[c] = pack_bf16x2(y.x, y.y);
   }
-#pragma unroll
-  for (int c = 0; c < 8; ++c) acc[c] = silu_tanh(acc[c]);
-  *reinterpret_cast<uint4*>(dst) = pack8(acc);
+  *reinterpret_cast<uint4*>(dst) = out;
 }
 
 template <int KW>
@@ -219,11 +276,19 @@ __global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
   if (c0 < p.key_dim) { dst = p.q + c0; ldd = p.key_dim; }
   else if (c0 < 2 * p.key_dim) { dst = p.k + (c0 - p.key_dim); ldd = p.key_dim; }
   else { dst = p.v + (c0 - 2 * p.key_dim); ldd = p.channels - 2 * p.key_dim; }
-  auto load_w = [&](float (&w)[KW][8]) {
+  auto load_w = [&](float2 (&w)[KW][4]) {  // 8 channels x KW taps: KW aligned 16-byte loads
+    float f[8 * KW];
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
+    for (int i = 0; i < KW; ++i) {
+      float e[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + (int64_t)c0 * KW) + i), e);
 #pragma unroll
-      for (int j = 0; j < KW; ++j) w[j][c] = __bfloat162float(p.w[(int64_t)(c0 + c) * KW + j]);
+      for (int u = 0; u < 8; ++u) f[8 * i + u] = e[u];
+    }
+#pragma unroll
+    for (int j = 0; j < KW; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[j][c] = make_float2(f[2 * c * KW + j], f[(2 * c + 1) * KW + j]);
   };
   if (job < p.nseg) {
     const int s = (int)job;
@@ -270,7 +335,7 @@ __global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
         *reinterpret_cast<uint4*>(p.hist_out + (to * HR + j) * p.channels + c0) = last[j];
     }
     if (n == 0) return;
-    float w[KW][8];
+    float2 w[KW][4];
     load_w(w);
 #pragma unroll
     for (int j = 0; j < HR; ++j) {
@@ -299,7 +364,7 @@ __global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
     const int64_t t = r0 - HR + j;
     raw[j] = t >= 0 && t < r1 ? ldg_stream(p.x + t * p.ld_x + c0) : zero;
   }
-  float w[KW][8];
+  float2 w[KW][4];
   load_w(w);
   int64_t begin = -1, end = -1;
 #pragma unroll
@@ -406,7 +471,7 @@ extern "C" int fdk_packed_conv_state(const void* x, int64_t ld_x, const void* we
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: fewer history slots than segments", what);
   if (ld_x < channels) return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: ld_x < channels", what);
   if (!aligned16(x) || ld_x % 8 || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(history) ||
-      !aligned16(new_history))
+      !aligned16(new_history) || !aligned16(weight))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and row stride must be 16-byte aligned", what);
   ConvParams p = {};
   p.x = static_cast<const bf16*>(x); p.ld_x = ld_x; p.w = static_cast<const bf16*>(weight);

@@ -486,7 +486,13 @@ def test_delta_in_place_step_by_step_equals_one_call():
         step = [t.reshape(S, n, *t.shape[2:])[:, i:i + 1] for t in (q, k, v, g, beta)]
         outs.append(ops.recurrent_gated_delta_rule_(*step, b))
     assert no_error()
-    assert torch.equal(a, b) and torch.equal(torch.cat(outs, 1), o1)
+    # Not bit-equal: the kernel keeps a segment's decay factored out of its registers and multiplies it in
+    # when it stores the state, after every token here and after six there.  Each of the two is within the
+    # header's bound of the exact result, so by the triangle inequality they differ by at most twice it.
+    assert (a - b).abs().max().item() <= 2 * 2e-5 * max(1.0, a.abs().max().item())
+    o2 = torch.cat(outs, 1).float()
+    o1 = o1.float()
+    assert ((o1 - o2).abs() <= 2 * (2 ** -8 * o1.abs() * (1 + 2 ** -7) + 2e-5 * max(1.0, o1.abs().max().item()))).all()
 
 
 def test_delta_forks_share_a_slot_and_no_l2norm():
