@@ -30,18 +30,21 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t sl
 // ------------------------------------------------------------------------------------------------
 // Recurrent gated delta rule.  Per token, with the state S [dk][dv] (float32) of one head:
 //     S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
-// Columns of S evolve on their own, so a warp owns 16 of the 128 columns and never talks to another:
-// lane (r, c) = (lane / 4, lane % 4) holds rows 16 r .. 16 r + 15 of columns 4 c .. 4 c + 3 in 64
-// registers, as pairs of rows (one packed operation works on two).  S^T k and S^T q of the old state are
-// reduced together, as o = scale (e^g S^T q + (k . q) u); the reduction over r leaves one of the eight
-// sums in each lane (7 shuffles instead of 24).
+// A CTA is one (segment, head).  Columns of S evolve on their own, so each of its 8 warps owns 16 of the 128
+// columns and they never exchange state: lane (r, c) = (lane / 4, lane % 4) holds rows 16 r .. 16 r + 15 of
+// columns 4 c .. 4 c + 3 in 64 registers, as pairs of rows (one packed operation works on two).
+// Up to 16 tokens at a time, the warps first share the work that every column needs: k and q normalised to
+// float32, k . q, e^g, beta and v go to shared memory.  The token loop then reads only that.
+// S^T k and S^T q of the old state are reduced together, as o = e^g S^T q + (k . q) u with q scaled; the
+// reduction over r leaves one of the eight sums in each lane (7 shuffles instead of 24).
 // The decay is not applied to the registers: they hold S / G with G the product of the decays so far, and
 // the update adds k (u / G), one operation an element instead of two.  When G leaves [1e-18, 1e18] it is
 // multiplied in and starts over at 1.
 // Bound by HBM where states dominate (64 KiB in, 64 KiB out a head and segment), by the float32 pipe at
-// several tokens a segment: about 240 operations a lane and token.
+// several tokens a segment.
 constexpr int DK = 128, DV = 128, CPW = 16;   // columns a warp
-constexpr int WARPS = 4;
+constexpr int WARPS = DV / CPW;
+constexpr int BATCH = 16;                     // tokens in shared memory at a time
 
 struct DeltaParams {
   const bf16* q;
@@ -65,24 +68,24 @@ struct DeltaParams {
   bf16* out;
 };
 
-// One token's inputs of a lane, loaded a token ahead.
-struct TokenIn {
-  uint4 k[2], q[2];
-  float v, g, beta;
+// k and q of a token are kept in the order the lanes read them: rows 16 r + 4 i .. + 3 at float4 8 i + r, so
+// the eight r of a warp read 128 consecutive bytes.
+struct Tokens {
+  float4 k[BATCH][DK / 4], q[BATCH][DK / 4];
+  float v[BATCH][DV];
+  float4 s[BATCH];  // e^g, beta, k . q
 };
 
-__global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const DeltaParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  const int slice = (int)(w & (DV / CPW - 1));
-  const int64_t sh = w / (DV / CPW);
-  const int s = (int)(sh / p.heads), h = (int)(sh - (int64_t)s * p.heads);
-  if (s >= p.nseg) return;
+__global__ void __launch_bounds__(32 * WARPS, 2) recurrent_delta_kernel(const DeltaParams p) {
+  __shared__ Tokens sm;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int s = (int)(blockIdx.x / (unsigned)p.heads), h = (int)(blockIdx.x % (unsigned)p.heads);
+  const bool report = threadIdx.x == 0 && h == 0;
   int64_t t0, t1;
   if (p.cu) {
     int b, e;
     if (!paged::segment_range(p.cu, s, p.tokens, b, e)) {
-      if (lane == 0) flag_error();
+      if (report) flag_error();
       b = e = 0;
     }
     t0 = b;
@@ -92,26 +95,11 @@ __global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const Delta
     t1 = t0 + p.period;
   }
   const int r = lane >> 2, c = lane & 3;
-  const int col = slice * CPW + c * 4;
+  const int col = warp * CPW + c * 4;
   const int hk = h / p.group;
-  const int64_t from = p.state_in ? slot_of(p.in_idx, s, p.in_slots, lane == 0) : -1;
-  const int64_t to = p.state_out ? slot_of(p.out_idx, s, p.out_slots, lane == 0) : -1;
+  const int64_t from = p.state_in ? slot_of(p.in_idx, s, p.in_slots, report) : -1;
+  const int64_t to = p.state_out ? slot_of(p.out_idx, s, p.out_slots, report) : -1;
   const int64_t in_slot = (int64_t)r * 16 * DV + col;
-  auto load = [&](int64_t t) {
-    TokenIn x;
-    const uint4* kp = reinterpret_cast<const uint4*>(p.k + t * p.ld_k + hk * DK + r * 16);
-    const uint4* qp = reinterpret_cast<const uint4*>(p.q + t * p.ld_q + hk * DK + r * 16);
-    x.k[0] = __ldg(kp);
-    x.k[1] = __ldg(kp + 1);
-    x.q[0] = __ldg(qp);
-    x.q[1] = __ldg(qp + 1);
-    x.v = __bfloat162float(p.v[t * p.ld_v + h * DV + col + (r & 3)]);
-    x.g = p.g[t * p.heads + h];
-    x.beta = __bfloat162float(p.beta[t * p.heads + h]);
-    return x;
-  };
-  TokenIn next = {};
-  if (t0 < t1) next = load(t0);
   float2 S[4][8];  // [column][pair of rows]
   if (from >= 0) {
     const float* src = p.state_in + (from * p.heads + h) * (DK * DV) + in_slot;
@@ -138,69 +126,83 @@ __global__ void __launch_bounds__(32 * WARPS) recurrent_delta_kernel(const Delta
 #pragma unroll
       for (int j = 0; j < 4; ++j) S[j][i] = __fmul2_rn(S[j][i], f2);
   };
-  for (int64_t t = t0; t < t1; ++t) {
-    const TokenIn x = next;
-    if (t + 1 < t1) next = load(t + 1);
-    float2 k[8], q[8];
-    const uint32_t kw[8] = {x.k[0].x, x.k[0].y, x.k[0].z, x.k[0].w, x.k[1].x, x.k[1].y, x.k[1].z, x.k[1].w};
-    const uint32_t qw[8] = {x.q[0].x, x.q[0].y, x.q[0].z, x.q[0].w, x.q[1].x, x.q[1].y, x.q[1].z, x.q[1].w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      k[i] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&kw[i]));
-      q[i] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qw[i]));
+  for (int64_t tb = t0; tb < t1; tb += BATCH) {
+    const int nt = (int)(t1 - tb < BATCH ? t1 - tb : BATCH);
+    if (tb > t0) __syncthreads();
+    for (int i = warp; i < nt; i += WARPS) {
+      const int64_t t = tb + i;
+      const uint2 kr = __ldg(reinterpret_cast<const uint2*>(p.k + t * p.ld_k + hk * DK) + lane);
+      const uint2 qr = __ldg(reinterpret_cast<const uint2*>(p.q + t * p.ld_q + hk * DK) + lane);
+      const uint2 vr = __ldg(reinterpret_cast<const uint2*>(p.v + t * p.ld_v + h * DV) + lane);
+      const float g = p.g[t * p.heads + h], beta = __bfloat162float(p.beta[t * p.heads + h]);
+      auto two = [](uint32_t w) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };
+      float2 k0 = two(kr.x), k1 = two(kr.y), q0 = two(qr.x), q1 = two(qr.y);
+      const float2 v0 = two(vr.x), v1 = two(vr.y);
+      float rk = 1.f, rq = p.scale;
+      if (p.l2norm) {
+        rk = rsqrtf(warp_sum(k0.x * k0.x + k0.y * k0.y + k1.x * k1.x + k1.y * k1.y) + 1e-6f);
+        rq *= rsqrtf(warp_sum(q0.x * q0.x + q0.y * q0.y + q1.x * q1.x + q1.y * q1.y) + 1e-6f);
+      }
+      const float4 kn = make_float4(k0.x * rk, k0.y * rk, k1.x * rk, k1.y * rk);
+      const float4 qn = make_float4(q0.x * rq, q0.y * rq, q1.x * rq, q1.y * rq);
+      const float kq = warp_sum(kn.x * qn.x + kn.y * qn.y + kn.z * qn.z + kn.w * qn.w);
+      const int at = (lane & 3) * 8 + (lane >> 2);
+      sm.k[i][at] = kn;
+      sm.q[i][at] = qn;
+      *reinterpret_cast<float4*>(&sm.v[i][4 * lane]) = make_float4(v0.x, v0.y, v1.x, v1.y);
+      if (lane == 0) sm.s[i] = make_float4(expf(g), beta, kq, 0.f);
     }
-    G *= expf(x.g);
-    if (!(G >= 1e-18f && G <= 1e18f)) {  // warp-uniform
-      scale_state(G);
-      G = 1.f;
-    }
-    float2 dot[8], kq = make_float2(0.f, 0.f), kk = kq, qq = kq;
+    __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+      const float4 sc = sm.s[t];
+      G *= sc.x;
+      if (!(G >= 1e-18f && G <= 1e18f)) {  // the same for the whole CTA
+        scale_state(G);
+        G = 1.f;
+      }
+      float2 k[8], dot[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dot[j] = make_float2(0.f, 0.f);
+      for (int j = 0; j < 8; ++j) dot[j] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        const float4 k4 = sm.k[t][i * 8 + r], q4 = sm.q[t][i * 8 + r];
+        k[2 * i] = make_float2(k4.x, k4.y);
+        k[2 * i + 1] = make_float2(k4.z, k4.w);
+        const float2 q0 = make_float2(q4.x, q4.y), q1 = make_float2(q4.z, q4.w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dot[j] = __ffma2_rn(S[j][2 * i], k[2 * i], dot[j]);
+          dot[4 + j] = __ffma2_rn(S[j][2 * i], q0, dot[4 + j]);
+          dot[j] = __ffma2_rn(S[j][2 * i + 1], k[2 * i + 1], dot[j]);
+          dot[4 + j] = __ffma2_rn(S[j][2 * i + 1], q1, dot[4 + j]);
+        }
+      }
+      float d[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = dot[j].x + dot[j].y;
+      // sum over r: lane r ends with sum r of S^T k (columns 0 .. 3), S^T q (columns 0 .. 3)
+#pragma unroll
+      for (int n = 4; n > 0; n >>= 1) {
+        const bool upper = (r & n) != 0;
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+          const float mine = upper ? d[n + j] : d[j], other = upper ? d[j] : d[n + j];
+          d[j] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
+        }
+      }
+      // lanes r < 4: u of column r; lanes r >= 4 pick it up for their output
+      const float gd = G * d[0];
+      const float u = sc.y * (sm.v[t][col + (r & 3)] - gd);
+      const float uo = __shfl_xor_sync(0xffffffffu, u, 16);
+      if (r >= 4) p.out[((tb + t) * p.heads + h) * DV + col + (r & 3)] = __float2bfloat16_rn(fmaf(sc.z, uo, gd));
+      const float ug = __fdividef(u, G);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        dot[j] = __ffma2_rn(S[j][i], k[i], dot[j]);
-        dot[4 + j] = __ffma2_rn(S[j][i], q[i], dot[4 + j]);
+        const float uj = __shfl_sync(0xffffffffu, ug, 4 * j + c);
+        const float2 uu = make_float2(uj, uj);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) S[j][i] = __ffma2_rn(k[i], uu, S[j][i]);
       }
-      kq = __ffma2_rn(k[i], q[i], kq);
-      kk = __ffma2_rn(k[i], k[i], kk);
-      qq = __ffma2_rn(q[i], q[i], qq);
-    }
-    float d[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] = dot[j].x + dot[j].y;
-    float skq = kq.x + kq.y, skk = kk.x + kk.y, sqq = qq.x + qq.y;
-    // sum over r: lane r ends with sum r of S^T k (columns 0 .. 3), S^T q (columns 0 .. 3)
-#pragma unroll
-    for (int n = 4; n > 0; n >>= 1) {
-      const bool upper = (r & n) != 0;
-#pragma unroll
-      for (int j = 0; j < n; ++j) {
-        const float mine = upper ? d[n + j] : d[j], other = upper ? d[j] : d[n + j];
-        d[j] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
-      }
-    }
-#pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      skq += __shfl_xor_sync(0xffffffffu, skq, off);
-      skk += __shfl_xor_sync(0xffffffffu, skk, off);
-      sqq += __shfl_xor_sync(0xffffffffu, sqq, off);
-    }
-    const float rk = p.l2norm ? rsqrtf(skk + 1e-6f) : 1.f;
-    const float rq = (p.l2norm ? rsqrtf(sqq + 1e-6f) : 1.f) * p.scale;
-    // lanes r < 4: u of column r times k's norm factor; lanes r >= 4 pick it up for their output
-    const float u = rk * x.beta * (x.v - G * rk * d[0]);
-    const float uo = __shfl_xor_sync(0xffffffffu, u, 16);
-    if (r >= 4) p.out[(t * p.heads + h) * DV + col + (r & 3)] = __float2bfloat16_rn(rq * fmaf(skq, uo, G * d[0]));
-    const float ug = u / G;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float uj = __shfl_sync(0xffffffffu, ug, 4 * j + c);
-      const float2 uu = make_float2(uj, uj);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) S[j][i] = __ffma2_rn(k[i], uu, S[j][i]);
     }
   }
   if (to >= 0) {
@@ -439,10 +441,8 @@ extern "C" int fdk_recurrent_gated_delta_rule_fwd(
   p.state_in = initial_state; p.in_idx = state_indices; p.in_slots = initial_slots;
   p.state_out = final_state; p.out_idx = final_indices; p.out_slots = final_slots;
   p.out = static_cast<bf16*>(out);
-  const int64_t warps = num_segments * heads * (DV / CPW);
-  const int64_t blocks = (warps + WARPS - 1) / WARPS;
-  if (blocks > 0x7fffffff) return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments", what);
-  recurrent_delta_kernel<<<(unsigned)blocks, 32 * WARPS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  if (num_segments * heads > 0x7fffffff) return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments", what);
+  recurrent_delta_kernel<<<(unsigned)(num_segments * heads), 32 * WARPS, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return check_launch(what);
 }
 

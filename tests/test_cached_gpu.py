@@ -534,6 +534,27 @@ def test_delta_transformers_signature_and_chunked_agree():
     assert no_error()
 
 
+@pytest.mark.parametrize("decay", [0.0, -3.0, -30.0, -80.0, -200.0, float("-inf"), 20.0])
+def test_delta_decays_of_any_size(decay):
+    # decays from none to total and growth, mixed with ordinary ones, over several tokens; with growth the
+    # state gets large, and bounds are relative to it
+    H, n = 3, 21
+    q, k, v, g, beta = delta_inputs(n, H, H, 68)
+    g[0, 2::3] = decay
+    g[0, 10] = decay
+    if decay > 0:
+        g[0, 2::3], g[0, 5] = 0.0, decay
+    pool = torch.randn(2, H, 128, 128, generator=gen(69)) * 0.5
+    d = pool.cuda()
+    o = ops.recurrent_gated_delta_rule_(q.cuda(), k.cuda(), v.cuda(), g.cuda(), beta.cuda(), d,
+                                        torch.tensor([0], dtype=torch.int32).cuda(),
+                                        torch.tensor([1], dtype=torch.int32).cuda())
+    assert no_error()
+    want, states = O.recurrent_delta(q[0], k[0], v[0], g[0], beta[0], pool[:1], [0, n])
+    delta_check(o[0], want)
+    state_check(d[1:], states)
+
+
 def test_delta_bad_metadata_and_refusals():
     H = 2
     q, k, v, g, beta = (t.cuda() for t in delta_inputs(6, H, H, 66))
