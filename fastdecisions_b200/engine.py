@@ -12,7 +12,11 @@ softmax, with the projections and MLP as cuBLAS GEMMs and every other op a kerne
   gate|up), the residual add is fused into the following RMSNorm, the attention output gate into
   the attention epilogue, and the last residual add into the slot readout (only slot rows);
 * fixed shapes (e.g. batch-1 decisions of one length) are captured once into a CUDA graph and
-  replayed, like the reference's bucketed graphs (engine.py:123-149).
+  replayed, like the reference's bucketed graphs (engine.py:123-149);
+* a prefix shared by many requests is computed once and kept on the device (``StateCache``: pages of
+  keys and values, convolution histories, recurrent states); requests behind it run their own tokens
+  only, straight from the shared pages and states (the reference copies transformers' dense caches
+  for every fork, src/decider/shared_prefix.py:42-200).
 """
 from __future__ import annotations
 
@@ -86,6 +90,87 @@ def pack(requests: Sequence[Request]) -> PackedBatch:
         raise ValueError("decision slot outside its request")
     nopts = np.array([r.nopts for r in requests], dtype=np.int32)
     return PackedBatch(ids, cu, pos, slots, nopts, int(lens.max()))
+
+
+# Gated-DeltaNet layers continued from a state: segments of at most this many tokens run the recurrent
+# form, longer ones the chunked one.
+RECURRENT_MAX_TOKENS = 32
+
+
+class Prefix:
+    """A token sequence whose keys, values and states are in a ``StateCache``."""
+
+    def __init__(self, cache: "StateCache", slot: int):
+        self.cache, self.slot, self.length, self.pages = cache, slot, 0, []
+
+    def release(self):
+        """Gives the pages and the state slot back (work already queued on the cache's stream order
+        still reads them first)."""
+        if self.slot is not None:
+            self.cache.free_pages.extend(self.pages)
+            self.cache.free_slots.append(self.slot)
+            self.slot, self.length, self.pages = None, 0, []
+
+
+class StateCache:
+    """Device state of cached prefixes for one engine: per attention layer a paged KV cache (``bf16`` or
+    ``e4m3`` with a scale per token and head), per Gated-DeltaNet layer a pool of convolution histories
+    and recurrent states.  Calls that use one cache must be on one stream (or ordered)."""
+
+    def __init__(self, cfg: ModelConfig, device, tokens: int, prefixes: int, page_size: int = 64,
+                 kv_dtype: str = "bf16"):
+        if kv_dtype not in ("bf16", "e4m3"):
+            raise ValueError("StateCache: kv_dtype must be 'bf16' or 'e4m3'")
+        if page_size not in (16, 32, 64, 128, 256) or tokens < 1 or prefixes < 1:
+            raise ValueError("StateCache: page_size 16 to 256 (a power of two), at least one token and prefix")
+        self.cfg, self.dev, self.page_size, self.kv_dtype = cfg, torch.device(device), page_size, kv_dtype
+        pages = -(-tokens // page_size)
+        hkv, D = cfg.num_key_value_heads, cfg.head_dim
+        Hk, Hv = cfg.linear_num_key_heads, cfg.linear_num_value_heads
+        C = 2 * Hk * cfg.linear_key_head_dim + Hv * cfg.linear_value_head_dim
+        kv = torch.float8_e4m3fn if kv_dtype == "e4m3" else torch.bfloat16
+        self.layers = []
+        for kind in cfg.layer_types:
+            if kind == "linear_attention":
+                self.layers.append(SimpleNamespace(
+                    conv=torch.zeros(prefixes, cfg.linear_conv_kernel_dim - 1, C, device=device, dtype=torch.bfloat16),
+                    state=torch.zeros(prefixes, Hv, cfg.linear_key_head_dim, cfg.linear_value_head_dim, device=device)))
+            else:
+                scale = [torch.zeros(pages, hkv, page_size, device=device, dtype=torch.uint8) if kv_dtype == "e4m3"
+                         else None for _ in range(2)]
+                self.layers.append(SimpleNamespace(
+                    k=torch.zeros(pages, hkv, page_size, D, device=device, dtype=kv),
+                    v=torch.zeros(pages, hkv, page_size, D, device=device, dtype=kv), ks=scale[0], vs=scale[1]))
+        self.free_pages = list(range(pages))[::-1]
+        self.free_slots = list(range(prefixes))[::-1]
+
+    def take_pages(self, n: int) -> list:
+        if n > len(self.free_pages):
+            raise RuntimeError(f"StateCache: {n} pages of {self.page_size} tokens needed, {len(self.free_pages)} free")
+        return [self.free_pages.pop() for _ in range(n)]
+
+    def copy_page(self, src: int, dst: torch.Tensor):
+        """Copies page ``src`` of every attention layer to the pages ``dst`` (int64, on the device)."""
+        for L in self.layers:
+            if hasattr(L, "k"):
+                for t in (L.k, L.v, L.ks, L.vs):
+                    if t is not None:
+                        u = t.view(torch.uint8)
+                        u[dst] = u[src].clone()
+
+
+@dataclass
+class CachedStep:
+    """Where one packed batch continues from: page table and lengths of its segments, the state slot each
+    starts from (-1: nothing before it) and leaves its state in (-1: nowhere)."""
+    cache: StateCache
+    page_table: torch.Tensor
+    kv_lens: torch.Tensor
+    max_kv_len: int
+    state_in: torch.Tensor
+    state_out: torch.Tensor
+    fresh: bool
+    keep: bool
 
 
 def plan_batches(lengths: Sequence[int], max_tokens: int) -> list:
@@ -242,11 +327,36 @@ class DecisionEngine:
             return _NULL
         return self.kernel_timer(name)
 
+    def _gdn_cached(self, L, state, proj: torch.Tensor, cu: torch.Tensor, max_seqlen: int, ws: torch.Tensor,
+                    step: CachedStep) -> torch.Tensor:
+        """The Gated-DeltaNet mixer core of ``proj`` continued from ``step``'s histories and states."""
+        c, tm = self.cfg, self._timed
+        Hk, Hv, Dk = c.linear_num_key_heads, c.linear_num_value_heads, c.linear_key_head_dim
+        kd, vd = Hk * Dk, Hv * c.linear_value_head_dim
+        C = 2 * kd + vd
+        with tm("packed_conv"):
+            q, k, v = ops.packed_conv_state_(proj[:, :C].unsqueeze(0), L.conv, state.conv, step.state_in,
+                                             step.state_out, kd, vd, Dk, cu)
+        with tm("gdn_gates"):
+            g, beta = ops.gdn_gates(proj[:, C + vd + Hv:C + vd + 2 * Hv], proj[:, C + vd:C + vd + Hv], L.A_log,
+                                    L.dt_bias)
+            g, beta = g.unsqueeze(0), beta.unsqueeze(0)
+        with tm("delta_rule"):
+            if max_seqlen <= RECURRENT_MAX_TOKENS:
+                return ops.recurrent_gated_delta_rule_(q, k, v, g, beta, state.state, step.state_in, step.state_out, cu)
+            init = None if step.fresh else state.state.index_select(0, step.state_in)
+            o, final = ops.chunk_gated_delta_rule(q, k, v, g, beta, initial_state=init, output_final_state=step.keep,
+                                                  cu_seqlens=cu, workspace=ws)
+            if step.keep:
+                state.state.index_copy_(0, step.state_out.long(), final)
+            return o
+
     def _mixer_mlp(self, i: int, x: torch.Tensor, h: torch.Tensor, cu: torch.Tensor, pos: torch.Tensor,
-                   max_seqlen: int, ws: torch.Tensor):
+                   max_seqlen: int, ws: torch.Tensor, step: Optional[CachedStep] = None):
         """Layer ``i`` given its normalised input ``x`` (bf16) and the residual stream ``h``:
         token mixer, residual add fused into post_attention_layernorm, SwiGLU MLP.  Updates ``h`` in
-        place to ``h + mixer`` and returns the MLP output (the caller adds it)."""
+        place to ``h + mixer`` and returns the MLP output (the caller adds it).  With ``step`` the
+        segments continue from cached state."""
         c = self.cfg
         L = self.layers[i]
         T = x.shape[0]
@@ -259,7 +369,9 @@ class DecisionEngine:
         if L.kind == "linear_attention":
             with tm("gemm"):
                 proj = torch.matmul(x, L.w_in.t())                                       # [T, C + vd + 2 Hv]
-            if self.fuse_gdn_prologue and Hk == Hv and Dk == Dv == 128:
+            if step is not None:
+                o = self._gdn_cached(L, step.cache.layers[i], proj, cu, max_seqlen, ws, step)
+            elif self.fuse_gdn_prologue and Hk == Hv and Dk == Dv == 128:
                 # conv + SiLU, gates and the chunked delta rule in one call on the projection
                 with tm("delta_rule"):
                     o = ops.gdn_fused_delta_rule(proj, L.conv, L.A_log, L.dt_bias, Hv, C + vd + Hv, C + vd, cu,
@@ -288,8 +400,16 @@ class DecisionEngine:
                 with tm("qk_norm_rope"):
                     q, k = ops.attn_qk_norm_rope(proj, L.q_norm, L.k_norm, pos, self.rope, hq, hkv, D, c.rms_norm_eps)
             v = proj[:, (2 * hq + hkv) * D:].view(T, hkv, D)
-            with tm("gqa_attention"):
-                o = ops.gqa_attention_varlen_(q, k, v, cu, max_seqlen, gate=proj[:, D:], gate_interleaved=True)
+            if step is not None:
+                kv = step.cache.layers[i]
+                with tm("paged_kv_write"):
+                    ops.paged_kv_write(k, v, kv.k, kv.v, step.page_table, cu, step.kv_lens, kv.ks, kv.vs)
+                with tm("gqa_attention"):
+                    o = ops.paged_gqa_attention(q, kv.k, kv.v, step.page_table, cu, step.kv_lens, max_seqlen,
+                                                step.max_kv_len, kv.ks, kv.vs, gate=proj[:, D:], gate_interleaved=True)
+            else:
+                with tm("gqa_attention"):
+                    o = ops.gqa_attention_varlen_(q, k, v, cu, max_seqlen, gate=proj[:, D:], gate_interleaved=True)
             mix_in, w_mix = o.view(T, hq * D), L.w_o
         fused_res = self.fused_residual_gemm and T >= FUSED_RESIDUAL_MIN_TOKENS
         H = c.hidden_size
@@ -332,9 +452,11 @@ class DecisionEngine:
     @torch.no_grad()
     def forward_device(self, ids: torch.Tensor, cu: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
                        nopts: torch.Tensor, max_seqlen: int, probs: Optional[torch.Tensor] = None,
-                       logits: Optional[torch.Tensor] = None, trace: Optional[list] = None):
+                       logits: Optional[torch.Tensor] = None, trace: Optional[list] = None,
+                       step: Optional[CachedStep] = None):
         """All inputs int32 on the engine's device.  Returns ``(probs, logits)`` float32 ``[S, K]``.
-        ``trace`` (a list, diagnostics only) receives the residual stream after every layer."""
+        ``trace`` (a list, diagnostics only) receives the residual stream after every layer.  ``step``:
+        the segments continue from cached state (``pos`` counts from their prefixes' ends)."""
         c = self.cfg
         ws = self._workspace(ids.numel(), cu.numel() - 1)
         self.stats["forwards"] += 1
@@ -346,7 +468,7 @@ class DecisionEngine:
                                         residual_fp32=self.residual_fp32)
         down = None
         for i in range(len(self.layers)):
-            down = self._mixer_mlp(i, x, h, cu, pos, max_seqlen, ws)
+            down = self._mixer_mlp(i, x, h, cu, pos, max_seqlen, ws, step)
             if isinstance(down, tuple):  # k-split partial planes of the down-projection
                 parts = self._partials(h.shape[0], down[1])
                 with tm("residual_rmsnorm"):
@@ -477,6 +599,104 @@ class DecisionEngine:
         order = np.concatenate([np.asarray(b, dtype=np.int64) for b in plan])
         result = np.empty((len(requests), K), dtype=np.float32)
         result[order] = host_out.numpy()
+        return result
+
+    # ------------------------------------------------------------------ cached prefixes
+    def open_cache(self, tokens: int, prefixes: int = 8, page_size: int = 64, kv_dtype: str = "bf16") -> StateCache:
+        """Device memory for ``prefixes`` cached prefixes and ``tokens`` cached positions in total, the ones
+        that ``score_after`` needs for its requests while they run included (``kv_dtype`` ``"e4m3"``
+        halves the positions' size)."""
+        return StateCache(self.cfg, self.dev, tokens, prefixes, page_size, kv_dtype)
+
+    def _run_cached(self, cache: StateCache, batch: PackedBatch, past: int, tables: Sequence[Sequence[int]],
+                    state_in: int, state_out: int) -> torch.Tensor:
+        """One packed batch whose segments all continue from ``past`` positions and state ``state_in``."""
+        S = batch.num_segments
+        lens = np.diff(batch.cu_seqlens) + past
+        width = max(len(t) for t in tables)
+        table = np.zeros((S, width), dtype=np.int32)
+        for row, t in zip(table, tables):
+            row[:len(t)] = t
+        meta = np.concatenate([lens.astype(np.int32), np.full(S, state_in, np.int32), np.full(S, state_out, np.int32),
+                               table.reshape(-1)])
+        batch = PackedBatch(batch.ids, batch.cu_seqlens, batch.positions + np.int32(past), batch.slots, batch.nopts,
+                            batch.max_seqlen)
+        (ids, cu, pos, slots, nopts), _ = self.to_device(batch)
+        dev = torch.from_numpy(meta).pin_memory().to(self.dev, non_blocking=True)
+        step = CachedStep(cache, dev[3 * S:].view(S, width), dev[:S], int(lens.max()), dev[S:2 * S], dev[2 * S:3 * S],
+                          fresh=state_in < 0, keep=state_out >= 0)
+        return self.forward_device(ids, cu, pos, slots, nopts, batch.max_seqlen, step=step)[0]
+
+    @torch.no_grad()
+    def extend(self, prefix: Prefix, ids) -> Prefix:
+        """Appends tokens to a cached prefix (its pages grow, its states advance in place)."""
+        ids = np.asarray(ids, dtype=np.int32).reshape(-1)
+        cache, total = prefix.cache, prefix.length + ids.size
+        if prefix.slot is None:
+            raise ValueError("extend: the prefix was released")
+        if ids.size < 1 or total > self.max_positions:
+            raise ValueError(f"extend: at least one token and at most {self.max_positions} positions")
+        prefix.pages += cache.take_pages(-(-total // cache.page_size) - len(prefix.pages))
+        batch = pack([Request(ids=ids, slot=ids.size - 1, nopts=1)])
+        self._run_cached(cache, batch, prefix.length, [prefix.pages], prefix.slot if prefix.length else -1, prefix.slot)
+        prefix.length = total
+        return prefix
+
+    def cache_prefix(self, cache: StateCache, ids) -> Prefix:
+        """Runs ``ids`` once and keeps their keys, values and states for ``score_after``."""
+        if not cache.free_slots:
+            raise RuntimeError("StateCache: no free prefix slot")
+        prefix = Prefix(cache, cache.free_slots.pop())
+        try:
+            return self.extend(prefix, ids)
+        except Exception:
+            prefix.release()
+            raise
+
+    @torch.no_grad()
+    def score_after(self, prefix: Prefix, requests: Sequence[Request], max_tokens: int = 32768) -> np.ndarray:
+        """``score`` of requests behind a cached prefix: probabilities ``[N, K]`` as if each request's ids
+        followed the prefix's (``slot`` counts within the request's own ids), running only the requests'
+        tokens.  Whole pages of the prefix are shared by all of them; the positions of its last, partial
+        page are copied to each request's first own page.  The prefix itself is not changed."""
+        if prefix.slot is None:
+            raise ValueError("score_after: the prefix was released")
+        if len(requests) == 0:
+            return np.zeros((0, self.letters.shape[0]), dtype=np.float32)
+        cache, past, size = prefix.cache, prefix.length, prefix.cache.page_size
+        lens = [int(r.ids.size) for r in requests]
+        if min(lens) < 1 or past + max(lens) > self.max_positions:
+            raise ValueError(f"score_after: at least one token a request and at most {self.max_positions} positions")
+        shared, part = past // size, past % size
+        result = np.empty((len(requests), self.letters.shape[0]), dtype=np.float32)
+        # batches of at most max_tokens tokens whose own pages are free: they are given back after each
+        plan, room = [], len(cache.free_pages)
+        for b in plan_batches(lens, max_tokens):
+            need, cur = 0, []
+            for i in b:
+                n = -(-(part + lens[i]) // size)
+                if n > room:
+                    raise RuntimeError(f"StateCache: {n} free pages needed for one request, {room} free")
+                if need + n > room:
+                    plan.append(cur)
+                    need, cur = 0, []
+                need += n
+                cur.append(i)
+            plan.append(cur)
+        outs = []
+        for b in plan:
+            batch = pack([requests[i] for i in b])
+            own = [cache.take_pages(-(-(part + lens[i]) // size)) for i in b]
+            try:
+                if part:
+                    first = torch.tensor([o[0] for o in own], dtype=torch.int64).pin_memory()
+                    cache.copy_page(prefix.pages[shared], first.to(self.dev, non_blocking=True))
+                outs.append(self._run_cached(cache, batch, past, [prefix.pages[:shared] + o for o in own], prefix.slot,
+                                             -1))
+            finally:
+                for o in own:  # the next batch's kernels are ordered behind this one's on the stream
+                    cache.free_pages.extend(o)
+        result[np.concatenate([np.asarray(b, dtype=np.int64) for b in plan])] = torch.cat(outs).cpu().numpy()
         return result
 
     # ------------------------------------------------------------------ CUDA graphs
