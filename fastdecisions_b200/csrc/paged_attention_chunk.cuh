@@ -8,7 +8,9 @@
 //     PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): the softmax of one tile overlaps the MMAs of the other.
 //     TMEM: S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512).
 //   head_dim 256: one tile (two would not fit TMEM), KV blocks of 64 keys, S ping-pong one block ahead.
-//     TMEM: S0 [0,64) S1 [64,128) O [256,512).
+//     TMEM: S0 [0,64) S1 [64,128) Q [128,256) O [256,512).  Q is the S MMA's A operand from TMEM: read
+//     from shared memory it would be 64 of the 192 KB a block moves there, and its 64 KB make room for
+//     more KV slots.
 //   P overwrites S in TMEM (A operand of the PV MMA).  Softmax: thread = row = TMEM lane, online in the
 //   exp2 domain, O rescaled only when the running maximum grows by more than 2^8.
 //
@@ -41,23 +43,25 @@ struct Geo {
   static constexpr int NBX = D / 64;                   // 64-column (128-byte) boxes of a row
   static constexpr uint32_t QBOX = 128 * 128, KBOX = (uint32_t)BN * 128;
   static constexpr uint32_t QT = NBX * QBOX, KT = NBX * KBOX;
+  static constexpr bool Q_TMEM = D == 256;
+  static constexpr uint32_t TM_Q = 128;
   static constexpr uint32_t TM_S(int i) { return (uint32_t)(BN * i); }         // tile i, or ping-pong buffer i
   static constexpr uint32_t TM_O(int i) { return 256u + 128u * (uint32_t)i; }  // tile i
 };
 // Shared memory: Q tiles, operand ring, raw ring (8-bit cache), barriers and small state.
 // barriers: F / E operand slot full / empty, RF / RE raw slot full / empty, S and P per tile or buffer;
 // VT: V of the block that ends past kv_lens, before its tail is zeroed
-enum { B_Q = 0, B_F, B_E = B_F + 4, B_RF = B_E + 4, B_RE = B_RF + 4, B_S = B_RE + 4, B_P = B_S + 2, B_VT = B_P + 2,
+enum { B_Q = 0, B_F, B_E = B_F + 6, B_RF = B_E + 6, B_RE = B_RF + 4, B_S = B_RE + 4, B_P = B_S + 2, B_VT = B_P + 2,
        B_PV, B_O, NBAR };
 constexpr int RAW_SLOTS = 4;
 template <int D, bool QUANT>
 struct Smem {
   using G = Geo<D>;
-  static constexpr int SLOTS = QUANT ? 3 : 4;
+  static constexpr int SLOTS = G::Q_TMEM ? (QUANT ? 4 : 6) : QUANT ? 3 : 4;
   static constexpr uint32_t RAWT = QUANT ? (uint32_t)(G::BN * D) : 0;  // bytes of a raw tile
-  static constexpr uint32_t OFF_Q = 0, OFF_KV = G::NT * G::QT, OFF_RAW = OFF_KV + SLOTS * G::KT,
+  static constexpr uint32_t OFF_Q = 0, OFF_KV = G::Q_TMEM ? 0 : G::NT * G::QT, OFF_RAW = OFF_KV + SLOTS * G::KT,
                             OFF_BAR = OFF_RAW + RAW_SLOTS * RAWT, OFF_MISC = OFF_BAR + 8 * NBAR,
-                            OFF_QS = OFF_MISC + 64,                       // row scale exponents of q: 256 bytes
+                            OFF_QS = OFF_MISC + 64,                       // row scale exponents of q: 256 bytes (head_dim 128)
                             OFF_FT = OFF_QS + (QUANT ? 256 : 0),          // row factors of two tiles: half2
                             BYTES = OFF_FT + (QUANT ? 1024 : 0) + 1024;   // + slack for 1024-byte alignment
   static_assert(OFF_MISC % 16 == 0, "alignment of the small state");
@@ -272,8 +276,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;
       if (i == B_P || i == B_P + 1) count = 128;
-      if (QUANT && i == B_Q) count = two ? 256 : 128;
-      if (QUANT && ((i >= B_F && i < B_F + 4) || (i >= B_RE && i < B_RE + 4))) count = 128;
+      if ((QUANT || G::Q_TMEM) && i == B_Q) count = two ? 256 : 128;
+      if (QUANT && ((i >= B_F && i < B_F + 6) || (i >= B_RE && i < B_RE + 4))) count = 128;
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -303,7 +307,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     if (lane == 0) {
       prefetch_tmap(&tk);
       prefetch_tmap(&tv);
-      if (!QUANT) {
+      if (!QUANT && !G::Q_TMEM) {
         const int tiles = two ? 2 : 1;
         mbar_expect_tx(bar(B_Q), (uint32_t)(tiles * NBX) * 128u * (uint32_t)rpt);
         for (int i = 0; i < tiles; ++i)
@@ -360,7 +364,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     }
     // drain: every issued load must have landed before shared memory is released
     if (lane == 0) {
-      if (!QUANT) drain(bar(B_Q), 0);
+      if (!QUANT && !G::Q_TMEM) drain(bar(B_Q), 0);
       for (int i = (issued > RING ? issued - RING : 0); i < issued; ++i) drain(bar(FULL + i % RING), (uint32_t)(i / RING) & 1u);
     }
   };
@@ -379,12 +383,13 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       constexpr uint32_t ID_QK = idesc(128, BN, false, QUANT);
       constexpr uint32_t ID_PV = idesc(128, D, true, QUANT);  // V is MN-major (columns contiguous)
       auto issue_s = [&](int j, int tile, uint32_t tm) {
-        const uint64_t dq = sdesc_sw128(base + M::OFF_Q + tile * G::QT, 16, 1024);
+        const uint64_t dq = G::Q_TMEM ? 0 : sdesc_sw128(base + M::OFF_Q + tile * G::QT, 16, 1024);
         const uint64_t dk = sdesc_sw128(base + M::OFF_KV + (2 * j % M::SLOTS) * G::KT, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t qo = ((kk >> 2) * G::QBOX + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * G::KBOX + (kk & 3) * 32) >> 4;
-          umma_ss(tmem + tm, dq + qo, dk + ko, ID_QK, kk > 0);
+          if (G::Q_TMEM) umma_ts(tmem + tm, tmem + G::TM_Q + 8 * kk, dk + ko, ID_QK, kk > 0);
+          else umma_ss(tmem + tm, dq + qo, dk + ko, ID_QK, kk > 0);
         }
       };
       auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o) {
@@ -574,7 +579,51 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     float r_run = -INFINITY, l_run = 0.f;  // running maximum (unscaled) and sum
     bool ok = tile == 0 || two;
     float sl2 = p.sl2;
-    if (QUANT && ok) {
+    if (G::Q_TMEM) {
+      // q's row of this thread to its TMEM lane, two elements a column; 8-bit cache: as fp16 with the row's
+      // largest magnitude in [1, 2)
+      const bf16* src = p.q + (int64_t)(seg.begin + (valid ? tok : 0)) * p.ld_q + (int64_t)(hk * p.group + (valid ? row % p.group : 0)) * D;
+      float inv = 1.f, unit = 1.f;
+      if (QUANT) {
+        float a = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < D / 8; ++c) {
+          float f[8];
+          unpack8(__ldg(reinterpret_cast<const uint4*>(src) + c), f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
+        }
+        const int e = a == 0.f ? 127 : min(max((int)(__float_as_uint(a) >> 23), 1), 253);
+        inv = __uint_as_float((uint32_t)(254 - e) << 23);
+        unit = __uint_as_float((uint32_t)e << 23);
+      }
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c) {
+        uint4 w[8];
+        uint32_t col[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(src) + c * 8 + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ww[u]));
+            col[4 * i + u] = QUANT ? pack_f16x2(x.x * inv, x.y * inv) : ww[u];
+          }
+        }
+        tmem_st32(tmem + lane_base + G::TM_Q + c * 32, col);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(bar(B_Q));
+      if (QUANT) {
+        // S of the first block follows the scale maxima
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_S), 0, abort_flag) ? 1 : 0);
+        // never 0: a masked score is -inf * sl2
+        if (ok) sl2 = fmaxf(sl2 * unit * scale_value(scale_max[0]), 1e-37f);
+      }
+    } else if (QUANT && ok) {
       // this tile's q: D / 8 threads a row, fp16 with the row's largest magnitude in [1, 2)
       constexpr int TPR = D / 8, RPP = 128 / TPR;
       const int ct = tid & 127, lc = ct % TPR, lr = ct / TPR;
@@ -809,7 +858,7 @@ static int launch(const Params& p, int64_t row_tiles, cudaStream_t s) {
   const cuuint64_t vs[3] = {(cuuint64_t)D * esz, ps * D * esz, (cuuint64_t)p.vpage};
   if (int st = encode(&mk, p.k_cache, QUANT, 4, kd, ks, kb)) return st;
   if (int st = encode(&mv, p.v_cache, QUANT, 4, kd, vs, kb)) return st;
-  if (!QUANT) {
+  if (!QUANT && !G::Q_TMEM) {
     const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)p.hq, (cuuint64_t)p.tokens};
     const cuuint64_t qs[2] = {(cuuint64_t)D * 2, (cuuint64_t)p.ld_q * 2};
     const cuuint32_t qb[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(128 / p.group)};
