@@ -50,6 +50,7 @@ struct Params {
   int64_t tokens, num_pages;
   int nseg, max_pages, page_shift, hq, hkv, group, nsplit, row_blocks;
   int split_keys;  // keys a split (a multiple of every tile's), the last one takes what is left
+  int block_rows;  // rows of a row block (a CTA's)
   int picked;      // many rows: x counts the call's row tiles, longest first
   float sl2;  // softmax scale * log2(e)
   const bf16* gate;
@@ -89,6 +90,9 @@ __device__ __forceinline__ void split_range(const Params& p, int split, int kend
   kb = (int)min((int64_t)kend, (int64_t)split * p.split_keys);
   ke = split == p.nsplit - 1 ? kend : (int)min((int64_t)kend, (int64_t)kb + p.split_keys);
 }
+// Whether a row block that sees keys [0, kend) is computed in parts.  One that fits a split is not: its CTA
+// writes the result and the join passes over its rows.
+__device__ __forceinline__ bool in_parts(const Params& p, int64_t kend) { return p.nsplit > 1 && kend > p.split_keys; }
 // Parts of a row that sees `visible` keys: the splits that hold one of them (at least one is written).
 __device__ __forceinline__ int parts_of(const Params& p, int64_t visible) {
   return visible <= p.split_keys ? 1 : (int)min((int64_t)p.nsplit, (visible + p.split_keys - 1) / p.split_keys);
@@ -539,7 +543,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     const int64_t tok = seg.begin + gr / p.group;
     const int head = hk * p.group + gr % p.group;
     const int64_t idx = tok * p.hq + head;
-    if (p.nsplit > 1) {
+    if (in_parts(p, kend)) {
       float* dst = p.part_o + ((int64_t)split * p.tokens * p.hq + idx) * D + c;
       *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
@@ -579,6 +583,10 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int64_t idx = tok * p.hq + head, plane = p.tokens * p.hq;
   int64_t len = p.kv_lens[s];
   if (len < 0 || len > ((int64_t)p.max_pages << p.page_shift)) len = 0;
+  // the last token of the row's block decides whether there are parts
+  const int n = end - p.cu[s], row = (int)(tok - p.cu[s]) * p.group + head % p.group;
+  const int last = min((row / p.block_rows + 1) * p.block_rows, n * p.group) - 1;
+  if (!in_parts(p, len - n + last / p.group + 1)) return;
   const int parts = parts_of(p, len - (end - tok) + 1);
   float mm = -INFINITY;
   for (int i = 0; i < parts; ++i) mm = fmaxf(mm, p.part_ml[i * plane + idx].x);
@@ -793,6 +801,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
   p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks; p.split_keys = pl.split_keys;
   p.picked = pl.picked;
+  p.block_rows = pl.many ? (head_dim == 128 ? 2 : 1) * (128 / p.group) * p.group : pl.rows;
   p.sl2 = scale * 1.4426950408889634f;
   p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
   p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);

@@ -5,7 +5,8 @@
 // padding of short chunks to 128 tokens a head, and K/V are read once a group, not once a head.
 //
 //   head_dim 128: a CTA owns two 128-row tiles A, B, KV blocks of 128 keys.  Issue order per block j:
-//     PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): the softmax of one tile overlaps the MMAs of the other.
+//     PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): the softmax of one tile overlaps the MMAs of the other, and
+//     PV starts on the block's first 64 keys while the softmax computes the weights of the other 64.
 //     TMEM: S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512).
 //   head_dim 256: one tile (two would not fit TMEM), KV blocks of 64 keys, S ping-pong one block ahead.
 //     TMEM: S0 [0,64) S1 [64,128) Q [128,256) O [256,512).  Q is the S MMA's A operand from TMEM: read
@@ -49,9 +50,11 @@ struct Geo {
   static constexpr uint32_t TM_O(int i) { return 256u + 128u * (uint32_t)i; }  // tile i
 };
 // Shared memory: Q tiles, operand ring, raw ring (8-bit cache), barriers and small state.
-// barriers: F / E operand slot full / empty, RF / RE raw slot full / empty, S and P per tile or buffer;
+// barriers: F / E operand slot full / empty, RF / RE raw slot full / empty, S and P per tile or buffer (P2: P's
+// second 64 keys, two tiles);
 // VT: V of the block that ends past kv_lens, before its tail is zeroed
-enum { B_Q = 0, B_F, B_E = B_F + 6, B_RF = B_E + 6, B_RE = B_RF + 4, B_S = B_RE + 4, B_P = B_S + 2, B_VT = B_P + 2,
+enum { B_Q = 0, B_F, B_E = B_F + 6, B_RF = B_E + 6, B_RE = B_RF + 4, B_S = B_RE + 4, B_P = B_S + 2, B_P2 = B_P + 2,
+       B_VT = B_P2 + 2,
        B_PV, B_O, NBAR };
 constexpr int RAW_SLOTS = 4;
 template <int D, bool QUANT>
@@ -106,6 +109,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// 2^x for two x <= 64 on the float32 pipe, for the share of the weights that would leave the softmax waiting for
+// the special-function unit (16 results a clock and SM, half of what its two tiles take): x = n + f with
+// |f| <= 1/2, 2^f by a cubic fitted to the least relative error (2^-13.7, below the fp16 and bf16
+// roundings of P), 2^n from the bits of n + 127.  x below -126.5 gives 0; NaN stays NaN.
+constexpr int EXP_POLY = 3;  // every 3rd pair of columns (2: 268 us, 3: 259, 4: 261, 6: 261, none: 264 for 2 x 2048 tokens behind 6144 and 7543)
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n" : "+f"(x.x));  // -127: the factor 2^n below is then 0
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n" : "+f"(x.y));
+  const float magic = 12582912.f + 127.f;  // 1.5 * 2^23: its sum with x holds round(x) + 127 in the low bits
+  const float2 t = __fadd2_rn(x, make_float2(magic, magic));
+  const float2 n = __fadd2_rn(t, make_float2(-magic, -magic));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 y = make_float2(0.0551716685f, 0.0551716685f);
+  y = __ffma2_rn(y, f, make_float2(0.2426111251f, 0.2426111251f));
+  y = __ffma2_rn(y, f, make_float2(0.6932609677f, 0.6932609677f));
+  y = __ffma2_rn(y, f, make_float2(0.9999280572f, 0.9999280572f));
+  return __fmul2_rn(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
@@ -256,16 +277,13 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   split_range(p, split, kend, kb, ke);
   if (kb >= ke && split > 0) return;  // the join does not read this part
   const int n_kv = (ke - kb + BN - 1) / BN;
-  if (n_kv == 0) {  // no keys at all: zeros, or an empty part
+  const bool part = in_parts(p, kend);
+  if (n_kv == 0) {  // no keys at all: zeros
     for (int e = tid; e < NT * rpt; e += R::THREADS) {
       const int64_t gr = (int64_t)tok0 * p.group + e;
       if (gr >= rows) break;
       const int64_t idx = (seg.begin + gr / p.group) * p.hq + hk * p.group + gr % p.group;
-      if (p.nsplit > 1) {
-        p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(-INFINITY, 0.f);
-      } else {
-        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(p.out + idx * D + c) = make_uint4(0u, 0u, 0u, 0u);
-      }
+      for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(p.out + idx * D + c) = make_uint4(0u, 0u, 0u, 0u);
     }
     return;
   }
@@ -275,7 +293,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   if (tid == 0) {
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;
-      if (i == B_P || i == B_P + 1) count = 128;
+      if (i >= B_P && i < B_P2 + 2) count = 128;
       if ((QUANT || G::Q_TMEM) && i == B_Q) count = two ? 256 : 128;
       if (QUANT && ((i >= B_F && i < B_F + 6) || (i >= B_RE && i < B_RE + 4))) count = 128;
       mbar_init(bar(i), count);
@@ -392,10 +410,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           else umma_ss(tmem + tm, dq + qo, dk + ko, ID_QK, kk > 0);
         }
       };
-      auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o) {
+      auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o, int k0) {
         const uint64_t dv = sdesc_sw128(base + M::OFF_KV + ((2 * j + 1) % M::SLOTS) * G::KT, G::KBOX, 1024);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
+        for (int kk = k0; kk < k0 + 4; ++kk)  // 64 keys
           umma_ts(tmem + tm_o, tmem + tm_p + 8 * kk, dv + (uint32_t)(kk * 2048 >> 4), ID_PV, (j > 0 || kk > 0) ? 1u : 0u);
       };
       auto wait = [&](int i, int parity) { return mbar_wait(bar(i), (uint32_t)parity & 1u, abort_flag); };
@@ -417,7 +435,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           const bool more = j + 1 < n_kv;
           if (!full(2 * j + 1) || !wait(B_P, j)) break;
           tc_fence_after();
-          issue_pv(j, G::TM_S(0), G::TM_O(0));
+          issue_pv(j, G::TM_S(0), G::TM_O(0), 0);
+          if (!wait(B_P2, j)) break;
+          tc_fence_after();
+          issue_pv(j, G::TM_S(0), G::TM_O(0), 4);
           if (more) {
             if (!full(2 * j + 2)) break;
             tc_fence_after();
@@ -427,7 +448,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           if (two) {
             if (!wait(B_P + 1, j)) break;
             tc_fence_after();
-            issue_pv(j, G::TM_S(1), G::TM_O(1));
+            issue_pv(j, G::TM_S(1), G::TM_O(1), 0);
+            if (!wait(B_P2 + 1, j)) break;
+            tc_fence_after();
+            issue_pv(j, G::TM_S(1), G::TM_O(1), 4);
           }
           release(2 * j + 1);
           if (more) {
@@ -455,7 +479,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         for (int j = 0; ok && j < n_kv; ++j) {
           if (!full(2 * j + 1) || !wait(B_P + (j & 1), j >> 1)) break;
           tc_fence_after();
-          issue_pv(j, G::TM_S(j & 1), G::TM_O(0));
+          issue_pv(j, G::TM_S(j & 1), G::TM_O(0), 0);
           umma_commit(bar(B_PV));
           release(2 * j + 1);
           if (j + 2 < n_kv) {
@@ -703,35 +727,6 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       // a row that has seen nothing yet: every exponent below is -inf
       const float r0 = r_run == -INFINITY ? 0.f : r_run;
       const float shift = r0 * sl2 - (QUANT ? P_SHIFT : 0.f);
-      float2 sum4[4];  // packed float32: two columns an operation
-#pragma unroll
-      for (int a = 0; a < 4; ++a) sum4[a] = make_float2(0.f, 0.f);
-      uint32_t pk[BN / 64][32];
-      auto weights = [&](auto expo) {
-#pragma unroll
-        for (int c = 0; c < BN / 2; ++c) {
-          const float2 x = expo(make_float2(__uint_as_float(sr[(2 * c) >> 5][(2 * c) & 31]),
-                                            __uint_as_float(sr[(2 * c + 1) >> 5][(2 * c + 1) & 31])));
-          const float2 e = make_float2(ex2(x.x), ex2(x.y));
-          sum4[c & 3] = __fadd2_rn(sum4[c & 3], e);
-          pk[c >> 5][c & 31] = QUANT ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
-        }
-      };
-      const float2 sl2v = make_float2(sl2, sl2);
-      // s * sl2 - shift in one operation, unless scores are so large that shift's own rounding (float32
-      // spacing 0.25 and more) would show in the exponent
-      if (!__any_sync(0xffffffffu, fabsf(shift) > 2097152.f))
-        weights([&](float2 x) { return __ffma2_rn(x, sl2v, make_float2(-shift, -shift)); });
-      else
-        weights([&](float2 x) {
-          const float up = QUANT ? P_SHIFT : 0.f;
-          return __ffma2_rn(make_float2(x.x - r0, x.y - r0), sl2v, make_float2(up, up));
-        });
-#pragma unroll
-      for (int c = 0; c < BN / 64; ++c) tmem_st32(tS + c * 32, pk[c]);
-      const float2 sum2 = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
-      const float sum = sum2.x + sum2.y;
-      l_run = l_run * alpha + sum;
       if (__any_sync(0xffffffffu, rescale)) {  // O row *= alpha
         // NT == 2: S_j's commit covers PV(j-1) of this tile; NT == 1: it covers PV(j-2), so wait for PV(j-1)
         if (NT == 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_PV), (j - 1) & 1, abort_flag) ? 1 : 0)) {
@@ -749,9 +744,40 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           tmem_st32(tO + c * 32, o);
         }
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(bar(B_P + buf));
+      float2 sum4[4];  // packed float32: two columns an operation
+#pragma unroll
+      for (int a = 0; a < 4; ++a) sum4[a] = make_float2(0.f, 0.f);
+      const float2 sl2v = make_float2(sl2, sl2);
+      // s * sl2 - shift in one operation, unless scores are so large that shift's own rounding (float32
+      // spacing 0.25 and more) would show in the exponent
+      const bool large = __any_sync(0xffffffffu, fabsf(shift) > 2097152.f);
+#pragma unroll
+      for (int half = 0; half < BN / 64; ++half) {
+        uint32_t pk[32];
+        auto weights = [&](auto expo) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int i = half * 64 + 2 * c;
+            const float2 x = expo(make_float2(__uint_as_float(sr[i >> 5][i & 31]), __uint_as_float(sr[(i + 1) >> 5][(i + 1) & 31])));
+            const float2 e = NT == 2 && c % EXP_POLY == EXP_POLY - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum4[c & 3] = __fadd2_rn(sum4[c & 3], e);
+            pk[c] = QUANT ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
+          }
+        };
+        if (!large)
+          weights([&](float2 x) { return __ffma2_rn(x, sl2v, make_float2(-shift, -shift)); });
+        else
+          weights([&](float2 x) {
+            const float up = QUANT ? P_SHIFT : 0.f;
+            return __ffma2_rn(make_float2(x.x - r0, x.y - r0), sl2v, make_float2(up, up));
+          });
+        tmem_st32(tS + half * 32, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar(half == 0 ? B_P + buf : B_P2 + buf));
+      }
+      const float2 sum2 = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
+      l_run = l_run * alpha + (sum2.x + sum2.y);
     }
     // ------------------------------------------------------------------ epilogue
     if (ok && __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0, abort_flag) ? 1 : 0)) {
@@ -761,8 +787,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       const int64_t idx = tk_ * p.hq + head;
       // l and O both carry 2^P_SHIFT with the 8-bit cache; O is in units of V's largest scale
       const float unit = QUANT ? scale_value(scale_max[1]) : 1.f;
-      const float inv = p.nsplit > 1 ? unit : (l_run > 0.f ? unit / l_run : (l_run == 0.f ? 0.f : l_run));
-      const bool part = p.nsplit > 1;
+      const float inv = part ? unit : (l_run > 0.f ? unit / l_run : (l_run == 0.f ? 0.f : l_run));
       float* prow = part ? p.part_o + ((int64_t)split * p.tokens * p.hq + idx) * D : nullptr;
       if (part && valid) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(r_run * sl2, l_run);
       bf16* orow = p.out + idx * D;
