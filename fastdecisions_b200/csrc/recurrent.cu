@@ -242,12 +242,18 @@ struct ConvParams {
   bf16* v;
 };
 
+// silu(x) = h + h tanh(h), h = x / 2, of two channels as bf16
+__device__ __forceinline__ uint32_t silu2(float2 x) {
+  const float2 h = __fmul2_rn(make_float2(0.5f, 0.5f), x);
+  const float2 y = __ffma2_rn(h, make_float2(tanh_approx(h.x), tanh_approx(h.y)), h);
+  return pack_bf16x2(y.x, y.y);
+}
+
 // One output row of 8 channels from its KW input rows, two channels an operation.
 template <int KW>
 __device__ __forceinline__ void conv_row(const uint4 (&rows)[KW], const float2 (&w)[KW][4], bf16* dst) {
   uint4 out;
   uint32_t* o = reinterpret_cast<uint32_t*>(&out);
-  const float2 half2_ = make_float2(0.5f, 0.5f);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     float2 acc = make_float2(0.f, 0.f);
@@ -257,9 +263,7 @@ __device__ __forceinline__ void conv_row(const uint4 (&rows)[KW], const float2 (
       const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b));
       acc = j == 0 ? __fmul2_rn(w[0][c], x) : __ffma2_rn(w[j][c], x, acc);
     }
-    const float2 h = __fmul2_rn(half2_, acc);  // silu(x) = h + h tanh(h), h = x / 2
-    const float2 y = __ffma2_rn(h, make_float2(tanh_approx(h.x), tanh_approx(h.y)), h);
-    o[c] = pack_bf16x2(y.x, y.y);
+    o[c] = silu2(acc);
   }
   *reinterpret_cast<uint4*>(dst) = out;
 }
@@ -352,6 +356,12 @@ __global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
   const int64_t r0 = (job - p.nseg) * RPT;
   if (r0 >= p.tokens) return;
   const int64_t r1 = r0 + RPT < p.tokens ? r0 + RPT : p.tokens;
+  uint4 raw[RPT + HR];  // loaded before the segment is looked up: neither needs the other
+#pragma unroll
+  for (int j = 0; j < RPT + HR; ++j) {
+    const int64_t t = r0 - HR + j;
+    raw[j] = active && t >= 0 && t < r1 ? ldg_stream(p.x + t * p.ld_x + c0) : zero;
+  }
   int s;
   if (p.cu) {
     s = paged::find_segment_warp(p.cu, p.nseg, (int)r0, lane);
@@ -360,29 +370,49 @@ __global__ void __launch_bounds__(128) conv_state_kernel(const ConvParams p) {
     s = (int)(r0 / p.period);
   }
   if (!active) return;
-  uint4 raw[RPT + HR];
-#pragma unroll
-  for (int j = 0; j < RPT + HR; ++j) {
-    const int64_t t = r0 - HR + j;
-    raw[j] = t >= 0 && t < r1 ? ldg_stream(p.x + t * p.ld_x + c0) : zero;
-  }
-  float2 w[KW][4];
-  load_w(w);
+  // which of the rows are this job's: at least HR tokens into a segment
+  uint32_t mine = 0;
   int64_t begin = -1, end = -1;
-#pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int64_t t = r0 + i;
-    if (t >= r1) break;
+  for (int64_t t = r0; t < r1;) {
     while (t >= end && s < p.nseg) {  // the segment that holds t (none: behind the last one)
       begin = p.cu ? p.cu[s] : s * p.period;
       end = p.cu ? p.cu[s + 1] : begin + p.period;
       ++s;
     }
-    if (t >= end || begin < 0 || end > p.tokens || t < begin + HR) continue;
-    uint4 win[KW];
+    if (t >= end) break;
+    const int64_t stop = end < r1 ? end : r1;
+    if (begin >= 0 && end <= p.tokens) {
+      const int64_t from = begin + HR > t ? begin + HR : t;
+      if (from < stop) mine |= ((1u << (stop - from)) - 1u) << (from - r0);
+    }
+    t = stop;
+  }
+  if (mine == 0) return;
+  float2 w[KW][4];
+  load_w(w);
+  // the rows go through a window of KW in float32: each is unpacked once, each output formed and stored if
+  // it is this job's
+  float2 win[KW][4];
+  auto unpack = [](const uint4& u, float2 (&f)[4]) {
+    const uint32_t b[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int m = 0; m < KW; ++m) win[m] = raw[i + m];
-    conv_row<KW>(win, w, dst + t * ldd);
+    for (int c = 0; c < 4; ++c) f[c] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b[c]));
+  };
+#pragma unroll
+  for (int j = 0; j < HR; ++j) unpack(raw[j], win[j]);
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    unpack(raw[i + HR], win[(i + HR) % KW]);
+    uint4 out;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float2 acc = __fmul2_rn(w[0][c], win[i % KW][c]);
+#pragma unroll
+      for (int j = 1; j < KW; ++j) acc = __ffma2_rn(w[j][c], win[(i + j) % KW][c], acc);
+      o[c] = silu2(acc);
+    }
+    if (mine >> i & 1u) *reinterpret_cast<uint4*>(dst + (r0 + i) * ldd) = out;
   }
 }
 
