@@ -18,7 +18,8 @@
 //   groups x WK = 4 / WM key groups.  Tiles stream through a ring of cp.async stages.  Each warp keeps
 //   its own running maximum (raised only when a score exceeds it by more than 2^8, so most tiles
 //   need no reduction across lanes), sum and O (fp32) over its keys; key groups are joined through
-//   shared memory at the end, splits through a float32 workspace by the second kernel.
+//   shared memory at the end.  Up to eight splits are a cluster and join through each other's shared memory,
+//   more through a float32 workspace and a second kernel.
 //   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S, V's multiplies
 //   P before its rounding to fp16, relative to the largest V scale so far (O is rescaled when that grows,
 //   as for the maximum).  q is brought to fp16 with a power of two a row.
@@ -51,6 +52,7 @@ struct Params {
   int nseg, max_pages, page_shift, hq, hkv, group, nsplit, row_blocks;
   int split_keys;  // keys a split (a multiple of every tile's), the last one takes what is left
   int block_rows;  // rows of a row block (a CTA's)
+  int clustered;   // few rows: the splits of a row block are one cluster
   int picked;      // many rows: x counts the call's row tiles, longest first
   float sl2;  // softmax scale * log2(e)
   const bf16* gate;
@@ -180,6 +182,27 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 
+// Cluster: barrier, and loads from the shared memory of CTA `rank` at this CTA's address `a`.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t a, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t a, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(map_rank(a, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t a, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_rank(a, rank)) : "memory");
+  return v;
+}
+
 constexpr float GROW = 8.f;     // the running maximum lags by at most 2^GROW
 constexpr int V_SHIFT = 6;      // fp16 P: times 2^V_SHIFT; at most 2^(GROW + V_SHIFT), weights down to 2^-30 stay
 
@@ -212,7 +235,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int kend = kend64 > 0 ? (int)kend64 : 0;       // keys the row block can see
   int kb, ke;
   split_range(p, split, kend, kb, ke);
-  if (kb >= ke && split > 0) return;  // the join does not read this part
+  if (kb >= ke && split > 0) return;  // no join reads this part
   const int ntiles = (ke - kb + BN - 1) / BN;
 
   // tile loads: chunk lc of rows lr + i * RPP; the rows of a pass lie in one group of 16 keys
@@ -518,6 +541,21 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     }
   __syncthreads();
   // 8 columns a thread: sum of the key groups, then the result or this split's part
+  const bool part = in_parts(p, kend);
+  auto finish = [&](float (&y)[8], float ll, int gr, int c) {
+    const int64_t tok = seg.begin + gr / p.group;
+    const int head = hk * p.group + gr % p.group;
+    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= inv;
+    if (p.gate) {
+      float gv[8];
+      unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
+    }
+    *reinterpret_cast<uint4*>(p.out + (tok * p.hq + head) * D + c) = pack8(y);
+  };
   for (int e = tid; e < BM * (D / 8); e += THREADS) {
     const int row = e / (D / 8), c = (e % (D / 8)) * 8;
     const int gr = row0 + row;
@@ -540,27 +578,54 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
       y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
       y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
     }
-    const int64_t tok = seg.begin + gr / p.group;
-    const int head = hk * p.group + gr % p.group;
-    const int64_t idx = tok * p.hq + head;
-    if (in_parts(p, kend)) {
+    if (!part) {
+      finish(y, ll, gr, c);
+    } else if (p.clustered) {  // in the place of the first key group, read by the cluster
+      float* dst = so + row * LDO + c;
+      *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
+      if (c == 0) sml[WK * BM + row] = make_float2(mm, ll);
+    } else {
+      const int64_t idx = (int64_t)(seg.begin + gr / p.group) * p.hq + hk * p.group + gr % p.group;
       float* dst = p.part_o + ((int64_t)split * p.tokens * p.hq + idx) * D + c;
       *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
       if (c == 0) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(mm, ll);
-    } else {
-      const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= inv;
-      if (p.gate) {
-        float gv[8];
-        unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
-      }
-      *reinterpret_cast<uint4*>(p.out + idx * D + c) = pack8(y);
     }
   }
+  if (!part || !p.clustered) return;
+  // join in the cluster: CTA `split` of the `parts` that have keys takes every parts-th piece.  The ones
+  // without keys have left already, which the cluster barrier counts as arrived.
+  __syncthreads();
+  cluster_sync();
+  const int parts = parts_of(p, kend);
+  for (int e = tid * parts + split; e < BM * (D / 8); e += THREADS * parts) {
+    const int row = e / (D / 8), c = (e % (D / 8)) * 8;
+    const int gr = row0 + row;
+    if (gr >= rows) break;
+    const uint32_t ml_at = smem_u32(sml + WK * BM + row), o_at = smem_u32(so + row * LDO + c);
+    float2 ml[8];
+    float mm = -INFINITY, ll = 0.f, y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ml[i] = i < parts ? cluster_load2(ml_at, i) : make_float2(-INFINITY, 0.f);
+      mm = fmaxf(mm, ml[i].x);
+      y[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < parts && ml[i].x != -INFINITY) {
+        const float f = ex2(ml[i].x - mm);
+        const float4 a = cluster_load4(o_at, i), b = cluster_load4(o_at + 16, i);
+        ll = fmaf(f, ml[i].y, ll);
+        y[0] = fmaf(f, a.x, y[0]); y[1] = fmaf(f, a.y, y[1]); y[2] = fmaf(f, a.z, y[2]); y[3] = fmaf(f, a.w, y[3]);
+        y[4] = fmaf(f, b.x, y[4]); y[5] = fmaf(f, b.y, y[5]); y[6] = fmaf(f, b.z, y[6]); y[7] = fmaf(f, b.w, y[7]);
+      }
+    }
+    finish(y, ll, gr, c);
+  }
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
 // Join of the splits: one warp a (token, head) row, 8 columns a lane (two rows a warp at D = 128).
@@ -620,12 +685,23 @@ template <int D, bool QUANT, int WM, int NR>
 static int launch_few(const Params& p, cudaStream_t s) {
   using G = Geo<D, QUANT>;
   constexpr int BM = 8 * NR * WM, WK = 4 / WM;
-  constexpr int join = WK * BM * (D + 4) * 4 + WK * BM * 8;
+  constexpr int join = WK * BM * (D + 4) * 4 + (WK + 1) * BM * 8;
   constexpr int bytes = G::RING > join ? G::RING : join;
   const void* fn = (const void*)few_rows_kernel<D, QUANT, WM, NR>;
   if (int st = ensure_smem_attr(fn, bytes, "paged_gqa")) return st;
-  const dim3 grid((unsigned)((int64_t)p.nseg * p.row_blocks * p.hkv), (unsigned)p.nsplit);
-  few_rows_kernel<D, QUANT, WM, NR><<<grid, THREADS, bytes, s>>>(p);
+  cudaLaunchAttribute cluster = {};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 1;
+  cluster.val.clusterDim.y = (unsigned)p.nsplit;
+  cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.nseg * p.row_blocks * p.hkv), (unsigned)p.nsplit);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = p.clustered ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, few_rows_kernel<D, QUANT, WM, NR>, p);
   return check_launch("paged_gqa");
 }
 
@@ -648,11 +724,11 @@ struct Plan {
   int rows;            // few-row kernel: rows a CTA
   int64_t row_blocks;  // row blocks (tiles) of the longest segment, a KV head
   int64_t tiles;       // many rows: row tiles in the grid, a KV head
-  bool picked;
+  bool picked, clustered;
   int nsplit, split_keys;
 };
 constexpr int SMS = 148;
-constexpr int MAX_SPLIT = 64;
+constexpr int MAX_SPLIT = 64, MAX_CLUSTER = 8;
 // The few-row kernel's time grows with the rows, the tcgen05 kernel's does not below a tile.  Measured, 64
 // segments x 8192 positions, 16 / 4 heads of 128 and 8 / 2 of 256, few against many rows in us, bf16: 16
 // rows 173 / 302 and 204 / 214, 32 rows 253 / 296 and 284 / 209, 64 rows 365 / 299 and 520 / 208; e4m3:
@@ -664,6 +740,11 @@ constexpr int few_rows_most(int64_t d, bool quant) { return d == 256 && !quant ?
 // fewer.  Parts below 256 keys gain nothing.
 constexpr int few_ctas(int64_t ctas, int rows) { return ctas < SMS ? 2 : rows <= 16 ? 8 : 4; }
 constexpr int MIN_SPLIT_KEYS_FEW = 256;
+// Splits as clusters while all of them run at once: one token behind 1535 positions 12.4 -> 10.3 us, 8 x 2048
+// 12.6 -> 9.6 us (bf16, head_dim 128).  With more CTAs the short parts would wait for the long ones: 64
+// segments of 500 to 8192, e4m3, 54 us with the second kernel, 70 in clusters.  At head_dim 256 in bf16 a CTA
+// fills an SM, and more than eight clusters no longer find their eight SMs in one GPC: 13 us against 20 at
+// 8 x 2048.
 // Many rows: a part costs its rows in float32 twice, about as much as 250 keys of work, and a CTA's start
 // about 10 us.  Measured, eight segments of 100 to 700 tokens behind 600 to 6902 positions, e4m3: 164 us
 // unsplit, 140 aiming at two CTAs an SM, 155 at three; 48 segments of 9 to 70 tokens behind 1490, bf16:
@@ -696,12 +777,19 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
   }
   if (split > MAX_SPLIT) split = MAX_SPLIT;
   if (split < 1) split = 1;
-  int64_t keys = (max_kv + split - 1) / split;
-  if (keys < least) keys = least;
-  keys = (keys + 127) / 128 * 128;
-  r.split_keys = (int)keys;
-  r.nsplit = (int)((max_kv + keys - 1) / keys);
-  if (r.nsplit < 1) r.nsplit = 1;
+  auto cut = [&](int64_t parts) {
+    int64_t keys = (max_kv + parts - 1) / parts;
+    if (keys < least) keys = least;
+    keys = (keys + 127) / 128 * 128;
+    r.split_keys = (int)keys;
+    r.nsplit = max_kv > keys ? (int)((max_kv + keys - 1) / keys) : 1;
+  };
+  cut(split);
+  // a cluster's join costs no launch and no workspace: a little over eight splits become eight
+  const int64_t in_cluster = r.nsplit < MAX_CLUSTER ? r.nsplit : MAX_CLUSTER;
+  r.clustered = !r.many && r.nsplit > 1 && r.nsplit <= 2 * MAX_CLUSTER &&
+                num_segments * hkv * r.row_blocks * in_cluster <= (d == 256 && !quant ? 64 : 2 * SMS);
+  if (r.clustered) cut(in_cluster);
   return r;
 }
 
@@ -741,7 +829,7 @@ extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max
                                                int cache_is_e4m3) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
   const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, cache_is_e4m3 != 0);
-  return pl.nsplit > 1 ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
+  return pl.nsplit > 1 && !pl.clustered ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
 }
 
 extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,
@@ -800,13 +888,13 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
   p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks; p.split_keys = pl.split_keys;
-  p.picked = pl.picked;
+  p.picked = pl.picked; p.clustered = pl.clustered;
   p.block_rows = pl.many ? (head_dim == 128 ? 2 : 1) * (128 / p.group) * p.group : pl.rows;
   p.sl2 = scale * 1.4426950408889634f;
   p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
   p.gate_hstride = (int)(gate_interleaved ? 2 * head_dim : head_dim);
   p.out = static_cast<bf16*>(out);
-  if (pl.nsplit > 1) {
+  if (pl.nsplit > 1 && !pl.clustered) {
     const size_t need = fdk_paged_gqa_workspace_size(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim, quant);
     if (!workspace || workspace_bytes < need)
       return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes needed", what, need);
@@ -823,7 +911,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       st = quant ? chunk::launch<256, true>(p, pl.tiles, s) : chunk::launch<256, false>(p, pl.tiles, s);
   } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.rows, s) : launch_rows<128, false>(p, pl.rows, s);
   else st = quant ? launch_rows<256, true>(p, pl.rows, s) : launch_rows<256, false>(p, pl.rows, s);
-  if (st || pl.nsplit == 1) return st;
+  if (st || pl.nsplit == 1 || pl.clustered) return st;
   const int64_t rpw = head_dim == 128 ? 2 : 1;
   const int64_t warps = tokens * ((hq + rpw - 1) / rpw);
   cudaLaunchAttribute early = {};
