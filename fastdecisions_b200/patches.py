@@ -66,6 +66,18 @@ def install_chunk_gated_delta_rule(core) -> int:
     return n
 
 
+def install_recurrent_gated_delta_rule(core) -> int:
+    """Only swap the token-by-token delta rule of each GDN module (the function its forward calls when a
+    cache holds a state and one token comes in) for the CUDA kernel."""
+    from transformers.models.qwen3_5.modeling_qwen3_5 import Qwen3_5GatedDeltaNet
+    n = 0
+    for m in core.modules():
+        if isinstance(m, Qwen3_5GatedDeltaNet):
+            m.recurrent_gated_delta_rule = ops.recurrent_gated_delta_rule
+            n += 1
+    return n
+
+
 # ------------------------------------------------------------------ decoder: residual + RMSNorm
 def _decoder_forward(self, hidden_states, position_embeddings, attention_mask=None, position_ids=None,
                      past_key_values=None, **kwargs):

@@ -127,3 +127,32 @@ def test_e4m3_cache(setup):
     want, _ = oracle(cfg, weights, ids, reqs)
     check(eng.score_after(prefix, reqs), want, 2 * BOUND)
     assert _lib.poll_device_error() == 0
+
+
+def test_installed_recurrent_rule_decodes_like_the_models_own(setup):
+    """transformers' cached forward, token by token behind a prompt, with the CUDA kernel in place of its
+    recurrent delta rule.  The two differ by float32 rounding inside the rule and bf16 rounding of its
+    output (2^-8); the framework's layer bound, 2e-2 of the largest output, covers that."""
+    mq = pytest.importorskip("transformers.models.qwen3_5.modeling_qwen3_5")
+    from fastdecisions_b200 import patches
+    cfg, weights, _ = setup
+    model = mq.Qwen3_5TextModel(cfg.to_transformers()).to("cuda", torch.bfloat16).eval()
+    model.load_state_dict({k: v.to("cuda", torch.bfloat16) for k, v in weights.items()}, strict=False)
+    prompt = torch.from_numpy(tokens(12, 77).astype(np.int64)).cuda()[None]
+
+    def run():
+        with torch.no_grad():
+            out = model(input_ids=prompt[:, :8], use_cache=True)
+            hidden = [out.last_hidden_state]
+            for i in range(8, 12):
+                out = model(input_ids=prompt[:, i:i + 1], past_key_values=out.past_key_values, use_cache=True)
+                hidden.append(out.last_hidden_state)
+        return torch.cat(hidden, 1).float()
+
+    want = run()
+    before = dict(_lib.call_counts)
+    assert patches.install_recurrent_gated_delta_rule(model) == 3
+    got = run()
+    assert _lib.launches_since(before) == 3 * 4
+    assert _lib.poll_device_error() == 0
+    assert (got - want).abs().max().item() <= 2e-2 * want.abs().max().item()
