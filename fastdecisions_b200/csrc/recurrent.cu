@@ -76,8 +76,310 @@ struct Tokens {
   float4 s[BATCH];  // e^g, beta, k . q
 };
 
+// ---- More than a few tokens: up to 16 at a time on the tensor cores, at float32 accuracy.  With the state S
+// before the batch, decays D_ij = e_{j+1} .. e_i (D_i0 from the batch's start) and normalised k, q:
+//     u_i = beta_i (v_i - D_i0 S^T k_i - sum_{j < i} D_ij (k_j . k_i) u_j)
+//     o_i = D_i0 S^T q_i + sum_{j <= i} D_ij (k_j . q_i) u_j
+//     S  <- D_n0 S + sum_j D_nj k_j u_j^T
+// so with L_ij = beta_i D_ij (k_j . k_i) (j < i), N_ij = D_ij (k_j . q_i) (j <= i), T = (I + L)^-1 and
+// R = beta (v - D_0 S^T k): U = T R, O = D_0 S^T q + N U.  No quotient of decays appears: any of them may be 0.
+// The raw k and q are bf16 and go into the products exactly, their norms are applied to the results; float32
+// operands (S, R, T, U, N) go in as three bf16 parts (24 bits), products below 2^-24 of the leading one
+// left out.
+// Warp w keeps S^T for 16 columns of S (dv) as the MMA's accumulators: row g of its tile is column 16 w + 2 g,
+// row g + 8 the next one, so that states are read 8 bytes a lane, and accumulators become A operands as they
+// are.  16 tokens cost about 2.5 times the work of one token walked alone (measured below).
+constexpr int WALK_MAX = 8;  // segments of at most this many tokens are walked token by token
+constexpr int LDV = DV + 4;  // row stride of v: the four token pairs of a warp's read fall into different banks
+struct Batch16 {
+  uint4 k[BATCH][DK / 8], q[BATCH][DK / 8];  // bf16 rows, 16-byte chunks XORed with the row
+  float v[BATCH * LDV];
+  float Lt[BATCH][BATCH], N[BATCH][BATCH], T[BATCH][BATCH];  // L transposed
+  alignas(16) float e[BATCH];
+  float beta[BATCH], rk[BATCH], rq[BATCH], d0[BATCH], dn[BATCH];
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
+  return r;
+}
+// (x, y) as three packed bf16 pairs whose sum has 24 bits
+__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  h = pack_bf16x2(x, y);
+  x -= __uint_as_float(h << 16);
+  y -= __uint_as_float(h & 0xffff0000u);
+  m = pack_bf16x2(x, y);
+  x -= __uint_as_float(m << 16);
+  y -= __uint_as_float(m & 0xffff0000u);
+  l = pack_bf16x2(x, y);
+}
+// accumulators of two neighbouring 8-column tiles as the A operand of 16 columns, in three parts
+__device__ __forceinline__ void split_a(const float (&c0)[4], const float (&c1)[4], uint32_t (&a)[3][4]) {
+  split3(c0[0], c0[1], a[0][0], a[1][0], a[2][0]);
+  split3(c0[2], c0[3], a[0][1], a[1][1], a[2][1]);
+  split3(c1[0], c1[1], a[0][2], a[1][2], a[2][2]);
+  split3(c1[2], c1[3], a[0][3], a[1][3], a[2][3]);
+}
+// c += A X^T for a float32 16 x 16 matrix X in shared memory (both in parts), 16 columns (tokens) of c.  The six
+// products go through two accumulators: half the chain of dependent MMAs.
+__device__ __forceinline__ void mma_xt(float (&c)[2][4], const uint32_t (&a)[3][4], const float (*X)[BATCH], int g, int t) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const float2 x0 = *reinterpret_cast<const float2*>(&X[8 * n + g][2 * t]);
+    const float2 x1 = *reinterpret_cast<const float2*>(&X[8 * n + g][2 * t + 8]);
+    uint32_t b[3][2];
+    split3(x0.x, x0.y, b[0][0], b[1][0], b[2][0]);
+    split3(x1.x, x1.y, b[0][1], b[1][1], b[2][1]);
+    float small[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_bf16(small, a[2], b[0][0], b[0][1]);
+    mma_bf16(c[n], a[1], b[0][0], b[0][1]);
+    mma_bf16(small, a[0], b[2][0], b[2][1]);
+    mma_bf16(c[n], a[0], b[1][0], b[1][1]);
+    mma_bf16(small, a[1], b[1][0], b[1][1]);
+    mma_bf16(c[n], a[0], b[0][0], b[0][1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[n][i] += small[i];
+  }
+}
+
+// Tokens t0 .. t1 - 1 of one (segment, head) by its CTA.
+__device__ __forceinline__ void batched_tokens(const DeltaParams& p, Batch16& sm, int64_t t0, int64_t t1, int h, int hk,
+                                               int64_t from, int64_t to) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int col = warp * CPW + 2 * g;  // this lane's two columns of S: rows g and g + 8 of its tile
+  // S^T: tile j holds rows (dk) 8 j + 2 t, + 1 of S
+  float S[DK / 8][4];
+  const int64_t head_at = (int64_t)h * (DK * DV) + (int64_t)(2 * t) * DV + col;
+  const int64_t pool_ld = (int64_t)p.heads * (DK * DV);
+  if (from >= 0) {
+    const float* src = p.state_in + from * pool_ld + head_at;
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j) {
+      const float2 a = *reinterpret_cast<const float2*>(src + 8 * j * DV), b = *reinterpret_cast<const float2*>(src + (8 * j + 1) * DV);
+      S[j][0] = a.x; S[j][1] = b.x; S[j][2] = a.y; S[j][3] = b.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[j][i] = 0.f;
+  }
+  const uint32_t kbase = (uint32_t)__cvta_generic_to_shared(&sm.k[0][0]), qbase = (uint32_t)__cvta_generic_to_shared(&sm.q[0][0]);
+  auto at = [](int row, int chunk) { return (uint32_t)((row * (DK / 8) + (chunk ^ (row & 7))) * 16); };
+  // a 16-byte chunk of k, q and v a thread, loaded a batch ahead; rows behind the last token are zeros (beta 0,
+  // decay 1)
+  const int li = tid >> 4, lcn = tid & 15;
+  uint4 kr, qr, vr;
+  float ge, be;
+  auto load_batch = [&](int64_t tb) {
+    const bool live = tb + li < t1;
+    const int64_t tok = live ? tb + li : t0;
+    kr = __ldg(reinterpret_cast<const uint4*>(p.k + tok * p.ld_k + hk * DK) + lcn);
+    qr = __ldg(reinterpret_cast<const uint4*>(p.q + tok * p.ld_q + hk * DK) + lcn);
+    vr = __ldg(reinterpret_cast<const uint4*>(p.v + tok * p.ld_v + h * DV) + lcn);
+    ge = p.g[tok * p.heads + h];
+    be = __bfloat162float(p.beta[tok * p.heads + h]);
+  };
+  load_batch(t0);
+  for (int64_t tb = t0; tb < t1; tb += BATCH) {
+    const int nt = (int)(t1 - tb < BATCH ? t1 - tb : BATCH);
+    if (tb > t0) __syncthreads();
+    {
+      if (li >= nt) {
+        kr = qr = vr = make_uint4(0u, 0u, 0u, 0u);
+        ge = be = 0.f;
+      }
+      if (lcn == 0) {
+        sm.e[li] = expf(ge);
+        sm.beta[li] = be;
+      }
+      sm.k[li][lcn ^ (li & 7)] = kr;
+      sm.q[li][lcn ^ (li & 7)] = qr;
+      float kf[8], qf[8], vf[8], kk = 0.f, qq = 0.f;
+      unpack8(kr, kf);
+      unpack8(qr, qf);
+      unpack8(vr, vf);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        kk = fmaf(kf[u], kf[u], kk);
+        qq = fmaf(qf[u], qf[u], qq);
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) {
+        kk += __shfl_xor_sync(0xffffffffu, kk, off);
+        qq += __shfl_xor_sync(0xffffffffu, qq, off);
+      }
+      if (lcn == 0) {
+        sm.rk[li] = p.l2norm ? rsqrtf(kk + 1e-6f) : 1.f;
+        sm.rq[li] = (p.l2norm ? rsqrtf(qq + 1e-6f) : 1.f) * p.scale;
+      }
+      float* vd = sm.v + li * LDV + 8 * lcn;
+      *reinterpret_cast<float4*>(vd) = make_float4(vf[0], vf[1], vf[2], vf[3]);
+      *reinterpret_cast<float4*>(vd + 4) = make_float4(vf[4], vf[5], vf[6], vf[7]);
+    }
+    __syncthreads();
+    if (tb + BATCH < t1) load_batch(tb + BATCH);
+    if (warp < 4) {  // L (warps 0, 1: eight columns each) and N (2, 3) from the Gram matrices of k and of q with k
+      const uint32_t abase = warp < 2 ? kbase : qbase;
+      float acc[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < DK / 16; kk += 2) {
+        uint32_t a0[4], a1[4], b[4];
+        ldsm4(a0, abase + at(lane & 15, 2 * kk + (lane >> 4)));
+        ldsm4(a1, abase + at(lane & 15, 2 * kk + 2 + (lane >> 4)));
+        ldsm4(b, kbase + at(8 * (warp & 1) + (lane & 7), 2 * kk + (lane >> 3)));
+        mma_bf16(acc[0], a0, b[0], b[1]);
+        mma_bf16(acc[1], a1, b[2], b[3]);
+      }
+      float e[BATCH];
+#pragma unroll
+      for (int m = 0; m < BATCH; m += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(&sm.e[m]);
+        e[m] = x.x; e[m + 1] = x.y; e[m + 2] = x.z; e[m + 3] = x.w;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = g + 8 * (c >> 1), j = 8 * (warp & 1) + 2 * t + (c & 1);
+        float d = 1.f;
+#pragma unroll
+        for (int m = 1; m < BATCH; ++m) d *= m > j && m <= i ? e[m] : 1.f;
+        const float x = (acc[0][c] + acc[1][c]) * sm.rk[j] * d;
+        if (warp < 2) sm.Lt[j][i] = j < i ? x * sm.rk[i] * sm.beta[i] : 0.f;
+        else sm.N[i][j] = j <= i ? x * sm.rq[i] : 0.f;
+      }
+    } else if (warp == 4 && lane < BATCH) {
+      float d0 = 1.f, dn = 1.f;
+#pragma unroll
+      for (int m = 0; m < BATCH; ++m) {
+        const float e = sm.e[m];
+        d0 *= m <= lane ? e : 1.f;
+        dn *= m > lane ? e : 1.f;
+      }
+      sm.d0[lane] = d0;
+      sm.dn[lane] = dn;
+    }
+    __syncthreads();
+    if (warp == 7 && lane < BATCH) {  // T = (I + L)^-1, a column a lane
+      float x[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) x[i] = i == lane ? 1.f : 0.f;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        sm.T[i][lane] = x[i];
+#pragma unroll
+        for (int m = (i + 1) & ~3; m < BATCH; m += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(&sm.Lt[i][m]);  // 0 up to the diagonal
+          x[m] = fmaf(-l.x, x[i], x[m]);
+          x[m + 1] = fmaf(-l.y, x[i], x[m + 1]);
+          x[m + 2] = fmaf(-l.z, x[i], x[m + 2]);
+          x[m + 3] = fmaf(-l.w, x[i], x[m + 3]);
+        }
+      }
+    }
+    // S^T k and S^T q of all tokens
+    float pk[2][4], pq[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk[n][i] = pq[n][i] = 0.f;
+    const int brow = (lane & 7) + ((lane >> 4) << 3), bchunk = (lane >> 3) & 1;
+#pragma unroll
+    for (int kk = 0; kk < DK / 16; ++kk) {
+      uint32_t a[3][4], bk[4], bq[4];
+      split_a(S[2 * kk], S[2 * kk + 1], a);
+      ldsm4(bk, kbase + at(brow, 2 * kk + bchunk));
+      ldsm4(bq, qbase + at(brow, 2 * kk + bchunk));
+#pragma unroll
+      for (int u = 2; u >= 0; --u) {
+        mma_bf16(pk[0], a[u], bk[0], bk[1]);
+        mma_bf16(pq[0], a[u], bq[0], bq[1]);
+        mma_bf16(pk[1], a[u], bk[2], bk[3]);
+        mma_bf16(pq[1], a[u], bq[2], bq[3]);
+      }
+    }
+    __syncthreads();  // T
+    // R, U = T R, O = D_0 S^T q + N U; tokens i = 8 n + 2 t (+ 1) of columns col, col + 1
+    float u[2][4], w[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 8 * n + 2 * t + e;
+        const float beta = sm.beta[i], d0 = sm.d0[i], dk = d0 * sm.rk[i], dq = d0 * sm.rq[i];
+        const float2 v = *reinterpret_cast<const float2*>(sm.v + i * LDV + col);
+        w[n][e] = beta * (v.x - dk * pk[n][e]);
+        w[n][2 + e] = beta * (v.y - dk * pk[n][2 + e]);
+        pq[n][e] *= dq;
+        pq[n][2 + e] *= dq;
+        u[n][e] = u[n][2 + e] = 0.f;
+      }
+    uint32_t a[3][4];
+    split_a(w[0], w[1], a);
+    mma_xt(u, a, sm.T, g, t);
+    split_a(u[0], u[1], a);
+    mma_xt(pq, a, sm.N, g, t);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {  // token 8 n + g, columns 16 w + 4 t .. + 3 after the transpose
+      const uint32_t even = transpose8(pack_bf16x2(pq[n][0], pq[n][1])), odd = transpose8(pack_bf16x2(pq[n][2], pq[n][3]));
+      if (8 * n + g < nt)
+        *reinterpret_cast<uint2*>(p.out + ((tb + 8 * n + g) * p.heads + h) * DV + warp * CPW + 4 * t) =
+            make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+    }
+    // S^T <- D_n0 S^T + sum_j (D_nj |k_j| u_j) k_j^T
+    const float dall = sm.d0[BATCH - 1];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 8 * n + 2 * t + e;
+        const float f = sm.dn[i] * sm.rk[i];
+        u[n][e] *= f;
+        u[n][2 + e] *= f;
+      }
+    split_a(u[0], u[1], a);
+#pragma unroll
+    for (int j = 0; j < DK / 8; j += 2) {
+      uint32_t b[4];
+      ldsm4t(b, kbase + at(lane & 15, j + (lane >> 4)));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[j + x][i] *= dall;
+#pragma unroll
+        for (int y = 2; y >= 0; --y) mma_bf16(S[j + x], a[y], b[2 * x], b[2 * x + 1]);
+      }
+    }
+  }
+  if (to >= 0) {
+    float* dst = p.state_out + to * pool_ld + head_at;
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j) {
+      *reinterpret_cast<float2*>(dst + 8 * j * DV) = make_float2(S[j][0], S[j][2]);
+      *reinterpret_cast<float2*>(dst + (8 * j + 1) * DV) = make_float2(S[j][1], S[j][3]);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrent_delta_kernel(const DeltaParams p) {
-  __shared__ Tokens sm;
+  __shared__ union { Tokens walk; Batch16 batch; } shared;
+  Tokens& sm = shared.walk;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s = (int)(blockIdx.x / (unsigned)p.heads), h = (int)(blockIdx.x % (unsigned)p.heads);
   const bool report = threadIdx.x == 0 && h == 0;
@@ -99,6 +401,10 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrent_delta_kernel(const De
   const int hk = h / p.group;
   const int64_t from = p.state_in ? slot_of(p.in_idx, s, p.in_slots, report) : -1;
   const int64_t to = p.state_out ? slot_of(p.out_idx, s, p.out_slots, report) : -1;
+  if (t1 - t0 > WALK_MAX) {
+    batched_tokens(p, shared.batch, t0, t1, h, hk, from, to);
+    return;
+  }
   const int64_t in_slot = (int64_t)r * 16 * DV + col;
   float2 S[4][8];  // [column][pair of rows]
   if (from >= 0) {
