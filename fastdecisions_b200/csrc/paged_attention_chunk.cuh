@@ -497,6 +497,16 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     if constexpr (R::SPLIT_REGS) reg_dec<88>();
     const int ct = tid - R::CONV * 32, cw = ct >> 5;
     auto slot_of = [&](int key) { return (hk << p.page_shift) + (key & page_mask); };
+    const int my = ct < BN ? ct : 0;
+    auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
+    auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
+      const bool live = (uint32_t)id < (uint32_t)p.num_pages && key < ke;  // a bad id is reported by the producer
+      const int b = __ldg(scales + ((live ? id : 0) * page_ld + slot_of(key)));
+      return live ? b : 0;
+    };
+    int id = page_at(kb + my);
+    int kbyte = scale_at(p.k_scale, p.kscale_page, kb + my, id), vbyte = scale_at(p.v_scale, p.vscale_page, kb + my, id);
+    id = page_at(kb + BN + my);
     // largest scale bytes of the range, 16 keys a load
     uint32_t mk = 0, mv = 0;
     for (int key = kb + ct * 16; key < ke; key += 128 * 16) {
@@ -537,16 +547,6 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     // piece lc (8 columns) of rows lr, lr + RPP, ..: 8 raw bytes become one 16-byte operand chunk.  Eight
     // neighbouring threads read 64 consecutive bytes and store all eight chunk positions: no conflicts.
     constexpr int PASSES = BN / RPP;
-    const int my = ct < BN ? ct : 0;
-    auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
-    auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
-      const bool live = (uint32_t)id < (uint32_t)p.num_pages && key < ke;  // a bad id is reported by the producer
-      const int b = __ldg(scales + ((live ? id : 0) * page_ld + slot_of(key)));
-      return live ? b : 0;
-    };
-    int id = page_at(kb + my);
-    int kbyte = scale_at(p.k_scale, p.kscale_page, kb + my, id), vbyte = scale_at(p.v_scale, p.vscale_page, kb + my, id);
-    id = page_at(kb + BN + my);
     // once a wait has run out, a thread only keeps step at the named barrier (the others may be behind it)
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
