@@ -25,6 +25,7 @@
 //   as for the maximum).  q is brought to fp16 with a power of two a row.
 #include <math.h>
 
+#include <algorithm>
 #include "paged.cuh"
 #include "sm100.cuh"
 
@@ -53,13 +54,16 @@ struct Params {
   int split_keys;  // keys a split (a multiple of every tile's), the last one takes what is left
   int block_rows;  // rows of a row block (a CTA's)
   int clustered;   // few rows: the splits of a row block are one cluster
-  int picked;      // many rows: x counts the call's row tiles, longest first
+  int picked;      // many rows: x counts the call's units of work, longest first
+  int units;       // ... and this many of them, a KV head
+  int part_cost;   // ... one part's float32 rows, written and read, in keys of a CTA's work
   float sl2;  // softmax scale * log2(e)
   const bf16* gate;
   int64_t ld_gate;
   int gate_hstride;
   bf16* out;
   float* part_o;   // [nsplit][tokens * hq][D], unnormalised
+  int* part_keys;  // many rows, picked: the part size
   float2* part_ml; // [nsplit][tokens * hq]: (running max in the exp2 domain, sum)
 };
 
@@ -88,16 +92,80 @@ __device__ __forceinline__ Seg segment(const Params& p, int s, bool report) {
 
 // Keys [kb, ke) of a split of a row block that sees keys [0, kend).  The split size is fixed, so short
 // sequences use few of the grid's splits.
-__device__ __forceinline__ void split_range(const Params& p, int split, int kend, int& kb, int& ke) {
-  kb = (int)min((int64_t)kend, (int64_t)split * p.split_keys);
-  ke = split == p.nsplit - 1 ? kend : (int)min((int64_t)kend, (int64_t)kb + p.split_keys);
+__device__ __forceinline__ void split_range(const Params& p, int part_keys, int split, int kend, int& kb, int& ke) {
+  kb = (int)min((int64_t)kend, (int64_t)split * part_keys);
+  ke = split == p.nsplit - 1 ? kend : (int)min((int64_t)kend, (int64_t)kb + part_keys);
 }
 // Whether a row block that sees keys [0, kend) is computed in parts.  One that fits a split is not: its CTA
 // writes the result and the join passes over its rows.
-__device__ __forceinline__ bool in_parts(const Params& p, int64_t kend) { return p.nsplit > 1 && kend > p.split_keys; }
+__device__ __forceinline__ bool in_parts(const Params& p, int part_keys, int64_t kend) {
+  return p.nsplit > 1 && kend > part_keys;
+}
 // Parts of a row that sees `visible` keys: the splits that hold one of them (at least one is written).
-__device__ __forceinline__ int parts_of(const Params& p, int64_t visible) {
-  return visible <= p.split_keys ? 1 : (int)min((int64_t)p.nsplit, (visible + p.split_keys - 1) / p.split_keys);
+__device__ __forceinline__ int parts_of(const Params& p, int part_keys, int64_t visible) {
+  return visible <= part_keys ? 1 : (int)min((int64_t)p.nsplit, (visible + part_keys - 1) / part_keys);
+}
+
+// Many rows, at most 32 * PICK segments: the call's row tiles, the segments spread over a warp's lanes.
+// Tile rb of a segment sees past + min((rb + 1) tokens, n) keys.
+constexpr int PICK = 2;
+struct Tiles {
+  int past[PICK], n[PICK], tiles[PICK];
+  int tokens, most;  // tokens a tile, keys of the longest one
+  uint32_t inv;
+  // x / tokens as a multiplication, exact for x < 2^32 / tokens: here x < 2^24 (the host's rule)
+  __device__ __forceinline__ int div_up(int x) const { return (int)__umulhi((uint32_t)(x + tokens - 1), inv); }
+  __device__ __forceinline__ void load(const Params& p, int tokens_a_tile, int lane) {
+    tokens = tokens_a_tile;
+    inv = 0xffffffffu / (uint32_t)tokens + 1u;
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < PICK; ++i) {
+      const int s = lane * PICK + i;
+      n[i] = past[i] = tiles[i] = 0;
+      if (s < p.nseg) {
+        const Seg g = segment(p, s, false);
+        n[i] = g.n;
+        past[i] = (int)g.past;
+        tiles[i] = div_up(g.n);
+        if (g.n > 0) m = max(m, past[i] + n[i]);
+      }
+    }
+    most = (int)__reduce_max_sync(0xffffffffu, (unsigned)m);
+  }
+};
+
+// Keys a part of such a call, from its lengths: lane j - 1 prices j parts of the longest range.  In units of
+// one key of a CTA's work: while every CTA has an SM the longest part is the time, else the whole work
+// shared out, with half a part more for its uneven end; a CTA's start is START, the join JOIN and the
+// float32 rows of each part written and read.  Measured against a rule on the longest range alone, which has
+// to favour even or ragged contexts: 8 segments of 100 to 700 tokens behind 600 to 8000 positions, e4m3, 110 us
+// (170 unsplit); 74 of 32 behind 4608, 2 KV heads of 256, 113 us (152 in two parts).  Every CTA gets the same answer (integers only); one leaves it
+// for the join, whose many warps would take 20 us to work it out again.
+constexpr int SMS = 148;
+constexpr int START_KEYS = 448, JOIN_KEYS = 256;
+__device__ __forceinline__ int best_part_keys(const Params& p, const Tiles& t, int lane) {
+  const int j = lane + 1;
+  const int most = max(t.most, 1);
+  const int keys = ((most + j - 1) / j + 127) / 128 * 128;
+  int64_t work = 0, ctas = 0;  // of one KV head
+#pragma unroll
+  for (int i = 0; i < PICK; ++i) {
+    // the launched units cover `ctas`, which counts every tile of a segment as its last one
+    for (int src = 0; src * PICK + i < p.nseg; ++src) {
+      const int past = __shfl_sync(0xffffffffu, t.past[i], src), n = __shfl_sync(0xffffffffu, t.n[i], src);
+      const int tiles = __shfl_sync(0xffffffffu, t.tiles[i], src);
+      ctas += (int64_t)tiles * max(((unsigned)(past + n) + keys - 1u) / keys, 1u);
+      work += (int64_t)tiles * max(past + n / 2, 0);
+    }
+  }
+  int64_t cost = keys;
+  if (ctas * p.hkv > SMS) cost = max(cost, (work + START_KEYS * ctas) * p.hkv / SMS + keys / 2);
+  if (j > 1) cost += JOIN_KEYS + j * (int64_t)p.part_cost;
+  if (j > 1 && (j > p.nsplit || ctas > p.units)) cost = 0x7fffffff;
+  const unsigned mine = (unsigned)min(cost, (int64_t)0x7fffffff);
+  const unsigned best = __reduce_min_sync(0xffffffffu, mine);
+  return __shfl_sync(0xffffffffu, keys, __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1);
 }
 
 // Page ids of the 16-key groups from `key0` on (page sizes are multiples of 16).  The index is clamped to
@@ -234,7 +302,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int64_t kend64 = seg.past + last_tok + 1;
   const int kend = kend64 > 0 ? (int)kend64 : 0;       // keys the row block can see
   int kb, ke;
-  split_range(p, split, kend, kb, ke);
+  split_range(p, p.split_keys, split, kend, kb, ke);
   if (kb >= ke && split > 0) return;  // no join reads this part
   const int ntiles = (ke - kb + BN - 1) / BN;
 
@@ -541,7 +609,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     }
   __syncthreads();
   // 8 columns a thread: sum of the key groups, then the result or this split's part
-  const bool part = in_parts(p, kend);
+  const bool part = in_parts(p, p.split_keys, kend);
   auto finish = [&](float (&y)[8], float ll, int gr, int c) {
     const int64_t tok = seg.begin + gr / p.group;
     const int head = hk * p.group + gr % p.group;
@@ -598,7 +666,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   // without keys have left already, which the cluster barrier counts as arrived.
   __syncthreads();
   cluster_sync();
-  const int parts = parts_of(p, kend);
+  const int parts = parts_of(p, p.split_keys, kend);
   for (int e = tid * parts + split; e < BM * (D / 8); e += THREADS * parts) {
     const int row = e / (D / 8), c = (e % (D / 8)) * 8;
     const int gr = row0 + row;
@@ -628,11 +696,11 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Join of the splits: one warp a (token, head) row, 8 columns a lane (two rows a warp at D = 128).
-// It is launched while the kernel before it drains and waits here for its parts.
+// Join of the splits: one warp a (token, head) row, 8 columns a lane (two rows a warp at D = 128), four parts
+// at a time so that their loads are in flight together.  It is launched while the kernel before it drains;
+// what that kernel does not write is read before the wait for the parts.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const Params p) {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int LPR = D / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -651,30 +719,54 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   // the last token of the row's block decides whether there are parts
   const int n = end - p.cu[s], row = (int)(tok - p.cu[s]) * p.group + head % p.group;
   const int last = min((row / p.block_rows + 1) * p.block_rows, n * p.group) - 1;
-  if (!in_parts(p, len - n + last / p.group + 1)) return;
-  const int parts = parts_of(p, len - (end - tok) + 1);
-  float mm = -INFINITY;
-  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, p.part_ml[i * plane + idx].x);
-  float ll = 0.f, y[8];
+  uint4 gate = {};
+  if (p.gate) gate = *reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int part_keys = p.picked ? *p.part_keys : p.split_keys;
+  if (!in_parts(p, part_keys, len - n + last / p.group + 1)) return;
+  const int parts = parts_of(p, part_keys, len - (end - tok) + 1);
+  float mm = -INFINITY, ll = 0.f, y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = 0.f;
-  if (mm != -INFINITY)
-    for (int i = 0; i < parts; ++i) {
-      const float2 ml = p.part_ml[i * plane + idx];
-      if (ml.x == -INFINITY) continue;
-      const float f = ex2(ml.x - mm);
-      const float* src = p.part_o + (i * plane + idx) * D + c;
-      const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-      ll = fmaf(f, ml.y, ll);
+  for (int i0 = 0; i0 < parts; i0 += 4) {
+    float2 ml[4];
+    float4 o[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ml[i] = make_float2(-INFINITY, 0.f);
+      o[i][0] = o[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + i < parts) {
+        const float* src = p.part_o + ((i0 + i) * plane + idx) * D + c;
+        ml[i] = p.part_ml[(i0 + i) * plane + idx];
+        o[i][0] = *reinterpret_cast<const float4*>(src);
+        o[i][1] = *reinterpret_cast<const float4*>(src + 4);
+      }
+    }
+    float m = mm;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i].x);
+    if (m == -INFINITY) continue;  // nothing visible so far: sums stay zero
+    const float keep = ex2(mm - m);
+    mm = m;
+    ll *= keep;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (ml[i].x == -INFINITY) continue;
+      const float f = ex2(ml[i].x - mm);
+      const float4 a = o[i][0], b = o[i][1];
+      ll = fmaf(f, ml[i].y, ll);
       y[0] = fmaf(f, a.x, y[0]); y[1] = fmaf(f, a.y, y[1]); y[2] = fmaf(f, a.z, y[2]); y[3] = fmaf(f, a.w, y[3]);
       y[4] = fmaf(f, b.x, y[4]); y[5] = fmaf(f, b.y, y[5]); y[6] = fmaf(f, b.z, y[6]); y[7] = fmaf(f, b.w, y[7]);
     }
+  }
   const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] *= inv;
   if (p.gate) {
     float gv[8];
-    unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
+    unpack8(gate, gv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
   }
@@ -723,33 +815,33 @@ struct Plan {
   bool many;           // the tcgen05 kernel
   int rows;            // few-row kernel: rows a CTA
   int64_t row_blocks;  // row blocks (tiles) of the longest segment, a KV head
-  int64_t tiles;       // many rows: row tiles in the grid, a KV head
+  int64_t tiles;       // many rows: row tiles that can exist, a KV head
+  int64_t units;       // ... and CTAs in the grid's first dimension
+  int64_t part_cost;   // ... a part's float32 rows in keys of a CTA's work
   bool picked, clustered;
   int nsplit, split_keys;
 };
-constexpr int SMS = 148;
 constexpr int MAX_SPLIT = 64, MAX_CLUSTER = 8;
 // The few-row kernel's time grows with the rows, the tcgen05 kernel's does not below a tile.  Measured, 64
 // segments x 8192 positions, 16 / 4 heads of 128 and 8 / 2 of 256, few against many rows in us, bf16: 16
 // rows 173 / 302 and 204 / 214, 32 rows 253 / 296 and 284 / 209, 64 rows 365 / 299 and 520 / 208; e4m3:
 // 32 rows 229 / 363 and 202 / 279, 64 rows 364 / 363 and 323 / 286.
 constexpr int few_rows_most(int64_t d, bool quant) { return d == 256 && !quant ? 16 : 32; }
-// Few rows, CTAs an SM to aim at.  A part costs its rows in float32 and a CTA's start, so equal contexts want
-// few (8 segments x 8192 positions, bf16: 31 us with 2 CTAs an SM, 35 with 4, 46 with 8); ragged ones want
-// many once every SM has one (64 segments of 500 to 8192, e4m3: 98, 80 and 75 us), the more rows the
-// fewer.  Parts below 256 keys gain nothing.
-constexpr int few_ctas(int64_t ctas, int rows) { return ctas < SMS ? 2 : rows <= 16 ? 8 : 4; }
-constexpr int MIN_SPLIT_KEYS_FEW = 256;
-// Splits as clusters while all of them run at once: one token behind 1535 positions 12.4 -> 10.3 us, 8 x 2048
-// 12.6 -> 9.6 us (bf16, head_dim 128).  With more CTAs the short parts would wait for the long ones: 64
+// Few rows, CTAs an SM to aim at.  A part costs its rows in float32 and a CTA's start, so below one CTA an SM
+// the parts fill the SMs once, with what a ring's shared memory leaves room for: one CTA of head_dim 256 in bf16,
+// two of 128, three of an 8-bit cache (8 segments x 8192 positions, 4 KV heads, bf16: 26 us with 8 parts, 34 with
+// 13).  Above, ragged contexts want many parts (64 segments of 500 to 8192, e4m3: 99 us unsplit, 59 in 4, 45 in 6),
+// even ones lose a little by them (64 x 8192, bf16: 153 us unsplit, 169 in 6), and more rows a part cost more.
+// Short parts pay while SMs are idle (20 segments of 190 to 725, 6 heads on one: 10.5 us in parts of 256 keys,
+// 8.7 of 128; 64 segments of 500 on 4 heads: 11.4 us unsplit, 15.7 in parts of 256).
+constexpr int few_ctas(int64_t ctas, int rows, int64_t d, bool quant) {
+  return ctas < SMS ? (quant ? 3 : d == 128 ? 2 : 1) : rows <= 16 ? 12 : 4;
+}
+// Splits as clusters while all of them run at once, up to eight, and eight where more would be short: one token
+// behind 1535 positions 12.4 -> 10.3 us, 8 x 2048 12.6 -> 9.6 us (bf16, head_dim 128).  With more CTAs the short parts would wait for the long ones: 64
 // segments of 500 to 8192, e4m3, 54 us with the second kernel, 70 in clusters.  At head_dim 256 in bf16 a CTA
 // fills an SM, and more than eight clusters no longer find their eight SMs in one GPC: 13 us against 20 at
 // 8 x 2048.
-// Many rows: a part costs its rows in float32 twice, about as much as 250 keys of work, and a CTA's start
-// about 10 us.  Measured, eight segments of 100 to 700 tokens behind 600 to 6902 positions, e4m3: 164 us
-// unsplit, 140 aiming at two CTAs an SM, 155 at three; 48 segments of 9 to 70 tokens behind 1490, bf16:
-// 59 us unsplit, 66 in two parts of 896 keys.  While half of the SMs have no CTA, parts may be short.
-constexpr int MIN_SPLIT_KEYS_MANY = 2048, MIN_SPLIT_KEYS_IDLE = 512;
 static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
                       int64_t group, int64_t d, bool quant) {
   Plan r = {};
@@ -759,21 +851,29 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
   if (r.many) {
     const int64_t per = (d == 128 ? 2 : 1) * (128 / group);  // tokens a CTA
     r.row_blocks = (max_seqlen + per - 1) / per;
-    // CTAs that have work: from the tokens, half a tile more a segment, not from the longest segment
-    int64_t ctas = hkv * (tokens / per + (num_segments + 1) / 2);
-    if (ctas > num_segments * hkv * r.row_blocks) ctas = num_segments * hkv * r.row_blocks;
-    // row tiles that can exist; few segments are sorted on the device (see pick_tile)
-    r.picked = num_segments <= 64 && tokens < 1 << 24;
+    // CTAs that have work: from the tokens, half a tile more a segment and one at least, not from the longest one
+    int64_t ctas = hkv * std::max(tokens / per + (num_segments + 1) / 2, std::min(num_segments, tokens));
+    const int64_t most = num_segments * hkv * r.row_blocks;
+    if (10 * ctas > 7 * most) ctas = most;  // even lengths
+    // More than half of the SMs busy: few segments are cut and sorted on the device, which knows their lengths.
+    r.picked = 2 * ctas > SMS && num_segments <= 64 && tokens < 1 << 24;
+    // upper bound of the parts where the device picks (see best_part_keys), else the parts
+    split = r.picked ? (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1) : SMS / (ctas > 0 ? ctas : 1);
+    if (split > 32) split = 32;
+    r.part_cost = tokens * group * hkv * d / 8192;  // 8 bytes a value; a key's work lasts as long as 64 KB of them
+    if (r.part_cost > 1 << 24) r.part_cost = 1 << 24;
+    // no more than can pay
+    while (split > 1 && max_kv * (split - 1) <= split * (JOIN_KEYS + split * r.part_cost)) --split;
+    if (split == 1 && most <= SMS) r.picked = false;  // one wave in any order
     r.tiles = num_segments * r.row_blocks;
     if (r.picked && tokens / per + num_segments < r.tiles) r.tiles = tokens / per + num_segments;
-    split = (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1);
-    least = 2 * ctas <= SMS ? MIN_SPLIT_KEYS_IDLE : MIN_SPLIT_KEYS_MANY;
+    least = 128;
   } else {
     r.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
     r.row_blocks = (rows + r.rows - 1) / r.rows;
     const int64_t ctas = num_segments * hkv * (r.row_blocks > 0 ? r.row_blocks : 1);
-    split = (few_ctas(ctas, r.rows) * SMS + ctas - 1) / ctas;
-    least = MIN_SPLIT_KEYS_FEW;
+    split = few_ctas(ctas, r.rows, d, quant) * SMS / ctas;
+    least = ctas >= SMS ? 512 : max_kv > 4096 ? 256 : 128;
   }
   if (split > MAX_SPLIT) split = MAX_SPLIT;
   if (split < 1) split = 1;
@@ -785,9 +885,14 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
     r.nsplit = max_kv > keys ? (int)((max_kv + keys - 1) / keys) : 1;
   };
   cut(split);
+  r.units = r.tiles;
+  if (r.picked && r.nsplit > 1) {
+    r.units += 2 * SMS / hkv;
+    if (r.units > r.tiles * r.nsplit) r.units = r.tiles * r.nsplit;
+  }
   // a cluster's join costs no launch and no workspace: a little over eight splits become eight
   const int64_t in_cluster = r.nsplit < MAX_CLUSTER ? r.nsplit : MAX_CLUSTER;
-  r.clustered = !r.many && r.nsplit > 1 && r.nsplit <= 2 * MAX_CLUSTER &&
+  r.clustered = !r.many && r.nsplit > 1 && (r.nsplit <= MAX_CLUSTER || max_kv <= 256 * MAX_CLUSTER) &&
                 num_segments * hkv * r.row_blocks * in_cluster <= (d == 256 && !quant ? 64 : 2 * SMS);
   if (r.clustered) cut(in_cluster);
   return r;
@@ -829,7 +934,7 @@ extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max
                                                int cache_is_e4m3) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
   const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, cache_is_e4m3 != 0);
-  return pl.nsplit > 1 && !pl.clustered ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) : 0;
+  return pl.nsplit > 1 && !pl.clustered ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) + 16 : 0;
 }
 
 extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,
@@ -876,7 +981,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
   Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, quant);
-  if (max_seqlen * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.tiles : num_segments * pl.row_blocks) > 0x7fffffff)
+  if (max_seqlen * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.units : num_segments * pl.row_blocks) > 0x7fffffff)
     return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
   Params p = {};
   p.q = static_cast<const bf16*>(q); p.ld_q = ld_q;
@@ -888,7 +993,8 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
   p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks; p.split_keys = pl.split_keys;
-  p.picked = pl.picked; p.clustered = pl.clustered;
+  p.picked = pl.picked; p.clustered = pl.clustered; p.units = (int)pl.units;
+  p.part_cost = (int)pl.part_cost;
   p.block_rows = pl.many ? (head_dim == 128 ? 2 : 1) * (128 / p.group) * p.group : pl.rows;
   p.sl2 = scale * 1.4426950408889634f;
   p.gate = static_cast<const bf16*>(gate); p.ld_gate = ld_gate;
@@ -901,14 +1007,15 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
     if (!aligned16(workspace)) return set_error(FDK_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", what);
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)pl.nsplit * tokens * hq * head_dim);
+    p.part_keys = reinterpret_cast<int*>(p.part_ml + (int64_t)pl.nsplit * tokens * hq);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st;
   if (pl.many) {
     if (head_dim == 128)
-      st = quant ? chunk::launch<128, true>(p, pl.tiles, s) : chunk::launch<128, false>(p, pl.tiles, s);
+      st = quant ? chunk::launch<128, true>(p, s) : chunk::launch<128, false>(p, s);
     else
-      st = quant ? chunk::launch<256, true>(p, pl.tiles, s) : chunk::launch<256, false>(p, pl.tiles, s);
+      st = quant ? chunk::launch<256, true>(p, s) : chunk::launch<256, false>(p, s);
   } else if (head_dim == 128) st = quant ? launch_rows<128, true>(p, pl.rows, s) : launch_rows<128, false>(p, pl.rows, s);
   else st = quant ? launch_rows<256, true>(p, pl.rows, s) : launch_rows<256, false>(p, pl.rows, s);
   if (st || pl.nsplit == 1 || pl.clustered) return st;

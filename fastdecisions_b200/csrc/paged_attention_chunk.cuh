@@ -139,37 +139,21 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)(c >> 3) * BOX + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) * 16);
 }
 
-// The `rank`-th longest row tile of the call (a warp's work): tiles of all segments in descending order of
-// the keys they see, so that the grid starts with the longest and the launched tiles are the ones that
-// exist.  Tile rb of a segment sees kend(rb) = past + min((rb + 1) tokens, n) keys; the number of tiles with
-// at least L keys has a closed form a segment, so L is found by bisection with the segments spread over
-// the lanes.  False when there are no more than `rank` tiles.  At most 32 * PICK segments.
-constexpr int PICK = 2;
+// The `rank`-th unit of work of the call (a warp's work), for calls whose segments fit one warp's lanes: the
+// whole parts of all row tiles first, then each tile's last part (or the tile that is not split), both in
+// descending order of the keys that the tile sees.  So the grid starts with the longest CTAs and launches
+// what exists.  The number of tiles with at least L keys has a closed form a segment, so a tile is found
+// by bisection over L with the segments spread over the lanes.  False when there are no more than `rank`
+// units.
 struct Unit {
-  int s, rb;
+  int s, rb, split;
 };
-__device__ __forceinline__ bool pick_tile(const Params& p, int tokens, int rank, int lane, Unit& u) {
-  int past[PICK], n[PICK], tiles[PICK], most = 0;
-  // x / tokens as a multiplication, exact for x < 2^32 / tokens: here x < 2^24 (the host's rule)
-  const uint32_t inv = 0xffffffffu / (uint32_t)tokens + 1u;
-  auto div_up = [&](int x) { return (int)__umulhi((uint32_t)(x + tokens - 1), inv); };
-#pragma unroll
-  for (int i = 0; i < PICK; ++i) {
-    const int s = lane * PICK + i;
-    n[i] = past[i] = tiles[i] = 0;
-    if (s < p.nseg) {
-      const Seg g = segment(p, s, false);
-      n[i] = g.n;
-      past[i] = (int)g.past;
-      tiles[i] = div_up(g.n);
-      most = max(most, past[i] + n[i]);
-    }
-  }
+__device__ __forceinline__ bool pick_unit(const Params& p, const Tiles& t, int part_keys, int rank, int lane, Unit& u) {
   auto count1 = [&](int i, int L) {  // tiles of the lane's segment i that see at least L keys
-    if (L <= 0) return tiles[i];
-    if (tiles[i] == 0 || past[i] + n[i] < L) return 0;
-    const int need = max(min(L - past[i], n[i]), 1);  // the first tile with (rb + 1) tokens >= need
-    return tiles[i] - div_up(need) + 1;
+    if (L <= 0) return t.tiles[i];
+    if (t.tiles[i] == 0 || t.past[i] + t.n[i] < L) return 0;
+    const int need = max(min(L - t.past[i], t.n[i]), 1);  // the first tile with (rb + 1) tokens >= need
+    return t.tiles[i] - t.div_up(need) + 1;
   };
   auto count = [&](int L) {
     int c = 0;
@@ -177,8 +161,19 @@ __device__ __forceinline__ bool pick_tile(const Params& p, int tokens, int rank,
     for (int i = 0; i < PICK; ++i) c += count1(i, L);
     return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
   };
+  u.split = -1;
+  for (int i = 0; i + 1 < p.nsplit; ++i) {  // tiles whose part i is a whole one and not their last
+    const int64_t more = (int64_t)(i + 1) * part_keys + 1;
+    const int c = more > t.most ? 0 : count((int)more);
+    if (c == 0) break;
+    if (rank < c) {
+      u.split = i;
+      break;
+    }
+    rank -= c;
+  }
   if (count(0) <= rank) return false;
-  int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) + 1;  // count(lo) > rank >= count(hi)
+  int lo = 0, hi = t.most + 1;  // count(lo) > rank >= count(hi)
   while (hi - lo > 1) {
     const int mid = lo + (hi - lo) / 2;
     if (count(mid) > rank) lo = mid;
@@ -200,7 +195,7 @@ __device__ __forceinline__ bool pick_tile(const Params& p, int tokens, int rank,
   for (int i = 0; i < PICK; ++i) {
     if (found < 0 && skip >= 0 && skip < eq[i]) {
       found = lane * PICK + i;
-      rb = tiles[i] - count1(i, lo) + skip;
+      rb = t.tiles[i] - count1(i, lo) + skip;
     }
     skip -= eq[i];
   }
@@ -208,6 +203,7 @@ __device__ __forceinline__ bool pick_tile(const Params& p, int tokens, int rank,
   const int src = __ffs(who) - 1;
   u.s = __shfl_sync(0xffffffffu, found, src);
   u.rb = __shfl_sync(0xffffffffu, rb, src);
+  if (u.split < 0) u.split = lo > part_keys ? (lo - 1) / part_keys : 0;  // lo: the tile's keys
   return true;
 }
 
@@ -235,32 +231,39 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tpt = 128 / p.group;                 // tokens a tile
   const int rpt = tpt * p.group;                 // rows of it in use
-  // grid: x = (row tiles of all segments, KV head) with the head fastest, y = split of the keys from the
-  // last one (only long ranges have it: short tiles come at the end).  With few
-  // segments the tiles are taken longest first (short calls end on their longest CTA, and only the device
-  // knows the lengths); with many, x counts each segment's tiles up to the longest one's number, from
-  // the last tile down.
+  // grid: with few segments x = (units of work, KV head), the head fastest, longest first (short calls end
+  // on their longest CTA, and only the device knows the lengths).  With many, x counts each segment's row
+  // tiles up to the longest one's number, from the last tile down, and y the splits of the keys from the
+  // last one (only long ranges have it: short tiles come at the end).
   const int hk = (int)(blockIdx.x % (unsigned)p.hkv), item = (int)(blockIdx.x / (unsigned)p.hkv);
-  const int split = p.nsplit - 1 - (int)blockIdx.y;
-  int s, rb;
+  int s, rb, split, part_keys = p.split_keys;
   if (p.picked) {
     int* pick = reinterpret_cast<int*>(gbase + M::OFF_MISC + 48);
     if (warp == 0) {
-      Unit u = {-1, 0};
-      const bool some = pick_tile(p, NT * tpt, item, lane, u);
+      Tiles t;
+      t.load(p, NT * tpt, lane);
+      if (p.nsplit > 1) part_keys = best_part_keys(p, t, lane);
+      Unit u = {-1, 0, 0};
+      const bool some = pick_unit(p, t, part_keys, item, lane, u);
       if (lane == 0) {
         pick[0] = some ? u.s : -1;
         pick[1] = u.rb;
+        pick[2] = u.split;
+        pick[3] = part_keys;
+        if (p.nsplit > 1 && item == 0 && hk == 0) *p.part_keys = part_keys;
       }
     }
     __syncthreads();
     s = pick[0];
     rb = pick[1];
+    split = pick[2];
+    part_keys = pick[3];
   } else {
     s = item % p.nseg;
     rb = p.row_blocks - 1 - item / p.nseg;
+    split = p.nsplit - 1 - (int)blockIdx.y;
   }
-  if (item == 0 && hk == 0 && split == 0) {  // one CTA reports what is wrong with the segments
+  if (item == 0 && hk == 0 && blockIdx.y == 0) {  // one CTA reports what is wrong with the segments
     for (int i = tid; i < p.nseg; i += R::THREADS)
       if (segment(p, i, true).n > p.row_blocks * NT * tpt) atomicOr(&g_error, 1);
   }
@@ -274,10 +277,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   const int kend = kend64 > 0 ? (int)kend64 : 0;
   const int kv_len = (int)(seg.past + seg.n);
   int kb, ke;
-  split_range(p, split, kend, kb, ke);
+  split_range(p, part_keys, split, kend, kb, ke);
   if (kb >= ke && split > 0) return;  // the join does not read this part
   const int n_kv = (ke - kb + BN - 1) / BN;
-  const bool part = in_parts(p, kend);
+  const bool part = in_parts(p, part_keys, kend);
   if (n_kv == 0) {  // no keys at all: zeros
     for (int e = tid; e < NT * rpt; e += R::THREADS) {
       const int64_t gr = (int64_t)tok0 * p.group + e;
@@ -873,7 +876,7 @@ static int encode(CUtensorMap* m, const void* ptr, bool bytes, int rank, const c
 }
 
 template <int D, bool QUANT>
-static int launch(const Params& p, int64_t row_tiles, cudaStream_t s) {
+static int launch(const Params& p, cudaStream_t s) {
   using G = Geo<D>;
   CUtensorMap mq = {}, mk = {}, mv = {};
   const cuuint64_t esz = QUANT ? 1 : 2, ps = (cuuint64_t)1 << p.page_shift;
@@ -892,7 +895,7 @@ static int launch(const Params& p, int64_t row_tiles, cudaStream_t s) {
   constexpr uint32_t bytes = Smem<D, QUANT>::BYTES;
   const void* fn = (const void*)many_rows_kernel<D, QUANT>;
   if (int st = ensure_smem_attr(fn, (int)bytes, "paged_gqa")) return st;
-  const dim3 grid((unsigned)(row_tiles * p.hkv), (unsigned)p.nsplit);
+  const dim3 grid((unsigned)((int64_t)p.units * p.hkv), p.picked ? 1u : (unsigned)p.nsplit);
   many_rows_kernel<D, QUANT><<<grid, Roles<D, QUANT>::THREADS, bytes, s>>>(mq, mk, mv, p);
   return check_launch("paged_gqa (many rows)");
 }

@@ -179,6 +179,22 @@ def test_attention_many_tokens_split_keys(hq, hkv, D, quant):
 
 
 @pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
+def test_attention_many_tokens_parts_cut_on_the_device(hq, hkv, D, quant):
+    # enough tiles for the part size to follow from the lengths, with contexts and tiles far from even;
+    # a segment of more tokens than positions, empty ones, and even lengths, where nothing is split
+    n = [500, 40, 0, 350, 64, 290, 1, 333]
+    run_attn(n, [530, 4500, 9, 3000, 64, 100, 2500, 333], hq, hkv, D, 64, quant, seed=42, gate=True)
+    run_attn(n, [500, 40, 0, 350, 64, 290, 1, 333], hq, hkv, D, 32, quant, seed=43)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_many_segments_split_keys(quant):
+    n = [33 if i % 7 else 1 for i in range(66)]
+    run_attn(n, [x + 23 * i for i, x in enumerate(n)], 6, 1, 128, 32, quant, seed=44)
+
+
+@pytest.mark.parametrize("quant", [False, True])
 def test_attention_empty_rows_and_segments(quant):
     # no tokens; no keys; more tokens than positions (the first ones see nothing and give zeros)
     run_attn([0, 4, 0, 6, 1, 2], [10, 0, 0, 3, 0, 2], 16, 4, 128, 16, quant, seed=3)
