@@ -36,6 +36,11 @@ using sm100::ex2;
 
 __device__ int g_error = 0;
 
+// sigmoid by the fast exponential and quotient: a relative error below 2^-16 for |x| < 88, where the rounding of
+// the result to bf16 has 2^-9.  Exact ones make a tile's epilogue wait: 1532 tokens of 8 heads of 256, 58 us
+// with, 42 without a gate; so 46.
+__device__ __forceinline__ float gate_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
 struct Params {
   const bf16* q;
   int64_t ld_q;
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
       float gv[8];
       unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
+      for (int i = 0; i < 8; ++i) y[i] *= gate_of(gv[i]);
     }
     *reinterpret_cast<uint4*>(p.out + (tok * p.hq + head) * D + c) = pack8(y);
   };
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
     float gv[8];
     unpack8(gate, gv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
+    for (int i = 0; i < 8; ++i) y[i] *= gate_of(gv[i]);
   }
   *reinterpret_cast<uint4*>(p.out + idx * D + c) = pack8(y);
 }

@@ -66,7 +66,8 @@ struct Smem {
                             OFF_BAR = OFF_RAW + RAW_SLOTS * RAWT, OFF_MISC = OFF_BAR + 8 * NBAR,
                             OFF_QS = OFF_MISC + 64,                       // row scale exponents of q: 256 bytes (head_dim 128)
                             OFF_FT = OFF_QS + (QUANT ? 256 : 0),          // row factors of two tiles: half2
-                            BYTES = OFF_FT + (QUANT ? 1024 : 0) + 1024;   // + slack for 1024-byte alignment
+                            OFF_STAGE = OFF_FT + (QUANT ? 1024 : 0),      // q on its way to TMEM: 4 KB a softmax warp
+                            BYTES = OFF_STAGE + (G::Q_TMEM ? 16384 : 0) + 1024;  // + slack for 1024-byte alignment
   static_assert(OFF_MISC % 16 == 0, "alignment of the small state");
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
@@ -608,37 +609,73 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     float sl2 = p.sl2;
     if (G::Q_TMEM) {
       // q's row of this thread to its TMEM lane, two elements a column; 8-bit cache: as fp16 with the row's
-      // largest magnitude in [1, 2)
-      const bf16* src = p.q + (int64_t)(seg.begin + (valid ? tok : 0)) * p.ld_q + (int64_t)(hk * p.group + (valid ? row % p.group : 0)) * D;
+      // largest magnitude in [1, 2).  Read with eight lanes to 128 bytes of a row, turned in shared memory.
+      const int64_t q_at = (int64_t)(seg.begin + (valid ? tok : 0)) * p.ld_q + (int64_t)(hk * p.group + (valid ? row % p.group : 0)) * D;
+      const int r8 = lane >> 3, c8 = lane & 7;  // a pass: rows 4 i + r8, columns 8 c8 .. + 7
+      // Straight code runs at the speed of instruction fetches: the loops stay rolled.
+      uint4 w[8];
+      auto load = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + __shfl_sync(0xffffffffu, q_at, 4 * i + r8) + c * 64 + c8 * 8));
+      };
       float inv = 1.f, unit = 1.f;
       if (QUANT) {
-        float a = 0.f;
-#pragma unroll 8
-        for (int c = 0; c < D / 8; ++c) {
-          float f[8];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(src) + c), f);
+        float m[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]));
+        for (int i = 0; i < 8; ++i) m[i] = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          load(c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            __nv_bfloat162 x = __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[i].x));
+            x = __hmax2(x, __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[i].y)));
+            x = __hmax2(x, __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[i].z)));
+            x = __hmax2(x, __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[i].w)));
+            m[i] = fmaxf(m[i], fmaxf(__low2float(x), __high2float(x)));
+          }
+        }
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+          const float x = __shfl_sync(0xffffffffu, m[i], (lane & 3) * 8);  // row 4 i + (lane & 3)
+          if (lane >> 2 == i) a = x;
         }
         const int e = a == 0.f ? 127 : min(max((int)(__float_as_uint(a) >> 23), 1), 253);
         inv = __uint_as_float((uint32_t)(254 - e) << 23);
         unit = __uint_as_float((uint32_t)e << 23);
       }
+      load(0);
+      const uint32_t stage = base + M::OFF_STAGE + (uint32_t)warp * 4096u;
 #pragma unroll 1
       for (int c = 0; c < D / 64; ++c) {
-        uint4 w[8];
-        uint32_t col[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(src) + c * 8 + i);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          const int r = 4 * i + r8;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + (uint32_t)(r * 128 + ((c8 ^ (r & 7)) * 16))),
+                       "r"(w[i].x), "r"(w[i].y), "r"(w[i].z), "r"(w[i].w)
+                       : "memory");
+        }
+        __syncwarp();
+        if (c + 1 < D / 64) load(c + 1);
+        uint32_t col[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t ww[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3])
+                       : "r"(stage + (uint32_t)(lane * 128 + ((i ^ (lane & 7)) * 16)))
+                       : "memory");
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ww[u]));
             col[4 * i + u] = QUANT ? pack_f16x2(x.x * inv, x.y * inv) : ww[u];
           }
         }
+        __syncwarp();
         tmem_st32(tmem + lane_base + G::TM_Q + c * 32, col);
       }
       tmem_st_wait();
@@ -783,57 +820,94 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       l_run = l_run * alpha + (sum2.x + sum2.y);
     }
     // ------------------------------------------------------------------ epilogue
+    // A thread's row of O is 2 D bytes from its neighbour's: stored (and its gate loaded) row by row, every
+    // access of a warp would touch 32 lines.  So 32 rows x 64 columns at a time go through the warp's part of
+    // the operands' shared memory, free by now, and eight lanes hold 128 bytes of one row.  The gate's rows follow it
+    // there, all of them at once.  16-byte chunks are XORed with the row: no bank conflicts either way.
+    // This code runs once a CTA, at the speed of instruction fetches: the loops stay rolled.
+    const int64_t tk_ = (int64_t)seg.begin + tok;
+    const int head = hk * p.group + row % p.group;
+    const int64_t idx = tk_ * p.hq + head;
+    const bool gated = p.gate != nullptr && !part;
+    const unsigned live = __ballot_sync(0xffffffffu, valid);
+    const int64_t gate_at = tk_ * p.ld_gate + (int64_t)head * p.gate_hstride;
+    const int r8 = lane >> 3, c8 = lane & 7;  // a pass: rows 4 i + r8, columns 8 c8 .. + 7
     if (ok && __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0, abort_flag) ? 1 : 0)) {
       tc_fence_after();
-      const int64_t tk_ = (int64_t)seg.begin + tok;
-      const int head = hk * p.group + row % p.group;
-      const int64_t idx = tk_ * p.hq + head;
       // l and O both carry 2^P_SHIFT with the 8-bit cache; O is in units of V's largest scale
       const float unit = QUANT ? scale_value(scale_max[1]) : 1.f;
       const float inv = part ? unit : (l_run > 0.f ? unit / l_run : (l_run == 0.f ? 0.f : l_run));
-      float* prow = part ? p.part_o + ((int64_t)split * p.tokens * p.hq + idx) * D : nullptr;
       if (part && valid) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(r_run * sl2, l_run);
-      bf16* orow = p.out + idx * D;
-      const bf16* grow = p.gate ? p.gate + tk_ * p.ld_gate + (int64_t)head * p.gate_hstride : nullptr;
-      uint4 gate_next[4];  // the gate's next 32 columns, loaded a step ahead
-      const bool gated = grow != nullptr && valid && !part;
+      constexpr uint32_t GATE = 64u * D;  // 32 rows of the gate
+      static_assert(G::NT * 4 * (8192 + GATE) <= M::OFF_RAW, "shared memory of the epilogue");
+      const uint32_t stage = base + (uint32_t)warp * (8192u + GATE), gates = stage + 8192u;
       if (gated) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) gate_next[i] = ldg_stream(grow + i * 8);
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {  // D / 8 lanes a row
+          const int e = i * 32 + lane, r = e / (D / 8), ch = e % (D / 8);
+          const int64_t at = __shfl_sync(0xffffffffu, gate_at, r);
+          const uint32_t to = gates + (uint32_t)(r * 2 * D + ((ch ^ (r & 7)) * 16));
+          if (live >> r & 1) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(p.gate + at + ch * 8) : "memory");
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
       }
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint4 gate_now[4];
+      for (int c = 0; c < D / 64; ++c) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 64 + h * 32, o);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gate_now[i] = gate_next[i];
-        if (gated && c + 1 < D / 32) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) gate_next[i] = ldg_stream(grow + (c + 1) * 32 + i * 8);
-        }
-        uint32_t o[32];
-        tmem_ld32(tO + c * 32, o);
-        tmem_ld_wait();
-        if (valid && part) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(prow + c * 32 + i) =
-                make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv,
-                            __uint_as_float(o[i + 3]) * inv);
-        } else if (valid) {
-#pragma unroll
-          for (int v8 = 0; v8 < 4; ++v8) {
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(o[v8 * 8 + i]) * inv;
-            if (gated) {
-              float gv[8];
-              unpack8(gate_now[v8], gv);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gv[i]);
-            }
-            *reinterpret_cast<uint4*>(orow + c * 32 + v8 * 8) = pack8(y);
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t at = stage + (uint32_t)lane * 256u + (uint32_t)(((8 * h + q) ^ (lane & 7)) * 16);
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "f"(__uint_as_float(o[4 * q]) * inv),
+                         "f"(__uint_as_float(o[4 * q + 1]) * inv), "f"(__uint_as_float(o[4 * q + 2]) * inv),
+                         "f"(__uint_as_float(o[4 * q + 3]) * inv)
+                         : "memory");
           }
         }
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncwarp();
+        auto staged = [&](int r, int chunk) {
+          float4 x;
+          const uint32_t at = stage + (uint32_t)r * 256u + (uint32_t)((chunk ^ (r & 7)) * 16);
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+          return x;
+        };
+        if (part) {
+#pragma unroll 2
+          for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            const int64_t at = __shfl_sync(0xffffffffu, idx, r);
+            const float4 x = staged(r, lane & 15);
+            if (live >> r & 1)
+              *reinterpret_cast<float4*>(p.part_o + ((int64_t)split * p.tokens * p.hq + at) * D + c * 64 + (lane & 15) * 4) = x;
+          }
+        } else {
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + r8;
+            const int64_t at = __shfl_sync(0xffffffffu, idx, r);
+            // the second half of the lanes reads its chunks in the other order: all eight differ in their bank
+            const float4 first = staged(r, 2 * c8 + (c8 >> 2)), second = staged(r, 2 * c8 + 1 - (c8 >> 2));
+            const float4 lo = c8 < 4 ? first : second, hi = c8 < 4 ? second : first;
+            float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            if (gated) {
+              float gv[8];
+              uint4 gw;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                           : "=r"(gw.x), "=r"(gw.y), "=r"(gw.z), "=r"(gw.w)
+                           : "r"(gates + (uint32_t)(r * 2 * D + (((c * 8 + c8) ^ (r & 7)) * 16)))
+                           : "memory");
+              unpack8(gw, gv);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) y[u] *= gate_of(gv[u]);
+            }
+            if (live >> r & 1) *reinterpret_cast<uint4*>(p.out + at * D + c * 64 + c8 * 8) = pack8(y);
+          }
+        }
+        __syncwarp();
       }
     }
   }
