@@ -37,8 +37,8 @@ using sm100::ex2;
 __device__ int g_error = 0;
 
 // sigmoid by the fast exponential and quotient: a relative error below 2^-16 for |x| < 88, where the rounding of
-// the result to bf16 has 2^-9.  Exact ones make a tile's epilogue wait: 1532 tokens of 8 heads of 256, 58 us
-// with, 42 without a gate; so 46.
+// the result to bf16 has 2^-9.  With the exact ones 1532 tokens of 8 heads of 256 behind a shared prefix of 1490
+// took 58 us, 42 without a gate; with these 46.
 __device__ __forceinline__ float gate_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 struct Params {
@@ -116,14 +116,14 @@ __device__ __forceinline__ int parts_of(const Params& p, int part_keys, int64_t 
 constexpr int PICK = 2;
 struct Tiles {
   int past[PICK], n[PICK], tiles[PICK];
-  int tokens, most;  // tokens a tile, keys of the longest one
+  int tokens, least, most;  // tokens a tile, keys of the shortest and of the longest tile
   uint32_t inv;
   // x / tokens as a multiplication, exact for x < 2^32 / tokens: here x < 2^24 (the host's rule)
   __device__ __forceinline__ int div_up(int x) const { return (int)__umulhi((uint32_t)(x + tokens - 1), inv); }
   __device__ __forceinline__ void load(const Params& p, int tokens_a_tile, int lane) {
     tokens = tokens_a_tile;
     inv = 0xffffffffu / (uint32_t)tokens + 1u;
-    int m = 0;
+    int m = 0, l = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < PICK; ++i) {
       const int s = lane * PICK + i;
@@ -133,10 +133,14 @@ struct Tiles {
         n[i] = g.n;
         past[i] = (int)g.past;
         tiles[i] = div_up(g.n);
-        if (g.n > 0) m = max(m, past[i] + n[i]);
+        if (g.n > 0) {
+          m = max(m, past[i] + n[i]);
+          l = min(l, max(past[i] + min(n[i], tokens), 0));
+        }
       }
     }
     most = (int)__reduce_max_sync(0xffffffffu, (unsigned)m);
+    least = min((int)__reduce_min_sync(0xffffffffu, (unsigned)l), most);
   }
 };
 

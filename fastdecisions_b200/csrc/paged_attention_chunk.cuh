@@ -174,7 +174,7 @@ __device__ __forceinline__ bool pick_unit(const Params& p, const Tiles& t, int p
     rank -= c;
   }
   if (count(0) <= rank) return false;
-  int lo = 0, hi = t.most + 1;  // count(lo) > rank >= count(hi)
+  int lo = t.least, hi = t.most + 1;  // count(lo) > rank >= count(hi)
   while (hi - lo > 1) {
     const int mid = lo + (hi - lo) / 2;
     if (count(mid) > rank) lo = mid;
@@ -513,18 +513,32 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     id = page_at(kb + BN + my);
     // largest scale bytes of the range, 16 keys a load
     uint32_t mk = 0, mv = 0;
-    for (int key = kb + ct * 16; key < ke; key += 128 * 16) {
-      const int64_t id = __ldg(table + (key >> p.page_shift));
-      if (id < 0 || id >= p.num_pages) continue;  // reported by the loads below
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p.k_scale + id * p.kscale_page + slot_of(key)));
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.v_scale + id * p.vscale_page + slot_of(key)));
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    constexpr int AHEAD = 4;  // page ids, then scales, of that many steps in flight
+    for (int key0 = kb + ct * 16; key0 < ke; key0 += AHEAD * 128 * 16) {
+      int64_t ids[AHEAD];
+      uint4 a[AHEAD], b[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int left = ke - (key + 4 * i);  // bytes of this word inside the range
-        const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-        mk = __vmaxu4(mk, aw[i] & mask);
-        mv = __vmaxu4(mv, bw[i] & mask);
+      for (int u = 0; u < AHEAD; ++u) ids[u] = __ldg(table + (min(key0 + u * 128 * 16, ke - 1) >> p.page_shift));
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int key = key0 + u * 128 * 16;
+        a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (key < ke && ids[u] >= 0 && ids[u] < p.num_pages) {  // a bad id is reported by the loads below
+          a[u] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + ids[u] * p.kscale_page + slot_of(key)));
+          b[u] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + ids[u] * p.vscale_page + slot_of(key)));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int key = key0 + u * 128 * 16;
+        const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int left = ke - (key + 4 * i);  // bytes of this word inside the range
+          const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          mk = __vmaxu4(mk, aw[i] & mask);
+          mv = __vmaxu4(mv, bw[i] & mask);
+        }
       }
     }
     auto byte_max = [](uint32_t w) { return max(max(w & 255u, (w >> 8) & 255u), max((w >> 16) & 255u, w >> 24)); };
@@ -876,7 +890,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           return x;
         };
         if (part) {
-#pragma unroll 2
+#pragma unroll 4
           for (int i = 0; i < 16; ++i) {
             const int r = 2 * i + (lane >> 4);
             const int64_t at = __shfl_sync(0xffffffffu, idx, r);
@@ -885,26 +899,41 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
               *reinterpret_cast<float4*>(p.part_o + ((int64_t)split * p.tokens * p.hq + at) * D + c * 64 + (lane & 15) * 4) = x;
           }
         } else {
-#pragma unroll 2
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + r8;
-            const int64_t at = __shfl_sync(0xffffffffu, idx, r);
-            // the second half of the lanes reads its chunks in the other order: all eight differ in their bank
-            const float4 first = staged(r, 2 * c8 + (c8 >> 2)), second = staged(r, 2 * c8 + 1 - (c8 >> 2));
-            const float4 lo = c8 < 4 ? first : second, hi = c8 < 4 ? second : first;
-            float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            if (gated) {
-              float gv[8];
-              uint4 gw;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                           : "=r"(gw.x), "=r"(gw.y), "=r"(gw.z), "=r"(gw.w)
-                           : "r"(gates + (uint32_t)(r * 2 * D + (((c * 8 + c8) ^ (r & 7)) * 16)))
-                           : "memory");
-              unpack8(gw, gv);
+#pragma unroll 1
+          for (int i0 = 0; i0 < 8; i0 += 4) {  // four rows a lane: their chains of exponential and quotient overlap
+            float4 first[4], second[4];
+            uint4 gw[4];
 #pragma unroll
-              for (int u = 0; u < 8; ++u) y[u] *= gate_of(gv[u]);
+            for (int i = 0; i < 4; ++i) {
+              const int r = 4 * (i0 + i) + r8;
+              // the second half of the lanes reads its chunks in the other order: all eight differ in their bank
+              first[i] = staged(r, 2 * c8 + (c8 >> 2));
+              second[i] = staged(r, 2 * c8 + 1 - (c8 >> 2));
+              if (gated)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                             : "=r"(gw[i].x), "=r"(gw[i].y), "=r"(gw[i].z), "=r"(gw[i].w)
+                             : "r"(gates + (uint32_t)(r * 2 * D + (((c * 8 + c8) ^ (r & 7)) * 16)))
+                             : "memory");
             }
-            if (live >> r & 1) *reinterpret_cast<uint4*>(p.out + at * D + c * 64 + c8 * 8) = pack8(y);
+            uint4 res[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 lo = c8 < 4 ? first[i] : second[i], hi = c8 < 4 ? second[i] : first[i];
+              float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+              if (gated) {
+                float gv[8];
+                unpack8(gw[i], gv);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) y[u] *= gate_of(gv[u]);
+              }
+              res[i] = pack8(y);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 4 * (i0 + i) + r8;
+              const int64_t at = __shfl_sync(0xffffffffu, idx, r);
+              if (live >> r & 1) *reinterpret_cast<uint4*>(p.out + at * D + c * 64 + c8 * 8) = res[i];
+            }
           }
         }
         __syncwarp();

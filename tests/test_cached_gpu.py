@@ -110,12 +110,12 @@ def attn_check(o, ref, quant, gate=None, rows=slice(None)):
 
 
 def run_attn(q_lens, kv_lens, hq, hkv, D, page, quant, seed=1, gate=False, interleaved=False, shared=0, spread=0.0,
-             q_scale=1.0, max_kv_len=None, strided=False, v_only=False):
+             q_scale=1.0, max_kv_len=None, strided=False, v_only=False, gate_scale=1.0):
     c = Cache(kv_lens, hkv, D, page, quant, seed, shared, spread, v_only)
     T = sum(q_lens)
     g = gen(seed + 1)
     q = (torch.randn(T, hq, D, generator=g) * q_scale).to(BF)
-    gt = torch.randn(T, 2 * hq * D, generator=g).to(BF) if gate else None
+    gt = (torch.randn(T, 2 * hq * D, generator=g) * gate_scale).to(BF) if gate else None
     cu = cu_of(q_lens)
     dev, kw = c.dev(interleaved)
     qd = q.cuda()
@@ -186,6 +186,14 @@ def test_attention_many_tokens_parts_cut_on_the_device(hq, hkv, D, quant):
     n = [500, 40, 0, 350, 64, 290, 1, 333]
     run_attn(n, [530, 4500, 9, 3000, 64, 100, 2500, 333], hq, hkv, D, 64, quant, seed=42, gate=True)
     run_attn(n, [500, 40, 0, 350, 64, 290, 1, 333], hq, hkv, D, 32, quant, seed=43)
+
+
+@pytest.mark.parametrize("n,kv", [([1, 2, 3], [700, 40, 9]), ([1], [5000]), ([80, 33], [90, 333]), ([70], [6000])])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
+def test_attention_gates_of_any_size(n, kv, hq, hkv, D):
+    # sigmoids from 0 to 1, infinite gates among them, in each kernel and in the join of parts
+    run_attn(n, kv, hq, hkv, D, 64, False, seed=45, gate=True, gate_scale=60.0)
+    run_attn(n, kv, hq, hkv, D, 64, False, seed=46, gate=True, gate_scale=3e38)
 
 
 @pytest.mark.parametrize("quant", [False, True])
