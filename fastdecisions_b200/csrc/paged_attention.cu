@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const int ntiles = (ke - kb + BN - 1) / BN;
 
   // tile loads: chunk lc of rows lr + i * RPP; the rows of a pass lie in one group of 16 keys
-  constexpr int RPP = THREADS / G::CH, PASSES = BN / RPP, GROUPS = BN / 16;
+  constexpr int RPP = THREADS / G::CH, GROUPS = BN / 16;
   const int lc = tid % G::CH, lr = tid / G::CH;
   const int32_t* table = p.table + (int64_t)s * p.ld_table;
   const int page_mask = (1 << p.page_shift) - 1;
