@@ -710,18 +710,19 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
 // what that kernel does not write is read before the wait for the parts.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const Params p) {
+  auto wait = [] { asm volatile("griddepcontrol.wait;\n" ::: "memory"); };  // every thread, also one that leaves
   constexpr int LPR = D / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int64_t per_tok = (p.hq + RPW - 1) / RPW;   // warps a token
   const int64_t tok = w / per_tok;
-  if (tok >= p.tokens) return;
+  if (tok >= p.tokens) return wait();
   const int s = paged::find_segment_warp(p.cu, p.nseg, (int)tok, lane);
-  if (s < 0 || s >= p.nseg) return;                 // behind the last segment
+  if (s < 0 || s >= p.nseg) return wait();          // behind the last segment
   const int end = p.cu[s + 1];
-  if (end <= tok || end > p.tokens || p.cu[s] < 0) return;
+  if (end <= tok || end > p.tokens || p.cu[s] < 0) return wait();
   const int head = (int)(w % per_tok) * RPW + lane / LPR, c = (lane % LPR) * 8;
-  if (head >= p.hq) return;
+  if (head >= p.hq) return wait();
   const int64_t idx = tok * p.hq + head, plane = p.tokens * p.hq;
   int64_t len = p.kv_lens[s];
   if (len < 0 || len > ((int64_t)p.max_pages << p.page_shift)) len = 0;
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int last = min((row / p.block_rows + 1) * p.block_rows, n * p.group) - 1;
   uint4 gate = {};
   if (p.gate) gate = *reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c);
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  wait();
   const int part_keys = p.picked ? *p.part_keys : p.split_keys;
   if (!in_parts(p, part_keys, len - n + last / p.group + 1)) return;
   const int parts = parts_of(p, part_keys, len - (end - tok) + 1);
@@ -943,7 +944,8 @@ extern "C" size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max
                                                int cache_is_e4m3) {
   if (!sizes_ok(num_segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim)) return 0;
   const pattn::Plan pl = pattn::make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, cache_is_e4m3 != 0);
-  return pl.nsplit > 1 && !pl.clustered ? (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) + 16 : 0;
+  if (pl.nsplit == 1 || pl.clustered) return 0;
+  return (size_t)pl.nsplit * tokens * hq * (head_dim * 4 + 8) + (pl.picked ? 16 : 0);  // + the part size
 }
 
 extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,

@@ -631,18 +631,28 @@ class DecisionEngine:
 
     @torch.no_grad()
     def extend(self, prefix: Prefix, ids) -> Prefix:
-        """Appends tokens to a cached prefix (its pages grow, its states advance in place)."""
+        """Appends tokens to a cached prefix (its pages grow, its states advance in place).  A run that fails
+        leaves states of unknown length: the prefix is released."""
         ids = np.asarray(ids, dtype=np.int32).reshape(-1)
         cache, total = prefix.cache, prefix.length + ids.size
-        if prefix.slot is None:
-            raise ValueError("extend: the prefix was released")
+        self._own(prefix, "extend")
         if ids.size < 1 or total > self.max_positions:
             raise ValueError(f"extend: at least one token and at most {self.max_positions} positions")
         prefix.pages += cache.take_pages(-(-total // cache.page_size) - len(prefix.pages))
         batch = pack([Request(ids=ids, slot=ids.size - 1, nopts=1)])
-        self._run_cached(cache, batch, prefix.length, [prefix.pages], prefix.slot if prefix.length else -1, prefix.slot)
+        try:
+            self._run_cached(cache, batch, prefix.length, [prefix.pages], prefix.slot if prefix.length else -1, prefix.slot)
+        except Exception:
+            prefix.release()
+            raise
         prefix.length = total
         return prefix
+
+    def _own(self, prefix: Prefix, what: str):
+        if prefix.slot is None:
+            raise ValueError(f"{what}: the prefix was released")
+        if prefix.cache.cfg != self.cfg:
+            raise ValueError(f"{what}: the prefix belongs to a cache of another model")
 
     def cache_prefix(self, cache: StateCache, ids) -> Prefix:
         """Runs ``ids`` once and keeps their keys, values and states for ``score_after``."""
@@ -661,8 +671,7 @@ class DecisionEngine:
         followed the prefix's (``slot`` counts within the request's own ids), running only the requests'
         tokens.  Whole pages of the prefix are shared by all of them; the positions of its last, partial
         page are copied to each request's first own page.  The prefix itself is not changed."""
-        if prefix.slot is None:
-            raise ValueError("score_after: the prefix was released")
+        self._own(prefix, "score_after")
         if len(requests) == 0:
             return np.zeros((0, self.letters.shape[0]), dtype=np.float32)
         cache, past, size = prefix.cache, prefix.length, prefix.cache.page_size

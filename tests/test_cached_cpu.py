@@ -1,11 +1,12 @@
 """Cached-state operators without a GPU: refusals, host-side sizes, installers and the oracle itself."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from fastdecisions_b200 import _lib, ops, patches, workloads as W
-from fastdecisions_b200.engine import StateCache
+from fastdecisions_b200.engine import DecisionEngine, Prefix, StateCache
 from oracle import cached as O
 from oracle import ops as R
 
@@ -119,3 +120,29 @@ def test_oracle_attention_and_recurrences_agree_with_the_uncached_oracle():
     ref = torch.cat([t.reshape(n, -1) for t in R.packed_conv_silu(x, w)], 1)
     assert (y - ref).abs().max() < 1e-4 and torch.equal(hist[0], x[0, -3:].double())
     assert math.isfinite(float(y.sum()))
+
+
+def test_prefix_of_another_model_and_failed_extension():
+    cfg = W.ModelConfig(num_hidden_layers=4, vocab_size=64)
+    eng = object.__new__(DecisionEngine)  # host logic only
+    eng.cfg, eng.dev, eng.max_positions = cfg, torch.device("cpu"), 4096
+    other = StateCache(W.ModelConfig(num_hidden_layers=8, vocab_size=64), "cpu", 64, 1, 16)
+    with pytest.raises(ValueError, match="another model"):
+        eng.extend(Prefix(other, 0), [1, 2])
+    cache = StateCache(cfg, "cpu", 64, 1, 16)
+    with pytest.raises(ValueError, match="another model"):
+        eng.score_after(Prefix(other, 0), [W.Request(ids=np.zeros(2, np.int32), slot=1, nopts=2)])
+
+    def fails(*_):
+        raise RuntimeError("launch failed")
+
+    eng._run_cached = lambda *_: None
+    prefix = eng.cache_prefix(cache, np.zeros(20, np.int32))
+    assert prefix.length == 20 and len(cache.free_pages) == 2 and not cache.free_slots
+    eng._run_cached = fails
+    with pytest.raises(RuntimeError, match="launch failed"):
+        eng.extend(prefix, np.zeros(20, np.int32))
+    assert prefix.slot is None and len(cache.free_pages) == 4 and len(cache.free_slots) == 1
+    with pytest.raises(RuntimeError, match="launch failed"):
+        eng.cache_prefix(cache, np.zeros(20, np.int32))
+    assert len(cache.free_pages) == 4 and len(cache.free_slots) == 1

@@ -330,6 +330,38 @@ def test_attention_graph_replay_with_other_lengths_and_stream():
         attn_check(out, O.paged_attention(q, *c.cache, c.table, cu_of([1, 1]), kv, *c.scale), True)
 
 
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_graph_replay_of_parts_cut_on_the_device(quant):
+    # the part size follows the lengths of each replay; token counts and contexts change, the second stream
+    # runs a call of its own meanwhile
+    n, kv = [500, 40, 0, 350, 64, 290, 1, 333], [530, 4500, 9, 3000, 64, 100, 2500, 333]
+    c = Cache([4600] * 8, 4, 128, 64, quant, 51)
+    dev, kw = c.dev()
+    T = sum(n)
+    q = torch.randn(T, 16, 128, generator=gen(6)).to(BF)
+    qd, cu, lens = q.cuda(), cu_of(n).cuda(), torch.tensor(kv, dtype=torch.int32, device="cuda")
+    ops.paged_gqa_attention(qd, *dev, cu, lens, 500, 4600, **kw)
+    torch.cuda.synchronize()
+    graph, other, side = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = ops.paged_gqa_attention(qd, *dev, cu, lens, 500, 4600, **kw)
+    with torch.cuda.graph(other):
+        out2 = ops.paged_gqa_attention(qd, *dev, cu, lens, 500, 4600, **kw)
+    for n2, kv2 in ((n, kv), ([200] * 7 + [178], [4600] * 8), ([500, 500, 500, 78, 0, 0, 0, 0], [501, 500, 499, 4000, 0, 7, 0, 1]),
+                    ([1] * 8, [4600, 1, 2, 3, 4, 5, 6, 7])):
+        cu.copy_(cu_of(n2))
+        lens.copy_(torch.tensor(kv2, dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            other.replay()
+        assert no_error()
+        ref = O.paged_attention(q, c.cache[0], c.cache[1], c.table, cu_of(n2), kv2, c.scale[0], c.scale[1])
+        rows = slice(0, sum(n2))
+        attn_check(out[rows], ref, quant, rows=rows)
+        attn_check(out2[rows], ref, quant, rows=rows)
+
+
 # --------------------------------------------------------------------------- cache write and read
 @pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("hkv,D,page", [(4, 128, 64), (2, 256, 16), (1, 128, 32), (3, 256, 128), (5, 128, 256)])
