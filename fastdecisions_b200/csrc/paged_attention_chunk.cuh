@@ -567,7 +567,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     constexpr int PASSES = BN / RPP;
     // Rows loaded before the first store (the compiler keeps their order, so a load behind a store waits for it): at
     // head_dim 256 the converters set the pace (74 x 32 tokens behind 4096 shared positions: 130 us with 1, 104
-    // with 4, 101 with 8); at 128 the rest does, and bursts only disturb it (37 x 64: 131, 134 with 4).
+    // with 4, 101 with 8); at 128 issue slots do, which the softmax needs as well (37 x 64: 114 us with 1, 115 with
+    // 2, 117 with 4; 131 with the test of `live` in full blocks too).
     constexpr int BURST = D == 128 ? 1 : 8;
     // once a wait has run out, a thread only keeps step at the named barrier (the others may be behind it)
     bool ok = true;
@@ -590,26 +591,30 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         const uint8_t* src = gbase + M::OFF_RAW + raw_slot * M::RAWT + lr * D + lc * 8;
         uint8_t* dst = gbase + M::OFF_KV + slot * G::KT;
         const uint32_t* fac = factor + which * BN + lr;
+        auto convert = [&](bool partial) {
 #pragma unroll
-        for (int i0 = 0; i0 < PASSES; i0 += BURST) {
-          uint2 w[BURST];
-          uint32_t f[BURST];
+          for (int i0 = 0; i0 < PASSES; i0 += BURST) {
+            uint2 w[BURST];
+            uint32_t f[BURST];
 #pragma unroll
-          for (int i = 0; i < BURST; ++i) {
-            w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * RPP * D);
-            f[i] = fac[(i0 + i) * RPP];
-            if (lr + (i0 + i) * RPP >= live) w[i] = make_uint2(0u, 0u);
+            for (int i = 0; i < BURST; ++i) {
+              w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * RPP * D);
+              if (partial && lr + (i0 + i) * RPP >= live) w[i] = make_uint2(0u, 0u);
+              f[i] = fac[(i0 + i) * RPP];
+            }
+#pragma unroll
+            for (int i = 0; i < BURST; ++i) {
+              uint4 h;
+              h.x = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].x), f[i]);
+              h.y = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].x >> 16)), f[i]);
+              h.z = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].y), f[i]);
+              h.w = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].y >> 16)), f[i]);
+              *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(lr + (i0 + i) * RPP, lc)) = h;
+            }
           }
-#pragma unroll
-          for (int i = 0; i < BURST; ++i) {
-            uint4 h;
-            h.x = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].x), f[i]);
-            h.y = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].x >> 16)), f[i]);
-            h.z = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].y), f[i]);
-            h.w = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].y >> 16)), f[i]);
-            *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(lr + (i0 + i) * RPP, lc)) = h;
-          }
-        }
+        };
+        if (live >= BN) convert(false);
+        else convert(true);
         fence_proxy_async_smem();
         mbar_arrive(bar(B_F + slot));
         mbar_arrive(bar(B_RE + raw_slot));

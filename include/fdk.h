@@ -280,14 +280,18 @@ size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, in
 /*
  * Causal GQA attention of the newest tokens over the paged cache: token i of segment s's n attends
  * to positions 0 .. kv_lens[s] - n + i (its own keys are in the cache already); a token that sees
- * nothing gets zeros.  q, gate, out, scale and the head mapping as fdk_gqa_fwd (any hq / hkv).
+ * nothing gets zeros.  q, gate, out and the head mapping as fdk_gqa_fwd (any hq / hkv); scale is
+ * positive and finite.
  * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows past the bound are
  * not computed).  max_kv_len is a hint for how far the keys are split: any lengths up to
  * max_pages * page_size are right with any hint.  Softmax statistics and accumulation are float32; P
- * is rounded to bf16 (bf16 cache) or fp16 (e4m3 cache) before P.V.  A non-finite V row may reach every
+ * is rounded to bf16 (bf16 cache) or fp16 (e4m3 cache) before P.V; calls of many query
+ * rows take e4m3 rows as fp16 relative to the largest scale among the keys a CTA reads: exact for scales
+ * down to 2^-15 of it, below that rounded to multiples of 2^-24 of it.
+ * A non-finite V row may reach every
  * row of its call that shares a tile with it, masked ones included; K rows and rows past kv_lens[s]
- * never do.  The caller's workspace holds float32 partial results; calls that overlap on the GPU
- * need separate ones.
+ * never do.  The caller's workspace holds float32 partial results and the size of the parts, which the
+ * device takes from the lengths; calls that overlap on the GPU need separate ones.
  */
 int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t ld_kpage,
                       const void* v_cache, int64_t ld_vpage, int cache_is_e4m3,
@@ -315,7 +319,9 @@ int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cache, int64_t 
  * The pools may be the same array and a segment's two slots the same slot; a slot that one segment
  * writes must not be read or written by another segment of the call.  Indices past the pool count as
  * negative and set bit 64 of the device error word, as an invalid segment range does (it counts as
- * empty).  dk == dv == 128; float32 states and arithmetic.
+ * empty).  Segments must not overlap.  dk == dv == 128; float32 states and sums.  Segments of more than
+ * eight tokens go 16 at a time through matrix products whose float32 operands enter as three bf16 parts
+ * (24 bits): the same accuracy, another order of the sums.
  */
 int fdk_recurrent_gated_delta_rule_fwd(
     const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
