@@ -28,6 +28,13 @@
 //   K and V blocks share one ring of operand slots, in the order K_0 V_0 K_1 V_1 ..: four slots for bf16,
 //   three for the 8-bit cache (PV of block j and S of block j + 1 hold two, the converters fill the
 //   third), which leaves room for a ring of four raw tiles.
+//
+// Measured (B200, device time): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 246 us,
+// 1.07 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050: the softmax's exponentials and the
+// operands' shared-memory traffic take as long each.  8 ragged chunks (2544 tokens behind 600 to 8000), e4m3, page
+// 16: 127 us; 4400 cycles a block, 22000 before the first, and uneven CTAs.  48 questions of 9 to 70 tokens behind
+// 1490 shared positions, 8 / 2 heads of 256, bf16: 45 us; a block of 64 keys brings 64 KB from L2, 32 bytes a clock
+// and SM, which sets its 2050 cycles; the start and the epilogue of the one wave are a third of the call.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -115,7 +122,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // the special-function unit (16 results a clock and SM, half of what its two tiles take): x = n + f with
 // |f| <= 1/2, 2^f by a cubic fitted to the least relative error (2^-13.7, below the fp16 and bf16
 // roundings of P), 2^n from the bits of n + 127.  x below -126.5 gives 0; NaN stays NaN.
-constexpr int EXP_POLY = 3;  // every 3rd pair of columns (2: 268 us, 3: 259, 4: 261, 6: 261, none: 264 for 2 x 2048 tokens behind 6144 and 7543)
+// Every 3rd pair of columns (2 x 2048 tokens behind 6144 and 14000, bf16, when it was chosen: none 275 us, every 2nd
+// 268, 3rd 259, 4th 261, 6th 261).  Not with an 8-bit cache, whose converters need the issue slots (37 x 64 tokens
+// behind 4096: 119 us with every 3rd, 115 without).
+constexpr int EXP_POLY = 3;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n" : "+f"(x.x));  // -127: the factor 2^n below is then 0
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n" : "+f"(x.y));
@@ -826,7 +836,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           for (int c = 0; c < 32; ++c) {
             const int i = half * 64 + 2 * c;
             const float2 x = expo(make_float2(__uint_as_float(sr[i >> 5][i & 31]), __uint_as_float(sr[(i + 1) >> 5][(i + 1) & 31])));
-            const float2 e = NT == 2 && c % EXP_POLY == EXP_POLY - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            const float2 e = NT == 2 && !QUANT && c % EXP_POLY == EXP_POLY - 1 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
             sum4[c & 3] = __fadd2_rn(sum4[c & 3], e);
             pk[c] = QUANT ? pack_f16x2(e.x, e.y) : pack_bf16x2(e.x, e.y);
           }

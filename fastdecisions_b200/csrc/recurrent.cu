@@ -40,8 +40,9 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t sl
 // The decay is not applied to the registers: they hold S / G with G the product of the decays so far, and
 // the update adds k (u / G), one operation an element instead of two.  When G leaves [1e-18, 1e18] it is
 // multiplied in and starts over at 1.
-// Bound by HBM where states dominate (64 KiB in, 64 KiB out a head and segment), by the float32 pipe at
-// several tokens a segment.
+// Bound by HBM where states dominate (64 KiB in, 64 KiB out a head and segment: 96 segments of one token forked from
+// one state 36 us, 101 MB written), else by the chain of dependent steps of the two CTAs an SM holds: 96 segments
+// of 1 to 24 tokens 65 us, issue slots 32% and tensor cores 10% busy.
 constexpr int DK = 128, DV = 128, CPW = 16;   // columns a warp
 constexpr int WARPS = DV / CPW;
 constexpr int BATCH = 16;                     // tokens in shared memory at a time
@@ -88,8 +89,10 @@ struct Tokens {
 // left out.
 // Warp w keeps S^T for 16 columns of S (dv) as the MMA's accumulators: row g of its tile is column 16 w + 2 g,
 // row g + 8 the next one, so that states are read 8 bytes a lane, and accumulators become A operands as they
-// are.  16 tokens cost about 2.5 times the work of one token walked alone (measured below).
-constexpr int WALK_MAX = 8;  // segments of at most this many tokens are walked token by token
+// are.  A batch costs the same for 2 to 16 tokens.
+// Segments of at most this many tokens are walked token by token.  Measured, 16 heads, walked / in batches: 96 segments
+// of 4 tokens 51 / 70 us, of 8 64 / 71, of 9 71 / 71, of 16 100 / 72; one segment of 4 7.2 / 9.3, of 16 13.7 / 9.3.
+constexpr int WALK_MAX = 8;
 constexpr int LDV = DV + 4;  // row stride of v: the four token pairs of a warp's read fall into different banks
 struct Batch16 {
   uint4 k[BATCH][DK / 8], q[BATCH][DK / 8];  // bf16 rows, 16-byte chunks XORed with the row
@@ -528,6 +531,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrent_delta_kernel(const De
 // Two kinds of work in one grid: jobs below nseg are a segment's head -- its first KW - 1 outputs, the
 // only ones that read the history, and the new history, so an in-place update cannot race -- and the
 // rest take eight consecutive tokens each and compute those at least KW - 1 tokens into their segment.
+// Memory-bound in bytes, in time bound by their latency: 96 segments, 3599 tokens of 6144 channels 27 us (3.4 TB/s,
+// 40% of the issue slots); more or fewer tokens a job (4, 16) and a forced occupancy were slower.
 constexpr int RPT = 8;
 
 struct ConvParams {
