@@ -5,8 +5,9 @@
 // position kv_lens[s] - (cu[s + 1] - t), in page page_table[s][position / page_size].
 // Both directions move every row once and compute next to nothing: HBM-bound (latency-bound for a
 // decoding step's few rows).  A warp owns a token and has four rows' loads in flight.  Measured, e4m3: 55899 cached
-// positions of 2 heads of 256 read back in 34 us (5.0 TB/s); 34198 tokens of 4 heads of 128 written and read back
-// in 48 us (4.4 TB/s), 55 with one row in flight; 64 tokens written and read back 8.3 us with both launches.
+// positions of 2 heads of 256 read back in 32.5 us (5.3 TB/s); 34198 tokens of 4 heads of 128 written and read back
+// in 40.6 us (5.2 TB/s; 55 with one row in flight, 46 with every address worked out in full); 64 tokens written and
+// read back 6.2 us with both launches.
 #include "paged.cuh"
 
 namespace fdk {
@@ -76,13 +77,16 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvParams p) {
   if (t >= p.tokens) return;
   const int sub = lane / LPR, c = (lane % LPR) * 8;
   const int rows = 2 * p.hkv;
+  // Issue slots bound the large calls, so every address is a base of the token, chosen once a row, plus the head's
+  // 32-bit offset.
+  auto pick = [&](bool is_v, auto* k, auto* v) { return is_v ? v : k; };
   uint4 raw[BATCH];
   auto load_new = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const int r = min(r0 + i * RPI + sub, rows - 1);
-      const bf16* src = r >= p.hkv ? p.v + t * p.ld_v + (r - p.hkv) * D : p.k + t * p.ld_k + r * D;
-      raw[i] = ldg_stream(src + c);
+      const bool is_v = r >= p.hkv;
+      raw[i] = ldg_stream(pick(is_v, p.k + t * p.ld_k + c, p.v + t * p.ld_v + c) + (is_v ? r - p.hkv : r) * D);
     }
   };
   if (!READ) load_new(0);
@@ -90,26 +94,33 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvParams p) {
   int off = 0;
   const Where where = locate(p, t, lane, page, off);
   if (where == OUTSIDE || (!READ && where == NONE)) return;
+  // `page` and `off` are 0 where there is no row: a valid place
+  constexpr int ESZ = QUANT ? 1 : 2;
+  uint8_t* const k_at = static_cast<uint8_t*>(p.k_cache) + (page * p.ld_kpage + off * D + c) * ESZ;
+  uint8_t* const v_at = static_cast<uint8_t*>(p.v_cache) + (page * p.ld_vpage + off * D + c) * ESZ;
+  uint8_t* const ks_at = QUANT ? p.k_scale + page * p.ld_kscale_page + off : nullptr;
+  uint8_t* const vs_at = QUANT ? p.v_scale + page * p.ld_vscale_page + off : nullptr;
   for (int r0 = 0; r0 < rows; r0 += BATCH * RPI) {
     if (READ) {
       int bytes[BATCH];
       uint2 q8[BATCH];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {  // `page` and `off` are 0 where there is no row: a valid place
+      for (int i = 0; i < BATCH; ++i) {
         const int r = min(r0 + i * RPI + sub, rows - 1);
         const bool is_v = r >= p.hkv;
-        const int64_t slot = ((int64_t)(is_v ? r - p.hkv : r) << p.page_shift) + off;
-        const int64_t at = page * (is_v ? p.ld_vpage : p.ld_kpage) + slot * D + c;
+        const int slot = (is_v ? r - p.hkv : r) << p.page_shift;
+        const uint8_t* src = pick(is_v, k_at, v_at) + slot * (D * ESZ);
         if (QUANT) {
-          q8[i] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + at));
-          bytes[i] = __ldg((is_v ? p.v_scale : p.k_scale) + page * (is_v ? p.ld_vscale_page : p.ld_kscale_page) + slot);
+          q8[i] = __ldg(reinterpret_cast<const uint2*>(src));
+          bytes[i] = __ldg(pick(is_v, ks_at, vs_at) + slot);
         } else {
-          raw[i] = ldg_stream(static_cast<const bf16*>(is_v ? p.v_cache : p.k_cache) + at);
+          raw[i] = ldg_stream(reinterpret_cast<const bf16*>(src));
         }
       }
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         const int r = r0 + i * RPI + sub;
+        const bool is_v = r >= p.hkv;
         if (QUANT) {
           const float s = scale_value(bytes[i]);
           const uint16_t q[4] = {(uint16_t)q8[i].x, (uint16_t)(q8[i].x >> 16), (uint16_t)q8[i].y, (uint16_t)(q8[i].y >> 16)};
@@ -117,15 +128,15 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvParams p) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const uint32_t h2 = e4m3x2_to_f16x2(q[u]);
-            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-            f[2 * u] = w.x * s;
-            f[2 * u + 1] = w.y * s;
+            const float2 w = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&h2)), make_float2(s, s));
+            f[2 * u] = w.x;
+            f[2 * u + 1] = w.y;
           }
           raw[i] = pack8(f);
         }
         if (where == NONE) raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows)
-          *reinterpret_cast<uint4*>((r >= p.hkv ? p.v_out + (t * p.hkv + r - p.hkv) * D : p.k_out + (t * p.hkv + r) * D) + c) = raw[i];
+        bf16* dst = pick(is_v, p.k_out + t * p.hkv * D + c, p.v_out + t * p.hkv * D + c) + (is_v ? r - p.hkv : r) * D;
+        if (r < rows) *reinterpret_cast<uint4*>(dst) = raw[i];
       }
     } else {
       if (r0 > 0) load_new(r0);
@@ -133,27 +144,30 @@ __global__ void __launch_bounds__(128) kv_rows_kernel(const KvParams p) {
       for (int i = 0; i < BATCH; ++i) {
         const int r = r0 + i * RPI + sub;
         const bool is_v = r >= p.hkv;
-        const int64_t slot = ((int64_t)(is_v ? r - p.hkv : r) << p.page_shift) + off;
-        const int64_t at = page * (is_v ? p.ld_vpage : p.ld_kpage) + slot * D + c;
+        const int slot = (is_v ? r - p.hkv : r) << p.page_shift;
+        uint8_t* dst = pick(is_v, k_at, v_at) + slot * (D * ESZ);
         if (!QUANT) {
-          if (r < rows) *reinterpret_cast<uint4*>(static_cast<bf16*>(is_v ? p.v_cache : p.k_cache) + at) = raw[i];
+          if (r < rows) *reinterpret_cast<uint4*>(dst) = raw[i];
         } else {
-          float f[8];
-          unpack8(raw[i], f);
-          float a = 0.f;
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
 #pragma unroll
-          for (int u = 0; u < 8; ++u) a = fmaxf(a, fabsf(f[u]));
+          for (int u = 1; u < 4; ++u) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[u])));
+          float a = fmaxf(__low2float(m), __high2float(m));
 #pragma unroll
           for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
           const int b = scale_byte(a);
           const float inv = scale_inverse(b);
           uint16_t q[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) q[u] = f32x2_to_e4m3x2(f[2 * u] * inv, f[2 * u + 1] * inv);
+          for (int u = 0; u < 4; ++u) {
+            const float2 f = __fmul2_rn(make_float2(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xffff0000u)),
+                                        make_float2(inv, inv));
+            q[u] = f32x2_to_e4m3x2(f.x, f.y);
+          }
           if (r < rows) {
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + at) =
-                make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
-            if (c == 0) (is_v ? p.v_scale : p.k_scale)[page * (is_v ? p.ld_vscale_page : p.ld_kscale_page) + slot] = (uint8_t)b;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
+            if (c == 0) pick(is_v, ks_at, vs_at)[slot] = (uint8_t)b;
           }
         }
       }
