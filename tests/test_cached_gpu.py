@@ -188,6 +188,15 @@ def test_attention_many_tokens_parts_cut_on_the_device(hq, hkv, D, quant):
     run_attn(n, [500, 40, 0, 350, 64, 290, 1, 333], hq, hkv, D, 32, quant, seed=43)
 
 
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", [(6, 1, 128), (10, 2, 128), (4, 4, 256), (7, 1, 256)])
+def test_attention_most_segments_the_device_sorts(hq, hkv, D, quant):
+    # 64 segments, groups that do not divide a tile, contexts shorter than the tokens among them
+    n = [37 * i % 90 for i in range(64)]
+    kv = [max(x + 311 * i % 1300 - 20, 0) for i, x in enumerate(n)]
+    run_attn(n, kv, hq, hkv, D, 64, quant, seed=47, gate=hkv == 2)
+
+
 @pytest.mark.parametrize("n,kv", [([1, 2, 3], [700, 40, 9]), ([1], [5000]), ([80, 33], [90, 333]), ([70], [6000])])
 @pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
 def test_attention_gates_of_any_size(n, kv, hq, hkv, D):
