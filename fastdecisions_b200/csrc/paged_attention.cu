@@ -152,9 +152,10 @@ struct Tiles {
 // one key of a CTA's work: while every CTA has an SM the longest part is the time, else the whole work
 // shared out, with half a part more for its uneven end; a CTA's start is START, the join JOIN and the
 // float32 rows of each part written and read.  Measured against a rule on the longest range alone, which has
-// to favour even or ragged contexts: 8 segments of 100 to 700 tokens behind 600 to 8000 positions, e4m3, 110 us
-// (170 unsplit); 74 of 32 behind 4608, 2 KV heads of 256, 113 us (152 in two parts).  Every CTA gets the same answer (integers only); one leaves it
-// for the join, whose many warps would take 20 us to work it out again.
+// to favour even or ragged contexts: 8 segments of 100 to 700 tokens behind 600 to 8000 positions, e4m3, page
+// 64, 107 us (170 unsplit); 74 of 32 behind 4608, 2 KV heads of 256, 113 us (152 in two parts).  Every CTA gets
+// the same answer (integers only); one leaves it for the join, whose many warps would take 20 us to work it out
+// again.
 constexpr int SMS = 148;
 constexpr int START_KEYS = 448, JOIN_KEYS = 256;
 __device__ __forceinline__ int best_part_keys(const Params& p, const Tiles& t, int lane) {
@@ -852,10 +853,10 @@ constexpr int few_ctas(int64_t ctas, int rows, int64_t d, bool quant) {
   return ctas < SMS ? (quant ? 3 : d == 128 ? 2 : 1) : rows <= 16 ? 12 : 4;
 }
 // Splits as clusters while all of them run at once, up to eight, and eight where more would be short: one token
-// behind 1535 positions 12.4 -> 10.3 us, 8 x 2048 12.6 -> 9.6 us (bf16, head_dim 128).  With more CTAs the short parts would wait for the long ones: 64
-// segments of 500 to 8192, e4m3, 54 us with the second kernel, 70 in clusters.  At head_dim 256 in bf16 a CTA
-// fills an SM, and more than eight clusters no longer find their eight SMs in one GPC: 13 us against 20 at
-// 8 x 2048.
+// behind 1535 positions 12.4 -> 10.3 us, 8 x 2048 12.6 -> 9.6 us (bf16, head_dim 128).  With more CTAs the short
+// parts would wait for the long ones: 64 segments of 500 to 8192, e4m3, 54 us with the second kernel, 70 in
+// clusters.  At head_dim 256 in bf16 a CTA fills an SM, and more than eight clusters no longer find their eight
+// SMs in one GPC: 13 us against 20 at 8 x 2048.
 static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
                       int64_t group, int64_t d, bool quant) {
   Plan r = {};
