@@ -19,7 +19,7 @@
 //   outside the cache is an out-of-range coordinate, which TMA fills with zeros.  V rows at or behind
 //   kv_lens[s] may hold anything (0 * NaN would reach the sums): the block that has them is zeroed there
 //   after its load and before the MMA warp sees it.
-//   8-bit cache: TMA brings the raw e4m3 rows; four converter warps turn them into fp16 operands (e4m3 ->
+//   8-bit cache: TMA brings the raw e4m3 rows; six converter warps turn them into fp16 operands (e4m3 ->
 //   fp16 is exact) multiplied by the row's scale relative to the largest one of the CTA's key range
 //   (exact for scales within 2^15 of it; smaller ones lose bits below 2^-33 of the range's largest
 //   element).  The largest K scale then folds into the softmax scale, V's into the final normalisation,
@@ -32,7 +32,7 @@
 // Measured (B200, device time): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 246 us,
 // 1.07 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050: the softmax's exponentials and the
 // operands' shared-memory traffic take as long each.  8 ragged chunks (2544 tokens behind 600 to 8000), e4m3, page
-// 16: 127 us; 4400 cycles a block, 22000 before the first, and uneven CTAs.  48 questions of 9 to 70 tokens behind
+// 16: 115 us; 3700 cycles a block, 20000 before the first, and uneven CTAs.  48 questions of 9 to 70 tokens behind
 // 1490 shared positions, 8 / 2 heads of 256, bf16: 45 us; a block of 64 keys brings 64 KB from L2, 32 bytes a clock
 // and SM, which sets its 2050 cycles; the start and the epilogue of the one wave are a third of the call.
 #pragma once
@@ -82,12 +82,13 @@ constexpr uint32_t TM_COLS = 512;
 constexpr float P_SHIFT = 6.f;  // fp16 P is scaled by 2^6: weights down to 2^-30 of the row's largest stay
 constexpr long long DRAIN_BUDGET = 2000000000LL;
 
-// warps: NT * 4 softmax, one producer, one MMA issuer and TMEM allocator; with the 8-bit cache four
-// converter warps on a warpgroup boundary
+// warps: NT * 4 softmax, one producer, one MMA issuer and TMEM allocator; with the 8-bit cache six
+// converter warps, which fill the warpgroups (with four of them 8 ragged chunks took 128 us, not 115)
 template <int D, bool QUANT>
 struct Roles {
-  static constexpr int PRODUCER = Geo<D>::NT * 4, MMA = PRODUCER + 1, CONV = PRODUCER + 4;
-  static constexpr int THREADS = QUANT ? (CONV + 4) * 32 : (MMA + 1) * 32;
+  static constexpr int PRODUCER = Geo<D>::NT * 4, MMA = PRODUCER + 1, CONV = MMA + 1;
+  static constexpr int CT = QUANT ? 192 : 0;  // converter threads
+  static constexpr int THREADS = CONV * 32 + CT;
   static constexpr bool SPLIT_REGS = QUANT && D == 128;
 };
 
@@ -235,7 +236,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + M::OFF_MISC);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + M::OFF_MISC + 4);
   volatile int* scale_max = reinterpret_cast<volatile int*>(gbase + M::OFF_MISC + 8);  // largest K, V scale byte
-  int* warp_max = reinterpret_cast<int*>(gbase + M::OFF_MISC + 16);                    // [4][2]
+  int* warp_max = reinterpret_cast<int*>(gbase + M::OFF_MISC + 16);                    // [6][2]; over `pick`, read by then
   uint8_t* q_exp = gbase + M::OFF_QS;
   uint32_t* factor = reinterpret_cast<uint32_t*>(gbase + M::OFF_FT);                   // [2][BN] half2
 
@@ -309,7 +310,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       uint32_t count = 1;
       if (i >= B_P && i < B_P2 + 2) count = 128;
       if ((QUANT || G::Q_TMEM) && i == B_Q) count = two ? 256 : 128;
-      if (QUANT && ((i >= B_F && i < B_F + 6) || (i >= B_RE && i < B_RE + 4))) count = 128;
+      if (QUANT && ((i >= B_F && i < B_F + 6) || (i >= B_RE && i < B_RE + 4))) count = R::CT;
       mbar_init(bar(i), count);
     }
     *abort_flag = 0;
@@ -401,233 +402,233 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     }
   };
 
-  if (warp == R::PRODUCER && !R::SPLIT_REGS) {
-    producer();
-  } else if (QUANT ? warp >= R::PRODUCER && warp < R::CONV : warp == R::MMA) {
+  if (warp >= R::PRODUCER) {
     // With the 8-bit cache at head_dim 128, 512 threads are launched with 128 registers each; the softmax
-    // needs more (a row of S and of P), the other warpgroups less: 256 * 192 + 128 * (40 + 88) = 65536.
-    if constexpr (R::SPLIT_REGS) {
-      reg_dec<40>();
-      if (warp == R::PRODUCER) producer();
-    }
-    // ------------------------------------------------------------------ MMA issuer
-    if (warp == R::MMA && lane == 0) {
-      constexpr uint32_t ID_QK = idesc(128, BN, false, QUANT);
-      constexpr uint32_t ID_PV = idesc(128, D, true, QUANT);  // V is MN-major (columns contiguous)
-      auto issue_s = [&](int j, int tile, uint32_t tm) {
-        const uint64_t dq = G::Q_TMEM ? 0 : sdesc_sw128(base + M::OFF_Q + tile * G::QT, 16, 1024);
-        const uint64_t dk = sdesc_sw128(base + M::OFF_KV + (2 * j % M::SLOTS) * G::KT, 16, 1024);
+    // needs more (a row of S and of P), the other two warpgroups less: 256 * 192 + 256 * 64 = 65536.
+    if constexpr (R::SPLIT_REGS) reg_dec<64>();
+    if (warp == R::PRODUCER) {
+      producer();
+    } else if (warp == R::MMA) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t ID_QK = idesc(128, BN, false, QUANT);
+        constexpr uint32_t ID_PV = idesc(128, D, true, QUANT);  // V is MN-major (columns contiguous)
+        auto issue_s = [&](int j, int tile, uint32_t tm) {
+          const uint64_t dq = G::Q_TMEM ? 0 : sdesc_sw128(base + M::OFF_Q + tile * G::QT, 16, 1024);
+          const uint64_t dk = sdesc_sw128(base + M::OFF_KV + (2 * j % M::SLOTS) * G::KT, 16, 1024);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t qo = ((kk >> 2) * G::QBOX + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * G::KBOX + (kk & 3) * 32) >> 4;
-          if (G::Q_TMEM) umma_ts(tmem + tm, tmem + G::TM_Q + 8 * kk, dk + ko, ID_QK, kk > 0);
-          else umma_ss(tmem + tm, dq + qo, dk + ko, ID_QK, kk > 0);
-        }
-      };
-      auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o, int k0) {
-        const uint64_t dv = sdesc_sw128(base + M::OFF_KV + ((2 * j + 1) % M::SLOTS) * G::KT, G::KBOX, 1024);
-#pragma unroll
-        for (int kk = k0; kk < k0 + 4; ++kk)  // 64 keys
-          umma_ts(tmem + tm_o, tmem + tm_p + 8 * kk, dv + (uint32_t)(kk * 2048 >> 4), ID_PV, (j > 0 || kk > 0) ? 1u : 0u);
-      };
-      auto wait = [&](int i, int parity) { return mbar_wait(bar(i), (uint32_t)parity & 1u, abort_flag); };
-      auto full = [&](int item) { return wait(B_F + item % M::SLOTS, item / M::SLOTS); };
-      auto release = [&](int item) { umma_commit(bar(B_E + item % M::SLOTS)); };
-      bool ok = wait(B_Q, 0) && full(0);
-      if (NT == 2) {
-        if (ok) {
-          tc_fence_after();
-          issue_s(0, 0, G::TM_S(0));
-          umma_commit(bar(B_S));
-          if (two) {
-            issue_s(0, 1, G::TM_S(1));
-            umma_commit(bar(B_S + 1));
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t qo = ((kk >> 2) * G::QBOX + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * G::KBOX + (kk & 3) * 32) >> 4;
+            if (G::Q_TMEM) umma_ts(tmem + tm, tmem + G::TM_Q + 8 * kk, dk + ko, ID_QK, kk > 0);
+            else umma_ss(tmem + tm, dq + qo, dk + ko, ID_QK, kk > 0);
           }
-          release(0);
-        }
-        for (int j = 0; ok && j < n_kv; ++j) {
-          const bool more = j + 1 < n_kv;
-          if (!full(2 * j + 1) || !wait(B_P, j)) break;
-          tc_fence_after();
-          issue_pv(j, G::TM_S(0), G::TM_O(0), 0);
-          if (!wait(B_P2, j)) break;
-          tc_fence_after();
-          issue_pv(j, G::TM_S(0), G::TM_O(0), 4);
-          if (more) {
-            if (!full(2 * j + 2)) break;
+        };
+        auto issue_pv = [&](int j, uint32_t tm_p, uint32_t tm_o, int k0) {
+          const uint64_t dv = sdesc_sw128(base + M::OFF_KV + ((2 * j + 1) % M::SLOTS) * G::KT, G::KBOX, 1024);
+#pragma unroll
+          for (int kk = k0; kk < k0 + 4; ++kk)  // 64 keys
+            umma_ts(tmem + tm_o, tmem + tm_p + 8 * kk, dv + (uint32_t)(kk * 2048 >> 4), ID_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        };
+        auto wait = [&](int i, int parity) { return mbar_wait(bar(i), (uint32_t)parity & 1u, abort_flag); };
+        auto full = [&](int item) { return wait(B_F + item % M::SLOTS, item / M::SLOTS); };
+        auto release = [&](int item) { umma_commit(bar(B_E + item % M::SLOTS)); };
+        bool ok = wait(B_Q, 0) && full(0);
+        if (NT == 2) {
+          if (ok) {
             tc_fence_after();
-            issue_s(j + 1, 0, G::TM_S(0));
+            issue_s(0, 0, G::TM_S(0));
             umma_commit(bar(B_S));
-          }
-          if (two) {
-            if (!wait(B_P + 1, j)) break;
-            tc_fence_after();
-            issue_pv(j, G::TM_S(1), G::TM_O(1), 0);
-            if (!wait(B_P2 + 1, j)) break;
-            tc_fence_after();
-            issue_pv(j, G::TM_S(1), G::TM_O(1), 4);
-          }
-          release(2 * j + 1);
-          if (more) {
             if (two) {
-              issue_s(j + 1, 1, G::TM_S(1));
+              issue_s(0, 1, G::TM_S(1));
               umma_commit(bar(B_S + 1));
             }
-            release(2 * j + 2);
+            release(0);
           }
-        }
-      } else {
-        auto s_block = [&](int j) {
-          issue_s(j, 0, G::TM_S(j & 1));
-          umma_commit(bar(B_S + (j & 1)));
-          release(2 * j);
-        };
-        if (ok) {
-          tc_fence_after();
-          s_block(0);
-          if (n_kv > 1 && (ok = full(2))) {
+          for (int j = 0; ok && j < n_kv; ++j) {
+            const bool more = j + 1 < n_kv;
+            if (!full(2 * j + 1) || !wait(B_P, j)) break;
             tc_fence_after();
-            s_block(1);
-          }
-        }
-        for (int j = 0; ok && j < n_kv; ++j) {
-          if (!full(2 * j + 1) || !wait(B_P + (j & 1), j >> 1)) break;
-          tc_fence_after();
-          issue_pv(j, G::TM_S(j & 1), G::TM_O(0), 0);
-          umma_commit(bar(B_PV));
-          release(2 * j + 1);
-          if (j + 2 < n_kv) {
-            if (!full(2 * j + 4)) break;
+            issue_pv(j, G::TM_S(0), G::TM_O(0), 0);
+            if (!wait(B_P2, j)) break;
             tc_fence_after();
-            s_block(j + 2);
+            issue_pv(j, G::TM_S(0), G::TM_O(0), 4);
+            if (more) {
+              if (!full(2 * j + 2)) break;
+              tc_fence_after();
+              issue_s(j + 1, 0, G::TM_S(0));
+              umma_commit(bar(B_S));
+            }
+            if (two) {
+              if (!wait(B_P + 1, j)) break;
+              tc_fence_after();
+              issue_pv(j, G::TM_S(1), G::TM_O(1), 0);
+              if (!wait(B_P2 + 1, j)) break;
+              tc_fence_after();
+              issue_pv(j, G::TM_S(1), G::TM_O(1), 4);
+            }
+            release(2 * j + 1);
+            if (more) {
+              if (two) {
+                issue_s(j + 1, 1, G::TM_S(1));
+                umma_commit(bar(B_S + 1));
+              }
+              release(2 * j + 2);
+            }
+          }
+        } else {
+          auto s_block = [&](int j) {
+            issue_s(j, 0, G::TM_S(j & 1));
+            umma_commit(bar(B_S + (j & 1)));
+            release(2 * j);
+          };
+          if (ok) {
+            tc_fence_after();
+            s_block(0);
+            if (n_kv > 1 && (ok = full(2))) {
+              tc_fence_after();
+              s_block(1);
+            }
+          }
+          for (int j = 0; ok && j < n_kv; ++j) {
+            if (!full(2 * j + 1) || !wait(B_P + (j & 1), j >> 1)) break;
+            tc_fence_after();
+            issue_pv(j, G::TM_S(j & 1), G::TM_O(0), 0);
+            umma_commit(bar(B_PV));
+            release(2 * j + 1);
+            if (j + 2 < n_kv) {
+              if (!full(2 * j + 4)) break;
+              tc_fence_after();
+              s_block(j + 2);
+            }
+          }
+        }
+        umma_commit(bar(B_O));  // arrives when every MMA above has completed
+        drain(bar(B_O), 0);
+      }
+    } else if constexpr (QUANT) {
+      // ------------------------------------------------------------------ converters
+      const int ct = tid - R::CONV * 32, cw = ct >> 5;
+      auto slot_of = [&](int key) { return (hk << p.page_shift) + (key & page_mask); };
+      const int my = ct < BN ? ct : 0;
+      auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
+      auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
+        const bool live = (uint32_t)id < (uint32_t)p.num_pages && key < ke;  // a bad id is reported by the producer
+        const int b = __ldg(scales + ((live ? id : 0) * page_ld + slot_of(key)));
+        return live ? b : 0;
+      };
+      int id = page_at(kb + my);
+      int kbyte = scale_at(p.k_scale, p.kscale_page, kb + my, id), vbyte = scale_at(p.v_scale, p.vscale_page, kb + my, id);
+      id = page_at(kb + BN + my);
+      // largest scale bytes of the range, 16 keys a load
+      uint32_t mk = 0, mv = 0;
+      constexpr int AHEAD = 4;  // page ids, then scales, of that many steps in flight
+      for (int key0 = kb + ct * 16; key0 < ke; key0 += AHEAD * R::CT * 16) {
+        int64_t ids[AHEAD];
+        uint4 a[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ids[u] = __ldg(table + (min(key0 + u * R::CT * 16, ke - 1) >> p.page_shift));
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int key = key0 + u * R::CT * 16;
+          a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (key < ke && ids[u] >= 0 && ids[u] < p.num_pages) {  // a bad id is reported by the loads below
+            a[u] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + ids[u] * p.kscale_page + slot_of(key)));
+            b[u] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + ids[u] * p.vscale_page + slot_of(key)));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int key = key0 + u * R::CT * 16;
+          const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int left = ke - (key + 4 * i);  // bytes of this word inside the range
+            const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+            mk = __vmaxu4(mk, aw[i] & mask);
+            mv = __vmaxu4(mv, bw[i] & mask);
           }
         }
       }
-      umma_commit(bar(B_O));  // arrives when every MMA above has completed
-      drain(bar(B_O), 0);
-    }
-  } else if (QUANT && warp >= R::CONV) {
-    // ------------------------------------------------------------------ converters (128 threads)
-    if constexpr (R::SPLIT_REGS) reg_dec<88>();
-    const int ct = tid - R::CONV * 32, cw = ct >> 5;
-    auto slot_of = [&](int key) { return (hk << p.page_shift) + (key & page_mask); };
-    const int my = ct < BN ? ct : 0;
-    auto page_at = [&](int key) { return __ldg(table + (min(key, ke - 1) >> p.page_shift)); };
-    auto scale_at = [&](const uint8_t* scales, int64_t page_ld, int key, int id) -> int {
-      const bool live = (uint32_t)id < (uint32_t)p.num_pages && key < ke;  // a bad id is reported by the producer
-      const int b = __ldg(scales + ((live ? id : 0) * page_ld + slot_of(key)));
-      return live ? b : 0;
-    };
-    int id = page_at(kb + my);
-    int kbyte = scale_at(p.k_scale, p.kscale_page, kb + my, id), vbyte = scale_at(p.v_scale, p.vscale_page, kb + my, id);
-    id = page_at(kb + BN + my);
-    // largest scale bytes of the range, 16 keys a load
-    uint32_t mk = 0, mv = 0;
-    constexpr int AHEAD = 4;  // page ids, then scales, of that many steps in flight
-    for (int key0 = kb + ct * 16; key0 < ke; key0 += AHEAD * 128 * 16) {
-      int64_t ids[AHEAD];
-      uint4 a[AHEAD], b[AHEAD];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) ids[u] = __ldg(table + (min(key0 + u * 128 * 16, ke - 1) >> p.page_shift));
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int key = key0 + u * 128 * 16;
-        a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (key < ke && ids[u] >= 0 && ids[u] < p.num_pages) {  // a bad id is reported by the loads below
-          a[u] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + ids[u] * p.kscale_page + slot_of(key)));
-          b[u] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + ids[u] * p.vscale_page + slot_of(key)));
-        }
+      auto byte_max = [](uint32_t w) { return max(max(w & 255u, (w >> 8) & 255u), max((w >> 16) & 255u, w >> 24)); };
+      mk = __reduce_max_sync(0xffffffffu, byte_max(mk));
+      mv = __reduce_max_sync(0xffffffffu, byte_max(mv));
+      if (lane == 0) {
+        warp_max[2 * cw] = (int)mk;
+        warp_max[2 * cw + 1] = (int)mv;
       }
+      asm volatile("bar.sync 1, 192;\n" ::: "memory");
+      int ek = 0, ev = 0;
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int key = key0 + u * 128 * 16;
-        const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int left = ke - (key + 4 * i);  // bytes of this word inside the range
-          const uint32_t mask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-          mk = __vmaxu4(mk, aw[i] & mask);
-          mv = __vmaxu4(mv, bw[i] & mask);
-        }
+      for (int i = 0; i < R::CT / 32; ++i) {
+        ek = max(ek, warp_max[2 * i]);
+        ev = max(ev, warp_max[2 * i + 1]);
       }
-    }
-    auto byte_max = [](uint32_t w) { return max(max(w & 255u, (w >> 8) & 255u), max((w >> 16) & 255u, w >> 24)); };
-    mk = __reduce_max_sync(0xffffffffu, byte_max(mk));
-    mv = __reduce_max_sync(0xffffffffu, byte_max(mv));
-    if (lane == 0) {
-      warp_max[2 * cw] = (int)mk;
-      warp_max[2 * cw + 1] = (int)mv;
-    }
-    asm volatile("bar.sync 1, 128;\n" ::: "memory");
-    int ek = 0, ev = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ek = max(ek, warp_max[2 * i]);
-      ev = max(ev, warp_max[2 * i + 1]);
-    }
-    if (ct == 0) {  // the softmax reads them behind the first S, the epilogue later still
-      scale_max[0] = ek;
-      scale_max[1] = ev;
-    }
-    constexpr int TPR = D / 8, RPP = 128 / TPR;  // threads a row, rows a pass (of 128 threads)
-    const int lc = ct % TPR, lr = ct / TPR;
-    // Items: thread ct is row ct's keeper (its scale byte, loaded a block ahead) and, for the conversion,
-    // piece lc (8 columns) of rows lr, lr + RPP, ..: 8 raw bytes become one 16-byte operand chunk.  Eight
-    // neighbouring threads read 64 consecutive bytes and store all eight chunk positions: no conflicts.
-    constexpr int PASSES = BN / RPP;
-    // Rows loaded before the first store (the compiler keeps their order, so a load behind a store waits for it): at
-    // head_dim 256 the converters set the pace (74 x 32 tokens behind 4096 shared positions: 130 us with 1, 104
-    // with 4, 101 with 8); at 128 issue slots do, which the softmax needs as well (37 x 64: 114 us with 1, 115 with
-    // 2, 117 with 4; 131 with the test of `live` in full blocks too).
-    constexpr int BURST = D == 128 ? 1 : 8;
-    // once a wait has run out, a thread only keeps step at the named barrier (the others may be behind it)
-    bool ok = true;
-    for (int j = 0; j < n_kv; ++j) {
-      const int key0 = kb + j * BN;
-      const uint32_t fk = half2_bits(scale_value(max(kbyte - ek + 127, 0))), fv = half2_bits(scale_value(max(vbyte - ev + 127, 0)));
-      // rows behind the range may hold anything, NaN included: their operands are zeros, not 0 * NaN
-      const int live = ke - key0;
-      kbyte = scale_at(p.k_scale, p.kscale_page, key0 + BN + my, id);
-      vbyte = scale_at(p.v_scale, p.vscale_page, key0 + BN + my, id);
-      id = page_at(key0 + 2 * BN + my);
+      if (ct == 0) {  // the softmax reads them behind the first S, the epilogue later still
+        scale_max[0] = ek;
+        scale_max[1] = ev;
+      }
+      constexpr int TPR = D / 8, RPP = R::CT / TPR;  // threads a row, rows a pass
+      const int lc = ct % TPR, lr = ct / TPR;
+      // Items: thread ct is row ct's keeper (its scale byte, loaded a block ahead) and, for the conversion,
+      // piece lc (8 columns) of rows lr, lr + RPP, ..: 8 raw bytes become one 16-byte operand chunk.  Eight
+      // neighbouring threads read 64 consecutive bytes and store all eight chunk positions: no conflicts.
+      constexpr int PASSES = (BN + RPP - 1) / RPP;  // the last one is short
+      // Rows loaded before the first store (the compiler keeps their order, so a load behind a store waits for it): at
+      // head_dim 256 the converters set the pace (74 x 32 tokens behind 4096 shared positions: 92 us with 4, 93
+      // with 6, 97 with 8; 130 with 1 and four warps); at 128 issue slots do, which the softmax needs as well (37 x
+      // 64: 95 us with 1, 96.5 with 2, 96 with 4; a test of `live` in full blocks too cost 15%).
+      constexpr int BURST = D == 128 ? 1 : 4;
+      // once a wait has run out, a thread only keeps step at the named barrier (the others may be behind it)
+      bool ok = true;
+      for (int j = 0; j < n_kv; ++j) {
+        const int key0 = kb + j * BN;
+        const uint32_t fk = half2_bits(scale_value(max(kbyte - ek + 127, 0))), fv = half2_bits(scale_value(max(vbyte - ev + 127, 0)));
+        // rows behind the range may hold anything, NaN included: their operands are zeros, not 0 * NaN
+        const int live = ke - key0;
+        kbyte = scale_at(p.k_scale, p.kscale_page, key0 + BN + my, id);
+        vbyte = scale_at(p.v_scale, p.vscale_page, key0 + BN + my, id);
+        id = page_at(key0 + 2 * BN + my);
 #pragma unroll 1
-      for (int which = 0; which < 2; ++which) {
-        const int item = 2 * j + which, raw_slot = item % RAW_SLOTS, slot = item % M::SLOTS;
-        if (ct < BN) factor[which * BN + ct] = which ? fv : fk;
-        asm volatile("bar.sync 1, 128;\n" ::: "memory");  // factors written; also: nobody still reads the other table
-        ok = ok && mbar_wait(bar(B_RF + raw_slot), (uint32_t)(item / RAW_SLOTS) & 1u, abort_flag) &&
-             (item < M::SLOTS || mbar_wait(bar(B_E + slot), (uint32_t)(item / M::SLOTS - 1) & 1u, abort_flag));
-        if (!ok) continue;
-        const uint8_t* src = gbase + M::OFF_RAW + raw_slot * M::RAWT + lr * D + lc * 8;
-        uint8_t* dst = gbase + M::OFF_KV + slot * G::KT;
-        const uint32_t* fac = factor + which * BN + lr;
-        auto convert = [&](bool partial) {
+        for (int which = 0; which < 2; ++which) {
+          const int item = 2 * j + which, raw_slot = item % RAW_SLOTS, slot = item % M::SLOTS;
+          if (ct < BN) factor[which * BN + ct] = which ? fv : fk;
+          asm volatile("bar.sync 1, 192;\n" ::: "memory");  // factors written; also: nobody still reads the other table
+          ok = ok && mbar_wait(bar(B_RF + raw_slot), (uint32_t)(item / RAW_SLOTS) & 1u, abort_flag) &&
+               (item < M::SLOTS || mbar_wait(bar(B_E + slot), (uint32_t)(item / M::SLOTS - 1) & 1u, abort_flag));
+          if (!ok) continue;
+          const uint8_t* src = gbase + M::OFF_RAW + raw_slot * M::RAWT + lr * D + lc * 8;
+          uint8_t* dst = gbase + M::OFF_KV + slot * G::KT;
+          const uint32_t* fac = factor + which * BN + lr;
+          auto convert = [&](bool partial) {
 #pragma unroll
-          for (int i0 = 0; i0 < PASSES; i0 += BURST) {
-            uint2 w[BURST];
-            uint32_t f[BURST];
+            for (int i0 = 0; i0 < PASSES; i0 += BURST) {
+              uint2 w[BURST];
+              uint32_t f[BURST];
 #pragma unroll
-            for (int i = 0; i < BURST; ++i) {
-              w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * RPP * D);
-              if (partial && lr + (i0 + i) * RPP >= live) w[i] = make_uint2(0u, 0u);
-              f[i] = fac[(i0 + i) * RPP];
+              for (int i = 0; i < BURST; ++i) {
+                if (i0 + i >= PASSES || ((i0 + i + 1) * RPP > BN && lr + (i0 + i) * RPP >= BN)) continue;
+                w[i] = *reinterpret_cast<const uint2*>(src + (i0 + i) * RPP * D);
+                if (partial && lr + (i0 + i) * RPP >= live) w[i] = make_uint2(0u, 0u);
+                f[i] = fac[(i0 + i) * RPP];
+              }
+#pragma unroll
+              for (int i = 0; i < BURST; ++i) {
+                if (i0 + i >= PASSES || ((i0 + i + 1) * RPP > BN && lr + (i0 + i) * RPP >= BN)) continue;
+                uint4 h;
+                h.x = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].x), f[i]);
+                h.y = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].x >> 16)), f[i]);
+                h.z = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].y), f[i]);
+                h.w = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].y >> 16)), f[i]);
+                *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(lr + (i0 + i) * RPP, lc)) = h;
+              }
             }
-#pragma unroll
-            for (int i = 0; i < BURST; ++i) {
-              uint4 h;
-              h.x = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].x), f[i]);
-              h.y = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].x >> 16)), f[i]);
-              h.z = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)w[i].y), f[i]);
-              h.w = hmul2_bits(paged::e4m3x2_to_f16x2((uint16_t)(w[i].y >> 16)), f[i]);
-              *reinterpret_cast<uint4*>(dst + chunk_at<G::KBOX>(lr + (i0 + i) * RPP, lc)) = h;
-            }
-          }
-        };
-        if (live >= BN) convert(false);
-        else convert(true);
-        fence_proxy_async_smem();
-        mbar_arrive(bar(B_F + slot));
-        mbar_arrive(bar(B_RE + raw_slot));
+          };
+          if (live >= BN) convert(false);
+          else convert(true);
+          fence_proxy_async_smem();
+          mbar_arrive(bar(B_F + slot));
+          mbar_arrive(bar(B_RE + raw_slot));
+        }
       }
     }
   } else {
