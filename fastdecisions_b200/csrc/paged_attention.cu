@@ -867,13 +867,15 @@ static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, 
     const int64_t per = (d == 128 ? 2 : 1) * (128 / group);  // tokens a CTA
     r.row_blocks = (max_seqlen + per - 1) / per;
     // CTAs that have work: from the tokens, half a tile more a segment and one at least, not from the longest one
-    int64_t ctas = hkv * std::max(tokens / per + (num_segments + 1) / 2, std::min(num_segments, tokens));
+    int64_t ctas = hkv * std::max((2 * tokens + per * (num_segments + 2) - 1) / (2 * per), std::min(num_segments, tokens));
     const int64_t most = num_segments * hkv * r.row_blocks;
-    if (10 * ctas > 7 * most) ctas = most;  // even lengths
+    const bool even = 10 * ctas > 7 * most;  // even lengths, `most` is exact; else `ctas` is rather too many
+    if (even) ctas = most;
+    ctas = std::max<int64_t>(ctas, 1);
     // More than half of the SMs busy: few segments are cut and sorted on the device, which knows their lengths.
     r.picked = 2 * ctas > SMS && num_segments <= 64 && tokens < 1 << 24;
     // upper bound of the parts where the device picks (see best_part_keys), else the parts
-    split = r.picked ? (2 * SMS + ctas / 2) / (ctas > 0 ? ctas : 1) : SMS / (ctas > 0 ? ctas : 1);
+    split = r.picked ? (2 * SMS + ctas / 2) / ctas : (SMS + (even ? 0 : ctas / 16)) / ctas;
     if (split > 32) split = 32;
     r.part_cost = tokens * group * hkv * d / 8192;  // 8 bytes a value; a key's work lasts as long as 64 KB of them
     if (r.part_cost > 1 << 24) r.part_cost = 1 << 24;
