@@ -125,7 +125,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // roundings of P), 2^n from the bits of n + 127.  x below -126.5 gives 0; NaN stays NaN.
 // Every 3rd pair of columns (2 x 2048 tokens behind 6144 and 14000, bf16, when it was chosen: none 275 us, every 2nd
 // 268, 3rd 259, 4th 261, 6th 261).  Not with an 8-bit cache, whose converters need the issue slots (37 x 64 tokens
-// behind 4096: 119 us with every 3rd, 115 without).
+// behind 4096 shared positions: 98 us without, 110 with every 3rd, 103 with every 6th).
 constexpr int EXP_POLY = 3;
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n" : "+f"(x.x));  // -127: the factor 2^n below is then 0
