@@ -29,8 +29,8 @@
 //   three for the 8-bit cache (PV of block j and S of block j + 1 hold two, the converters fill the
 //   third), which leaves room for a ring of four raw tiles.
 //
-// Measured (B200, device time): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 246 us,
-// 1.07 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050: the softmax's exponentials and the
+// Measured (B200, device time): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 250 us,
+// 1.06 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050: the softmax's exponentials and the
 // operands' shared-memory traffic take as long each.  8 ragged chunks (2544 tokens behind 600 to 8000), e4m3, page
 // 16: 115 us; 3700 cycles a block, 20000 before the first, and uneven CTAs.  48 questions of 9 to 70 tokens behind
 // 1490 shared positions, 8 / 2 heads of 256, bf16: 45 us; a block of 64 keys brings 64 KB from L2, 32 bytes a clock
