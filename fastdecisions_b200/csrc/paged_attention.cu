@@ -122,8 +122,12 @@ struct Tiles {
   int past[PICK], n[PICK], tiles[PICK];
   int tokens, least, most;  // tokens a tile, keys of the shortest and of the longest tile
   uint32_t inv;
-  // x / tokens as a multiplication, exact for x < 2^32 / tokens: here x < 2^24 (the host's rule)
-  __device__ __forceinline__ int div_up(int x) const { return (int)__umulhi((uint32_t)(x + tokens - 1), inv); }
+  // ceil(x / tokens) for x < 2^24 (the host's rule).  floor(y / tokens) as a multiplication is exact for any y where
+  // tokens is a power of two, else for y < 2^32 / tokens, and then tokens <= 84; the reciprocal of one token does not
+  // fit 32 bits.
+  __device__ __forceinline__ int div_up(int x) const {
+    return tokens == 1 ? x : (int)__umulhi((uint32_t)(x + tokens - 1), inv);
+  }
   __device__ __forceinline__ void load(const Params& p, int tokens_a_tile, int lane) {
     tokens = tokens_a_tile;
     inv = 0xffffffffu / (uint32_t)tokens + 1u;
