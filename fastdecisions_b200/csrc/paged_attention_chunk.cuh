@@ -215,7 +215,8 @@ __device__ __forceinline__ bool pick_unit(const Params& p, const Tiles& t, int p
   const int src = __ffs(who) - 1;
   u.s = __shfl_sync(0xffffffffu, found, src);
   u.rb = __shfl_sync(0xffffffffu, rb, src);
-  if (u.split < 0) u.split = lo > part_keys ? (lo - 1) / part_keys : 0;  // lo: the tile's keys
+  // lo: the tile's keys.  Without parts part_keys is the host's, from its hint, and bounds nothing.
+  if (u.split < 0) u.split = p.nsplit > 1 ? min((lo - 1) / part_keys, p.nsplit - 1) : 0;
   return true;
 }
 

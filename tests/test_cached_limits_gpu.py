@@ -52,3 +52,47 @@ def test_attention_more_heads_than_a_tile(group, D, quant):
     c = Cache(kv, 1, D, 16, quant, group)
     q = queries(q_lens, group, D, 2)
     attn_check(attend(c, q, q_lens), oracle(c, q, q_lens), quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("D,n", [(128, 600), (256, 300)])
+def test_attention_hint_shorter_than_the_contexts(D, n, quant):
+    # 32 heads a KV head, more tiles than SMs: sorted on the device, and too much work for parts to pay
+    for q_lens, kv in (([n], [1500]), ([n, 40, 7], [1400, 1500, 900])):
+        c = Cache(kv, 2, D, 64, quant, D)
+        q = queries(q_lens, 64, D, 3)
+        ref = oracle(c, q, q_lens)
+        for hint in (1, 750):
+            attn_check(attend(c, q, q_lens, max_kv_len=hint), ref, quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
+def test_attention_hint_shorter_than_the_contexts_in_parts(hq, hkv, D, quant):
+    # parts cut by the host, parts cut by the device, and neither
+    for q_lens, kv in (([70, 30], [2500, 60]), ([500, 40, 0, 350, 64, 290, 1, 333], [530, 4500, 9, 3000, 64, 100, 2500, 333])):
+        c = Cache(kv, hkv, D, 64, quant, D + 1)
+        q = queries(q_lens, hq, D, 4)
+        ref = oracle(c, q, q_lens)
+        for hint in (1, max(kv) // 2, 100000):
+            attn_check(attend(c, q, q_lens, max_kv_len=hint), ref, quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_replay_with_contexts_beyond_the_captured_hint(quant):
+    q_lens = [600]
+    c = Cache([1500], 2, 128, 64, quant, 5)
+    dev, kw = c.dev()
+    q = queries(q_lens, 64, 128, 5)
+    qd, cu, lens = q.cuda(), cu_of(q_lens).cuda(), torch.tensor([640], dtype=torch.int32, device="cuda")
+    ops.paged_gqa_attention(qd, *dev, cu, lens, 600, 640, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_gqa_attention(qd, *dev, cu, lens, 600, 640, **kw)
+    for kv in (640, 1500, 1000):
+        lens.fill_(kv)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _lib.poll_device_error() == 0
+        attn_check(out, O.paged_attention(q, *c.cache, c.table, cu_of(q_lens), [kv], *c.scale), quant)
