@@ -138,10 +138,11 @@ struct Tiles {
       n[i] = past[i] = tiles[i] = 0;
       if (s < p.nseg) {
         const Seg g = segment(p, s, false);
-        n[i] = g.n;
+        // a segment past the call's bound has the bound's tiles: more would take other segments' places in the grid
+        n[i] = (int)min((int64_t)g.n, (int64_t)p.row_blocks * tokens);
         past[i] = (int)g.past;
-        tiles[i] = div_up(g.n);
-        if (g.n > 0) {
+        tiles[i] = div_up(n[i]);
+        if (n[i] > 0) {
           m = max(m, past[i] + n[i]);
           l = min(l, max(past[i] + min(n[i], tokens), 0));
         }
@@ -737,6 +738,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   if (len < 0 || len > ((int64_t)p.max_pages << p.page_shift)) len = 0;
   // the last token of the row's block decides whether there are parts
   const int n = end - p.cu[s], row = (int)(tok - p.cu[s]) * p.group + head % p.group;
+  if (row / p.block_rows >= p.row_blocks) return wait();  // past the call's bound: not computed
   const int last = min((row / p.block_rows + 1) * p.block_rows, n * p.group) - 1;
   uint4 gate = {};
   if (p.gate) gate = *reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c);

@@ -96,3 +96,19 @@ def test_attention_replay_with_contexts_beyond_the_captured_hint(quant):
         torch.cuda.synchronize()
         assert _lib.poll_device_error() == 0
         attn_check(out, O.paged_attention(q, *c.cache, c.table, cu_of(q_lens), [kv], *c.scale), quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D,most,per", [(16, 4, 128, 200, 64), (8, 2, 256, 100, 32)])
+def test_attention_segment_longer_than_the_bound(hq, hkv, D, most, per, quant):
+    # in a call that the device sorts, the rows of the other segments and its own up to the bound are right, the
+    # error bit is set and rows behind the bound's last tile are left as they were
+    q_lens = [700] + [most] * 11 + [most // 2] * (0 if D == 128 else 13)
+    for kv in ([1600] + [most + 3 * i for i in range(len(q_lens) - 1)], [700 + 3900] + [most + 70 * i for i in range(len(q_lens) - 1)]):
+        c = Cache(kv, hkv, D, 64, quant, 12)
+        q = queries(q_lens, hq, D, 9)
+        o = attend(c, q, q_lens, max_seqlen=most, code=32)
+        ref = oracle(c, q, q_lens)
+        attn_check(o[700:], ref, quant, rows=slice(700, None))
+        attn_check(o[:most], ref, quant, rows=slice(0, most))
+        assert o[-(-most // per) * per:700].isnan().all()
