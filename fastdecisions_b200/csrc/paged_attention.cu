@@ -60,6 +60,7 @@ struct Params {
   const int32_t* kv_lens;
   int64_t tokens, num_pages;
   int nseg, max_pages, page_shift, hq, hkv, group, nsplit, row_blocks;
+  int max_seqlen;  // the caller's bound on a segment's tokens
   int split_keys;  // keys a split (a multiple of every tile's), the last one takes what is left
   int block_rows;  // rows of a row block (a CTA's)
   int clustered;   // few rows: the splits of a row block are one cluster
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   const Seg seg = segment(p, s, first);
   const int rows = seg.n * p.group;
   const int row0 = rb * BM;
-  if (first && rows > p.row_blocks * BM) atomicOr(&g_error, 1);
+  if (first && seg.n > p.max_seqlen) atomicOr(&g_error, 1);
   if (row0 >= rows) return;
   const int last_tok = (min(row0 + BM, rows) - 1) / p.group;
   const int64_t kend64 = seg.past + last_tok + 1;
@@ -866,6 +867,7 @@ constexpr int few_ctas(int64_t ctas, int rows, int64_t d, bool quant) {
 static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
                       int64_t group, int64_t d, bool quant) {
   Plan r = {};
+  if (max_seqlen < 1) max_seqlen = 1;  // a bound of no tokens is still checked against the segments
   const int64_t rows = max_seqlen * group;
   int64_t split, least;
   r.many = rows > few_rows_most(d, quant) && group <= 128;
@@ -984,7 +986,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   for (int i = 4; i <= 8; ++i)
     if (page_size == (int64_t)1 << i) shift = i;
   if (!shift) return set_error(FDK_ERR_UNSUPPORTED, "%s: page_size=%lld (16, 32, 64, 128 or 256)", what, (long long)page_size);
-  if (tokens == 0 || max_seqlen == 0) return FDK_OK;
+  if (tokens == 0) return FDK_OK;
   if (!q || !k_cache || !v_cache || !page_table || !cu_seqlens || !kv_lens || !out)
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   const bool quant = cache_is_e4m3 != 0;
@@ -1017,6 +1019,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   p.tokens = tokens; p.num_pages = num_pages; p.nseg = (int)num_segments; p.max_pages = (int)max_pages;
   p.page_shift = shift; p.hq = (int)hq; p.hkv = (int)hkv; p.group = (int)(hq / hkv);
   p.nsplit = pl.nsplit; p.row_blocks = (int)pl.row_blocks; p.split_keys = pl.split_keys;
+  p.max_seqlen = (int)max_seqlen;
   p.picked = pl.picked; p.clustered = pl.clustered; p.units = (int)pl.units;
   p.part_cost = (int)pl.part_cost;
   p.block_rows = pl.many ? (head_dim == 128 ? 2 : 1) * (128 / p.group) * p.group : pl.rows;

@@ -278,7 +278,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   }
   if (item == 0 && hk == 0 && blockIdx.y == 0) {  // one CTA reports what is wrong with the segments
     for (int i = tid; i < p.nseg; i += R::THREADS)
-      if (segment(p, i, true).n > p.row_blocks * NT * tpt) atomicOr(&g_error, 1);
+      if (segment(p, i, true).n > p.max_seqlen) atomicOr(&g_error, 1);
   }
   if (s < 0) return;
   const Seg seg = segment(p, s, false);

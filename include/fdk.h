@@ -282,8 +282,8 @@ size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, in
  * to positions 0 .. kv_lens[s] - n + i (its own keys are in the cache already); a token that sees
  * nothing gets zeros.  q, gate, out and the head mapping as fdk_gqa_fwd (any hq / hkv); scale is
  * positive and finite.
- * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows past the bound are
- * not computed).  max_kv_len is a hint for how far the keys are split: any lengths up to
+ * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows up to the bound are
+ * computed, those past it right or left as they were).  max_kv_len is a hint for how far the keys are split: any lengths up to
  * max_pages * page_size are right with any hint.  Softmax statistics and accumulation are float32; P
  * is rounded to bf16 (bf16 cache) or fp16 (e4m3 cache) before P.V; calls of many query
  * rows take e4m3 rows as fp16 relative to the largest scale among the keys a CTA reads: exact for scales

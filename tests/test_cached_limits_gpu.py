@@ -112,3 +112,21 @@ def test_attention_segment_longer_than_the_bound(hq, hkv, D, most, per, quant):
         attn_check(o[700:], ref, quant, rows=slice(700, None))
         attn_check(o[:most], ref, quant, rows=slice(0, most))
         assert o[-(-most // per) * per:700].isnan().all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_bound_is_exact(quant):
+    # a segment of one token more sets the error bit in either kernel, one at the bound does not
+    for q_lens, kv in (([2, 1, 2], [60, 5000, 2]), ([9, 70, 1], [80, 70, 4000])):
+        c = Cache(kv, 4, 128, 16, quant, 13)
+        q = queries(q_lens, 16, 128, 10)
+        attn_check(attend(c, q, q_lens), oracle(c, q, q_lens), quant)
+        attend(c, q, q_lens, max_seqlen=max(q_lens) - 1, code=32)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_attention_bound_of_zero(quant):
+    c = Cache([60, 20], 4, 128, 16, quant, 14)
+    q = queries([2, 1], 16, 128, 11)
+    attend(c, q, [2, 1], max_seqlen=0, code=32)
+    assert attend(c, q, [0, 0], max_seqlen=0).isnan().all()  # padding only
