@@ -72,9 +72,9 @@ struct Params {
   int64_t ld_gate;
   int gate_hstride;
   bf16* out;
-  float* part_o;   // [nsplit][tokens * hq][D], unnormalised
+  float* part_o;   // [nsplit][tokens * hq][D], each divided by its sum: no larger than the largest V row
   int* part_keys;  // many rows, picked: the part size
-  float2* part_ml; // [nsplit][tokens * hq]: (running max in the exp2 domain, sum)
+  float2* part_ml; // [nsplit][tokens * hq]: (running max in the exp2 domain, sum); the sum weighs the row in the join
 };
 
 // One segment's metadata, checked.  n: new tokens, past: cached positions before them (may be negative:
@@ -187,6 +187,17 @@ __device__ __forceinline__ int best_part_keys(const Params& p, const Tiles& t, i
   const unsigned best = __reduce_min_sync(0xffffffffu, mine);
   return __shfl_sync(0xffffffffu, keys, __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1);
 }
+
+// 1 / a softmax sum; 0 for a row that saw no key, NaN for one that met a NaN.  FAST: to two units in the last place
+// (few rows: the exact quotient costs one token behind 1535 positions 0.1 us; in the join it costs nothing, and
+// without it the compiler no longer keeps four parts' loads in flight: 64 segments of 500 to 8192, e4m3, 49.5 us, 50.7)
+template <bool FAST = false>
+__device__ __forceinline__ float reciprocal_sum(float l) {
+  return l > 0.f ? (FAST ? __fdividef(1.f, l) : 1.f / l) : (l == 0.f ? 0.f : l);
+}
+// What a part's row, of maximum m and sum l, counts beside a common maximum.  A sum of 0 is a part without a visible
+// key; a row of NaN scores has a NaN for its sum and no maximum.
+__device__ __forceinline__ float part_weight(float m, float l, float common) { return l == 0.f ? 0.f : l * ex2(m - common); }
 
 // Page ids of the 16-key groups from `key0` on (page sizes are multiples of 16).  The index is clamped to
 // the range's last key, so the loads need no branch and are all in flight at once; they are issued a
@@ -616,10 +627,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int row = (wm * NR + nr) * 8 + 2 * t4 + u;
-      float mj = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) mj = fmaxf(mj, sml[w * BM + row].x);
-      const float f = m[nr][u] == -INFINITY ? 0.f : ex2(m[nr][u] - mj) * unit;
+      const float f = reciprocal_sum<true>(l[nr][u]) * unit;
       float* dst = so + (wk * BM + row) * LDO;
 #pragma unroll
       for (int i = 0; i < KK; ++i) {
@@ -630,12 +638,9 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   __syncthreads();
   // 8 columns a thread: sum of the key groups, then the result or this split's part
   const bool part = in_parts(p, p.split_keys, kend);
-  auto finish = [&](float (&y)[8], float ll, int gr, int c) {
+  auto finish = [&](float (&y)[8], int gr, int c) {
     const int64_t tok = seg.begin + gr / p.group;
     const int head = hk * p.group + gr % p.group;
-    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= inv;
     if (p.gate) {
       float gv[8];
       unpack8(*reinterpret_cast<const uint4*>(p.gate + tok * p.ld_gate + (int64_t)head * p.gate_hstride + c), gv);
@@ -648,26 +653,28 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
     const int row = e / (D / 8), c = (e % (D / 8)) * 8;
     const int gr = row0 + row;
     if (gr >= rows) break;
-    float mm = -INFINITY, ll = 0.f;
+    float mm = -INFINITY, ll = 0.f, f[WK];
 #pragma unroll
     for (int w = 0; w < WK; ++w) mm = fmaxf(mm, sml[w * BM + row].x);
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
       const float2 x = sml[w * BM + row];
-      if (x.x != -INFINITY) ll += x.y * ex2(x.x - mm);
+      ll += f[w] = part_weight(x.x, x.y, mm);
     }
+    const float inv = reciprocal_sum<true>(ll);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
+      f[w] *= inv;
       const float4 a = *reinterpret_cast<const float4*>(so + (w * BM + row) * LDO + c);
       const float4 b = *reinterpret_cast<const float4*>(so + (w * BM + row) * LDO + c + 4);
-      y[0] += a.x; y[1] += a.y; y[2] += a.z; y[3] += a.w;
-      y[4] += b.x; y[5] += b.y; y[6] += b.z; y[7] += b.w;
+      y[0] = fmaf(f[w], a.x, y[0]); y[1] = fmaf(f[w], a.y, y[1]); y[2] = fmaf(f[w], a.z, y[2]); y[3] = fmaf(f[w], a.w, y[3]);
+      y[4] = fmaf(f[w], b.x, y[4]); y[5] = fmaf(f[w], b.y, y[5]); y[6] = fmaf(f[w], b.z, y[6]); y[7] = fmaf(f[w], b.w, y[7]);
     }
     if (!part) {
-      finish(y, ll, gr, c);
+      finish(y, gr, c);
     } else if (p.clustered) {  // in the place of the first key group, read by the cluster
       float* dst = so + row * LDO + c;
       *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
@@ -701,16 +708,18 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
       y[i] = 0.f;
     }
 #pragma unroll
+    for (int i = 0; i < 8; ++i) ll += ml[i].y = part_weight(ml[i].x, ml[i].y, mm);
+    const float inv = reciprocal_sum<true>(ll);
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < parts && ml[i].x != -INFINITY) {
-        const float f = ex2(ml[i].x - mm);
+      if (i < parts) {
+        const float f = ml[i].y * inv;
         const float4 a = cluster_load4(o_at, i), b = cluster_load4(o_at + 16, i);
-        ll = fmaf(f, ml[i].y, ll);
         y[0] = fmaf(f, a.x, y[0]); y[1] = fmaf(f, a.y, y[1]); y[2] = fmaf(f, a.z, y[2]); y[3] = fmaf(f, a.w, y[3]);
         y[4] = fmaf(f, b.x, y[4]); y[5] = fmaf(f, b.y, y[5]); y[6] = fmaf(f, b.z, y[6]); y[7] = fmaf(f, b.w, y[7]);
       }
     }
-    finish(y, ll, gr, c);
+    finish(y, gr, c);
   }
   __syncthreads();
   cluster_sync();  // no CTA leaves while another reads its shared memory
@@ -767,25 +776,23 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
     float m = mm;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i].x);
-    if (m == -INFINITY) continue;  // nothing visible so far: sums stay zero
-    const float keep = ex2(mm - m);
-    mm = m;
-    ll *= keep;
+    // y is the mean over the parts so far, of weight ll beside the maximum mm
+    const float keep = part_weight(mm, ll, m);
+    ll = keep;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] *= keep;
+    for (int i = 0; i < 4; ++i) ll += ml[i].y = part_weight(ml[i].x, ml[i].y, m);
+    mm = m;
+    const float inv = reciprocal_sum(ll);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] *= keep * inv;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (ml[i].x == -INFINITY) continue;
-      const float f = ex2(ml[i].x - mm);
+      const float f = ml[i].y * inv;
       const float4 a = o[i][0], b = o[i][1];
-      ll = fmaf(f, ml[i].y, ll);
       y[0] = fmaf(f, a.x, y[0]); y[1] = fmaf(f, a.y, y[1]); y[2] = fmaf(f, a.z, y[2]); y[3] = fmaf(f, a.w, y[3]);
       y[4] = fmaf(f, b.x, y[4]); y[5] = fmaf(f, b.y, y[5]); y[6] = fmaf(f, b.z, y[6]); y[7] = fmaf(f, b.w, y[7]);
     }
   }
-  const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= inv;
   if (p.gate) {
     float gv[8];
     unpack8(gate, gv);

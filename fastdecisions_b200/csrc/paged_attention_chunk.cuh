@@ -875,7 +875,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       tc_fence_after();
       // l and O both carry 2^P_SHIFT with the 8-bit cache; O is in units of V's largest scale
       const float unit = QUANT ? scale_value(scale_max[1]) : 1.f;
-      const float inv = part ? unit : (l_run > 0.f ? unit / l_run : (l_run == 0.f ? 0.f : l_run));
+      const float inv = reciprocal_sum(l_run) * unit;
       if (part && valid) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(r_run * sl2, l_run);
       constexpr uint32_t GATE = 64u * D;  // 32 rows of the gate
       static_assert(G::NT * 4 * (8192 + GATE) <= M::OFF_RAW, "shared memory of the epilogue");

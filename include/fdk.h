@@ -280,7 +280,7 @@ size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, in
 /*
  * Causal GQA attention of the newest tokens over the paged cache: token i of segment s's n attends
  * to positions 0 .. kv_lens[s] - n + i (its own keys are in the cache already); a token that sees
- * nothing gets zeros.  q, gate, out and the head mapping as fdk_gqa_fwd (any hq / hkv); scale is
+ * nothing gets zeros, one whose scores include a NaN gets NaN.  q, gate, out and the head mapping as fdk_gqa_fwd (any hq / hkv); scale is
  * positive and finite.
  * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows up to the bound are
  * computed, those past it right or left as they were).  max_kv_len is a hint for how far the keys are split: any lengths up to

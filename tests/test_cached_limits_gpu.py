@@ -130,3 +130,41 @@ def test_attention_bound_of_zero(quant):
     q = queries([2, 1], 16, 128, 11)
     attend(c, q, [2, 1], max_seqlen=0, code=32)
     assert attend(c, q, [0, 0], max_seqlen=0).isnan().all()  # padding only
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:2])
+@pytest.mark.parametrize("q_lens,kv", [([1, 2, 1], [90, 5, 700]), ([1], [1500]), ([1], [9000]), ([70, 9], [80, 9]), ([70], [6000])])
+def test_attention_nan_queries_and_keys_show(q_lens, kv, hq, hkv, D, quant):
+    # a query of NaN, and a query that meets a NaN key, give NaN in each kernel and in each join of parts; the others
+    # are what they are without
+    c = Cache(kv, hkv, D, 64, quant, 19)
+    q = queries(q_lens, hq, D, 17)
+    ref = oracle(c, q, q_lens)
+    T = sum(q_lens)
+    q[T - 1, hq - 1] = float("nan")
+    q[0, 0, 5] = float("nan")
+    o = attend(c, q, q_lens)
+    assert o[T - 1, hq - 1].isnan().all() and o[0, 0].isnan().all()
+    rest = torch.ones(T, hq, dtype=torch.bool)
+    rest[T - 1, hq - 1] = rest[0, 0] = False
+    attn_check(o.cpu()[rest], tuple(t[rest] for t in ref), quant)
+    q = queries(q_lens, hq, D, 17)
+    last = kv[-1] - 1                                     # seen by the last token only
+    c.cache[0][int(c.table[-1, last // 64]), 0, last % 64] = float("nan")
+    o = attend(c, q, q_lens)
+    assert o[T - 1, :hq // hkv].isnan().all()
+    rest = torch.ones(T, hq, dtype=torch.bool)
+    rest[T - 1, :hq // hkv] = False
+    attn_check(o.cpu()[rest], tuple(t[rest] for t in ref), quant)
+
+
+@pytest.mark.parametrize("q_lens,kv", [([2, 1], [90, 7]), ([1], [1500]), ([1], [9000]), ([60, 50], [90, 70]), ([60, 50], [1900, 70])])
+def test_attention_rows_near_the_largest_number(q_lens, kv):
+    # V rows of 2^113 times e4m3: sums of weights times V leave float32, their quotients do not
+    c = Cache(kv, 4, 128, 16, True, 16)
+    for s, length in enumerate(kv):
+        pos = torch.arange(length)
+        c.scale[1][c.table[s].long()[pos // 16], :, pos % 16] = 240
+    q = queries(q_lens, 16, 128, 16)
+    attn_check(attend(c, q, q_lens), oracle(c, q, q_lens), True)
