@@ -20,10 +20,11 @@
 //   kv_lens[s] may hold anything (0 * NaN would reach the sums): the block that has them is zeroed there
 //   after its load and before the MMA warp sees it.
 //   8-bit cache: TMA brings the raw e4m3 rows; six converter warps turn them into fp16 operands (e4m3 ->
-//   fp16 is exact) multiplied by the row's scale relative to the largest one of the CTA's key range
-//   (exact for scales within 2^15 of it; smaller ones lose bits below 2^-33 of the range's largest
-//   element).  The largest K scale then folds into the softmax scale, V's into the final normalisation,
-//   so the softmax costs what it does for bf16.  q goes to fp16 with a power of two a row.
+//   fp16 is exact) multiplied by the row's scale relative to the largest one of the CTA's key range and by
+//   2^7, which takes e4m3's 448 to 57344, just inside fp16.  So scales within 2^22 of the largest are exact, down to
+//   2^-31 of it elements are rounded to multiples of 2^-31 of it, and below the factor itself is 0.  The largest K
+//   scale then folds into the softmax scale, V's into the final normalisation, so the softmax costs what it
+//   does for bf16.  q goes to fp16 with a power of two a row.
 //
 //   K and V blocks share one ring of operand slots, in the order K_0 V_0 K_1 V_1 ..: four slots for bf16,
 //   three for the 8-bit cache (PV of block j and S of block j + 1 hold two, the converters fill the
@@ -80,6 +81,8 @@ struct Smem {
 };
 constexpr uint32_t TM_COLS = 512;
 constexpr float P_SHIFT = 6.f;  // fp16 P is scaled by 2^6: weights down to 2^-30 of the row's largest stay
+constexpr int ROW_SHIFT = 7;    // fp16 K and V of the 8-bit cache are scaled by 2^7
+constexpr float ROW_UNIT = 1.f / (1 << ROW_SHIFT);
 constexpr long long DRAIN_BUDGET = 2000000000LL;
 
 // warps: NT * 4 softmax, one producer, one MMA issuer and TMEM allocator; with the 8-bit cache six
@@ -583,7 +586,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       bool ok = true;
       for (int j = 0; j < n_kv; ++j) {
         const int key0 = kb + j * BN;
-        const uint32_t fk = half2_bits(scale_value(max(kbyte - ek + 127, 0))), fv = half2_bits(scale_value(max(vbyte - ev + 127, 0)));
+        const uint32_t fk = half2_bits(scale_value(max(kbyte - ek + 127 + ROW_SHIFT, 0)));
+        const uint32_t fv = half2_bits(scale_value(max(vbyte - ev + 127 + ROW_SHIFT, 0)));
         // rows behind the range may hold anything, NaN included: their operands are zeros, not 0 * NaN
         const int live = ke - key0;
         kbyte = scale_at(p.k_scale, p.kscale_page, key0 + BN + my, id);
@@ -724,7 +728,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         // S of the first block follows the scale maxima
         ok = __all_sync(0xffffffffu, mbar_wait(bar(B_S), 0, abort_flag) ? 1 : 0);
         // never 0: a masked score is -inf * sl2
-        if (ok) sl2 = fmaxf(sl2 * unit * scale_value(scale_max[0]), 1e-37f);
+        if (ok) sl2 = fmaxf(sl2 * ROW_UNIT * unit * scale_value(scale_max[0]), 1e-37f);
       }
     } else if (QUANT && ok) {
       // this tile's q: D / 8 threads a row, fp16 with the row's largest magnitude in [1, 2)
@@ -763,7 +767,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       // S of the first block follows every thread's q and the scale maxima
       ok = __all_sync(0xffffffffu, mbar_wait(bar(B_S + (NT == 2 ? tile : 0)), 0, abort_flag) ? 1 : 0);
       // never 0: a masked score is -inf * sl2
-      if (ok) sl2 = fmaxf(sl2 * scale_value(q_exp[tile * 128 + row]) * scale_value(scale_max[0]), 1e-37f);
+      if (ok) sl2 = fmaxf(sl2 * ROW_UNIT * scale_value(q_exp[tile * 128 + row]) * scale_value(scale_max[0]), 1e-37f);
     }
     const int n_blocks = ok ? n_kv : 0;
     for (int j = 0; j < n_blocks; ++j) {
@@ -873,9 +877,10 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     const int r8 = lane >> 3, c8 = lane & 7;  // a pass: rows 4 i + r8, columns 8 c8 .. + 7
     if (ok && __all_sync(0xffffffffu, mbar_wait(bar(B_O), 0, abort_flag) ? 1 : 0)) {
       tc_fence_after();
-      // l and O both carry 2^P_SHIFT with the 8-bit cache; O is in units of V's largest scale
+      // l and O both carry 2^P_SHIFT with the 8-bit cache; O is in units of V's largest scale over 2^ROW_SHIFT, which
+      // is multiplied in last: the smallest scale's unit divided by l would be subnormal
       const float unit = QUANT ? scale_value(scale_max[1]) : 1.f;
-      const float inv = reciprocal_sum(l_run) * unit;
+      const float inv = (QUANT ? ROW_UNIT : 1.f) * reciprocal_sum(l_run);
       if (part && valid) p.part_ml[(int64_t)split * p.tokens * p.hq + idx] = make_float2(r_run * sl2, l_run);
       constexpr uint32_t GATE = 64u * D;  // 32 rows of the gate
       static_assert(G::NT * 4 * (8192 + GATE) <= M::OFF_RAW, "shared memory of the epilogue");
@@ -900,9 +905,9 @@ many_rows_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const uint32_t at = stage + (uint32_t)lane * 256u + (uint32_t)(((8 * h + q) ^ (lane & 7)) * 16);
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "f"(__uint_as_float(o[4 * q]) * inv),
-                         "f"(__uint_as_float(o[4 * q + 1]) * inv), "f"(__uint_as_float(o[4 * q + 2]) * inv),
-                         "f"(__uint_as_float(o[4 * q + 3]) * inv)
+            auto value = [&](int i) { return QUANT ? __uint_as_float(o[i]) * inv * unit : __uint_as_float(o[i]) * inv; };
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "f"(value(4 * q)), "f"(value(4 * q + 1)),
+                         "f"(value(4 * q + 2)), "f"(value(4 * q + 3))
                          : "memory");
           }
         }

@@ -168,3 +168,73 @@ def test_attention_rows_near_the_largest_number(q_lens, kv):
         c.scale[1][c.table[s].long()[pos // 16], :, pos % 16] = 240
     q = queries(q_lens, 16, 128, 16)
     attn_check(attend(c, q, q_lens), oracle(c, q, q_lens), True)
+
+
+def scales_check(o, c, q, q_lens):
+    """attn_check's bound and, for an 8-bit cache, one term more.
+
+    More than 32 rows a KV head: V rows are fp16 in units of 2^-7 of the largest scale that the CTA reads.  Where the
+    segment's scales lie within 2^31 of each other, an element is off by at most half of fp16's smallest step, 2^-25
+    of that unit; else rows of smaller scales may read as zero, elements of at most 448 times 2^-32.  A mean of them is
+    off by no more.  Weights are fp16 with the row's largest at 2^6 or above: off by at most half the smallest step,
+    2^-31 of the largest weight, each times its |v|.
+
+    Up to 32 rows: P is fp16 times a power of two a row, so that the row's largest contribution p 2^(scale) is at
+    least 2^6: a weight is off by at most 2^-31 of that contribution, times the e4m3 value it meets."""
+    want, mag, size = oracle(c, q, q_lens)
+    if c.quant:
+        T, hq, D = q.shape
+        rep, cu = hq // c.hkv, cu_of(q_lens)
+        tail = torch.zeros(T, hq, D, dtype=torch.float64)
+        for s, n in enumerate(q_lens):
+            length = int(c.kv_lens[s])
+            k = O.cache_rows(c.cache[0], c.scale[0], c.table[s], length)
+            v8 = O.cache_rows(c.cache[1], torch.full_like(c.scale[1], 127), c.table[s], length).abs()
+            pos = torch.arange(length)
+            scale = torch.exp2(c.scale[1][c.table[s].long()[pos // c.page], :, pos % c.page].double() - 127)
+            for i in range(n):
+                t, seen = int(cu[s]) + i, length - n + i + 1
+                for h in range(hq if seen > 0 else 0):
+                    sc, v = scale[:, h // rep], v8[:seen, h // rep]
+                    p = torch.softmax(k[:seen, h // rep] @ q[t, h].double() * D ** -0.5, 0)
+                    if max(q_lens) * rep > 32:
+                        lost = 2.0 ** -32 * sc.max() * (1 if sc.max() <= 2 ** 31 * sc.min() else 448)
+                        tail[t, h] = lost + 2.0 ** -31 * p.max() * (v * sc[:seen, None]).sum(0)
+                    else:
+                        tail[t, h] = 2.0 ** -31 * (p * sc[:seen]).max() * v.sum(0)
+        mag = mag + tail / 2 ** -11
+    attn_check(o, (want, mag, size), c.quant)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("up", [0, 14, 21, 24, 30, 40])
+def test_attention_many_rows_behind_large_scales(hq, hkv, D, quant, up):
+    # the last token's V row is larger than the others by 2^up; first seen by itself only, then by every row
+    n = 33 * hkv // hq + 1
+    for q_lens, kv, at in (([n, n + 3, n + 1], [n, n + 90, n + 20], -1), ([n, n], [n + 200, n + 9], 3)):
+        c = Cache(kv, hkv, D, 16, quant, D + up)
+        for s, length in enumerate(kv):
+            pos = at % length
+            page = int(c.table[s, pos // 16])
+            if quant:
+                c.scale[1][page, :, pos % 16] += up
+            else:
+                c.cache[1][page, :, pos % 16] *= 2.0 ** up
+        q = queries(q_lens, hq, D, 15)
+        scales_check(attend(c, q, q_lens), c, q, q_lens)
+
+
+def test_attention_many_rows_smallest_and_largest_scales():
+    # scale bytes at both ends of what a write leaves
+    for byte in (0, 1, 2, 30, 240):
+        for kv in ([90, 70], [1900, 70]):
+            c = Cache(kv, 4, 128, 16, True, 16)
+            for s, length in enumerate(kv):
+                pos = torch.arange(length)
+                c.scale[1][c.table[s].long()[pos // 16], :, pos % 16] = byte
+            q = queries([60, 50], 16, 128, 16)
+            o = attend(c, q, [60, 50])
+            want = oracle(c, q, [60, 50])[0]
+            # bf16 of this size may be subnormal: half a step of 2^-133 besides the relative bound
+            assert ((o.double().cpu() - want).abs() <= 2 ** -7 * want.abs().amax(-1, keepdim=True) + 2.0 ** -134).all()
