@@ -20,12 +20,16 @@
 //   need no reduction across lanes), sum and O (fp32) over its keys; key groups are joined through
 //   shared memory at the end.  Up to eight splits are a cluster and join through each other's shared memory,
 //   more through a float32 workspace and a second kernel.
-//   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S, V's multiplies
-//   P before its rounding to fp16, relative to the largest V scale so far (O is rescaled when that grows,
-//   as for the maximum).  q is brought to fp16 with a power of two a row.
+//   8-bit cache: e4m3 -> fp16 is exact, one instruction a pair; K's row scale multiplies S, V's enters P
+//   before its rounding to fp16.  So P V is in units of the row's largest weight times scale so far, a second
+//   running maximum beside the one that the sum is relative to: what a row loses depends on the keys it sees
+//   only (one unit for all rows of a warp, from every key of a tile, lost the weights of early tokens behind a
+//   later token's large V row; the second exponential a weight costs 64 sequences x 8 tokens, e4m3, 127 us for 122,
+//   one token each nothing).  q is brought to fp16 with a power of two a row.
 //
 // Measured: one token behind 1535 positions, 16 / 4 heads of 128, bf16, 10.3 us with the launch; 64 ragged sequences of
 // 500 to 8192, e4m3, 51 us, 3.8 TB/s (issue 40% of the slots, DRAM 49%); 64 x 8192, bf16, 153 us unsplit, 7 TB/s.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -303,7 +307,8 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t a, int rank) {
 }
 
 constexpr float GROW = 8.f;     // the running maximum lags by at most 2^GROW
-constexpr int V_SHIFT = 6;      // fp16 P: times 2^V_SHIFT; at most 2^(GROW + V_SHIFT), weights down to 2^-30 stay
+// fp16 P: times 2^V_SHIFT, at most 2^(GROW + V_SHIFT); contributions down to 2^-30 of the row's largest stay
+constexpr float V_SHIFT = 6.f;
 
 template <int D, bool QUANT, int WM, int NR>
 __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
@@ -457,10 +462,13 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
   for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      m[nr][u] = -INFINITY;
+      m[nr][u] = -FLT_MAX;  // finite: a hidden key's score of -inf is -inf beside it
       l[nr][u] = 0.f;
     }
-  int ev = 0;  // O is in units of 2^(ev - 127) (8-bit cache)
+  // 8-bit cache: O of a row is in units of 2^(un - m - 127), un the running maximum of score + scale byte - V_SHIFT
+  float un[NR][2];
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) un[nr][0] = un[nr][1] = -FLT_MAX;
 
   for (int j = 0; j < ntiles; ++j) {
     cp_wait<G::STAGES - 2>();
@@ -503,11 +511,11 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
           }
         }
       }
-      int vb[2] = {0, 0};
+      float vb[2] = {0.f, 0.f};  // V's scale bytes; any byte where the key is hidden: its score is -inf
       if (QUANT) {
         const float k0 = pow2_byte(scales[krow + g]), k1 = pow2_byte(scales[krow + g + 8]);
-        vb[0] = key0 + g < ke ? scales[BN + krow + g] : 0;
-        vb[1] = key0 + g + 8 < ke ? scales[BN + krow + g + 8] : 0;
+        vb[0] = scales[BN + krow + g];
+        vb[1] = scales[BN + krow + g + 8];
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           sc[nr][0] *= k0 * qs[nr][0];
@@ -528,53 +536,65 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
           for (int c = 0; c < 4; ++c)
             if (key0 + g + 8 * (c >> 1) > min(lim[nr][c & 1], ke - 1)) sc[nr][c] = -INFINITY;
       }
-      // raise the maxima (and the unit of O) only where needed
-      bool up = QUANT && max(vb[0], vb[1]) > ev;
+      // the keys' exponents beside the running maxima: d of their weights, e of what they add to O (with the scale: one
+      // more float32 rounding of the score)
+      float d[NR][4], e[NR][4];
+      bool up = false;
+      auto exponents = [&] {
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
+        for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) up |= fmaxf(sc[nr][u], sc[nr][2 + u]) > m[nr][u] + GROW;
-      if (__any_sync(0xffffffffu, up)) {
-        float fv = 1.f;
-        if (QUANT) {
-          const int e = __reduce_max_sync(0xffffffffu, max(vb[0], vb[1]));
-          if (e > ev) {
-            fv = ev == 0 ? 0.f : pow2_byte(ev - e + 127);
-            ev = e;
+          for (int c = 0; c < 4; ++c) {
+            d[nr][c] = sc[nr][c] - m[nr][c & 1];
+            if (QUANT) e[nr][c] = (sc[nr][c] + vb[c >> 1]) - un[nr][c & 1];
           }
+          up |= fmaxf(fmaxf(d[nr][0], d[nr][1]), fmaxf(d[nr][2], d[nr][3])) > GROW;
+          if (QUANT) up |= fmaxf(fmaxf(e[nr][0], e[nr][1]), fmaxf(e[nr][2], e[nr][3])) > GROW + V_SHIFT;
         }
+      };
+      exponents();
+      // raise the maxima (and the units of O) only where needed
+      if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            float mx = fmaxf(sc[nr][u], sc[nr][2 + u]);
+            float mx = fmaxf(sc[nr][u], sc[nr][2 + u]), cx = fmaxf(sc[nr][u] + vb[0], sc[nr][2 + u] + vb[1]) - V_SHIFT;
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            for (int off = 4; off < 32; off <<= 1) {
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              if (QUANT) cx = fmaxf(cx, __shfl_xor_sync(0xffffffffu, cx, off));
+            }
             float corr = 1.f;
             if (mx > m[nr][u]) {
               corr = ex2(m[nr][u] - mx);  // 0 when nothing was visible before
               m[nr][u] = mx;
             }
             l[nr][u] *= corr;
-            corr *= fv;
+            if (QUANT) {
+              corr = 1.f;
+              if (cx > un[nr][u]) {
+                corr = ex2(un[nr][u] - cx);
+                un[nr][u] = cx;
+              }
+            }
 #pragma unroll
             for (int i = 0; i < KK; ++i) {
               o[i][nr][u] *= corr;
               o[i][nr][2 + u] *= corr;
             }
           }
+        exponents();
       }
       // P^T, this lane's part of the row sums (of the unrounded weights), and O^T += V^T P^T
-      const float w0 = QUANT ? pow2_byte(vb[0] - ev + 127 + V_SHIFT) : 1.f, w1 = QUANT ? pow2_byte(vb[1] - ev + 127 + V_SHIFT) : 1.f;
       uint32_t pb[NR][2];
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
-        const float m0 = m[nr][0] == -INFINITY ? 0.f : m[nr][0], m1 = m[nr][1] == -INFINITY ? 0.f : m[nr][1];
-        const float p0 = ex2(sc[nr][0] - m0), p1 = ex2(sc[nr][1] - m1), p2 = ex2(sc[nr][2] - m0), p3 = ex2(sc[nr][3] - m1);
+        const float p0 = ex2(d[nr][0]), p1 = ex2(d[nr][1]), p2 = ex2(d[nr][2]), p3 = ex2(d[nr][3]);
         l[nr][0] += p0 + p2;
         l[nr][1] += p1 + p3;
-        pb[nr][0] = transpose8(QUANT ? pack_f16x2(p0 * w0, p1 * w0) : pack_bf16x2(p0, p1));
-        pb[nr][1] = transpose8(QUANT ? pack_f16x2(p2 * w1, p3 * w1) : pack_bf16x2(p2, p3));
+        pb[nr][0] = transpose8(QUANT ? pack_f16x2(ex2(e[nr][0]), ex2(e[nr][1])) : pack_bf16x2(p0, p1));
+        pb[nr][1] = transpose8(QUANT ? pack_f16x2(ex2(e[nr][2]), ex2(e[nr][3])) : pack_bf16x2(p2, p3));
       }
       if (!QUANT) {
 #pragma unroll
@@ -621,18 +641,19 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(const Params p) {
       if (g == 0) sml[wk * BM + (wm * NR + nr) * 8 + 2 * t4 + u] = make_float2(m[nr][u], l[nr][u]);
     }
   __syncthreads();
-  const float unit = QUANT ? scale_value(ev) * (1.f / (1 << V_SHIFT)) : 1.f;
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int row = (wm * NR + nr) * 8 + 2 * t4 + u;
-      const float f = reciprocal_sum<true>(l[nr][u]) * unit;
+      // 8-bit cache: the unit's root twice, as the unit itself may leave float32's range where the result does not
+      const float root = !QUANT ? 1.f : l[nr][u] == 0.f ? 0.f : ex2(0.5f * (un[nr][u] - m[nr][u] - 127.f));
+      const float f = reciprocal_sum<true>(l[nr][u]) * root;
       float* dst = so + (wk * BM + row) * LDO;
 #pragma unroll
       for (int i = 0; i < KK; ++i) {
-        dst[i * 16 + (QUANT ? 2 * g : g)] = o[i][nr][u] * f;
-        dst[i * 16 + (QUANT ? 2 * g + 1 : g + 8)] = o[i][nr][2 + u] * f;
+        dst[i * 16 + (QUANT ? 2 * g : g)] = o[i][nr][u] * f * root;
+        dst[i * 16 + (QUANT ? 2 * g + 1 : g + 8)] = o[i][nr][2 + u] * f * root;
       }
     }
   __syncthreads();

@@ -238,3 +238,49 @@ def test_attention_many_rows_smallest_and_largest_scales():
             want = oracle(c, q, [60, 50])[0]
             # bf16 of this size may be subnormal: half a step of 2^-133 besides the relative bound
             assert ((o.double().cpu() - want).abs() <= 2 ** -7 * want.abs().amax(-1, keepdim=True) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS)
+@pytest.mark.parametrize("up", [12, 24, 60, 100])
+def test_attention_few_rows_behind_hidden_scales(hq, hkv, D, quant, up):
+    # the last token's V row, which the others may not see, is larger than theirs by 2^up: their results are
+    # what they are without it
+    for q_lens, past in (([2, 4, 3, 1], 0), ([2, 8, 1, 5], 70)):
+        kv = [n + past for n in q_lens]
+        c = Cache(kv, hkv, D, 16, quant, D + up)
+        for s, n in enumerate(kv):
+            page, off = int(c.table[s, (n - 1) // 16]), (n - 1) % 16
+            if quant:
+                c.scale[1][page, :, off] += up
+            else:
+                c.cache[1][page, :, off] *= 2.0 ** up
+        q = queries(q_lens, hq, D, 6)
+        scales_check(attend(c, q, q_lens), c, q, q_lens)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("hq,hkv,D", HEADS[:3])
+@pytest.mark.parametrize("spread", [6.0, 20.0])
+def test_attention_few_rows_scales_far_apart(hq, hkv, D, quant, spread):
+    # V rows of any size in any order; most of a result may come from keys of small weight and large rows
+    for q_lens, kv in (([1, 3, 4, 1], [400, 333, 5, 64]), ([8, 1], [150, 1700]), ([1], [3000])):
+        c = Cache(kv, hkv, D, 16, quant, 9, spread=spread, v_only=True)
+        q = queries(q_lens, hq, D, 7)
+        scales_check(attend(c, q, q_lens), c, q, q_lens)
+
+
+def test_attention_few_rows_smallest_and_largest_scales():
+    # scale bytes at both ends of what a write leaves
+    for byte in (0, 1, 2, 240):
+        c = Cache([90, 7], 4, 128, 16, True, 11)
+        for s, n in enumerate((90, 7)):
+            pos = torch.arange(n)
+            c.scale[1][c.table[s].long()[pos // 16], :, pos % 16] = byte
+            if byte < 240:
+                c.scale[1][int(c.table[s, (n - 1) // 16]), :, 3] = byte + 1
+        q = queries([2, 1], 16, 128, 8)
+        o = attend(c, q, [2, 1])
+        want = oracle(c, q, [2, 1])[0]
+        # bf16 of this size may be subnormal: half a step of 2^-133 besides the relative bound
+        assert ((o.double().cpu() - want).abs() <= 2 ** -7 * want.abs().amax(-1, keepdim=True) + 2.0 ** -134).all()
