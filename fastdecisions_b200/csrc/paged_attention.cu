@@ -859,6 +859,10 @@ static int launch_rows(const Params& p, int rows, cudaStream_t s) {
   }
 }
 
+// Positions of a sequence.  The kernels step through them in 32 bits and look ahead: the scan of the scale bytes by
+// 7 x 3072 keys, the others by less than 512.
+constexpr int64_t MOST_POSITIONS = 0x7fff0000;
+
 // Tiling of a call: the kernel, its rows a CTA and the split of the keys.  All follow from host-side
 // sizes only, so a captured call replays with any lengths.
 struct Plan {
@@ -1020,9 +1024,9 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
   const bool quant = cache_is_e4m3 != 0;
   if (quant && (!k_scale || !v_scale))
     return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: an e4m3 cache needs k_scale and v_scale", what);
-  if (num_pages < 1 || num_pages > 0x7fffffff || max_pages < 1 || ld_table < max_pages ||
-      max_pages * page_size > 0x7fffff00)
-    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad page counts (at most 2^31 positions a sequence)", what);
+  if (num_pages < 1 || num_pages > 0x7fffffff || max_pages < 1 || max_pages > 0x7fffffff || ld_table < max_pages ||
+      max_pages * page_size > MOST_POSITIONS)
+    return set_error(FDK_ERR_INVALID_ARGUMENT, "%s: bad page counts (at most 2^31 - 2^16 positions a sequence)", what);
   const int64_t page_elems = page_size * hkv * head_dim;
   if (ld_kpage < page_elems || ld_vpage < page_elems ||
       (quant && (ld_kscale_page < page_size * hkv || ld_vscale_page < page_size * hkv)))

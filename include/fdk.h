@@ -284,13 +284,13 @@ size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, in
  * fdk_gqa_fwd (any hq / hkv); scale is positive and finite.
  * max_seqlen bounds the tokens of a segment (a longer one sets bit 32; its rows up to the bound are
  * computed, those past it right or left as they were).  max_kv_len is a hint for how far the keys are
- * split: any lengths up to max_pages * page_size are right with any hint.  Softmax statistics and
- * accumulation are float32; P is rounded to bf16 (bf16 cache) or fp16 (e4m3 cache) before P.V.  e4m3
- * cache: calls of up to 32 query rows a KV head round weight times V's scale, contributions below
- * 2^-20 of the row's largest to multiples of 2^-30 of it; other calls (group sizes
- * hq / hkv above 128 excepted) take e4m3 rows as fp16 relative to the largest scale among the keys a CTA reads, later tokens'
- * than a row's own among them: exact for scales down to 2^-22 of it, rounded to multiples of 2^-31 of
- * it for scales down to 2^-31, zeros below.
+ * split: any lengths up to max_pages * page_size (at most 2^31 - 2^16) are right with any hint.
+ * Softmax statistics and accumulation are float32; P is rounded to bf16 (bf16 cache) or fp16 (e4m3
+ * cache) before P.V.  e4m3 cache: calls of up to 32 query rows a KV head round weight times V's scale,
+ * contributions below 2^-20 of the row's largest to multiples of 2^-30 of it; other calls (group sizes
+ * hq / hkv above 128 excepted) take e4m3 rows as fp16 relative to the largest scale among the keys a
+ * CTA reads, later tokens' than a row's own among them: exact for scales down to 2^-22 of it, rounded
+ * to multiples of 2^-31 of it for scales down to 2^-31, zeros below.
  * A non-finite V row may reach every row of its call that shares a tile with it, masked ones included;
  * K rows and rows past kv_lens[s] never do.  The caller's workspace holds float32 partial results and
  * the size of the parts, which the device takes from the lengths; calls that overlap on the GPU need

@@ -284,3 +284,24 @@ def test_attention_few_rows_smallest_and_largest_scales():
         want = oracle(c, q, [2, 1])[0]
         # bf16 of this size may be subnormal: half a step of 2^-133 besides the relative bound
         assert ((o.double().cpu() - want).abs() <= 2 ** -7 * want.abs().amax(-1, keepdim=True) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("q_lens", [[1], [40]])
+def test_attention_longest_page_table(q_lens):
+    # positions are counted in 32 bits with steps past the last one: tables that reach 2^31 are refused, the longest
+    # allowed one works
+    c = Cache([70], 4, 128, 256, True, 20)
+    (k, v, table), kw = c.dev()
+    q = queries(q_lens, 16, 128, 18)
+    ref = oracle(c, q, q_lens)
+    cu, lens = cu_of(q_lens).cuda(), c.kv_lens.cuda()
+    for pages, ok in ((2 ** 23 - 1, False), (2 ** 23 - 2 ** 8 + 1, False), (2 ** 23 - 2 ** 8, True)):
+        wide = torch.zeros(1, pages, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        if ok:
+            attn_check(ops.paged_gqa_attention(q.cuda(), k, v, wide, cu, lens, q_lens[0], **kw), ref, True)
+        else:
+            with pytest.raises(ValueError, match="positions"):
+                ops.paged_gqa_attention(q.cuda(), k, v, wide, cu, lens, q_lens[0], **kw)
+    torch.cuda.synchronize()
+    assert _lib.poll_device_error() == 0
