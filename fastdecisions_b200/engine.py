@@ -21,6 +21,7 @@ softmax, with the projections and MLP as cuBLAS GEMMs and every other op a kerne
 from __future__ import annotations
 
 import contextlib
+import weakref
 from dataclasses import dataclass
 from types import SimpleNamespace
 from typing import Optional, Sequence
@@ -117,7 +118,9 @@ class Prefix:
 class StateCache:
     """Device state of cached prefixes for one engine: per attention layer a paged KV cache (``bf16`` or
     ``e4m3`` with a scale per token and head), per Gated-DeltaNet layer a pool of convolution histories
-    and recurrent states.  Calls that use one cache must be on one stream (or ordered)."""
+    and recurrent states.  It belongs to the engine that opened it (``open_cache``), one made on its own to
+    the first engine that caches a prefix in it: what it holds comes from that engine's weights.  Calls that
+    use one cache must be on one stream (or ordered)."""
 
     def __init__(self, cfg: ModelConfig, device, tokens: int, prefixes: int, page_size: int = 64,
                  kv_dtype: str = "bf16"):
@@ -126,6 +129,7 @@ class StateCache:
         if page_size not in (16, 32, 64, 128, 256) or tokens < 1 or prefixes < 1:
             raise ValueError("StateCache: page_size 16 to 256 (a power of two), at least one token and prefix")
         self.cfg, self.dev, self.page_size, self.kv_dtype = cfg, torch.device(device), page_size, kv_dtype
+        self.engine = None  # weak reference to the engine it belongs to
         pages = -(-tokens // page_size)
         hkv, D = cfg.num_key_value_heads, cfg.head_dim
         Hk, Hv = cfg.linear_num_key_heads, cfg.linear_num_value_heads
@@ -608,7 +612,9 @@ class DecisionEngine:
         """Device memory for ``prefixes`` cached prefixes and ``tokens`` cached positions in total, the ones
         that ``score_after`` needs for its requests while they run included (``kv_dtype`` ``"e4m3"``
         halves the positions' size)."""
-        return StateCache(self.cfg, self.dev, tokens, prefixes, page_size, kv_dtype)
+        cache = StateCache(self.cfg, self.dev, tokens, prefixes, page_size, kv_dtype)
+        cache.engine = weakref.ref(self)
+        return cache
 
     def _run_cached(self, cache: StateCache, batch: PackedBatch, past: int, tables: Sequence[Sequence[int]],
                     state_in: int, state_out: int) -> torch.Tensor:
@@ -651,8 +657,13 @@ class DecisionEngine:
     def _own(self, prefix: Prefix, what: str):
         if prefix.slot is None:
             raise ValueError(f"{what}: the prefix was released")
-        if prefix.cache.cfg != self.cfg:
+        cache = prefix.cache
+        if cache.cfg != self.cfg:
             raise ValueError(f"{what}: the prefix belongs to a cache of another model")
+        if cache.engine is None:
+            cache.engine = weakref.ref(self)
+        if cache.engine() is not self:
+            raise ValueError(f"{what}: the prefix belongs to a cache of another engine (another model's weights)")
 
     def cache_prefix(self, cache: StateCache, ids) -> Prefix:
         """Runs ``ids`` once and keeps their keys, values and states for ``score_after``."""

@@ -146,3 +146,27 @@ def test_prefix_of_another_model_and_failed_extension():
     with pytest.raises(RuntimeError, match="launch failed"):
         eng.cache_prefix(cache, np.zeros(20, np.int32))
     assert len(cache.free_pages) == 4 and len(cache.free_slots) == 1
+
+
+def test_prefix_of_another_engine():
+    # equal configurations say nothing about the weights (or the device) a cache was filled with
+    cfg = W.ModelConfig(num_hidden_layers=4, vocab_size=64)
+    a, b = (object.__new__(DecisionEngine) for _ in range(2))  # host logic only
+    for eng in (a, b):
+        eng.cfg, eng.dev, eng.max_positions = cfg, torch.device("cpu"), 4096
+        eng._run_cached = lambda *_: None
+    ids = np.zeros(20, np.int32)
+    opened = a.open_cache(64, 2, 16)
+    prefix = a.cache_prefix(opened, ids)
+    own = StateCache(cfg, "cpu", 64, 2, 16)               # belongs to the first engine that uses it
+    second = b.cache_prefix(own, ids)
+    for eng, other, cache in ((b, prefix, opened), (a, second, own)):
+        with pytest.raises(ValueError, match="another engine"):
+            eng.score_after(other, [W.Request(ids=ids, slot=1, nopts=2)])
+        with pytest.raises(ValueError, match="another engine"):
+            eng.extend(other, ids)
+        with pytest.raises(ValueError, match="another engine"):
+            eng.cache_prefix(cache, ids)
+        assert other.length == 20 and len(cache.free_pages) == 2 and len(cache.free_slots) == 1
+    a.extend(prefix, ids[:4])
+    assert prefix.length == 24
