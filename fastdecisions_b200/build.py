@@ -3,7 +3,8 @@
 ``python -m fastdecisions_b200.build`` compiles every ``csrc/*.cu`` to an object file under
 ``fastdecisions_b200/_build/`` (in parallel, skipped when up to date) and links
 ``fastdecisions_b200/libfdk.so``, and the Python binding of the cached-state operators,
-``_fdk_torch.so``, with g++.  No GPU is needed: nvcc cross-compiles for sm_100a.
+``_fdk_torch.so``, with g++ where torch is installed (a host of the C library needs neither).  No GPU
+is needed: nvcc cross-compiles for sm_100a.
 """
 from __future__ import annotations
 
@@ -63,7 +64,12 @@ def build(verbose_ptxas: bool = False, jobs: int | None = None) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
-    build_binding()
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        print(f"torch is not installed: {os.path.basename(BINDING)} is not built, the C library is complete")
+    else:
+        build_binding()
     return LIB
 
 

@@ -1,5 +1,8 @@
 """Cached-state operators without a GPU: refusals, host-side sizes, installers and the oracle itself."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -170,3 +173,14 @@ def test_prefix_of_another_engine():
         assert other.length == 20 and len(cache.free_pages) == 2 and len(cache.free_slots) == 1
     a.extend(prefix, ids[:4])
     assert prefix.length == 24
+
+
+def test_the_c_library_builds_without_torch():
+    # in a process where torch cannot be imported; the library here counts as up to date, so nothing is compiled
+    code = ("import sys; sys.modules['torch'] = None; sys.path.insert(0, sys.argv[1]); import build; "
+            "build._compile = lambda *_: ''; build.os.path.getmtime = lambda _: 0; print(build.build())")
+    package = os.path.dirname(os.path.abspath(_lib.__file__))
+    r = subprocess.run([sys.executable, "-c", code, package], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    said, path = r.stdout.strip().splitlines()
+    assert "_fdk_torch.so is not built" in said and path == _lib.LIB_PATH
