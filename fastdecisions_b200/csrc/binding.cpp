@@ -102,13 +102,13 @@ struct Paged {
     if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || (d != 128 && d != 256))
       bad(name, "page sizes 16, 32, 64, 128 and 256 and head_dim 128 or 256 supported");
     for (const at::Tensor* t : {&k, &v})
-      if (t->stride(1) != page_size * d || t->stride(2) != d || t->stride(3) != 1)
+      if ((hkv > 1 && t->stride(1) != page_size * d) || t->stride(2) != d || t->stride(3) != 1)
         bad(name, "a cache page must be contiguous (only the page stride is free)");
     if (quant) {
       for (const at::Tensor* t : {ks, vs}) {
         if (!t || !is(*t, at::kByte, {pages, hkv, page_size}))
           bad(name, "an e4m3 cache needs uint8 k_scale and v_scale [pages, kv heads, page size]");
-        if (t->stride(1) != page_size || t->stride(2) != 1)
+        if ((hkv > 1 && t->stride(1) != page_size) || t->stride(2) != 1)
           bad(name, "the scales of a page must be contiguous (only the page stride is free)");
       }
     } else if (ks || vs) {
@@ -123,8 +123,12 @@ struct Paged {
     max_pages = table.size(1);
     ld_table = segments > 1 ? table.stride(0) : max_pages;
   }
-  int64_t ld_ks() const { return quant ? ks->stride(0) : 0; }
-  int64_t ld_vs() const { return quant ? vs->stride(0) : 0; }
+  // Page strides; a single page has none of its own.
+  int64_t page_stride(const at::Tensor& t, int64_t elems) const { return pages > 1 ? t.stride(0) : elems; }
+  int64_t ld_k() const { return page_stride(k, hkv * page_size * d); }
+  int64_t ld_v() const { return page_stride(v, hkv * page_size * d); }
+  int64_t ld_ks() const { return quant ? page_stride(*ks, hkv * page_size) : 0; }
+  int64_t ld_vs() const { return quant ? page_stride(*vs, hkv * page_size) : 0; }
 };
 
 // Token stride of bf16 rows [tokens, heads, d].
@@ -146,8 +150,8 @@ PyObject* paged_kv_write(PyObject* const* a) {
   const int64_t ldk = token_rows(name, "k", k, c.hkv, c.d), ldv = token_rows(name, "v", v, c.hkv, c.d);
   if (v.size(0) != k.size(0)) bad(name, "k and v must have the same tokens");
   Launch l(dev);
-  status(name, fdk_paged_kv_write(k.data_ptr(), ldk, v.data_ptr(), ldv, kc.data_ptr(), kc.stride(0), vc.data_ptr(),
-                                  vc.stride(0), c.quant, ptr(ks), c.ld_ks(), ptr(vs), c.ld_vs(), c.pages, c.page_size,
+  status(name, fdk_paged_kv_write(k.data_ptr(), ldk, v.data_ptr(), ldv, kc.data_ptr(), c.ld_k(), vc.data_ptr(),
+                                  c.ld_v(), c.quant, ptr(ks), c.ld_ks(), ptr(vs), c.ld_vs(), c.pages, c.page_size,
                                   ptr<int32_t>(&table), c.ld_table, c.max_pages, ptr<int32_t>(&cu), ptr<int32_t>(&lens),
                                   c.segments, k.size(0), c.hkv, c.d, l.stream));
   Py_RETURN_NONE;
@@ -167,7 +171,7 @@ PyObject* paged_kv_read(PyObject* const* a) {
   Launch l(dev);
   const auto opt = kc.options().dtype(at::kBFloat16);
   const at::Tensor k = ko ? *ko : at::empty({tokens, c.hkv, c.d}, opt), v = vo ? *vo : at::empty({tokens, c.hkv, c.d}, opt);
-  status(name, fdk_paged_kv_read(kc.data_ptr(), kc.stride(0), vc.data_ptr(), vc.stride(0), c.quant, ptr(ks), c.ld_ks(),
+  status(name, fdk_paged_kv_read(kc.data_ptr(), c.ld_k(), vc.data_ptr(), c.ld_v(), c.quant, ptr(ks), c.ld_ks(),
                                  ptr(vs), c.ld_vs(), c.pages, c.page_size, ptr<int32_t>(&table), c.ld_table, c.max_pages,
                                  ptr<int32_t>(&cu), ptr<int32_t>(&lens), c.segments, tokens, c.hkv, c.d, k.data_ptr(),
                                  v.data_ptr(), l.stream));
@@ -218,7 +222,7 @@ PyObject* paged_gqa_attention(PyObject* const* a) {
       ws = &scratch;
     }
   }
-  status(name, fdk_paged_gqa_fwd(q.data_ptr(), ldq, kc.data_ptr(), kc.stride(0), vc.data_ptr(), vc.stride(0), c.quant,
+  status(name, fdk_paged_gqa_fwd(q.data_ptr(), ldq, kc.data_ptr(), c.ld_k(), vc.data_ptr(), c.ld_v(), c.quant,
                                  ptr(ks), c.ld_ks(), ptr(vs), c.ld_vs(), c.pages, c.page_size, ptr<int32_t>(&table),
                                  c.ld_table, c.max_pages, ptr<int32_t>(&cu), ptr<int32_t>(&lens), c.segments, max_seqlen,
                                  max_kv, T, hq, c.hkv, d, (float)scale, ptr(gate), ldg, inter, o.data_ptr(), ptr(ws),

@@ -305,3 +305,36 @@ def test_attention_longest_page_table(q_lens):
                 ops.paged_gqa_attention(q.cuda(), k, v, wide, cu, lens, q_lens[0], **kw)
     torch.cuda.synchronize()
     assert _lib.poll_device_error() == 0
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_one_head_or_one_page_in_any_layout(quant):
+    # a dimension of one element has no stride of its own
+    c = Cache([100], 1, 128, 16, quant, 15)
+    q = queries([3], 6, 128, 12)
+    ref = oracle(c, q, [3])
+    cu, lens = cu_of([3]).cuda(), c.kv_lens.cuda()
+
+    def lay(t):  # [pages, page size, heads, ..] in memory, heads second as the operators take it
+        m = torch.empty_strided(t.shape, (t.stride(0), t.stride(2)) + t.stride()[2:], dtype=t.dtype, device="cuda")
+        return m.copy_(t)
+
+    (_, _, table), _ = c.dev()
+    k, v = (lay(t.view(torch.uint8)).view(t.dtype) for t in c.cache)
+    kw = dict(k_scale=lay(c.scale[0]), v_scale=lay(c.scale[1])) if quant else {}
+    attn_check(ops.paged_gqa_attention(q.cuda(), k, v, table, cu, lens, 3, **kw), ref, quant)
+    x = torch.randn(3, 1, 128, generator=gen(16)).to(BF).cuda()
+    ops.paged_kv_write(x, x, k, v, table, cu, lens, **kw)
+    rk, rv = ops.paged_kv_read(k, v, table, cu, lens, 3, **kw)
+    want = O.quantise(x.cpu())[1].to(BF) if quant else x.cpu()
+    assert torch.equal(rk.cpu(), want) and torch.equal(rv.cpu(), want)
+    one = Cache([9], 4, 128, 16, quant, 17)
+    (k, v, table), kw = one.dev()
+    page = int(one.table[0, 0])
+    flat = lambda t: torch.as_strided(t[page:page + 1], t[:1].shape, (1,) + t.stride()[1:], t[page:page + 1].storage_offset())
+    kw = {name: flat(t) for name, t in kw.items()}
+    q = queries([2], 16, 128, 13)
+    o = ops.paged_gqa_attention(q.cuda(), flat(k), flat(v), torch.zeros_like(table[:, :1]), cu_of([2]).cuda(), one.kv_lens.cuda(), 2, **kw)
+    torch.cuda.synchronize()
+    assert _lib.poll_device_error() == 0
+    attn_check(o, oracle(one, q, [2]), quant)
