@@ -40,7 +40,11 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Bad("an integer was expected");
   return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Bad("a truth value was expected");
+  return v == 1;
+}
 
 // The one CUDA device of all given tensors.
 int device_of(std::initializer_list<const at::Tensor*> ts) {

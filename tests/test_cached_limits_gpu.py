@@ -338,3 +338,12 @@ def test_one_head_or_one_page_in_any_layout(quant):
     torch.cuda.synchronize()
     assert _lib.poll_device_error() == 0
     attn_check(o, oracle(one, q, [2]), quant)
+
+
+def test_truth_value_that_cannot_be_taken():
+    c = Cache([10], 4, 128, 16, False, 18)
+    dev, _ = c.dev()
+    q = queries([1], 16, 128, 14).cuda()
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.paged_gqa_attention(q, *dev, cu_of([1]).cuda(), c.kv_lens.cuda(), 1, gate_interleaved=torch.zeros(2))
+    assert torch.isfinite(ops.paged_gqa_attention(q, *dev, cu_of([1]).cuda(), c.kv_lens.cuda(), 1).float()).all()
