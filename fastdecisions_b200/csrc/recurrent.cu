@@ -33,8 +33,8 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t sl
 // A CTA is one (segment, head).  Columns of S evolve on their own, so each of its 8 warps owns 16 of the 128
 // columns and they never exchange state: lane (r, c) = (lane / 4, lane % 4) holds rows 16 r .. 16 r + 15 of
 // columns 4 c .. 4 c + 3 in 64 registers, as pairs of rows (one packed operation works on two).
-// Up to 16 tokens at a time, the warps first share the work that every column needs: k and q normalised to
-// float32, k . q, e^g, beta and v go to shared memory.  The token loop then reads only that.
+// Segments of up to eight tokens are walked.  The warps first share the work that every column needs: k and q
+// normalised to float32, k . q, e^g, beta and v of all tokens go to shared memory.  The token loop then reads only that.
 // S^T k and S^T q of the old state are reduced together, as o = e^g S^T q + (k . q) u with q scaled; the
 // reduction over r leaves one of the eight sums in each lane (7 shuffles instead of 24).
 // The decay is not applied to the registers: they hold S / G with G the product of the decays so far, and
@@ -45,7 +45,10 @@ __device__ __forceinline__ int64_t slot_of(const int32_t* idx, int s, int64_t sl
 // of 1 to 24 tokens 65 us, issue slots 32% and tensor cores 10% busy.
 constexpr int DK = 128, DV = 128, CPW = 16;   // columns a warp
 constexpr int WARPS = DV / CPW;
-constexpr int BATCH = 16;                     // tokens in shared memory at a time
+// Segments of at most this many tokens are walked token by token.  Measured, 16 heads, walked / in batches: 96 segments
+// of 4 tokens 51 / 70 us, of 8 64 / 71, of 9 71 / 71, of 16 100 / 72; one segment of 4 7.2 / 9.3, of 16 13.7 / 9.3.
+constexpr int WALK_MAX = 8;
+constexpr int BATCH = 16;                     // tokens of a batch
 
 struct DeltaParams {
   const bf16* q;
@@ -72,9 +75,9 @@ struct DeltaParams {
 // k and q of a token are kept in the order the lanes read them: rows 16 r + 4 i .. + 3 at float4 8 i + r, so
 // the eight r of a warp read 128 consecutive bytes.
 struct Tokens {
-  float4 k[BATCH][DK / 4], q[BATCH][DK / 4];
-  float v[BATCH][DV];
-  float4 s[BATCH];  // e^g, beta, k . q
+  float4 k[WALK_MAX][DK / 4], q[WALK_MAX][DK / 4];
+  float v[WALK_MAX][DV];
+  float4 s[WALK_MAX];  // e^g, beta, k . q
 };
 
 // ---- More than a few tokens: up to 16 at a time on the tensor cores, at float32 accuracy.  With the state S
@@ -90,9 +93,6 @@ struct Tokens {
 // Warp w keeps S^T for 16 columns of S (dv) as the MMA's accumulators: row g of its tile is column 16 w + 2 g,
 // row g + 8 the next one, so that states are read 8 bytes a lane, and accumulators become A operands as they
 // are.  A batch costs the same for 2 to 16 tokens.
-// Segments of at most this many tokens are walked token by token.  Measured, 16 heads, walked / in batches: 96 segments
-// of 4 tokens 51 / 70 us, of 8 64 / 71, of 9 71 / 71, of 16 100 / 72; one segment of 4 7.2 / 9.3, of 16 13.7 / 9.3.
-constexpr int WALK_MAX = 8;
 constexpr int LDV = DV + 4;  // row stride of v: the four token pairs of a warp's read fall into different banks
 struct Batch16 {
   uint4 k[BATCH][DK / 8], q[BATCH][DK / 8];  // bf16 rows, 16-byte chunks XORed with the row
@@ -435,83 +435,82 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrent_delta_kernel(const De
 #pragma unroll
       for (int j = 0; j < 4; ++j) S[j][i] = __fmul2_rn(S[j][i], f2);
   };
-  for (int64_t tb = t0; tb < t1; tb += BATCH) {
-    const int nt = (int)(t1 - tb < BATCH ? t1 - tb : BATCH);
-    if (tb > t0) __syncthreads();
-    for (int i = warp; i < nt; i += WARPS) {
-      const int64_t t = tb + i;
-      const uint2 kr = __ldg(reinterpret_cast<const uint2*>(p.k + t * p.ld_k + hk * DK) + lane);
-      const uint2 qr = __ldg(reinterpret_cast<const uint2*>(p.q + t * p.ld_q + hk * DK) + lane);
-      const uint2 vr = __ldg(reinterpret_cast<const uint2*>(p.v + t * p.ld_v + h * DV) + lane);
-      const float g = p.g[t * p.heads + h], beta = __bfloat162float(p.beta[t * p.heads + h]);
-      auto two = [](uint32_t w) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };
-      float2 k0 = two(kr.x), k1 = two(kr.y), q0 = two(qr.x), q1 = two(qr.y);
-      const float2 v0 = two(vr.x), v1 = two(vr.y);
-      float rk = 1.f, rq = p.scale;
-      if (p.l2norm) {
-        rk = rsqrtf(warp_sum(k0.x * k0.x + k0.y * k0.y + k1.x * k1.x + k1.y * k1.y) + 1e-6f);
-        rq *= rsqrtf(warp_sum(q0.x * q0.x + q0.y * q0.y + q1.x * q1.x + q1.y * q1.y) + 1e-6f);
-      }
-      const float4 kn = make_float4(k0.x * rk, k0.y * rk, k1.x * rk, k1.y * rk);
-      const float4 qn = make_float4(q0.x * rq, q0.y * rq, q1.x * rq, q1.y * rq);
-      const float kq = warp_sum(kn.x * qn.x + kn.y * qn.y + kn.z * qn.z + kn.w * qn.w);
-      const int at = (lane & 3) * 8 + (lane >> 2);
-      sm.k[i][at] = kn;
-      sm.q[i][at] = qn;
-      *reinterpret_cast<float4*>(&sm.v[i][4 * lane]) = make_float4(v0.x, v0.y, v1.x, v1.y);
-      if (lane == 0) sm.s[i] = make_float4(expf(g), beta, kq, 0.f);
+  const int nt = (int)(t1 - t0);
+  static_assert(WALK_MAX <= WARPS, "a warp a token");
+  if (warp < nt) {
+    const int i = warp;
+    const int64_t t = t0 + i;
+    const uint2 kr = __ldg(reinterpret_cast<const uint2*>(p.k + t * p.ld_k + hk * DK) + lane);
+    const uint2 qr = __ldg(reinterpret_cast<const uint2*>(p.q + t * p.ld_q + hk * DK) + lane);
+    const uint2 vr = __ldg(reinterpret_cast<const uint2*>(p.v + t * p.ld_v + h * DV) + lane);
+    const float g = p.g[t * p.heads + h], beta = __bfloat162float(p.beta[t * p.heads + h]);
+    auto two = [](uint32_t w) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };
+    float2 k0 = two(kr.x), k1 = two(kr.y), q0 = two(qr.x), q1 = two(qr.y);
+    const float2 v0 = two(vr.x), v1 = two(vr.y);
+    float rk = 1.f, rq = p.scale;
+    if (p.l2norm) {
+      rk = rsqrtf(warp_sum(k0.x * k0.x + k0.y * k0.y + k1.x * k1.x + k1.y * k1.y) + 1e-6f);
+      rq *= rsqrtf(warp_sum(q0.x * q0.x + q0.y * q0.y + q1.x * q1.x + q1.y * q1.y) + 1e-6f);
     }
-    __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-      const float4 sc = sm.s[t];
-      G *= sc.x;
-      if (!(G >= 1e-18f && G <= 1e18f)) {  // the same for the whole CTA
-        scale_state(G);
-        G = 1.f;
-      }
-      float2 k[8], dot[8];
+    const float4 kn = make_float4(k0.x * rk, k0.y * rk, k1.x * rk, k1.y * rk);
+    const float4 qn = make_float4(q0.x * rq, q0.y * rq, q1.x * rq, q1.y * rq);
+    const float kq = warp_sum(kn.x * qn.x + kn.y * qn.y + kn.z * qn.z + kn.w * qn.w);
+    const int at = (lane & 3) * 8 + (lane >> 2);
+    sm.k[i][at] = kn;
+    sm.q[i][at] = qn;
+    *reinterpret_cast<float4*>(&sm.v[i][4 * lane]) = make_float4(v0.x, v0.y, v1.x, v1.y);
+    if (lane == 0) sm.s[i] = make_float4(expf(g), beta, kq, 0.f);
+  }
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const float4 sc = sm.s[t];
+    G *= sc.x;
+    if (!(G >= 1e-18f && G <= 1e18f)) {  // the same for the whole CTA
+      scale_state(G);
+      G = 1.f;
+    }
+    float2 k[8], dot[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot[j] = make_float2(0.f, 0.f);
+    for (int j = 0; j < 8; ++j) dot[j] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 k4 = sm.k[t][i * 8 + r], q4 = sm.q[t][i * 8 + r];
-        k[2 * i] = make_float2(k4.x, k4.y);
-        k[2 * i + 1] = make_float2(k4.z, k4.w);
-        const float2 q0 = make_float2(q4.x, q4.y), q1 = make_float2(q4.z, q4.w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          dot[j] = __ffma2_rn(S[j][2 * i], k[2 * i], dot[j]);
-          dot[4 + j] = __ffma2_rn(S[j][2 * i], q0, dot[4 + j]);
-          dot[j] = __ffma2_rn(S[j][2 * i + 1], k[2 * i + 1], dot[j]);
-          dot[4 + j] = __ffma2_rn(S[j][2 * i + 1], q1, dot[4 + j]);
-        }
-      }
-      float d[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = dot[j].x + dot[j].y;
-      // sum over r: lane r ends with sum r of S^T k (columns 0 .. 3), S^T q (columns 0 .. 3)
-#pragma unroll
-      for (int n = 4; n > 0; n >>= 1) {
-        const bool upper = (r & n) != 0;
-#pragma unroll
-        for (int j = 0; j < n; ++j) {
-          const float mine = upper ? d[n + j] : d[j], other = upper ? d[j] : d[n + j];
-          d[j] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
-        }
-      }
-      // lanes r < 4: u of column r; lanes r >= 4 pick it up for their output
-      const float gd = G * d[0];
-      const float u = sc.y * (sm.v[t][col + (r & 3)] - gd);
-      const float uo = __shfl_xor_sync(0xffffffffu, u, 16);
-      if (r >= 4) p.out[((tb + t) * p.heads + h) * DV + col + (r & 3)] = __float2bfloat16_rn(fmaf(sc.z, uo, gd));
-      const float ug = __fdividef(u, G);
+    for (int i = 0; i < 4; ++i) {
+      const float4 k4 = sm.k[t][i * 8 + r], q4 = sm.q[t][i * 8 + r];
+      k[2 * i] = make_float2(k4.x, k4.y);
+      k[2 * i + 1] = make_float2(k4.z, k4.w);
+      const float2 q0 = make_float2(q4.x, q4.y), q1 = make_float2(q4.z, q4.w);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float uj = __shfl_sync(0xffffffffu, ug, 4 * j + c);
-        const float2 uu = make_float2(uj, uj);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) S[j][i] = __ffma2_rn(k[i], uu, S[j][i]);
+        dot[j] = __ffma2_rn(S[j][2 * i], k[2 * i], dot[j]);
+        dot[4 + j] = __ffma2_rn(S[j][2 * i], q0, dot[4 + j]);
+        dot[j] = __ffma2_rn(S[j][2 * i + 1], k[2 * i + 1], dot[j]);
+        dot[4 + j] = __ffma2_rn(S[j][2 * i + 1], q1, dot[4 + j]);
       }
+    }
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = dot[j].x + dot[j].y;
+    // sum over r: lane r ends with sum r of S^T k (columns 0 .. 3), S^T q (columns 0 .. 3)
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1) {
+      const bool upper = (r & n) != 0;
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        const float mine = upper ? d[n + j] : d[j], other = upper ? d[j] : d[n + j];
+        d[j] = mine + __shfl_xor_sync(0xffffffffu, other, 4 * n);
+      }
+    }
+    // lanes r < 4: u of column r; lanes r >= 4 pick it up for their output
+    const float gd = G * d[0];
+    const float u = sc.y * (sm.v[t][col + (r & 3)] - gd);
+    const float uo = __shfl_xor_sync(0xffffffffu, u, 16);
+    if (r >= 4) p.out[((t0 + t) * p.heads + h) * DV + col + (r & 3)] = __float2bfloat16_rn(fmaf(sc.z, uo, gd));
+    const float ug = __fdividef(u, G);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float uj = __shfl_sync(0xffffffffu, ug, 4 * j + c);
+      const float2 uu = make_float2(uj, uj);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) S[j][i] = __ffma2_rn(k[i], uu, S[j][i]);
     }
   }
   if (to >= 0) {

@@ -347,3 +347,24 @@ def test_truth_value_that_cannot_be_taken():
     with pytest.raises((ValueError, RuntimeError)):
         ops.paged_gqa_attention(q, *dev, cu_of([1]).cuda(), c.kv_lens.cuda(), 1, gate_interleaved=torch.zeros(2))
     assert torch.isfinite(ops.paged_gqa_attention(q, *dev, cu_of([1]).cuda(), c.kv_lens.cuda(), 1).float()).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 8, 9, 21])
+@pytest.mark.parametrize("decay", [0.0, -3.0, -30.0, -80.0, -200.0, float("-inf"), 20.0])
+def test_delta_decays_of_any_size_and_length(decay, n):
+    # walked token by token (up to 8) and in batches: extreme decays among the first eight tokens, several in a row;
+    # growth passes 1e18 on the way
+    H = 3
+    for place in ([0], [0, 1, 2], [1, 2, 4, 5, 7], [2, 7, 8, 20]):
+        q, k, v, g, beta = delta_inputs(n, H, H, 90 + n)
+        at = [i for i in place if i < n]
+        g[0, at[:3] if decay > 0 else at] = decay
+        pool = torch.randn(2, H, 128, 128, generator=gen(91)) * 0.5
+        d = pool.cuda()
+        idx = lambda i: torch.tensor([i], dtype=torch.int32).cuda()
+        o = ops.recurrent_gated_delta_rule_(q.cuda(), k.cuda(), v.cuda(), g.cuda(), beta.cuda(), d, idx(0), idx(1))
+        torch.cuda.synchronize()
+        assert _lib.poll_device_error() == 0
+        want, states = O.recurrent_delta(q[0], k[0], v[0], g[0], beta[0], pool[:1], [0, n])
+        delta_check(o[0], want)
+        state_check(d[1:], states)
