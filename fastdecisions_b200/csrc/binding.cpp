@@ -208,8 +208,10 @@ PyObject* paged_gqa_attention(PyObject* const* a) {
   }
   if (out && (!is(*out, at::kBFloat16, {T, hq, d}) || !out->is_contiguous())) bad(name, "out must be contiguous bf16 shaped like q");
   if (ws && !ws->is_contiguous()) bad(name, "workspace must be contiguous");
-  const int64_t max_seqlen = std::min(integer(a[6]), T), reach = c.max_pages * c.page_size;
-  const int64_t max_kv = a[7] == Py_None ? reach : std::min(integer(a[7]), reach);
+  // cut to what the library takes; to the table's reach only where no workspace was sized for the caller's own value
+  const int64_t reach = c.max_pages * c.page_size, most = ws ? 0x7fffff00 : std::min<int64_t>(reach, 0x7fffff00);
+  const int64_t max_seqlen = std::min<int64_t>(integer(a[6]), 0x7fffffff);
+  const int64_t max_kv = std::min(a[7] == Py_None ? reach : integer(a[7]), most);
   if (max_seqlen < 0 || max_kv < 0) bad(name, "max_seqlen and max_kv_len must not be negative");
   double scale = 1.0 / std::sqrt((double)d);
   if (a[10] != Py_None) {

@@ -899,6 +899,7 @@ constexpr int few_ctas(int64_t ctas, int rows, int64_t d, bool quant) {
 static Plan make_plan(int64_t num_segments, int64_t max_seqlen, int64_t max_kv, int64_t tokens, int64_t hkv,
                       int64_t group, int64_t d, bool quant) {
   Plan r = {};
+  if (max_seqlen > tokens) max_seqlen = tokens;
   if (max_seqlen < 1) max_seqlen = 1;  // a bound of no tokens is still checked against the segments
   const int64_t rows = max_seqlen * group;
   int64_t split, least;
@@ -1039,7 +1040,7 @@ extern "C" int fdk_paged_gqa_fwd(const void* q, int64_t ld_q, const void* k_cach
       (quant && (!aligned16(k_scale) || !aligned16(v_scale) || ld_kscale_page % 16 || ld_vscale_page % 16)))
     return set_error(FDK_ERR_ALIGNMENT, "%s: pointers and strides must be 16-byte aligned", what);
   Plan pl = make_plan(num_segments, max_seqlen, max_kv_len, tokens, hkv, hq / hkv, head_dim, quant);
-  if (max_seqlen * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.units : num_segments * pl.row_blocks) > 0x7fffffff)
+  if (std::min(max_seqlen, tokens) * (hq / hkv) > 0x7fffffff || hkv * (pl.many ? pl.units : num_segments * pl.row_blocks) > 0x7fffffff)
     return set_error(FDK_ERR_UNSUPPORTED, "%s: too many segments or query rows", what);
   Params p = {};
   p.q = static_cast<const bf16*>(q); p.ld_q = ld_q;

@@ -724,8 +724,10 @@ def paged_kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
 
 def paged_gqa_workspace_bytes(segments: int, max_seqlen: int, max_kv_len: int, tokens: int, hq: int, hkv: int,
                               head_dim: int, e4m3: bool = False) -> int:
-    """Scratch bytes of ``paged_gqa_attention`` for these sizes (0 when the keys are not split)."""
-    return _lib.load().fdk_paged_gqa_workspace_size(segments, max_seqlen, max_kv_len, tokens, hq, hkv, head_dim, e4m3)
+    """Scratch bytes of ``paged_gqa_attention`` for these sizes (0 when the keys are not split): the call's own
+    arguments, where it has no ``max_kv_len`` the columns of the page table times the page size."""
+    return _lib.load().fdk_paged_gqa_workspace_size(segments, min(max_seqlen, 0x7fffffff), min(max_kv_len, 0x7fffff00), tokens,
+                                                    hq, hkv, head_dim, e4m3)
 
 
 def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

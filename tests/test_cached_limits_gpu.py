@@ -368,3 +368,24 @@ def test_delta_decays_of_any_size_and_length(decay, n):
         want, states = O.recurrent_delta(q[0], k[0], v[0], g[0], beta[0], pool[:1], [0, n])
         delta_check(o[0], want)
         state_check(d[1:], states)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("q_lens,kv", [([1] * 20, [700] * 20), ([100], [4500]), ([70, 30, 5], [4500, 60, 900])])
+def test_attention_workspace_for_loose_bounds(q_lens, kv, quant):
+    # a workspace as the size function gives it serves the call with the same arguments, also where they exceed what
+    # the tensors hold
+    c = Cache(kv, 4, 128, 64, quant, 21)
+    dev, kw = c.dev()
+    q = queries(q_lens, 16, 128, 19)
+    ref = oracle(c, q, q_lens)
+    reach = dev[2].shape[1] * 64
+    for max_seqlen in (max(q_lens), 5000, 2 ** 40):
+        for hint in (None, 1, max(kv), 10000, 2 ** 20, 2 ** 40):
+            need = ops.paged_gqa_workspace_bytes(len(q_lens), max_seqlen, reach if hint is None else hint, sum(q_lens), 16, 4, 128,
+                                                 quant)
+            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+            o = ops.paged_gqa_attention(q.cuda(), *dev, cu_of(q_lens).cuda(), c.kv_lens.cuda(), max_seqlen, hint, workspace=ws, **kw)
+            attn_check(o, ref, quant)
+    torch.cuda.synchronize()
+    assert _lib.poll_device_error() == 0
