@@ -27,8 +27,9 @@
 //   later token's large V row; the second exponential a weight costs 64 sequences x 8 tokens, e4m3, 127 us for 122,
 //   one token each nothing).  q is brought to fp16 with a power of two a row.
 //
-// Measured: one token behind 1535 positions, 16 / 4 heads of 128, bf16, 10.3 us with the launch; 64 ragged sequences of
-// 500 to 8192, e4m3, 51 us, 3.8 TB/s (issue 40% of the slots, DRAM 49%); 64 x 8192, bf16, 153 us unsplit, 7 TB/s.
+// Measured (back to back in a graph): one token behind 1535 positions, 16 / 4 heads of 128, bf16, 7.8 us; 64 x 8192, e4m3,
+// 97 us, 5.6 TB/s, bf16 170 us in the parts that the rule below takes, 6.3 TB/s: near the copy rate.  64 ragged sequences of 500 to 8192, e4m3,
+// 48.7 us, 4.0 TB/s, and bf16 69.5 us, 5.5 TB/s: what the shorter call loses is its start, its uneven end and the join.
 #include <float.h>
 #include <math.h>
 
@@ -44,8 +45,9 @@ using sm100::ex2;
 
 __device__ int g_error = 0;
 
-// sigmoid by the fast exponential and quotient: a relative error below 2^-16 for |x| < 88, where the rounding of
-// the result to bf16 has 2^-9.  With the exact ones 1532 tokens of 8 heads of 256 behind a shared prefix of 1490
+// sigmoid by the fast exponential and quotient: a relative error below 2^-16 for x > -87.3, where the rounding of
+// the result to bf16 has 2^-8; below that 0 (the quotient's divisor passes 2^126), where the sigmoid is less than 2^-125.
+// With the exact ones 1532 tokens of 8 heads of 256 behind a shared prefix of 1490
 // took 58 us, 42 without a gate; with these 46.
 __device__ __forceinline__ float gate_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 

@@ -30,12 +30,15 @@
 //   three for the 8-bit cache (PV of block j and S of block j + 1 hold two, the converters fill the
 //   third), which leaves room for a ring of four raw tiles.
 //
-// Measured (B200, device time): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 250 us,
-// 1.06 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050: the softmax's exponentials and the
-// operands' shared-memory traffic take as long each.  8 ragged chunks (2544 tokens behind 600 to 8000), e4m3, page
-// 16: 115 us; 3700 cycles a block, 20000 before the first, and uneven CTAs.  48 questions of 9 to 70 tokens behind
-// 1490 shared positions, 8 / 2 heads of 256, bf16: 45 us; a block of 64 keys brings 64 KB from L2, 32 bytes a clock
-// and SM, which sets its 2050 cycles; the start and the epilogue of the one wave are a third of the call.
+// Measured (B200, back to back in a graph): 2 x 2048 tokens behind 6144 and 14000 positions, 16 / 4 heads of 128, bf16: 241
+// us, 1.10 PF/s; a block of 128 keys takes 3500 cycles where its MMAs take 2050, as long as the softmax's exponentials
+// and the operands' shared-memory traffic each: no unit is full, a tile's chain of S, softmax, P and PV is what is
+// left.  8 ragged chunks (2544 tokens behind 600 to 8000), e4m3, page 16: 109 us; 3700 cycles a block, 20000 before
+// the first, and uneven CTAs (tensor pipe 27%, issue slots 30%).  48 questions of 9 to 70 tokens behind 1490 shared
+// positions, 8 / 2 heads of 256, bf16: 42 us; a block of 64 keys brings 64 KB to an SM in its 2050 cycles, L2 as a whole
+// 16% busy (which of the copies' latency and the SM's share of L2 sets this was not separated); the start and the
+// epilogue of the one wave are a third of the call.  74 x 32 tokens behind 4096 shared positions, 8 / 2 heads of 256,
+// e4m3: 93 us.  Whole prompts, no history, 16 / 4 heads of 128, bf16: 8192 tokens 252 us, 32 x 1024 299 us.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>

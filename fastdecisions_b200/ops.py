@@ -701,7 +701,7 @@ def _counted(name: str):
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                    page_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
-    """Writes ``k, v [T, Hkv, D]`` (bf16, token stride free) into the paged cache ``k_cache, v_cache
+    """Writes ``k, v [T, Hkv, D]`` (bf16, token stride free, rows 16-byte aligned) into the paged cache ``k_cache, v_cache
     [pages, Hkv, page size, D]``: bf16, or ``float8_e4m3fn`` with uint8 ``k_scale, v_scale [pages, Hkv,
     page size]`` (byte b: the row times ``2 ** (b - 127)``).  Segment s's tokens ``cu_seqlens[s] ..
     cu_seqlens[s + 1] - 1`` are the last of its ``kv_lens[s]`` positions; position p is row ``p % page
@@ -736,11 +736,11 @@ def paged_gqa_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                         gate: Optional[torch.Tensor] = None, gate_interleaved: bool = False,
                         out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Causal attention of ``q [T, Hq, D]`` (token stride free), the newest tokens of each segment, over
-    the paged cache (see ``paged_kv_write``, which has written their own keys): token i of a segment's
+    """Causal attention of ``q [T, Hq, D]`` (token stride free, rows 16-byte aligned), the newest tokens of each
+    segment, over the paged cache (see ``paged_kv_write``, which has written their own keys): token i of a segment's
     n attends to positions ``0 .. kv_lens[s] - n + i``; one that sees nothing gets zeros.  ``max_seqlen``
-    bounds the tokens of a segment; ``max_kv_len`` (default: the page table's reach) only guides how the
-    keys are split.  ``gate`` / ``gate_interleaved`` / ``scale`` as ``gqa_attention_varlen_``.  A
+    bounds the tokens of a segment (a longer one is reported by the device error word); ``max_kv_len`` (default:
+    the page table's reach) only guides how the keys are split.  ``gate`` / ``gate_interleaved`` / ``scale`` as ``gqa_attention_varlen_``.  A
     ``workspace`` (``paged_gqa_workspace_bytes``) may serve calls that do not overlap on the GPU; without
     one it is allocated."""
     return _counted("fdk_paged_gqa_fwd").paged_gqa_attention(
@@ -795,6 +795,7 @@ def packed_conv_state_(x: torch.Tensor, weight: torch.Tensor, state: torch.Tenso
     """``packed_conv_qkv`` continued from cached inputs: ``state [slots, K - 1, C]`` bf16 holds the last
     ``K - 1`` input rows of each sequence (oldest first) and is updated in place; ``state_indices`` /
     ``final_indices`` as ``recurrent_gated_delta_rule_`` (a negative index: zeros before the segment).
-    ``x [B, T, C]`` (unit column stride, any row stride) -> ``q, k, v [B, T, heads, head_dim]``."""
+    ``x [B, T, C]`` (unit column stride, any row stride that keeps rows 16-byte aligned) ->
+    ``q, k, v [B, T, heads, head_dim]``."""
     return _counted("fdk_packed_conv_state").packed_conv_state(x, weight, state, state_indices, final_indices, key_dim,
                                                                value_dim, head_dim, cu_seqlens)

@@ -292,7 +292,8 @@ size_t fdk_paged_gqa_workspace_size(int64_t num_segments, int64_t max_seqlen, in
  * CTA reads, later tokens' than a row's own among them: exact for scales down to 2^-22 of it, rounded
  * to multiples of 2^-31 of it for scales down to 2^-31, zeros below.
  * A non-finite V row may reach every row of its call that shares a tile with it, masked ones included;
- * K rows and rows past kv_lens[s] never do.  The caller's workspace holds float32 partial results and
+ * K rows and rows past kv_lens[s] never do (an infinity written to an e4m3 cache is a finite row of a
+ * large scale, for which the bounds above hold).  The caller's workspace holds float32 partial results and
  * the size of the parts, which the device takes from the lengths; calls that overlap on the GPU need
  * separate ones.
  */
