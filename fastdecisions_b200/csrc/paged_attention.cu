@@ -27,9 +27,10 @@
 //   later token's large V row; the second exponential a weight costs 64 sequences x 8 tokens, e4m3, 127 us for 122,
 //   one token each nothing).  q is brought to fp16 with a power of two a row.
 //
-// Measured (back to back in a graph): one token behind 1535 positions, 16 / 4 heads of 128, bf16, 7.8 us; 64 x 8192, e4m3,
-// 97 us, 5.6 TB/s, bf16 170 us in the parts that the rule below takes, 6.3 TB/s: near the copy rate.  64 ragged sequences of 500 to 8192, e4m3,
-// 48.7 us, 4.0 TB/s, and bf16 69.5 us, 5.5 TB/s: what the shorter call loses is its start, its uneven end and the join.
+// Measured (back to back in a graph): one token behind 1535 positions, 16 / 4 heads of 128, bf16, 7.8 us; 64 x 8192,
+// e4m3, 97 us, 5.6 TB/s, bf16 170 us in the parts that the rule below takes, 6.3 TB/s: near the copy rate.  64 ragged
+// sequences of 500 to 8192, e4m3, 48.7 us, 4.0 TB/s, and bf16 69.5 us, 5.5 TB/s: what the shorter call loses is its
+// start, its uneven end and the join.
 #include <float.h>
 #include <math.h>
 
@@ -46,9 +47,9 @@ using sm100::ex2;
 __device__ int g_error = 0;
 
 // sigmoid by the fast exponential and quotient: a relative error below 2^-16 for x > -87.3, where the rounding of
-// the result to bf16 has 2^-8; below that 0 (the quotient's divisor passes 2^126), where the sigmoid is less than 2^-125.
-// With the exact ones 1532 tokens of 8 heads of 256 behind a shared prefix of 1490
-// took 58 us, 42 without a gate; with these 46.
+// the result to bf16 has 2^-8; below that 0 (the quotient's divisor passes 2^126), where the sigmoid is less than
+// 2^-125.  With the exact ones 1532 tokens of 8 heads of 256 behind a shared prefix of 1490 took 58 us, 42 without a
+// gate; with these 46.
 __device__ __forceinline__ float gate_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 struct Params {
@@ -861,8 +862,8 @@ static int launch_rows(const Params& p, int rows, cudaStream_t s) {
   }
 }
 
-// Positions of a sequence.  The kernels step through them in 32 bits and look ahead: the scan of the scale bytes by
-// 7 x 3072 keys, the others by less than 512.
+// Positions of a sequence.  The kernels step through them in 32 bits and look ahead: the scan of the scale bytes by up
+// to 21504 keys, the others by less than 512.
 constexpr int64_t MOST_POSITIONS = 0x7fff0000;
 
 // Tiling of a call: the kernel, its rows a CTA and the split of the keys.  All follow from host-side
